@@ -1,0 +1,882 @@
+// emmy_paged_attention.cu -- attention of ragged chunks of new tokens, from one
+// token a sequence upwards, over a paged key/value cache.
+//
+//   s_j = scale q.k_j,  o = sum_j e^(s_j - m) v_j / l,  l = sum_j e^(s_j - m)
+//
+// in one pass over the keys with a running maximum and sum.  The G query heads
+// of a key head are stacked with the tokens (row = token * G + head of the
+// group), so a key tile is read once for all of them, whatever G is.
+//
+// One persistent CTA an SM walks its list of units (emmy_paged.h).  Its roles:
+//   warps 0-3, 4-7  softmax of stream 0 and 1, one thread a row;
+//   warp 8          issues the tensor-core products and loads the query tiles;
+//   warp 9          loads key and value tiles, page by page, into one ring;
+//   warps 10-11     fill the warpgroup that gives registers to the softmax.
+// A unit with two query tiles gives one to each stream and both see every key
+// tile; a unit with one query tile (decode) gives it to both streams, which
+// take the key tiles in turn and are joined at the end.  Either way one
+// stream's softmax runs while the tensor cores work for the other.
+//
+// Tensor memory: S_t at column 128 t, P_t over it (two 16-bit weights a
+// column), O_t at 256 + 128 t.  S = Q K^T and O += P V are 128 x 128 x D and
+// 128 x D x 128 tcgen05.mma chains; both accumulate in 32 bits.  P is rounded
+// to the type of V, which the product needs; the sum l is taken before that.
+//
+// Every wait is bounded; one that runs out sets the plan's status word, and
+// from then on nothing more is issued.
+#include "emmy_paged.h"
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+
+int emmy_internal_fail(int code, const char *msg);   // emmy_runtime.cpp
+
+namespace {
+
+using emmy_paged::kTile;
+using emmy_paged::Unit;
+
+constexpr int kThreads = 384;
+// registers a thread: at launch, then those of the softmax warps, which hold a
+// row of scores, and of the others; the shares add up to what was launched
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
+constexpr int kMmaWarp = 8;             // the next warp loads
+constexpr int kSmem = 227 * 1024;
+constexpr float kNoMax = -1e30f;        // exponent base of a row that has seen no key
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct alignas(64) Params {
+  CUtensorMap q, k, v;
+  const Unit *units;
+  const int *cta_first;
+  const int *table;
+  unsigned *counters, *status;
+  float *part_o;
+  float2 *part_ml;
+  void *out;
+  float *lse;
+  int64_t table_stride, out_stride[2];
+  int q_heads, group, per_tile, page_size, box, causal, window;
+  float scale_log2;
+};
+
+template <int D> struct Shape {
+  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kStages = D == 128 ? 5 : 12;      // key and value tiles in flight
+  static constexpr int kRing = 2 * kTileBytes;           // after two query tiles
+  static constexpr int kBars = kRing + kStages * kTileBytes;
+  static constexpr int kEnd = kBars + (2 * kStages + 8) * 8 + 32 + kTile * 8;
+  static_assert(kEnd + 1024 <= kSmem, "shared memory");
+};
+
+// ---------------------------------------------------------------- PTX
+__device__ __forceinline__ uint32_t smem_addr(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+// What a role needs to give up: the CTA's flag (any role may set it) and the
+// plan's status word.
+struct Guard {
+  volatile int *dead;
+  unsigned *status;
+  // false once a wait of this CTA ran out (2 s); the caller then issues nothing more
+  __device__ __forceinline__ bool slow(uint32_t bar, uint32_t parity, int code) const {
+    const uint64_t t0 = now_ns();
+    for (;;) {
+      if (bar_try(bar, parity)) return true;
+      if (*dead) return false;
+      if (now_ns() - t0 > 2000000000ull) {
+        *dead = 1;
+        atomicExch(status, code);
+        return false;
+      }
+    }
+  }
+  // one answer for the warp
+  __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int code) const {
+    const bool ok = bar_try(bar, parity);
+    return __all_sync(~0u, ok) || __all_sync(~0u, slow(bar, parity, code));
+  }
+};
+
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// a and b: low words of the operands' descriptors, `high` the high word of both
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(static_cast<uint32_t>(acc))
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(static_cast<uint32_t>(acc))
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// the registers of a load are valid only after this: they pass through it so
+// that no use of them can move above it
+template <int N> __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float &x, float &y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+template <bool BF16> __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if (BF16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Shared-memory operand descriptor: 128-byte swizzle, leading and stride byte
+// offsets in 16-byte units.  Keys and queries are K-major (rows of 64
+// components, 8-row groups 1024 bytes apart); values are MN-major (64 columns
+// of one key a row, the next 64 columns 16 KiB further).
+constexpr uint32_t kOperandHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t operand(uint32_t addr, uint32_t lead) {
+  uint32_t low = ((addr >> 4) & 0x3fff) | ((lead >> 4) << 16);
+  asm volatile("" : "+r"(low));      // the steps along it are added where used, not kept
+  return low;
+}
+template <bool BF16> __host__ __device__ constexpr uint32_t instruction(int n, bool b_mn_major) {
+  return (1u << 4) | (uint32_t(BF16) << 7) | (uint32_t(BF16) << 10) | (uint32_t(b_mn_major) << 16) | (uint32_t(n >> 3) << 17) |
+         (uint32_t(kTile >> 4) << 24);
+}
+
+// ---------------------------------------------------------------- roles
+template <int D> struct Smem {
+  uint32_t base;       // 1024-byte aligned
+  char *ptr;           // the same, generic
+  __device__ uint32_t query(int t) const { return base + t * Shape<D>::kTileBytes; }
+  __device__ uint32_t stage(int s) const { return base + Shape<D>::kRing + s * Shape<D>::kTileBytes; }
+  __device__ uint32_t bar(int i) const { return base + Shape<D>::kBars + 8 * i; }
+  __device__ uint32_t full(int s) const { return bar(s); }
+  __device__ uint32_t empty(int s) const { return bar(Shape<D>::kStages + s); }
+  __device__ uint32_t q_full() const { return bar(2 * Shape<D>::kStages); }
+  __device__ uint32_t s_full(int t) const { return bar(2 * Shape<D>::kStages + 1 + t); }
+  __device__ uint32_t p_ready(int t) const { return bar(2 * Shape<D>::kStages + 3 + t); }
+  __device__ uint32_t final(int t) const { return bar(2 * Shape<D>::kStages + 5 + t); }
+  __device__ uint32_t drain() const { return bar(2 * Shape<D>::kStages + 7); }
+  __device__ volatile int *words() const { return reinterpret_cast<volatile int *>(ptr + Shape<D>::kBars + (2 * Shape<D>::kStages + 8) * 8); }
+  __device__ float2 *ml() const { return reinterpret_cast<float2 *>(ptr + Shape<D>::kBars + (2 * Shape<D>::kStages + 8) * 8 + 32); }
+};
+// words(): 0 dead, 1 tensor memory address, 2 + t "last to arrive" of stream t
+
+template <int D> struct Ring {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == Shape<D>::kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// Read anew where it is used (from L1): a unit kept in registers across the
+// loop over its key tiles would cost the softmax warps 16 of them.
+__device__ __forceinline__ Unit read_unit(const Params &p, int i) {
+  Unit u;
+  const Unit *at = p.units + i;
+  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.seq), "=r"(u.kvh), "=r"(u.tok0), "=r"(u.ntok) : "l"(at));
+  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4+16];" : "=r"(u.pos0), "=r"(u.tile0), "=r"(u.ntiles), "=r"(u.lo) : "l"(at));
+  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4+32];" : "=r"(u.hi), "=r"(u.kv_len), "=r"(u.wide), "=r"(u.item) : "l"(at));
+  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4+48];" : "=r"(u.split), "=r"(u.nsplit), "=r"(u.part_row), "=r"(u.pad) : "l"(at));
+  return u;
+}
+
+// Keys and values: lane b of the warp copies box b of a tile (a page, or 128
+// tokens of one).  Boxes without a key that the item sees are left out; what
+// the stage then holds in their place is masked (keys) or cleared (values).
+template <int D> __device__ void load_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last) {
+  const int lane = threadIdx.x % 32;
+  const int boxes = kTile / p.box;
+  Ring<D> ring;
+  int issued = 0;
+  bool alive = true;
+  for (int i = first; i < last && alive; ++i) {
+    const Unit u = read_unit(p, i);
+    if (!u.ntiles) continue;
+    const int ahead = u.wide ? 1 : 2;
+    const int *row = p.table + u.seq * p.table_stride;
+    auto page_of = [&](int tile) {           // the page of this lane's box; -1: no box
+      const int key = (u.tile0 + tile) * kTile + lane * p.box;
+      const bool wanted = tile < u.ntiles && lane < boxes && key < u.hi && key + p.box > u.lo;
+      return wanted ? max(-1, __ldg(row + key / p.page_size)) : INT_MIN;
+    };
+    auto load = [&](const CUtensorMap *map, int tile, int page) {
+      alive = alive && g.wait(sm.empty(ring.stage), ring.phase ^ 1, 1);
+      if (!alive) return;
+      const int key = (u.tile0 + tile) * kTile + lane * p.box;
+      const bool wanted = page != INT_MIN;
+      const uint32_t bar = sm.full(ring.stage);
+      const int n = __popc(__ballot_sync(~0u, wanted));
+      if (lane == 0) bar_expect(bar, n * p.box * D * 2);
+      __syncwarp();
+      if (wanted) {
+        const uint32_t dst = sm.stage(ring.stage) + lane * p.box * 128;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+          load_box(dst + h * (kTile * 128), map, bar, 64 * h, key % p.page_size, u.kvh, page);
+      }
+      ring.next();
+      ++issued;
+    };
+    int p0 = page_of(0), p1 = page_of(1), p2 = page_of(2);
+    load(&p.k, 0, p0);
+    if (ahead == 2 && u.ntiles > 1) load(&p.k, 1, p1);
+    for (int n = 0; n < u.ntiles; ++n) {
+      const int p3 = page_of(n + 3);
+      load(&p.v, n, p0);
+      if (n + ahead < u.ntiles) load(&p.k, n + ahead, ahead == 1 ? p1 : p2);
+      p0 = p1;
+      p1 = p2;
+      p2 = p3;
+    }
+  }
+  if (!alive) {       // copies in flight land before the CTA ends
+    const int n = min(issued, Shape<D>::kStages);
+    for (int k = 0; k < n; ++k) {
+      if (ring.stage == 0) {
+        ring.stage = Shape<D>::kStages;
+        ring.phase ^= 1;
+      }
+      --ring.stage;
+      const uint64_t t0 = now_ns();
+      while (!bar_try(sm.full(ring.stage), ring.phase) && now_ns() - t0 < 100000000ull) {
+      }
+    }
+  }
+}
+
+template <int D, bool BF16> __device__ void mma_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last, uint32_t tmem) {
+  const int lane = threadIdx.x % 32;
+  constexpr uint32_t kQk = instruction<BF16>(kTile, false), kPv = instruction<BF16>(D, true);
+  Ring<D> ring;
+  uint32_t q_phase = 0, p_phase[2] = {0, 0};
+  bool alive = true, q_pending = false;
+  uint32_t q_awaited = 0;
+  const int rows_bytes = p.group * p.per_tile * 128;
+  auto wait = [&](uint32_t bar, uint32_t parity) { alive = alive && g.wait(bar, parity, 2); };
+  auto issue_qk = [&](int t, int q, int stage) {      // S_t = Q_q K^T
+    if (lane == 0 && alive) {
+      const uint32_t a = operand(sm.query(q), 16), b = operand(sm.stage(stage), 16);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const int off = (k % 4) * 2 + (k / 4) * (kTile * 128 / 16);
+        mma_ss(tmem + kTile * t, a + off, b + off, kOperandHigh, kQk, k > 0);
+      }
+      commit(sm.s_full(t));
+    }
+  };
+  auto issue_pv = [&](int t, int stage, bool acc) {   // O_t (+)= P_t V
+    if (lane == 0 && alive) {
+      const uint32_t b = operand(sm.stage(stage), kTile * 128);
+#pragma unroll
+      for (int k = 0; k < kTile / 16; ++k)
+        mma_ts(tmem + 2 * kTile + kTile * t, tmem + kTile * t + 8 * k, b + k * (16 * 128 / 16), kOperandHigh, kPv, acc || k > 0);
+    }
+  };
+  auto release = [&](int stage) {
+    if (lane == 0 && alive) commit(sm.empty(stage));
+  };
+  auto clear_values = [&](const Unit &u, int tile, int stage) {
+    // values of keys that no token of the item sees are unwritten or another's:
+    // their weight is 0, but 0 times an infinity is not
+    const int key0 = (u.tile0 + tile) * kTile;
+    const int above = min(kTile, max(0, u.hi - key0)), below = min(kTile, max(0, u.lo - key0));
+    if (above == kTile && below == 0) return;
+    constexpr int kChunks = D / 8;        // of 16 bytes a key
+    for (int i = lane; i < (below + kTile - above) * kChunks; i += 32) {
+      int key = i / kChunks;
+      key = key < below ? key : key - below + above;
+      const int chunk = i % kChunks;
+      const uint32_t at = sm.stage(stage) + (chunk / 8) * (kTile * 128) + key * 128 + (chunk % 8) * 16;
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+  };
+  for (int i = first; i < last; ++i) {
+    const Unit u = read_unit(p, i);
+    if (!u.ntiles) continue;
+    if (alive) {
+      // every product that read the last unit's queries has completed: the
+      // softmax warps have since used its scores
+      if (lane == 0) {
+        bar_expect(sm.q_full(), (u.wide ? 2 : 1) * (D / 64) * rows_bytes);
+        for (int t = 0; t < (u.wide ? 2 : 1); ++t)
+          for (int h = 0; h < D / 64; ++h)
+            load_box(sm.query(t) + h * (kTile * 128), &p.q, sm.q_full(), 64 * h, 0, u.kvh, u.tok0 + t * p.per_tile);
+      }
+      q_pending = true;
+      q_awaited = q_phase;
+      __syncwarp();
+    }
+    wait(sm.q_full(), q_phase);
+    if (alive) q_pending = false;
+    q_phase ^= 1;
+    const int ahead = u.wide ? 1 : 2;
+    for (int n = 0; n < min(ahead, u.ntiles); ++n) {
+      wait(sm.full(ring.stage), ring.phase);
+      fence_after();
+      if (u.wide) {
+        issue_qk(0, 0, ring.stage);
+        issue_qk(1, 1, ring.stage);
+      } else {
+        issue_qk(n, 0, ring.stage);
+      }
+      release(ring.stage);
+      ring.next();
+    }
+    for (int n = 0; n < u.ntiles; ++n) {
+      const int v_stage = ring.stage;
+      wait(sm.full(v_stage), ring.phase);
+      ring.next();
+      if (alive) clear_values(u, n, v_stage);
+      const bool more = n + ahead < u.ntiles;
+      const int k_stage = ring.stage;
+      if (more) {
+        wait(sm.full(k_stage), ring.phase);
+        ring.next();
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!u.wide && t != n % 2) continue;
+        wait(sm.p_ready(t), p_phase[t]);
+        p_phase[t] ^= 1;
+        fence_after();
+        issue_pv(t, v_stage, n >= ahead);
+        if (more)
+          issue_qk(t, u.wide ? t : 0, k_stage);
+        else if (lane == 0 && alive)
+          commit(sm.final(t));
+      }
+      release(v_stage);
+      if (more) release(k_stage);
+    }
+  }
+  // nothing of this thread's is in flight when the CTA gives up its memory
+  if (lane == 0) commit(sm.drain());
+  const uint64_t t0 = now_ns();
+  while (!bar_try(sm.drain(), 0) && now_ns() - t0 < 100000000ull) {
+  }
+  while (q_pending && !bar_try(sm.q_full(), q_awaited) && now_ns() - t0 < 100000000ull) {
+  }
+}
+
+__device__ __forceinline__ void group_sync(int id, int threads) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+template <int D, bool BF16> __device__ void softmax_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last, uint32_t tmem) {
+  // exponents may run 8 over the base before it moves; 16-bit floats of 5
+  // exponent bits get a base 6 lower, so that small weights keep their bits
+  constexpr float kShift = BF16 ? 0.f : 6.f, kGrow = 8.f;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, t = warp / 4, wid = warp % 4;
+  const int row = threadIdx.x % kTile;
+  const uint32_t lanes = tmem + (uint32_t(wid * 32) << 16);
+  const uint32_t s_at = lanes + kTile * t, o_at = lanes + 2 * kTile + kTile * t;
+  const float c = p.scale_log2;
+  uint32_t s_phase = 0, f_phase = 0;
+  bool alive = true;
+  // this stream's tile of queries: its first token in the unit, and its rows
+  auto first_token = [&](const Unit &u) { return u.wide ? t * p.per_tile : 0; };
+  auto stream_rows = [&](const Unit &u) { return min(u.ntok - first_token(u), p.per_tile) * p.group; };
+  for (int i = first; i < last; ++i) {
+    int my_lo, my_hi, step, key0, end;      // keys seen by this row; first key of a tile
+    bool warp_active;
+    {
+      const Unit u = read_unit(p, i);
+      const int rows = stream_rows(u);
+      warp_active = wid * 32 < rows;
+      const int pos = u.pos0 + first_token(u) + min(row, rows - 1) / p.group;
+      my_hi = p.causal ? min(u.kv_len, pos + 1) : u.kv_len;
+      my_lo = p.window ? max(0, pos - p.window + 1) : 0;
+      step = u.wide ? kTile : 2 * kTile;
+      key0 = (u.tile0 + (u.wide ? 0 : t)) * kTile;
+      end = (u.tile0 + u.ntiles) * kTile;
+    }
+    const int min_hi = __reduce_min_sync(~0u, my_hi), max_lo = __reduce_max_sync(~0u, my_lo);
+    float m = kNoMax, l = 0.f;
+    bool begun = false;
+    for (; key0 < end; key0 += step) {
+      alive = alive && g.wait(sm.s_full(t), s_phase, 3);
+      s_phase ^= 1;
+      if (warp_active && alive) {
+        fence_after();
+        uint32_t s[kTile];
+#pragma unroll
+        for (int k = 0; k < kTile; k += 32) tmem_ld32(s_at + k, s + k);
+        tmem_ld_wait(s);
+        if (key0 < max_lo || key0 + kTile > min_hi) {
+          const int from = my_lo - key0;
+          const unsigned span = my_hi > my_lo ? my_hi - my_lo : 0;
+#pragma unroll
+          for (int k = 0; k < kTile; ++k)
+            if (unsigned(k - from) >= span) s[k] = __float_as_uint(-INFINITY);
+        }
+        const uint64_t c2 = pair(c, c);
+        float sum;
+        for (;;) {
+          const uint64_t base2 = pair(-m, -m);
+          uint64_t part[4] = {0, 0, 0, 0};
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            uint32_t w[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+              const float x = __uint_as_float(s[32 * h + 2 * q]), y = __uint_as_float(s[32 * h + 2 * q + 1]);
+              top[q % 4] = fmaxf(fmaxf(top[q % 4], x), y);
+              float e, f;
+              unpair(fma2(pair(x, y), c2, base2), e, f);
+              e = exp2_approx(e);
+              f = exp2_approx(f);
+              part[q % 4] = add2(part[q % 4], pair(e, f));
+              w[q] = pack16<BF16>(e, f);
+            }
+            tmem_st16(s_at + 16 * h, w);
+          }
+          float x, y;
+          unpair(add2(add2(part[0], part[1]), add2(part[2], part[3])), x, y);
+          sum = x + y;
+          const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+          const bool need = best > m + (kShift + kGrow);
+          if (!__any_sync(~0u, need)) break;
+          // a new base, and the weights again from it; the running sum and
+          // output (idle: the last product is complete) come down to it
+          const float to = need ? best - kShift : m;
+          const float by = need ? exp2_approx(m - to) : 1.f;
+          m = to;
+          l *= by;
+          if (begun) {
+            const uint64_t by2 = pair(by, by);
+#pragma unroll 1
+            for (int k = 0; k < D; k += 16) {
+              uint32_t o[16];
+              tmem_ld16(o_at + k, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                float x, y;
+                unpair(mul2(pair(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])), by2), x, y);
+                o[2 * q] = __float_as_uint(x);
+                o[2 * q + 1] = __float_as_uint(y);
+              }
+              tmem_st16(o_at + k, o);
+            }
+          }
+        }
+        l += sum;
+        tmem_st_wait();
+        fence_before();
+      }
+      begun = true;
+      __syncwarp();
+      if (lane == 0) bar_arrive(sm.p_ready(t));
+    }
+
+    // ------------------------------------------------------------ the unit's end
+    const Unit u = read_unit(p, i);
+    const int rows = stream_rows(u), row0 = first_token(u) * p.group;
+    const bool joined = !u.wide && u.ntiles > 1;      // stream 1 saw keys too
+    if (begun) {
+      alive = alive && g.wait(sm.final(t), f_phase, 4);
+      f_phase ^= 1;
+      fence_after();
+    }
+    float by0 = 1.f, by1 = 0.f;
+    if (joined) {
+      if (t == 1) sm.ml()[row] = make_float2(m, l);
+      fence_before();
+      group_sync(3, 256);           // stream 1's output is complete as well
+      if (t == 0) {
+        const float2 other = sm.ml()[row];
+        const float top = fmaxf(m, other.x);
+        by0 = exp2_approx(m - top);
+        by1 = exp2_approx(other.x - top);
+        l = l * by0 + other.y * by1;
+        m = top;
+      }
+    }
+    if (t == 0 || u.wide) {
+      fence_after();
+      const bool mine = warp_active && row < rows && alive;
+      const int64_t out_token = u.tok0 + first_token(u) + row / p.group;
+      const int head = u.kvh * p.group + row % p.group;
+      const bool split = u.nsplit > 1;
+      const int64_t part = u.part_row + int64_t(u.split) * u.ntok * p.group + row0 + row;
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const float f0 = split ? by0 : by0 * inv, f1 = split ? by1 : by1 * inv;
+      if (warp_active && alive) {
+#pragma unroll 1
+        for (int k = 0; k < D; k += 32) {
+          uint32_t o[32];
+          if (begun) {
+            tmem_ld32(o_at + k, o);
+            tmem_ld_wait(o);
+          }
+#pragma unroll
+          for (int q = 0; q < 32; ++q) o[q] = begun && l != 0.f ? __float_as_uint(__uint_as_float(o[q]) * f0) : 0u;
+          if (joined) {
+            uint32_t o1[32];
+            tmem_ld32(o_at + kTile + k, o1);
+            tmem_ld_wait(o1);
+#pragma unroll
+            for (int q = 0; q < 32; ++q)
+              if (l != 0.f) o[q] = __float_as_uint(fmaf(__uint_as_float(o1[q]), f1, __uint_as_float(o[q])));
+          }
+          if (mine && split) {
+            float4 *dst = reinterpret_cast<float4 *>(p.part_o + part * D + k);
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              __stcg(dst + q, make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]),
+                                          __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3])));
+          } else if (mine) {
+            uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + out_token * p.out_stride[0] +
+                                                   head * p.out_stride[1] + k);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t w[4];
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                w[r] = pack16<BF16>(__uint_as_float(o[8 * q + 2 * r]), __uint_as_float(o[8 * q + 2 * r + 1]));
+              dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+        if (mine && split) __stcg(p.part_ml + part, make_float2(m, l));
+        if (mine && !split && p.lse)
+          p.lse[out_token * p.q_heads + head] = l > 0.f ? (m + log2f(l)) * kLn2 : (l == 0.f ? -INFINITY : l);
+      }
+      fence_before();
+      if (split) {
+        // the stream that arrives last joins the parts, in their order
+        __threadfence();
+        group_sync(1 + t, kTile);
+        if (row == 0) {
+          unsigned *counter = p.counters + 2 * u.item + t;
+          const bool is_last = alive && atomicAdd(counter, 1u) == unsigned(u.nsplit - 1);
+          if (is_last) *counter = 0;
+          __threadfence();
+          sm.words()[2 + t] = is_last;
+        }
+        group_sync(1 + t, kTile);
+        if (sm.words()[2 + t]) {
+          constexpr int kWidth = D / 32;            // components a lane
+          for (int r = wid; r < rows; r += 4) {
+            const int64_t at = u.part_row + row0 + r, stride = int64_t(u.ntok) * p.group;
+            float top = kNoMax;
+            for (int s = lane; s < u.nsplit; s += 32) top = fmaxf(top, __ldcg(p.part_ml + at + s * stride).x);
+#pragma unroll
+            for (int k = 16; k; k /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, k));
+            float acc[kWidth] = {}, total = 0.f;
+            for (int s0 = 0; s0 < u.nsplit; s0 += 32) {
+              float2 ml = make_float2(kNoMax, 0.f);
+              if (s0 + lane < u.nsplit) ml = __ldcg(p.part_ml + at + (s0 + lane) * stride);
+              const float by = ml.y == 0.f ? 0.f : exp2_approx(ml.x - top);
+              total += by * ml.y;
+              const int n = min(32, u.nsplit - s0);
+#pragma unroll 8
+              for (int s = 0; s < n; ++s) {
+                const float w = __shfl_sync(~0u, by, s);
+                const float *src = p.part_o + (at + (s0 + s) * stride) * D + lane * kWidth;
+                if constexpr (kWidth == 4) {
+                  const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
+                  acc[0] += w * v.x, acc[1] += w * v.y, acc[2] += w * v.z, acc[3] += w * v.w;
+                } else {
+                  const float2 v = __ldcg(reinterpret_cast<const float2 *>(src));
+                  acc[0] += w * v.x, acc[1] += w * v.y;
+                }
+              }
+            }
+#pragma unroll
+            for (int k = 16; k; k /= 2) total += __shfl_xor_sync(~0u, total, k);
+            const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
+            const int64_t tok = u.tok0 + first_token(u) + r / p.group;
+            const int h = u.kvh * p.group + r % p.group;
+            uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + tok * p.out_stride[0] +
+                                                         h * p.out_stride[1] + lane * kWidth);
+            if constexpr (kWidth == 4)
+              *reinterpret_cast<uint2 *>(dst) = make_uint2(pack16<BF16>(acc[0] * inv, acc[1] * inv), pack16<BF16>(acc[2] * inv, acc[3] * inv));
+            else
+              *dst = pack16<BF16>(acc[0] * inv, acc[1] * inv);
+            if (lane == 0 && p.lse)
+              p.lse[tok * p.q_heads + h] = total > 0.f ? (top + log2f(total)) * kLn2 : (total == 0.f ? -INFINITY : total);
+          }
+        }
+      }
+    }
+    if (joined) group_sync(3, 256);       // stream 1's output and sums have been read
+  }
+}
+
+template <int D, bool BF16> __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __grid_constant__ Params p) {
+  extern __shared__ char raw[];
+  Smem<D> sm;
+  sm.ptr = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+  sm.base = smem_addr(sm.ptr);
+  const int warp = threadIdx.x / 32;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Shape<D>::kStages; ++s) {
+      bar_init(sm.full(s), 1);
+      bar_init(sm.empty(s), 1);
+    }
+    bar_init(sm.q_full(), 1);
+    for (int t = 0; t < 2; ++t) {
+      bar_init(sm.s_full(t), 1);
+      bar_init(sm.p_ready(t), 4);
+      bar_init(sm.final(t), 1);
+    }
+    bar_init(sm.drain(), 1);
+    sm.words()[0] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(const_cast<int *>(sm.words() + 1))) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sm.words()[1];
+  const Guard g{sm.words(), p.status};
+  const int first = p.cta_first[blockIdx.x], last = p.cta_first[blockIdx.x + 1];
+  if (warp < kMmaWarp) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    softmax_role<D, BF16>(p, sm, g, first, last, tmem);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kMmaWarp)
+      mma_role<D, BF16>(p, sm, g, first, last, tmem);
+    else if (warp == kMmaWarp + 1)
+      load_role<D>(p, sm, g, first, last);
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// ---------------------------------------------------------------- host
+int fail(const char *fmt, long a = 0, long b = 0) {
+  char buf[256];
+  snprintf(buf, sizeof buf, fmt, a, b);
+  return emmy_internal_fail(EMMY_EINVAL, buf);
+}
+int cuda_fail(const char *what, cudaError_t e) {
+  char buf[256];
+  snprintf(buf, sizeof buf, "%s: %s", what, cudaGetErrorString(e));
+  return emmy_internal_fail(static_cast<int>(e), buf);
+}
+
+// A stride in bytes; that of an extent of 1 is never used, whatever it says.
+uint64_t step(int64_t stride, int64_t extent) { return extent == 1 ? 16 : static_cast<uint64_t>(stride) * 2; }
+bool bad_stride(int64_t stride, int64_t extent) { return extent != 1 && (stride <= 0 || stride % 8 || stride >= (int64_t(1) << 38)); }
+
+template <int D, bool BF16> int launch(const Params &p, int ctas, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};     // a bit for each device
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return cuda_fail("emmy_paged_attention: cudaGetDevice", e);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev > 63 || !(ready.load() & bit)) {
+    if (cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem))
+      return cuda_fail("emmy_paged_attention: shared memory", e);
+    // the softmax warps wait for the registers of the split: they must exist
+    cudaFuncAttributes attr;
+    if (cudaError_t e = cudaFuncGetAttributes(&attr, paged_attention_kernel<D, BF16>))
+      return cuda_fail("emmy_paged_attention: attributes", e);
+    if (attr.numRegs != kLaunchRegs) return fail("emmy_paged_attention: built with %ld registers, not %ld", attr.numRegs, kLaunchRegs);
+    if (dev <= 63) ready.fetch_or(bit);
+  }
+  paged_attention_kernel<D, BF16><<<ctas, kThreads, kSmem, s>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : cuda_fail("emmy_paged_attention: launch", e);
+}
+
+}  // namespace
+
+extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, void *stream) {
+  if (!plan || !a) return fail("emmy_paged_attention: bad argument");
+  if (a->dtype != 6 && a->dtype != 9) return fail("emmy_paged_attention: dtype %ld (f16 or bf16)", a->dtype);
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail("emmy_paged_attention: scale must be positive and finite");
+  if (plan->tokens == 0) return 0;
+  const int ps = a->page_size;
+  if (ps < 8 || (ps < kTile ? (ps & (ps - 1)) != 0 : ps % kTile != 0))
+    return fail("emmy_paged_attention: page_size %ld (8, 16, 32, 64 or a multiple of 128)", ps);
+  if (a->pages < 1) return fail("emmy_paged_attention: a cache of %ld pages", a->pages);
+  if (a->table_width < 0 || int64_t(a->table_width) * ps < plan->max_kv)
+    return fail("emmy_paged_attention: a table of %ld pages a sequence does not hold %ld tokens", a->table_width, plan->max_kv);
+  if (!a->q || !a->out || !a->k_cache || !a->v_cache || !a->table || !a->plan_words || (plan->part_rows && !a->scratch))
+    return fail("emmy_paged_attention: null address");
+  if ((a->q | a->out | a->k_cache | a->v_cache | a->plan_words | a->scratch) % 16 || (a->table | a->lse) % 4)
+    return fail("emmy_paged_attention: address not a multiple of 16 bytes");
+  const int group = plan->q_heads / plan->kv_heads, d = plan->head_dim;
+  const int64_t extent[3] = {a->pages, ps, plan->kv_heads};
+  for (int i = 0; i < 3; ++i)
+    if (bad_stride(a->k_cache_stride[i], extent[i]) || bad_stride(a->v_cache_stride[i], extent[i]))
+      return fail("emmy_paged_attention: cache stride %ld not a positive multiple of 8 elements", i);
+  const int64_t rows[2] = {plan->tokens, plan->q_heads};
+  for (int i = 0; i < 2; ++i)
+    if (bad_stride(a->q_stride[i], rows[i]) || bad_stride(a->out_stride[i], rows[i]))
+      return fail("emmy_paged_attention: q or out stride %ld not a positive multiple of 8 elements", i);
+  Params p;
+  memset(&p, 0, sizeof p);
+  const uint32_t box = ps < kTile ? ps : kTile;
+  const int per_tile = kTile / group;
+  const uint64_t q_dims[4] = {uint64_t(d), uint64_t(group), uint64_t(plan->kv_heads), uint64_t(plan->tokens)};
+  const uint64_t q_steps[3] = {step(a->q_stride[1], plan->q_heads), group * step(a->q_stride[1], plan->q_heads), step(a->q_stride[0], plan->tokens)};
+  const uint32_t q_box[4] = {64, uint32_t(group), 1, uint32_t(per_tile)};
+  if (int e = emmy_tensormap_encode(&p.q, a->dtype, 4, a->q, q_dims, q_steps, q_box, 3)) return e;
+  const uint64_t dims[4] = {uint64_t(d), uint64_t(ps), uint64_t(plan->kv_heads), uint64_t(a->pages)};
+  const uint32_t kv_box[4] = {64, box, 1, 1};
+  for (int i = 0; i < 2; ++i) {
+    const int64_t *st = i ? a->v_cache_stride : a->k_cache_stride;
+    const uint64_t steps[3] = {step(st[1], ps), step(st[2], plan->kv_heads), step(st[0], a->pages)};
+    if (int e = emmy_tensormap_encode(i ? &p.v : &p.k, a->dtype, 4, i ? a->v_cache : a->k_cache, dims, steps, kv_box, 3)) return e;
+  }
+  int *words = reinterpret_cast<int *>(a->plan_words);
+  p.status = reinterpret_cast<unsigned *>(words);
+  p.cta_first = words + 4;
+  p.counters = reinterpret_cast<unsigned *>(words + plan->at.counters);
+  p.units = reinterpret_cast<const Unit *>(words + plan->at.units);
+  p.table = reinterpret_cast<const int *>(a->table);
+  p.table_stride = a->table_stride;
+  p.part_o = reinterpret_cast<float *>(a->scratch);
+  p.part_ml = reinterpret_cast<float2 *>(p.part_o + plan->part_rows * d);
+  p.out = reinterpret_cast<void *>(a->out);
+  p.out_stride[0] = a->out_stride[0];
+  p.out_stride[1] = a->out_stride[1];
+  p.lse = reinterpret_cast<float *>(a->lse);
+  p.q_heads = plan->q_heads;
+  p.group = group;
+  p.per_tile = per_tile;
+  p.page_size = ps;
+  p.box = box;
+  p.causal = plan->causal;
+  p.window = plan->window;
+  p.scale_log2 = a->scale * kLog2e;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int n = plan->at.ctas;
+  if (d == 128) return a->dtype == 9 ? launch<128, true>(p, n, s) : launch<128, false>(p, n, s);
+  return a->dtype == 9 ? launch<64, true>(p, n, s) : launch<64, false>(p, n, s);
+}
+
+extern "C" EMMY_API int emmy_paged_plan_status(emmy_paged_plan_t plan, uint64_t plan_words, void *stream) {
+  if (!plan || !plan_words) return fail("emmy_paged_plan_status: bad argument");
+  int status = 0;
+  if (int e = emmy_memcpy_dtoh_async(&status, plan_words, sizeof status, stream)) return e;
+  if (int e = emmy_stream_sync(stream)) return e;
+  if (!status) return 0;
+  char buf[128];
+  snprintf(buf, sizeof buf, "emmy_paged_attention: a wait ran out (code %d)", status);
+  return emmy_internal_fail(EMMY_EKERNEL, buf);
+}

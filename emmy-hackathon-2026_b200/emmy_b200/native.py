@@ -19,6 +19,9 @@ REPO = ROOT.parent
 LIB_PATH = PKG / "libemmy_b200.so"
 SRC = ROOT / "csrc" / "emmy_runtime.cpp"
 NOALLOC_SRC = ROOT / "csrc" / "emmy_noalloc.cu"
+PLAN_SRC = ROOT / "csrc" / "emmy_paged_plan.cpp"
+PAGED_SRCS = [ROOT / "csrc" / "emmy_rotate_append.cu", ROOT / "csrc" / "emmy_paged_attention.cu"]
+PAGED_HEADER = ROOT / "csrc" / "emmy_paged.h"
 HEADER = REPO / "include" / "emmy_b200.h"
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 
@@ -31,6 +34,8 @@ EXPORTS = [
     "emmy_memcpy_htod_async", "emmy_memcpy_dtoh_async", "emmy_stream_sync", "emmy_mem_alloc",
     "emmy_mem_free", "emmy_ipc_handle", "emmy_ipc_open", "emmy_ipc_close",
     "emmy_time_launches", "emmy_run_host", "emmy_rmsnorm_noalloc",
+    "emmy_rotate_append", "emmy_paged_plan_make", "emmy_paged_plan_data", "emmy_paged_plan_free",
+    "emmy_paged_attention", "emmy_paged_plan_status",
 ]
 
 
@@ -41,31 +46,37 @@ class EmmyError(RuntimeError):
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the runtime library in-tree (host C++ only; the GPU code is the
-    PTX each IR compiles to)."""
-    deps = [SRC, NOALLOC_SRC, HEADER]
+    """Compile the runtime library in-tree: host C++, and by nvcc the entry
+    points that carry GPU code of their own (the GPU code of an IR is the PTX
+    it compiles to)."""
+    deps = [SRC, NOALLOC_SRC, HEADER, PLAN_SRC, *PAGED_SRCS, PAGED_HEADER]
     if LIB_PATH.exists() and not force and all(
             LIB_PATH.stat().st_mtime >= d.stat().st_mtime for d in deps):
         return LIB_PATH
     inc = CUDA_HOME / "include"
     ptxc = CUDA_HOME / "lib64" / "libnvptxcompiler_static.a"
     tmp = LIB_PATH.with_suffix(".so.tmp")
-    # the no-allocation entry point holds its scratch in a __device__ array:
-    # its one .cu file is compiled by nvcc for sm_100a, with the CUDA runtime
-    # linked statically
-    obj = LIB_PATH.with_suffix(".noalloc.o")
-    r = subprocess.run([str(CUDA_HOME / "bin" / "nvcc"), "-c", "-O2", "-std=c++17",
-                        "-gencode", "arch=compute_100a,code=sm_100a",
-                        "-Xcompiler", "-fPIC,-fvisibility=hidden", str(NOALLOC_SRC),
-                        "-o", str(obj)], capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"compiling {NOALLOC_SRC.name} failed:\n{r.stderr[-4000:]}")
+    # the no-allocation entry point holds its scratch in a __device__ array and
+    # the paged-cache operators are CUDA kernels: these .cu files are compiled
+    # by nvcc for sm_100a, with the CUDA runtime linked statically
+    objs = []
+    for cu in [NOALLOC_SRC, *PAGED_SRCS]:
+        objs.append(LIB_PATH.with_suffix(f".{cu.stem}.o"))
+        r = subprocess.run([str(CUDA_HOME / "bin" / "nvcc"), "-c", "-O3", "-std=c++17",
+                            "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
+                            "-Xptxas", "-v", "-Xcompiler", "-fPIC,-fvisibility=hidden", str(cu),
+                            "-o", str(objs[-1])], capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"compiling {cu.name} failed:\n{r.stderr[-4000:]}")
+        if verbose:
+            print(*(ln for ln in r.stderr.splitlines() if "spill" in ln or "Used" in ln), sep="\n")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wextra",
            "-fvisibility=hidden", "-Wl,--exclude-libs,ALL", "-s",
-           f"-I{inc}", str(SRC), str(obj), "-o", str(tmp), str(ptxc),
+           f"-I{inc}", str(SRC), str(PLAN_SRC), *map(str, objs), "-o", str(tmp), str(ptxc),
            f"-L{CUDA_HOME / 'lib64'}", "-lcudart_static", "-ldl", "-lpthread", "-lrt"]
     r = subprocess.run(cmd, capture_output=True, text=True)
-    obj.unlink(missing_ok=True)
+    for obj in objs:
+        obj.unlink(missing_ok=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {LIB_PATH.name} failed:\n{r.stderr[-4000:]}")
     if verbose and r.stderr:
@@ -139,6 +150,14 @@ def lib() -> ctypes.CDLL:
         L.emmy_rmsnorm_noalloc.argtypes = [ctypes.c_void_p, c_u32p, c_u32p, ctypes.c_void_p,
                                            c_u32p, c_u32p] + [ctypes.c_uint64] * 5 + [
                                            ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
+        L.emmy_rotate_append.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        L.emmy_paged_plan_make.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p)]
+        L.emmy_paged_plan_data.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p)] + [
+            ctypes.POINTER(ctypes.c_size_t)] * 2
+        L.emmy_paged_plan_free.argtypes = [ctypes.c_void_p]
+        L.emmy_paged_plan_free.restype = None
+        L.emmy_paged_attention.argtypes = [ctypes.c_void_p] * 3
+        L.emmy_paged_plan_status.argtypes = [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]
         _LIB = L
     return _LIB
 

@@ -1,0 +1,255 @@
+"""A paged key/value cache and the two operators of a serving step around it.
+
+* :func:`rotate_append` turns new queries and keys by their positions (rotary
+  positions of one or several axes) and writes keys and values to the cache;
+* :func:`attention` is the attention of a ragged chunk of new tokens, one token
+  a sequence (decoding) upwards, over that cache.
+
+A cache is two tensors, keys and values, of shape [pages, page_size, kv_heads,
+head_dim] with any strides of the outer dimensions, so ``[pages, kv_heads,
+page_size, head_dim]`` storage is passed as its ``transpose(1, 2)``.  Both
+operators run on the current stream of their tensors' device, or on the CUDA
+stream ``stream`` (its address), and return without waiting.  They are thin over
+the C ABI (``emmy_rotate_append``, ``emmy_paged_attention`` in
+``include/emmy_b200.h``) and raise :class:`~.native.EmmyError` with its message
+on arguments it refuses, ``ValueError`` on what only Python can see.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import native
+
+_DTYPES = {torch.float16: 6, torch.float32: 7, torch.bfloat16: 9}
+
+_i32, _i64, _u64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64
+
+
+class _RotateAppendArgs(ctypes.Structure):
+    _fields_ = ([(n, _i32) for n in ("dtype", "tokens", "q_heads", "kv_heads", "head_dim", "rotary_dim", "axes",
+                                     "interleaved", "pages", "page_size")]
+                + [(n, _u64) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "positions", "slots",
+                                       "frequencies", "pair_axis")]
+                + [("q_stride", _i64 * 2), ("k_stride", _i64 * 2), ("v_stride", _i64 * 2), ("q_out_stride", _i64 * 2),
+                   ("k_cache_stride", _i64 * 3), ("v_cache_stride", _i64 * 3), ("positions_stride", _i64)])
+
+
+class _PlanArgs(ctypes.Structure):
+    _fields_ = [("sequences", _i32), ("q_lens", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p),
+                ("q_heads", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("causal", _i32), ("window", _i32),
+                ("ctas", _i32)]
+
+
+class _AttentionArgs(ctypes.Structure):
+    _fields_ = ([(n, _i32) for n in ("dtype", "pages", "page_size", "table_width")] + [("scale", ctypes.c_float)]
+                + [(n, _u64) for n in ("q", "out", "lse", "k_cache", "v_cache", "table", "plan_words", "scratch")]
+                + [("q_stride", _i64 * 2), ("out_stride", _i64 * 2), ("k_cache_stride", _i64 * 3),
+                   ("v_cache_stride", _i64 * 3), ("table_stride", _i64)])
+
+
+def _need(ok, text):
+    if not ok:
+        raise ValueError(text)
+
+
+def _check(name, t, ndim, dtype, device, rows=True):
+    """A tensor of the cache operators: on the GPU, its innermost stride 1."""
+    _need(isinstance(t, torch.Tensor) and t.dim() == ndim, f"{name}: a tensor of {ndim} dimensions is wanted")
+    _need(t.dtype == dtype, f"{name}: {dtype} is wanted, not {t.dtype}")
+    _need(t.device == device, f"{name}: on {t.device}, not on {device}")
+    _need(not rows or t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: the innermost stride must be 1")
+
+
+def _cuda_device(name, t):
+    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name}: a CUDA tensor is wanted")
+    return t.device
+
+
+def _cache(k_cache, v_cache, dtype, device):
+    _check("k_cache", k_cache, 4, dtype, device)
+    _check("v_cache", v_cache, 4, dtype, device)
+    _need(k_cache.shape == v_cache.shape, "k_cache and v_cache have different shapes")
+
+
+def _call(fn, device, stream, *args):
+    """One C-ABI call with ``device`` current, on its current stream unless one is given."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(fn, device, stream, *args)
+    if stream is None:
+        stream = torch.cuda.current_stream(device).cuda_stream
+    native.check(fn(*args, ctypes.c_void_p(stream)))
+
+
+class Rotation:
+    """Rotary positions: ``frequencies`` (float32, on the GPU) has the radians
+    per position of each pair, so its length is half of the components that
+    turn, the leading ones of a head.  ``axes[i]`` (host integers; default 0) is
+    the row of ``positions`` that turns pair i: a video token has time, height
+    and width.  Pair i is components (2i, 2i+1) when ``interleaved``, otherwise
+    (i, i + len(frequencies))."""
+
+    def __init__(self, frequencies, axes=None, interleaved=False):
+        device = _cuda_device("frequencies", frequencies)
+        _check("frequencies", frequencies, 1, torch.float32, device)
+        self.frequencies = frequencies.contiguous()
+        self.interleaved = bool(interleaved)
+        self.axes = 1
+        self.pair_axis = None
+        if axes is not None:
+            axes = [int(x) for x in axes]
+            _need(len(axes) == len(frequencies), f"axes: {len(frequencies)} pairs, {len(axes)} entries")
+            _need(all(0 <= x < 16 for x in axes), "axes: entries must be 0..15")
+            if any(axes):
+                self.axes = max(axes) + 1
+                self.pair_axis = torch.tensor(axes, dtype=torch.int32, device=device)
+
+
+def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=None, stream=None):
+    """Rotated queries; rotated keys, and values, written to the cache in place.
+
+    ``q`` [tokens, q_heads, dim], ``k`` and ``v`` [tokens, kv_heads, dim] (views
+    of a joint projection are fine), all of one type with the cache: bfloat16,
+    float16 or float32.  ``positions`` int32 [tokens], or [axes, tokens] for a
+    rotation of several axes.  ``slots`` int32 [tokens]: token ``s % page_size``
+    of page ``s // page_size``; a slot outside the cache (-1, say) stores
+    nothing.  ``q_out`` may be ``q`` itself.  Rotates in 32 bits, with angles
+    formed in 64, and rounds once."""
+    device = _cuda_device("q", q)
+    dtype = q.dtype
+    _need(dtype in _DTYPES, f"q: bfloat16, float16 or float32 is wanted, not {dtype}")
+    _check("q", q, 3, dtype, device)
+    _check("k", k, 3, dtype, device)
+    _check("v", v, 3, dtype, device)
+    _cache(k_cache, v_cache, dtype, device)
+    tokens, q_heads, dim = q.shape
+    pages, page_size, kv_heads, _ = k_cache.shape
+    _need(k.shape == (tokens, kv_heads, dim) and v.shape == k.shape and k_cache.shape[3] == dim,
+          "q, k, v and the caches do not fit together")
+    if positions.dim() == 1:
+        positions = positions[None]
+    _check("positions", positions, 2, torch.int32, device)
+    _need(positions.shape[1] == tokens and positions.shape[0] >= rotation.axes,
+          f"positions: [{rotation.axes}, {tokens}] is wanted, not {list(positions.shape)}")
+    _check("slots", slots, 1, torch.int32, device)
+    _need(slots.shape[0] == tokens, f"slots: {tokens} are wanted, not {slots.shape[0]}")
+    _need(rotation.frequencies.device == device, "rotation: on another device")
+    if q_out is None:
+        q_out = torch.empty((tokens, q_heads, dim), dtype=dtype, device=device)
+    else:
+        _check("q_out", q_out, 3, dtype, device)
+        _need(q_out.shape == q.shape, "q_out: another shape than q")
+    pair_axis = rotation.pair_axis
+    a = _RotateAppendArgs(
+        _DTYPES[dtype], tokens, q_heads, kv_heads, dim, 2 * rotation.frequencies.shape[0], positions.shape[0],
+        rotation.interleaved, pages, page_size, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+        rotation.frequencies.data_ptr(), 0 if pair_axis is None else pair_axis.data_ptr(),
+        q.stride()[:2], k.stride()[:2], v.stride()[:2], q_out.stride()[:2], k_cache.stride()[:3],
+        v_cache.stride()[:3], positions.stride(0))
+    _call(native.lib().emmy_rotate_append, device, stream, ctypes.byref(a))
+    return q_out
+
+
+class AttentionPlan:
+    """How the attention of one batch is cut into units of work: made once from
+    the host's lengths, used by every layer's call.
+
+    Sequence s brings ``q_lens[s]`` new tokens to a cache that then holds
+    ``kv_lens[s]`` of its tokens, the new ones last.  ``causal`` tokens see
+    their own position and those before it, with a ``window`` only the last
+    ``window`` of them; otherwise every token sees all ``kv_lens[s]``.
+    ``q_heads`` is ``kv_heads`` times at most 128; ``head_dim`` is 64 or 128.
+    ``ctas``: over how many CTAs the work is spread, one for each SM by default.
+
+    A plan holds device memory (``words``, ``scratch``) that its calls write:
+    they must not overlap on the GPU, so calls on several streams need a plan
+    each."""
+
+    def __init__(self, q_lens, kv_lens, q_heads, kv_heads, head_dim, causal=True, window=None, device=None,
+                 ctas=None):
+        self._h = None
+        q_lens, kv_lens = [int(x) for x in q_lens], [int(x) for x in kv_lens]
+        _need(len(q_lens) == len(kv_lens), "q_lens and kv_lens have different lengths")
+        _need(all(0 <= x <= 1 << 30 for x in q_lens + kv_lens), "lengths must be 0..2^30")
+        _need(window is None or window >= 1, "window: at least 1, or None")
+        device = torch.device("cuda" if device is None else device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        if ctas is None:
+            ctas = torch.cuda.get_device_properties(device).multi_processor_count
+        n = len(q_lens)
+        a = _PlanArgs(n, None, None, q_heads, kv_heads, head_dim, bool(causal), window or 0, ctas)
+        lens = (_i32 * (2 * n))(*q_lens, *kv_lens)
+        a.q_lens, a.kv_lens = ctypes.addressof(lens), ctypes.addressof(lens) + 4 * n
+        L = native.lib()
+        h = ctypes.c_void_p()
+        native.check(L.emmy_paged_plan_make(ctypes.byref(a), ctypes.byref(h)))
+        self._h = h
+        words, count, scratch = ctypes.c_void_p(), ctypes.c_size_t(), ctypes.c_size_t()
+        native.check(L.emmy_paged_plan_data(h, ctypes.byref(words), ctypes.byref(count), ctypes.byref(scratch)))
+        host = torch.frombuffer((_i32 * count.value).from_address(words.value), dtype=torch.int32)
+        self.words = host.to(device, copy=True)
+        self.scratch = torch.empty(scratch.value, dtype=torch.uint8, device=device)
+        self.device, self.tokens, self.sequences = device, sum(q_lens), n
+        self.q_heads, self.kv_heads, self.head_dim = int(q_heads), int(kv_heads), int(head_dim)
+
+    def __del__(self):
+        if self._h is not None:
+            try:
+                native.lib().emmy_paged_plan_free(self._h)
+            except Exception:
+                pass
+
+    def check(self, stream=None):
+        """Waits for the calls so far and raises if one of them gave up."""
+        _call(native.lib().emmy_paged_plan_status, self.device, stream, self._h, self.words.data_ptr())
+
+
+def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, stream=None):
+    """``(out, lse)``: softmax(scale q k^T) v of every new token over the keys
+    that it sees, and the natural logarithm of the softmax's sum (float32
+    [tokens, q_heads]; what joins attention over several parts of a cache).
+
+    ``q`` [tokens, q_heads, head_dim], the sequences' tokens in order;
+    bfloat16 or float16 like the cache.  ``table`` int32 [sequences, pages]:
+    the pages of each sequence in order (entries after its last page are not
+    read; a page outside the cache reads as zeros).  page_size is 8, 16, 32, 64
+    or a multiple of 128.  ``scale`` defaults to 1/sqrt(head_dim).  A token
+    that sees no key gets 0, and -inf.  What lies in the cache beyond a
+    sequence's length is never used, whatever it holds; of the keys and values
+    that count, those that some tokens of a chunk see and others do not must be
+    finite."""
+    device = _cuda_device("q", q)
+    dtype = q.dtype
+    _need(dtype in (torch.bfloat16, torch.float16), f"q: bfloat16 or float16 is wanted, not {dtype}")
+    _check("q", q, 3, dtype, device)
+    _need(device == plan.device, f"q: on {device}, the plan on {plan.device}")
+    shape = (plan.tokens, plan.q_heads, plan.head_dim)
+    _need(q.shape == shape, f"q: the plan is for {list(shape)}, not {list(q.shape)}")
+    _cache(k_cache, v_cache, dtype, device)
+    pages, page_size, kv_heads, dim = k_cache.shape
+    _need((kv_heads, dim) == (plan.kv_heads, plan.head_dim),
+          f"k_cache: the plan is for {plan.kv_heads} heads of {plan.head_dim}, not {kv_heads} of {dim}")
+    _check("table", table, 2, torch.int32, device)
+    _need(table.shape[0] == plan.sequences, f"table: {plan.sequences} rows are wanted, not {table.shape[0]}")
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=device)
+    else:
+        _check("out", out, 3, dtype, device)
+        _need(out.shape == shape, "out: another shape than q")
+    if lse is None:
+        lse = torch.empty(shape[:2], dtype=torch.float32, device=device)
+    else:
+        _check("lse", lse, 2, torch.float32, device)
+        _need(lse.shape == shape[:2] and lse.is_contiguous(), f"lse: contiguous {list(shape[:2])} is wanted")
+    a = _AttentionArgs(
+        _DTYPES[dtype], pages, page_size, table.shape[1], 1 / math.sqrt(plan.head_dim) if scale is None else scale,
+        q.data_ptr(), out.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
+        plan.words.data_ptr(), plan.scratch.data_ptr(), q.stride()[:2], out.stride()[:2], k_cache.stride()[:3],
+        v_cache.stride()[:3], table.stride(0))
+    _call(native.lib().emmy_paged_attention, device, stream, plan._h, ctypes.byref(a))
+    return out, lse

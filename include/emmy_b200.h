@@ -201,6 +201,92 @@ EMMY_API int emmy_rmsnorm_noalloc(emmy_kernel_t meansq, const uint32_t grid1[3],
                                   uint64_t mean_count, uint64_t add_c1, uint64_t x, uint64_t w,
                                   uint64_t y, int rows, int cols, void *stream);
 
+/* ------------------------------------------------------------------------ */
+/* Serving: a paged key/value cache and the two operators around it.  No     */
+/* counterpart in the reference.                                             */
+/*                                                                          */
+/* A cache is two tensors (keys and values) of pages x page_size x kv_heads  */
+/* x head_dim elements; strides are in elements, in that order, so both the  */
+/* [page][token][head] and the [page][head][token] layout fit; the innermost */
+/* stride is 1.  Slot s is token s % page_size of page s / page_size.        */
+/* dtype uses the tensor-map numbering: 6=f16 7=f32 9=bf16.                  */
+/* ------------------------------------------------------------------------ */
+typedef struct {
+  int32_t dtype;         /* of q, k, v, q_out and both caches: 6, 7 or 9        */
+  int32_t tokens;        /* may be 0: nothing is launched                       */
+  int32_t q_heads;       /* may be 0: no queries                                */
+  int32_t kv_heads;      /* may be 0: no keys or values                         */
+  int32_t head_dim;      /* 1..1024                                             */
+  int32_t rotary_dim;    /* leading components that turn: even, 0..head_dim     */
+  int32_t axes;          /* position axes, 1..16                                */
+  int32_t interleaved;   /* pairs are (2i, 2i+1), else (i, i + rotary_dim/2)    */
+  int32_t pages, page_size;
+  uint64_t q, k, v;      /* [tokens][heads][head_dim]                           */
+  uint64_t q_out;        /* rotated queries; may be q itself                    */
+  uint64_t k_cache, v_cache;
+  uint64_t positions;    /* int32 [axes][tokens]                                */
+  uint64_t slots;        /* int32 [tokens]; outside the cache: token not stored */
+  uint64_t frequencies;  /* f32 [rotary_dim/2], radians per position            */
+  uint64_t pair_axis;    /* int32 [rotary_dim/2], or 0: every pair on axis 0    */
+  int64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2]; /* token, head */
+  int64_t k_cache_stride[3], v_cache_stride[3];  /* page, token of a page, head */
+  int64_t positions_stride;                      /* of an axis                  */
+} emmy_rotate_append_args;
+
+/* Turns every pair of the leading rotary_dim components of q and k by          */
+/* position x frequency, writes the queries to q_out and the keys and values    */
+/* to the cache slots of their tokens.  Two tokens with one slot: either stays. */
+EMMY_API int emmy_rotate_append(const emmy_rotate_append_args *a, void *stream);
+
+typedef struct emmy_paged_plan_s *emmy_paged_plan_t;
+
+typedef struct {
+  int32_t sequences;        /* may be 0                                          */
+  const int32_t *q_lens;    /* host: new tokens of each sequence, >= 0           */
+  const int32_t *kv_lens;   /* host: cached tokens of each, the new ones included */
+  int32_t q_heads, kv_heads;/* q_heads = G * kv_heads, G <= 128                  */
+  int32_t head_dim;         /* 64 or 128                                         */
+  int32_t causal;           /* a token sees its own position and those before it */
+  int32_t window;           /* the last `window` positions only (0: all; causal) */
+  int32_t ctas;             /* CTAs to spread the work over (SMs of the device)  */
+} emmy_paged_plan_args;
+
+/* How the work of one set of lengths is cut into units and dealt to the CTAs, */
+/* made on the host and used by every layer's call.  The plan's words (32-bit) */
+/* go to device memory as they are (16-byte aligned); beside them the caller    */
+/* keeps `scratch` bytes of device memory, not initialised, 16-byte aligned.    */
+/* Calls that share the device words must not overlap on the GPU.               */
+EMMY_API int emmy_paged_plan_make(const emmy_paged_plan_args *a, emmy_paged_plan_t *out);
+EMMY_API int emmy_paged_plan_data(emmy_paged_plan_t plan, const int32_t **words, size_t *n_words,
+                                  size_t *scratch);
+EMMY_API void emmy_paged_plan_free(emmy_paged_plan_t plan);
+
+typedef struct {
+  int32_t dtype;            /* of q, out and both caches: 6 or 9                 */
+  int32_t pages, page_size; /* page_size: 8, 16, 32, 64 or a multiple of 128     */
+  int32_t table_width;      /* pages a row of the table holds                    */
+  float scale;              /* of the scores, > 0                                */
+  uint64_t q, out;          /* [tokens][q_heads][head_dim], sequences in order   */
+  uint64_t lse;             /* f32 [tokens][q_heads], dense, or 0                */
+  uint64_t k_cache, v_cache;
+  uint64_t table;           /* int32 [sequences][table_width]: pages in order    */
+  uint64_t plan_words;      /* the plan's words on the device                    */
+  uint64_t scratch;
+  int64_t q_stride[2], out_stride[2];           /* token, head                   */
+  int64_t k_cache_stride[3], v_cache_stride[3]; /* page, token of a page, head   */
+  int64_t table_stride;
+} emmy_paged_attention_args;
+
+/* out = softmax(scale q k^T) v of each new token over the cached tokens that it */
+/* sees, lse the natural logarithm of the sum; a token that sees none gets 0 and */
+/* -inf.  A page number outside the cache reads as zeros.  q and the caches need */
+/* 16-byte aligned addresses and strides.                                       */
+EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_paged_attention_args *a,
+                                  void *stream);
+/* Reads the plan's status word (waits for `stream`): EMMY_EKERNEL when a call   */
+/* that used these device words gave up on a wait, and its outputs are void.     */
+EMMY_API int emmy_paged_plan_status(emmy_paged_plan_t plan, uint64_t plan_words, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
