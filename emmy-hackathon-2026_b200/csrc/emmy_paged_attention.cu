@@ -9,9 +9,9 @@
 //
 // One persistent CTA an SM walks its list of units (emmy_paged.h).  Its roles:
 //   warps 0-3, 4-7  softmax of stream 0 and 1, one thread a row;
-//   warp 8          issues the tensor-core products and loads the query tiles;
+//   warps 10, 11    issue the tensor-core products of stream 0 and 1;
 //   warp 9          loads key and value tiles, page by page, into one ring;
-//   warps 10-11     fill the warpgroup that gives registers to the softmax.
+//   warp 8          loads the query tiles.
 // A unit with two query tiles gives one to each stream and both see every key
 // tile; a unit with one query tile (decode) gives it to both streams, which
 // take the key tiles in turn and are joined at the end.  Either way one
@@ -50,7 +50,7 @@ constexpr int kThreads = 384;
 // row of scores, and of the others; the shares add up to what was launched
 constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
-constexpr int kMmaWarp = 8;             // the next warp loads
+constexpr int kSoftmaxWarps = 8, kLoadWarp = 9, kMmaWarp = 10;
 constexpr int kSmem = 227 * 1024;
 constexpr float kNoMax = -1e30f;        // exponent base of a row that has seen no key
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -66,7 +66,7 @@ struct alignas(64) Params {
   void *out;
   float *lse;
   int64_t table_stride, out_stride[2];
-  int q_heads, group, per_tile, page_size, box, causal, window;
+  int q_heads, group, per_tile, page_size, box, causal, window, aligned32;
   float scale_log2;
 };
 
@@ -75,7 +75,7 @@ template <int D> struct Shape {
   static constexpr int kStages = D == 128 ? 5 : 12;      // key and value tiles in flight
   static constexpr int kRing = 2 * kTileBytes;           // after two query tiles
   static constexpr int kBars = kRing + kStages * kTileBytes;
-  static constexpr int kEnd = kBars + (2 * kStages + 8) * 8 + 32 + kTile * 8;
+  static constexpr int kWords = kBars + (2 * kStages + 14) * 8, kEnd = kWords + 32 + kTile * 8;
   static_assert(kEnd + 1024 <= kSmem, "shared memory");
 };
 
@@ -112,17 +112,19 @@ __device__ __forceinline__ uint64_t now_ns() {
 // What a role needs to give up: the CTA's flag (any role may set it) and the
 // plan's status word.
 struct Guard {
-  volatile int *dead;
-  unsigned *status;
+  uint32_t dead;          // shared-memory address
+  const Params &p;
   // false once a wait of this CTA ran out (2 s); the caller then issues nothing more
   __device__ __forceinline__ bool slow(uint32_t bar, uint32_t parity, int code) const {
     const uint64_t t0 = now_ns();
     for (;;) {
       if (bar_try(bar, parity)) return true;
-      if (*dead) return false;
+      int gave_up;
+      asm volatile("ld.volatile.shared.b32 %0, [%1];" : "=r"(gave_up) : "r"(dead) : "memory");
+      if (gave_up) return false;
       if (now_ns() - t0 > 2000000000ull) {
-        *dead = 1;
-        atomicExch(status, code);
+        asm volatile("st.volatile.shared.b32 [%0], 1;" ::"r"(dead) : "memory");
+        atomicExch(p.status, code);
         return false;
       }
     }
@@ -139,6 +141,14 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, u
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
       "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
+}
+// true for one lane of a converged warp.  Compared with `lane == 0` the compiler
+// knows that one lane at most is active, and passes a tensor instruction's
+// operands without a loop over the lanes.
+__device__ __forceinline__ bool elected() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes;
 }
 __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -188,10 +198,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t *r) {
 }
 // the registers of a load are valid only after this: they pass through it so
 // that no use of them can move above it
-template <int N> __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[N]) {
+template <int N> __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[N], int from = 0, int to = N) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+  for (int i = from; i < to; ++i) asm volatile("" : "+r"(r[i]));
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -199,6 +209,11 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float max3(uint32_t x, uint32_t y, uint32_t z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(__uint_as_float(x)), "f"(__uint_as_float(y)), "f"(__uint_as_float(z)));
+  return r;
 }
 __device__ __forceinline__ uint64_t pair(float x, float y) {
   uint64_t r;
@@ -238,9 +253,9 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack16(float lo, float 
 // of one key a row, the next 64 columns 16 KiB further).
 constexpr uint32_t kOperandHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t operand(uint32_t addr, uint32_t lead) {
-  uint32_t low = ((addr >> 4) & 0x3fff) | ((lead >> 4) << 16);
-  asm volatile("" : "+r"(low));      // the steps along it are added where used, not kept
-  return low;
+  // a reduction's result is known to be the same in every lane, so that it and
+  // the steps along it stay in uniform registers, which the products read
+  return __reduce_or_sync(~0u, ((addr >> 4) & 0x3fff) | ((lead >> 4) << 16));
 }
 template <bool BF16> __host__ __device__ constexpr uint32_t instruction(int n, bool b_mn_major) {
   return (1u << 4) | (uint32_t(BF16) << 7) | (uint32_t(BF16) << 10) | (uint32_t(b_mn_major) << 16) | (uint32_t(n >> 3) << 17) |
@@ -250,19 +265,22 @@ template <bool BF16> __host__ __device__ constexpr uint32_t instruction(int n, b
 // ---------------------------------------------------------------- roles
 template <int D> struct Smem {
   uint32_t base;       // 1024-byte aligned
-  char *ptr;           // the same, generic
   __device__ uint32_t query(int t) const { return base + t * Shape<D>::kTileBytes; }
   __device__ uint32_t stage(int s) const { return base + Shape<D>::kRing + s * Shape<D>::kTileBytes; }
   __device__ uint32_t bar(int i) const { return base + Shape<D>::kBars + 8 * i; }
   __device__ uint32_t full(int s) const { return bar(s); }
   __device__ uint32_t empty(int s) const { return bar(Shape<D>::kStages + s); }
   __device__ uint32_t q_full() const { return bar(2 * Shape<D>::kStages); }
-  __device__ uint32_t s_full(int t) const { return bar(2 * Shape<D>::kStages + 1 + t); }
-  __device__ uint32_t p_ready(int t) const { return bar(2 * Shape<D>::kStages + 3 + t); }
-  __device__ uint32_t final(int t) const { return bar(2 * Shape<D>::kStages + 5 + t); }
-  __device__ uint32_t drain() const { return bar(2 * Shape<D>::kStages + 7); }
-  __device__ volatile int *words() const { return reinterpret_cast<volatile int *>(ptr + Shape<D>::kBars + (2 * Shape<D>::kStages + 8) * 8); }
-  __device__ float2 *ml() const { return reinterpret_cast<float2 *>(ptr + Shape<D>::kBars + (2 * Shape<D>::kStages + 8) * 8 + 32); }
+  __device__ uint32_t q_empty() const { return bar(2 * Shape<D>::kStages + 1); }
+  __device__ uint32_t s_full(int t) const { return bar(2 * Shape<D>::kStages + 2 + t); }
+  // the weights of a tile's first and last 64 keys
+  __device__ uint32_t p_ready(int t, int half) const { return bar(2 * Shape<D>::kStages + 4 + 2 * t + half); }
+  __device__ uint32_t final(int t) const { return bar(2 * Shape<D>::kStages + 8 + t); }
+  __device__ uint32_t drain(int t) const { return bar(2 * Shape<D>::kStages + 10 + t); }
+  // wide units: stream t may issue
+  __device__ uint32_t turn(int t) const { return bar(2 * Shape<D>::kStages + 12 + t); }
+  __device__ volatile int *words() const { return static_cast<volatile int *>(__cvta_shared_to_generic(base + Shape<D>::kWords)); }
+  __device__ float2 *ml() const { return static_cast<float2 *>(__cvta_shared_to_generic(base + Shape<D>::kWords + 32)); }
 };
 // words(): 0 dead, 1 tensor memory address, 2 + t "last to arrive" of stream t
 
@@ -301,6 +319,7 @@ template <int D> __device__ void load_role(const Params &p, const Smem<D> &sm, c
   for (int i = first; i < last && alive; ++i) {
     const Unit u = read_unit(p, i);
     if (!u.ntiles) continue;
+    if (i + 1 < last) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.units + i + 1));
     const int ahead = u.wide ? 1 : 2;
     const int *row = p.table + u.seq * p.table_stride;
     auto page_of = [&](int tile) {           // the page of this lane's box; -1: no box
@@ -353,40 +372,78 @@ template <int D> __device__ void load_role(const Params &p, const Smem<D> &sm, c
   }
 }
 
-template <int D, bool BF16> __device__ void mma_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last, uint32_t tmem) {
+// Query tiles: one 128-row tile for a stream of a wide unit, one for both of a
+// narrow one, each a box of group x tokens_per_tile rows.
+template <int D> __device__ void query_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last) {
+  const int bytes = p.group * p.per_tile * 128 * (D / 64);
+  uint32_t phase = 0;
+  for (int i = first; i < last; ++i) {
+    const Unit u = read_unit(p, i);
+    if (!u.ntiles) continue;
+    if (!g.wait(sm.q_empty(), phase ^ 1, 5)) break;
+    phase ^= 1;
+    const int tiles = u.wide ? 2 : 1;
+    if (elected()) {
+      bar_expect(sm.q_full(), tiles * bytes);
+      for (int t = 0; t < tiles; ++t)
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+          load_box(sm.query(t) + h * (kTile * 128), &p.q, sm.q_full(), 64 * h, 0, u.kvh, u.tok0 + t * p.per_tile);
+    }
+    __syncwarp();
+  }
+  // the last load lands before the CTA ends, also when its users gave up
+  const uint64_t t0 = now_ns();
+  while (!bar_try(sm.q_full(), phase ^ 1) && now_ns() - t0 < 100000000ull) {
+  }
+}
+
+// The products of stream t.  In a wide unit the streams issue in turn, so that
+// one's products run while the other's softmax does; left alone they fall into
+// step and wait for the exponentials and for the tensor cores together.  Both streams' warps walk the whole ring: a stage is
+// free when both have arrived, the one that uses it by the completion of its
+// products, the other at once.
+template <int D, bool BF16> __device__ void mma_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last, uint32_t tmem, int t) {
   const int lane = threadIdx.x % 32;
   constexpr uint32_t kQk = instruction<BF16>(kTile, false), kPv = instruction<BF16>(D, true);
+  const uint32_t s_at = tmem + kTile * t, o_at = tmem + 2 * kTile + kTile * t;
   Ring<D> ring;
-  uint32_t q_phase = 0, p_phase[2] = {0, 0};
-  bool alive = true, q_pending = false;
-  uint32_t q_awaited = 0;
-  const int rows_bytes = p.group * p.per_tile * 128;
+  uint32_t q_phase = 0, p_phase = 0, turn_phase = t ^ 1;
+  bool alive = true;
   auto wait = [&](uint32_t bar, uint32_t parity) { alive = alive && g.wait(bar, parity, 2); };
-  auto issue_qk = [&](int t, int q, int stage) {      // S_t = Q_q K^T
-    if (lane == 0 && alive) {
-      const uint32_t a = operand(sm.query(q), 16), b = operand(sm.stage(stage), 16);
+  auto issue_qk = [&](uint32_t a, uint32_t b, int stage) {   // S_t = Q K^T
+    if (alive && elected()) {
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         const int off = (k % 4) * 2 + (k / 4) * (kTile * 128 / 16);
-        mma_ss(tmem + kTile * t, a + off, b + off, kOperandHigh, kQk, k > 0);
+        mma_ss(s_at, a + off, b + off, kOperandHigh, kQk, k > 0);
       }
       commit(sm.s_full(t));
+      commit(sm.empty(stage));
     }
   };
-  auto issue_pv = [&](int t, int stage, bool acc) {   // O_t (+)= P_t V
-    if (lane == 0 && alive) {
-      const uint32_t b = operand(sm.stage(stage), kTile * 128);
+  auto issue_pv = [&](uint32_t b, int half, bool acc) {      // O_t (+)= P_t V over 64 keys
+    if (alive && elected()) {
 #pragma unroll
-      for (int k = 0; k < kTile / 16; ++k)
-        mma_ts(tmem + 2 * kTile + kTile * t, tmem + kTile * t + 8 * k, b + k * (16 * 128 / 16), kOperandHigh, kPv, acc || k > 0);
+      for (int k = 4 * half; k < 4 * half + 4; ++k)
+        mma_ts(o_at, s_at + 8 * k, b + k * (16 * 128 / 16), kOperandHigh, kPv, acc || k > 0);
     }
   };
-  auto release = [&](int stage) {
-    if (lane == 0 && alive) commit(sm.empty(stage));
+  auto take_turn = [&](bool wide) {
+    if (!wide) return;
+    wait(sm.turn(t), turn_phase);
+    turn_phase ^= 1;
+  };
+  auto give_turn = [&](bool wide) {
+    if (wide && alive && elected()) bar_arrive(sm.turn(t ^ 1));
+  };
+  auto pass_by = [&](int stage) {
+    if (alive && lane == 0) bar_arrive(sm.empty(stage));
   };
   auto clear_values = [&](const Unit &u, int tile, int stage) {
     // values of keys that no token of the item sees are unwritten or another's:
-    // their weight is 0, but 0 times an infinity is not
+    // their weight is 0, but 0 times an infinity is not.  Both warps of a wide
+    // unit do it, each before its own products.
     const int key0 = (u.tile0 + tile) * kTile;
     const int above = min(kTile, max(0, u.hi - key0)), below = min(kTile, max(0, u.lo - key0));
     if (above == kTile && below == 0) return;
@@ -404,73 +461,132 @@ template <int D, bool BF16> __device__ void mma_role(const Params &p, const Smem
   for (int i = first; i < last; ++i) {
     const Unit u = read_unit(p, i);
     if (!u.ntiles) continue;
-    if (alive) {
-      // every product that read the last unit's queries has completed: the
-      // softmax warps have since used its scores
-      if (lane == 0) {
-        bar_expect(sm.q_full(), (u.wide ? 2 : 1) * (D / 64) * rows_bytes);
-        for (int t = 0; t < (u.wide ? 2 : 1); ++t)
-          for (int h = 0; h < D / 64; ++h)
-            load_box(sm.query(t) + h * (kTile * 128), &p.q, sm.q_full(), 64 * h, 0, u.kvh, u.tok0 + t * p.per_tile);
-      }
-      q_pending = true;
-      q_awaited = q_phase;
-      __syncwarp();
-    }
-    wait(sm.q_full(), q_phase);
-    if (alive) q_pending = false;
-    q_phase ^= 1;
     const int ahead = u.wide ? 1 : 2;
+    const uint32_t q_op = operand(sm.query(u.wide ? t : 0), 16);
+    wait(sm.q_full(), q_phase);
+    q_phase ^= 1;
+    auto done_with_queries = [&](bool products) {
+      if (alive && elected()) {
+        if (products)
+          commit(sm.q_empty());
+        else
+          bar_arrive(sm.q_empty());
+      }
+    };
     for (int n = 0; n < min(ahead, u.ntiles); ++n) {
       wait(sm.full(ring.stage), ring.phase);
-      fence_after();
-      if (u.wide) {
-        issue_qk(0, 0, ring.stage);
-        issue_qk(1, 1, ring.stage);
+      if (u.wide || n == t) {
+        take_turn(u.wide);
+        fence_after();
+        issue_qk(q_op, operand(sm.stage(ring.stage), 16), ring.stage);
+        give_turn(u.wide);
+        if (n + ahead >= u.ntiles) done_with_queries(true);
       } else {
-        issue_qk(n, 0, ring.stage);
+        pass_by(ring.stage);
       }
-      release(ring.stage);
       ring.next();
     }
+    if (!u.wide && t >= u.ntiles) done_with_queries(false);
     for (int n = 0; n < u.ntiles; ++n) {
+      const bool mine = u.wide || n % 2 == t, more = n + ahead < u.ntiles;
       const int v_stage = ring.stage;
       wait(sm.full(v_stage), ring.phase);
       ring.next();
-      if (alive) clear_values(u, n, v_stage);
-      const bool more = n + ahead < u.ntiles;
       const int k_stage = ring.stage;
-      if (more) {
-        wait(sm.full(k_stage), ring.phase);
-        ring.next();
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (!u.wide && t != n % 2) continue;
-        wait(sm.p_ready(t), p_phase[t]);
-        p_phase[t] ^= 1;
+      if (mine) {
+        if (alive) clear_values(u, n, v_stage);
+        if (more) {
+          wait(sm.full(k_stage), ring.phase);
+          ring.next();
+        }
+        const uint32_t v_op = operand(sm.stage(v_stage), kTile * 128), k_op = operand(sm.stage(k_stage), 16);
+        take_turn(u.wide);
+        wait(sm.p_ready(t, 0), p_phase);
         fence_after();
-        issue_pv(t, v_stage, n >= ahead);
-        if (more)
-          issue_qk(t, u.wide ? t : 0, k_stage);
-        else if (lane == 0 && alive)
-          commit(sm.final(t));
+        issue_pv(v_op, 0, n >= ahead);
+        wait(sm.p_ready(t, 1), p_phase);
+        p_phase ^= 1;
+        fence_after();
+        issue_pv(v_op, 1, true);
+        if (more) issue_qk(q_op, k_op, k_stage);
+        give_turn(u.wide);
+        if (more) {
+          if (n + 2 * ahead >= u.ntiles) done_with_queries(true);
+        }
+        if (alive && elected()) {
+          if (!more) commit(sm.final(t));
+          commit(sm.empty(v_stage));
+        }
+      } else {
+        pass_by(v_stage);
+        if (more) {
+          wait(sm.full(k_stage), ring.phase);
+          ring.next();
+          pass_by(k_stage);
+        }
       }
-      release(v_stage);
-      if (more) release(k_stage);
     }
   }
   // nothing of this thread's is in flight when the CTA gives up its memory
-  if (lane == 0) commit(sm.drain());
+  if (elected()) commit(sm.drain(t));
   const uint64_t t0 = now_ns();
-  while (!bar_try(sm.drain(), 0) && now_ns() - t0 < 100000000ull) {
-  }
-  while (q_pending && !bar_try(sm.q_full(), q_awaited) && now_ns() - t0 < 100000000ull) {
+  while (!bar_try(sm.drain(t), 0) && now_ns() - t0 < 100000000ull) {
   }
 }
 
 __device__ __forceinline__ void group_sync(int id, int threads) {
   asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// 32 bytes of a row; at once where the address is on that grid.  A lane's rows
+// lie apart, so that each store is a line of its own: fewer and larger ones are
+// what counts (16-byte stores took 4 us a unit of 256 rows).
+__device__ __forceinline__ void store32(void *at, const uint32_t *w, bool aligned32) {
+  if (aligned32) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4 *>(at)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4 *>(at)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
+// Reciprocal of a row's sum: 0 for a row that saw no key, NaN stays.
+__device__ __forceinline__ float reciprocal(float l) { return l > 0.f ? __frcp_rn(l) : l; }
+__device__ __forceinline__ float log_sum(float m, float l) { return l > 0.f ? (m + log2f(l)) * kLn2 : (l == 0.f ? -INFINITY : l); }
+
+// The parts of `rows` rows, joined in their order: weights 2^(m - top), eight
+// lanes a row and four rows a warp at once, so that 16 loads are in flight.
+template <int D, bool BF16> __device__ void join_parts(const Params &p, const Unit &u, int rows, int row0, int first_tok, int wid, int lane) {
+  constexpr int kPieces = D / 32;           // of 4 components a lane
+  const int64_t stride = int64_t(u.ntok) * p.group;
+  for (int r = wid * 4 + lane / 8; r < rows; r += 16) {
+    const int64_t at = u.part_row + row0 + r;
+    float top = kNoMax, total = 0.f, acc[kPieces][4] = {};
+#pragma unroll 4
+    for (int s = 0; s < u.nsplit; ++s) top = fmaxf(top, __ldcg(p.part_ml + at + s * stride).x);
+#pragma unroll 4
+    for (int s = 0; s < u.nsplit; ++s) {
+      const float2 ml = __ldcg(p.part_ml + at + s * stride);
+      const float by = exp2_approx(ml.x - top);
+      total += by * ml.y;
+      const float4 *src = reinterpret_cast<const float4 *>(p.part_o + (at + s * stride) * D) + lane % 8;
+#pragma unroll
+      for (int k = 0; k < kPieces; ++k) {
+        const float4 v = __ldcg(src + 8 * k);
+        acc[k][0] += by * v.x, acc[k][1] += by * v.y, acc[k][2] += by * v.z, acc[k][3] += by * v.w;
+      }
+    }
+    const float inv = reciprocal(total);
+    const int64_t token = u.tok0 + first_tok + r / p.group;
+    const int head = u.kvh * p.group + r % p.group;
+    uint2 *dst = reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + token * p.out_stride[0] + head * p.out_stride[1]) + lane % 8;
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k)
+      dst[8 * k] = make_uint2(pack16<BF16>(acc[k][0] * inv, acc[k][1] * inv), pack16<BF16>(acc[k][2] * inv, acc[k][3] * inv));
+    if (lane % 8 == 0 && p.lse) p.lse[token * p.q_heads + head] = log_sum(top, total);
+  }
 }
 
 template <int D, bool BF16> __device__ void softmax_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last, uint32_t tmem) {
@@ -485,23 +601,36 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
   uint32_t s_phase = 0, f_phase = 0;
   bool alive = true;
   // this stream's tile of queries: its first token in the unit, and its rows
+  const int row_token = row / p.group, row_head = row % p.group;
   auto first_token = [&](const Unit &u) { return u.wide ? t * p.per_tile : 0; };
   auto stream_rows = [&](const Unit &u) { return min(u.ntok - first_token(u), p.per_tile) * p.group; };
+  // the keys that this thread's row sees; rows after the last take its place
+  auto seen_by_row = [&](const Unit &u, int &lo, int &hi) {
+    const int pos = u.pos0 + first_token(u) + min(row_token, min(u.ntok - first_token(u), p.per_tile) - 1);
+    hi = p.causal ? min(u.kv_len, pos + 1) : u.kv_len;
+    lo = p.window ? max(0, pos - p.window + 1) : 0;
+  };
+  auto weights_stored = [&](int half) {
+    tmem_st_wait();
+    fence_before();
+    __syncwarp();
+    if (lane == 0) bar_arrive(sm.p_ready(t, half));
+  };
   for (int i = first; i < last; ++i) {
-    int my_lo, my_hi, step, key0, end;      // keys seen by this row; first key of a tile
+    int step, key0, end;           // first key of a tile, and past the last
+    int min_hi, max_lo;            // every row of the warp sees the keys between
     bool warp_active;
     {
       const Unit u = read_unit(p, i);
-      const int rows = stream_rows(u);
-      warp_active = wid * 32 < rows;
-      const int pos = u.pos0 + first_token(u) + min(row, rows - 1) / p.group;
-      my_hi = p.causal ? min(u.kv_len, pos + 1) : u.kv_len;
-      my_lo = p.window ? max(0, pos - p.window + 1) : 0;
+      warp_active = wid * 32 < stream_rows(u);
+      int lo, hi;
+      seen_by_row(u, lo, hi);
+      min_hi = __reduce_min_sync(~0u, hi);
+      max_lo = __reduce_max_sync(~0u, lo);
       step = u.wide ? kTile : 2 * kTile;
       key0 = (u.tile0 + (u.wide ? 0 : t)) * kTile;
       end = (u.tile0 + u.ntiles) * kTile;
     }
-    const int min_hi = __reduce_min_sync(~0u, my_hi), max_lo = __reduce_max_sync(~0u, my_lo);
     float m = kNoMax, l = 0.f;
     bool begun = false;
     for (; key0 < end; key0 += step) {
@@ -509,47 +638,47 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
       s_phase ^= 1;
       if (warp_active && alive) {
         fence_after();
-        uint32_t s[kTile];
-#pragma unroll
-        for (int k = 0; k < kTile; k += 32) tmem_ld32(s_at + k, s + k);
-        tmem_ld_wait(s);
         if (key0 < max_lo || key0 + kTile > min_hi) {
-          const int from = my_lo - key0;
-          const unsigned span = my_hi > my_lo ? my_hi - my_lo : 0;
+          // some row of the warp does not see the whole tile: the scores are
+          // masked where they lie, so that the way below has no branches
+          int lo, hi;
+          seen_by_row(read_unit(p, i), lo, hi);
+          const int from = lo - key0;
+          const unsigned span = max(0, hi - lo);
+#pragma unroll 1
+          for (int column = 0; column < kTile; column += 16) {
+            uint32_t v[16];
+            tmem_ld16(s_at + column, v);
+            tmem_ld_wait(v);
 #pragma unroll
-          for (int k = 0; k < kTile; ++k)
-            if (unsigned(k - from) >= span) s[k] = __float_as_uint(-INFINITY);
-        }
-        const uint64_t c2 = pair(c, c);
-        float sum;
-        for (;;) {
-          const uint64_t base2 = pair(-m, -m);
-          uint64_t part[4] = {0, 0, 0, 0};
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            uint32_t w[16];
-#pragma unroll
-            for (int q = 0; q < 16; ++q) {
-              const float x = __uint_as_float(s[32 * h + 2 * q]), y = __uint_as_float(s[32 * h + 2 * q + 1]);
-              top[q % 4] = fmaxf(fmaxf(top[q % 4], x), y);
-              float e, f;
-              unpair(fma2(pair(x, y), c2, base2), e, f);
-              e = exp2_approx(e);
-              f = exp2_approx(f);
-              part[q % 4] = add2(part[q % 4], pair(e, f));
-              w[q] = pack16<BF16>(e, f);
-            }
-            tmem_st16(s_at + 16 * h, w);
+            for (int k = 0; k < 16; ++k)
+              if (unsigned(column + k - from) >= span) v[k] = __float_as_uint(-INFINITY);
+            tmem_st16(s_at + column, v);
           }
-          float x, y;
-          unpair(add2(add2(part[0], part[1]), add2(part[2], part[3])), x, y);
-          sum = x + y;
-          const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-          const bool need = best > m + (kShift + kGrow);
-          if (!__any_sync(~0u, need)) break;
-          // a new base, and the weights again from it; the running sum and
-          // output (idle: the last product is complete) come down to it
+          tmem_st_wait();
+        }
+        // the row's scores stay in registers
+        uint32_t s[kTile];
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto take_in = [&](int from) {
+#pragma unroll
+          for (int k = from; k < from + 64; k += 8)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) top[q] = max3(__float_as_uint(top[q]), s[k + q], s[k + 4 + q]);
+        };
+        tmem_ld32(s_at, s);
+        tmem_ld32(s_at + 32, s + 32);
+        tmem_ld_wait(s, 0, 64);
+        tmem_ld32(s_at + 64, s + 64);
+        tmem_ld32(s_at + 96, s + 96);
+        take_in(0);
+        tmem_ld_wait(s, 64, 128);
+        take_in(64);
+        const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+        const bool need = best > m + (kShift + kGrow);
+        if (__any_sync(~0u, need)) {
+          // a new base: the running sum and output (idle, the last product is
+          // complete) come down to it
           const float to = need ? best - kShift : m;
           const float by = need ? exp2_approx(m - to) : 1.f;
           m = to;
@@ -563,22 +692,48 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
               tmem_ld_wait(o);
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
-                float x, y;
-                unpair(mul2(pair(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])), by2), x, y);
-                o[2 * q] = __float_as_uint(x);
-                o[2 * q + 1] = __float_as_uint(y);
+                float e, f;
+                unpair(mul2(pair(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])), by2), e, f);
+                o[2 * q] = __float_as_uint(e);
+                o[2 * q + 1] = __float_as_uint(f);
               }
               tmem_st16(o_at + k, o);
             }
           }
         }
-        l += sum;
-        tmem_st_wait();
-        fence_before();
+        const uint64_t c2 = pair(c, c);
+        const uint64_t base2 = pair(-m, -m);
+        uint64_t part[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          // a branch that is always taken keeps the last chunk's exponentials
+          // from being scheduled before the first half is handed on
+          if (h == 3 && !p.group) break;
+          uint32_t w[16];
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            float e, f;
+            unpair(fma2(pair(__uint_as_float(s[32 * h + 2 * q]), __uint_as_float(s[32 * h + 2 * q + 1])), c2, base2), e, f);
+            e = exp2_approx(e);
+            f = exp2_approx(f);
+            part[q % 4] = add2(part[q % 4], pair(e, f));
+            w[q] = pack16<BF16>(e, f);
+          }
+          if (h == 2) weights_stored(0);      // of the first 64 keys
+          tmem_st16(s_at + 16 * h, w);
+        }
+        weights_stored(1);
+        float even, odd;
+        unpair(add2(add2(part[0], part[1]), add2(part[2], part[3])), even, odd);
+        l += even + odd;
+      } else {
+        __syncwarp();
+        if (lane == 0) {
+          bar_arrive(sm.p_ready(t, 0));
+          bar_arrive(sm.p_ready(t, 1));
+        }
       }
       begun = true;
-      __syncwarp();
-      if (lane == 0) bar_arrive(sm.p_ready(t));
     }
 
     // ------------------------------------------------------------ the unit's end
@@ -606,57 +761,65 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
     }
     if (t == 0 || u.wide) {
       fence_after();
-      const bool mine = warp_active && row < rows && alive;
-      const int64_t out_token = u.tok0 + first_token(u) + row / p.group;
-      const int head = u.kvh * p.group + row % p.group;
-      const bool split = u.nsplit > 1;
+      const bool mine = row < rows && alive, split = u.nsplit > 1;
+      const int64_t out_token = u.tok0 + first_token(u) + row_token;
+      const int head = u.kvh * p.group + row_head;
       const int64_t part = u.part_row + int64_t(u.split) * u.ntok * p.group + row0 + row;
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      const float f0 = split ? by0 : by0 * inv, f1 = split ? by1 : by1 * inv;
+      const float inv = split ? 1.f : reciprocal(l);
       if (warp_active && alive) {
+        const uint64_t f0 = pair(by0 * inv, by0 * inv), f1 = pair(by1 * inv, by1 * inv);
+        char *to = split ? reinterpret_cast<char *>(p.part_o + part * D)
+                         : static_cast<char *>(p.out) + 2 * (out_token * p.out_stride[0] + head * p.out_stride[1]);
 #pragma unroll 1
         for (int k = 0; k < D; k += 32) {
           uint32_t o[32];
           if (begun) {
             tmem_ld32(o_at + k, o);
             tmem_ld_wait(o);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 32; ++q) o[q] = 0;
           }
 #pragma unroll
-          for (int q = 0; q < 32; ++q) o[q] = begun && l != 0.f ? __float_as_uint(__uint_as_float(o[q]) * f0) : 0u;
+          for (int q = 0; q < 32; q += 2) {
+            float x, y;
+            unpair(mul2(pair(__uint_as_float(o[q]), __uint_as_float(o[q + 1])), f0), x, y);
+            o[q] = __float_as_uint(x);
+            o[q + 1] = __float_as_uint(y);
+          }
           if (joined) {
             uint32_t o1[32];
             tmem_ld32(o_at + kTile + k, o1);
             tmem_ld_wait(o1);
 #pragma unroll
-            for (int q = 0; q < 32; ++q)
-              if (l != 0.f) o[q] = __float_as_uint(fmaf(__uint_as_float(o1[q]), f1, __uint_as_float(o[q])));
+            for (int q = 0; q < 32; q += 2) {
+              float x, y;
+              unpair(fma2(pair(__uint_as_float(o1[q]), __uint_as_float(o1[q + 1])), f1,
+                          pair(__uint_as_float(o[q]), __uint_as_float(o[q + 1]))), x, y);
+              o[q] = __float_as_uint(x);
+              o[q + 1] = __float_as_uint(y);
+            }
           }
           if (mine && split) {
-            float4 *dst = reinterpret_cast<float4 *>(p.part_o + part * D + k);
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              __stcg(dst + q, make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]),
-                                          __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3])));
+            for (int q = 0; q < 32; q += 8) store32(to + 4 * (k + q), o + q, true);
           } else if (mine) {
-            uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + out_token * p.out_stride[0] +
-                                                   head * p.out_stride[1] + k);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t w[4];
+            for (int q = 0; q < 32; q += 16) {
+              uint32_t w[8];
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                w[r] = pack16<BF16>(__uint_as_float(o[8 * q + 2 * r]), __uint_as_float(o[8 * q + 2 * r + 1]));
-              dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int r = 0; r < 8; ++r)
+                w[r] = pack16<BF16>(__uint_as_float(o[q + 2 * r]), __uint_as_float(o[q + 2 * r + 1]));
+              store32(to + 2 * (k + q), w, p.aligned32);
             }
           }
         }
         if (mine && split) __stcg(p.part_ml + part, make_float2(m, l));
-        if (mine && !split && p.lse)
-          p.lse[out_token * p.q_heads + head] = l > 0.f ? (m + log2f(l)) * kLn2 : (l == 0.f ? -INFINITY : l);
+        if (mine && !split && p.lse) p.lse[out_token * p.q_heads + head] = log_sum(m, l);
       }
       fence_before();
       if (split) {
-        // the stream that arrives last joins the parts, in their order
+        // the stream that arrives last joins the parts
         __threadfence();
         group_sync(1 + t, kTile);
         if (row == 0) {
@@ -667,49 +830,7 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
           sm.words()[2 + t] = is_last;
         }
         group_sync(1 + t, kTile);
-        if (sm.words()[2 + t]) {
-          constexpr int kWidth = D / 32;            // components a lane
-          for (int r = wid; r < rows; r += 4) {
-            const int64_t at = u.part_row + row0 + r, stride = int64_t(u.ntok) * p.group;
-            float top = kNoMax;
-            for (int s = lane; s < u.nsplit; s += 32) top = fmaxf(top, __ldcg(p.part_ml + at + s * stride).x);
-#pragma unroll
-            for (int k = 16; k; k /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, k));
-            float acc[kWidth] = {}, total = 0.f;
-            for (int s0 = 0; s0 < u.nsplit; s0 += 32) {
-              float2 ml = make_float2(kNoMax, 0.f);
-              if (s0 + lane < u.nsplit) ml = __ldcg(p.part_ml + at + (s0 + lane) * stride);
-              const float by = ml.y == 0.f ? 0.f : exp2_approx(ml.x - top);
-              total += by * ml.y;
-              const int n = min(32, u.nsplit - s0);
-#pragma unroll 8
-              for (int s = 0; s < n; ++s) {
-                const float w = __shfl_sync(~0u, by, s);
-                const float *src = p.part_o + (at + (s0 + s) * stride) * D + lane * kWidth;
-                if constexpr (kWidth == 4) {
-                  const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
-                  acc[0] += w * v.x, acc[1] += w * v.y, acc[2] += w * v.z, acc[3] += w * v.w;
-                } else {
-                  const float2 v = __ldcg(reinterpret_cast<const float2 *>(src));
-                  acc[0] += w * v.x, acc[1] += w * v.y;
-                }
-              }
-            }
-#pragma unroll
-            for (int k = 16; k; k /= 2) total += __shfl_xor_sync(~0u, total, k);
-            const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
-            const int64_t tok = u.tok0 + first_token(u) + r / p.group;
-            const int h = u.kvh * p.group + r % p.group;
-            uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + tok * p.out_stride[0] +
-                                                         h * p.out_stride[1] + lane * kWidth);
-            if constexpr (kWidth == 4)
-              *reinterpret_cast<uint2 *>(dst) = make_uint2(pack16<BF16>(acc[0] * inv, acc[1] * inv), pack16<BF16>(acc[2] * inv, acc[3] * inv));
-            else
-              *dst = pack16<BF16>(acc[0] * inv, acc[1] * inv);
-            if (lane == 0 && p.lse)
-              p.lse[tok * p.q_heads + h] = total > 0.f ? (top + log2f(total)) * kLn2 : (total == 0.f ? -INFINITY : total);
-          }
-        }
+        if (sm.words()[2 + t]) join_parts<D, BF16>(p, u, rows, row0, first_token(u), wid, lane);
       }
     }
     if (joined) group_sync(3, 256);       // stream 1's output and sums have been read
@@ -719,21 +840,23 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
 template <int D, bool BF16> __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __grid_constant__ Params p) {
   extern __shared__ char raw[];
   Smem<D> sm;
-  sm.ptr = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-  sm.base = smem_addr(sm.ptr);
+  sm.base = (smem_addr(raw) + 1023) & ~1023u;
   const int warp = threadIdx.x / 32;
   if (threadIdx.x == 0) {
     for (int s = 0; s < Shape<D>::kStages; ++s) {
       bar_init(sm.full(s), 1);
-      bar_init(sm.empty(s), 1);
+      bar_init(sm.empty(s), 2);
     }
     bar_init(sm.q_full(), 1);
+    bar_init(sm.q_empty(), 2);
     for (int t = 0; t < 2; ++t) {
       bar_init(sm.s_full(t), 1);
-      bar_init(sm.p_ready(t), 4);
+      bar_init(sm.p_ready(t, 0), 4);
+      bar_init(sm.p_ready(t, 1), 4);
       bar_init(sm.final(t), 1);
+      bar_init(sm.drain(t), 1);
+      bar_init(sm.turn(t), 1);
     }
-    bar_init(sm.drain(), 1);
     sm.words()[0] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -744,22 +867,30 @@ template <int D, bool BF16> __global__ void __launch_bounds__(kThreads, 1) paged
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = sm.words()[1];
-  const Guard g{sm.words(), p.status};
+  const uint32_t tmem = __reduce_or_sync(~0u, sm.words()[1]);
+  const Guard g{sm.base + Shape<D>::kWords, p};
   const int first = p.cta_first[blockIdx.x], last = p.cta_first[blockIdx.x + 1];
-  if (warp < kMmaWarp) {
+  if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     softmax_role<D, BF16>(p, sm, g, first, last, tmem);
+    // an end of their own: code shared with the other warps would have to do
+    // with their registers
+    __syncwarp();
+    fence_before();
+    asm volatile("barrier.cta.sync 0;" ::: "memory");
+    return;
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == kMmaWarp)
-      mma_role<D, BF16>(p, sm, g, first, last, tmem);
-    else if (warp == kMmaWarp + 1)
+    if (warp >= kMmaWarp)
+      mma_role<D, BF16>(p, sm, g, first, last, tmem, warp - kMmaWarp);
+    else if (warp == kLoadWarp)
       load_role<D>(p, sm, g, first, last);
+    else
+      query_role<D>(p, sm, g, first, last);
   }
   __syncwarp();
   fence_before();
-  __syncthreads();
+  asm volatile("barrier.cta.sync 0;" ::: "memory");
   if (warp == kMmaWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
@@ -817,8 +948,8 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
     return fail("emmy_paged_attention: a table of %ld pages a sequence does not hold %ld tokens", a->table_width, plan->max_kv);
   if (!a->q || !a->out || !a->k_cache || !a->v_cache || !a->table || !a->plan_words || (plan->part_rows && !a->scratch))
     return fail("emmy_paged_attention: null address");
-  if ((a->q | a->out | a->k_cache | a->v_cache | a->plan_words | a->scratch) % 16 || (a->table | a->lse) % 4)
-    return fail("emmy_paged_attention: address not a multiple of 16 bytes");
+  if ((a->q | a->out | a->k_cache | a->v_cache | a->plan_words) % 16 || a->scratch % 32 || (a->table | a->lse) % 4)
+    return fail("emmy_paged_attention: address not a multiple of 16 bytes (scratch: 32)");
   const int group = plan->q_heads / plan->kv_heads, d = plan->head_dim;
   const int64_t extent[3] = {a->pages, ps, plan->kv_heads};
   for (int i = 0; i < 3; ++i)
@@ -861,6 +992,7 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
   p.per_tile = per_tile;
   p.page_size = ps;
   p.box = box;
+  p.aligned32 = (a->out % 32 == 0) && (rows[0] == 1 || a->out_stride[0] % 16 == 0) && (rows[1] == 1 || a->out_stride[1] % 16 == 0);
   p.causal = plan->causal;
   p.window = plan->window;
   p.scale_log2 = a->scale * kLog2e;

@@ -22,8 +22,9 @@ using emmy_paged::Unit;
 
 namespace {
 
-// Costs in units of a quarter of a one-query-tile key tile.
-constexpr int64_t kNarrowTile = 4, kNarrowUnit = 4, kWideTile = 6, kWideUnit = 12;
+// Costs in units of a quarter of a one-query-tile key tile; kWidePart is what a
+// part of a cut wide unit spends on its partial result.
+constexpr int64_t kNarrowTile = 4, kNarrowUnit = 4, kWideTile = 6, kWideUnit = 12, kWidePart = 20;
 constexpr int kMinNarrow = 2;    // tiles: the two streams of a CTA take one each
 constexpr int kMinWide = 16;     // tiles: under this a split costs more than it gives
 
@@ -107,7 +108,7 @@ void make(const emmy_paged_plan_args &a, emmy_paged_plan_s &plan) {
         const int b = part(wide[i], k, n), e = part(wide[i], k + 1, n);
         Slot s = least.top();
         least.pop();
-        s.first += kWideUnit + kWideTile * (e - b);
+        s.first += kWideUnit + kWideTile * (e - b) + (n > 1 ? kWidePart : 0);
         end = std::max(end, s.first);
         least.push(s);
         if (!keep) continue;

@@ -254,7 +254,7 @@ typedef struct {
 /* How the work of one set of lengths is cut into units and dealt to the CTAs, */
 /* made on the host and used by every layer's call.  The plan's words (32-bit) */
 /* go to device memory as they are (16-byte aligned); beside them the caller    */
-/* keeps `scratch` bytes of device memory, not initialised, 16-byte aligned.    */
+/* keeps `scratch` bytes of device memory, not initialised, 32-byte aligned.    */
 /* Calls that share the device words must not overlap on the GPU.               */
 EMMY_API int emmy_paged_plan_make(const emmy_paged_plan_args *a, emmy_paged_plan_t *out);
 EMMY_API int emmy_paged_plan_data(emmy_paged_plan_t plan, const int32_t **words, size_t *n_words,
