@@ -17,7 +17,7 @@ on arguments it refuses, ``ValueError`` on what only Python can see.
 from __future__ import annotations
 
 import ctypes
-import math
+import struct
 
 import torch
 
@@ -25,16 +25,12 @@ from . import native
 
 _DTYPES = {torch.float16: 6, torch.float32: 7, torch.bfloat16: 9}
 
-_i32, _i64, _u64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64
+# the argument structures of the C ABI, packed in one go: 1 us against 6 for a
+# ctypes structure of as many fields, on calls of 3 us on the GPU
+_ROTATE_APPEND_ARGS = struct.Struct("@10i10Q15q")
+_ATTENTION_ARGS = struct.Struct("@4if8Q11q")
 
-
-class _RotateAppendArgs(ctypes.Structure):
-    _fields_ = ([(n, _i32) for n in ("dtype", "tokens", "q_heads", "kv_heads", "head_dim", "rotary_dim", "axes",
-                                     "interleaved", "pages", "page_size")]
-                + [(n, _u64) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "positions", "slots",
-                                       "frequencies", "pair_axis")]
-                + [("q_stride", _i64 * 2), ("k_stride", _i64 * 2), ("v_stride", _i64 * 2), ("q_out_stride", _i64 * 2),
-                   ("k_cache_stride", _i64 * 3), ("v_cache_stride", _i64 * 3), ("positions_stride", _i64)])
+_i32 = ctypes.c_int32
 
 
 class _PlanArgs(ctypes.Structure):
@@ -43,45 +39,54 @@ class _PlanArgs(ctypes.Structure):
                 ("ctas", _i32)]
 
 
-class _AttentionArgs(ctypes.Structure):
-    _fields_ = ([(n, _i32) for n in ("dtype", "pages", "page_size", "table_width")] + [("scale", ctypes.c_float)]
-                + [(n, _u64) for n in ("q", "out", "lse", "k_cache", "v_cache", "table", "plan_words", "scratch")]
-                + [("q_stride", _i64 * 2), ("out_stride", _i64 * 2), ("k_cache_stride", _i64 * 3),
-                   ("v_cache_stride", _i64 * 3), ("table_stride", _i64)])
-
-
 def _need(ok, text):
     if not ok:
         raise ValueError(text)
 
 
-def _check(name, t, ndim, dtype, device, rows=True):
+def _check(name, t, ndim, dtype, device):
     """A tensor of the cache operators: on the GPU, its innermost stride 1."""
-    _need(isinstance(t, torch.Tensor) and t.dim() == ndim, f"{name}: a tensor of {ndim} dimensions is wanted")
-    _need(t.dtype == dtype, f"{name}: {dtype} is wanted, not {t.dtype}")
-    _need(t.device == device, f"{name}: on {t.device}, not on {device}")
-    _need(not rows or t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: the innermost stride must be 1")
+    if not isinstance(t, torch.Tensor) or t.ndim != ndim:
+        raise ValueError(f"{name}: a tensor of {ndim} dimensions is wanted")
+    if t.dtype is not dtype:
+        raise ValueError(f"{name}: {dtype} is wanted, not {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name}: on {t.device}, not on {device}")
+    stride = t.stride()
+    if stride[-1] != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name}: the innermost stride must be 1")
+    return stride
 
 
 def _cuda_device(name, t):
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name}: a CUDA tensor is wanted")
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor is wanted")
     return t.device
 
 
 def _cache(k_cache, v_cache, dtype, device):
-    _check("k_cache", k_cache, 4, dtype, device)
-    _check("v_cache", v_cache, 4, dtype, device)
-    _need(k_cache.shape == v_cache.shape, "k_cache and v_cache have different shapes")
+    strides = _check("k_cache", k_cache, 4, dtype, device)[:3], _check("v_cache", v_cache, 4, dtype, device)[:3]
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache have different shapes")
+    return strides
 
 
-def _call(fn, device, stream, *args):
+_fns = {}
+
+
+def _call(name, device, stream, *args):
     """One C-ABI call with ``device`` current, on its current stream unless one is given."""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(native.lib(), name)
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _call(fn, device, stream, *args)
+            return _call(name, device, stream, *args)
     if stream is None:
-        stream = torch.cuda.current_stream(device).cuda_stream
-    native.check(fn(*args, ctypes.c_void_p(stream)))
+        stream = torch._C._cuda_getCurrentRawStream(device.index)
+    rc = fn(*args, stream)
+    if rc:
+        native.check(rc)
 
 
 class Rotation:
@@ -106,6 +111,8 @@ class Rotation:
             if any(axes):
                 self.axes = max(axes) + 1
                 self.pair_axis = torch.tensor(axes, dtype=torch.int32, device=device)
+        self.components = 2 * self.frequencies.shape[0]
+        self.pair_axis_ptr = 0 if self.pair_axis is None else self.pair_axis.data_ptr()
 
 
 def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=None, stream=None):
@@ -120,37 +127,40 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
     formed in 64, and rounds once."""
     device = _cuda_device("q", q)
     dtype = q.dtype
-    _need(dtype in _DTYPES, f"q: bfloat16, float16 or float32 is wanted, not {dtype}")
-    _check("q", q, 3, dtype, device)
-    _check("k", k, 3, dtype, device)
-    _check("v", v, 3, dtype, device)
-    _cache(k_cache, v_cache, dtype, device)
+    if dtype not in _DTYPES:
+        raise ValueError(f"q: bfloat16, float16 or float32 is wanted, not {dtype}")
+    q_stride = _check("q", q, 3, dtype, device)
+    k_stride = _check("k", k, 3, dtype, device)
+    v_stride = _check("v", v, 3, dtype, device)
+    k_cache_stride, v_cache_stride = _cache(k_cache, v_cache, dtype, device)
     tokens, q_heads, dim = q.shape
-    pages, page_size, kv_heads, _ = k_cache.shape
-    _need(k.shape == (tokens, kv_heads, dim) and v.shape == k.shape and k_cache.shape[3] == dim,
-          "q, k, v and the caches do not fit together")
-    if positions.dim() == 1:
+    pages, page_size, kv_heads, cache_dim = k_cache.shape
+    if k.shape != (tokens, kv_heads, dim) or v.shape != k.shape or cache_dim != dim:
+        raise ValueError("q, k, v and the caches do not fit together")
+    if positions.ndim == 1:
         positions = positions[None]
-    _check("positions", positions, 2, torch.int32, device)
-    _need(positions.shape[1] == tokens and positions.shape[0] >= rotation.axes,
-          f"positions: [{rotation.axes}, {tokens}] is wanted, not {list(positions.shape)}")
+    positions_stride = _check("positions", positions, 2, torch.int32, device)[0]
+    axes = positions.shape[0]
+    if positions.shape[1] != tokens or axes < rotation.axes:
+        raise ValueError(f"positions: [{rotation.axes}, {tokens}] is wanted, not {list(positions.shape)}")
     _check("slots", slots, 1, torch.int32, device)
-    _need(slots.shape[0] == tokens, f"slots: {tokens} are wanted, not {slots.shape[0]}")
-    _need(rotation.frequencies.device == device, "rotation: on another device")
+    if slots.shape[0] != tokens:
+        raise ValueError(f"slots: {tokens} are wanted, not {slots.shape[0]}")
+    if rotation.frequencies.device != device:
+        raise ValueError("rotation: on another device")
     if q_out is None:
         q_out = torch.empty((tokens, q_heads, dim), dtype=dtype, device=device)
+        q_out_stride = q_heads * dim, dim
     else:
-        _check("q_out", q_out, 3, dtype, device)
-        _need(q_out.shape == q.shape, "q_out: another shape than q")
-    pair_axis = rotation.pair_axis
-    a = _RotateAppendArgs(
-        _DTYPES[dtype], tokens, q_heads, kv_heads, dim, 2 * rotation.frequencies.shape[0], positions.shape[0],
-        rotation.interleaved, pages, page_size, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(),
-        k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(), slots.data_ptr(),
-        rotation.frequencies.data_ptr(), 0 if pair_axis is None else pair_axis.data_ptr(),
-        q.stride()[:2], k.stride()[:2], v.stride()[:2], q_out.stride()[:2], k_cache.stride()[:3],
-        v_cache.stride()[:3], positions.stride(0))
-    _call(native.lib().emmy_rotate_append, device, stream, ctypes.byref(a))
+        q_out_stride = _check("q_out", q_out, 3, dtype, device)[:2]
+        if q_out.shape != q.shape:
+            raise ValueError("q_out: another shape than q")
+    a = _ROTATE_APPEND_ARGS.pack(
+        _DTYPES[dtype], tokens, q_heads, kv_heads, dim, rotation.components, axes, rotation.interleaved, pages, page_size,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        positions.data_ptr(), slots.data_ptr(), rotation.frequencies.data_ptr(), rotation.pair_axis_ptr,
+        *q_stride[:2], *k_stride[:2], *v_stride[:2], *q_out_stride, *k_cache_stride, *v_cache_stride, positions_stride)
+    _call("emmy_rotate_append", device, stream, a)
     return q_out
 
 
@@ -196,6 +206,7 @@ class AttentionPlan:
         self.scratch = torch.empty(scratch.value, dtype=torch.uint8, device=device)
         self.device, self.tokens, self.sequences = device, sum(q_lens), n
         self.q_heads, self.kv_heads, self.head_dim = int(q_heads), int(kv_heads), int(head_dim)
+        self.shape = (self.tokens, self.q_heads, self.head_dim)
 
     def __del__(self):
         if self._h is not None:
@@ -206,7 +217,7 @@ class AttentionPlan:
 
     def check(self, stream=None):
         """Waits for the calls so far and raises if one of them gave up."""
-        _call(native.lib().emmy_paged_plan_status, self.device, stream, self._h, self.words.data_ptr())
+        _call("emmy_paged_plan_status", self.device, stream, self._h, self.words.data_ptr())
 
 
 def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, stream=None):
@@ -225,31 +236,38 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     finite."""
     device = _cuda_device("q", q)
     dtype = q.dtype
-    _need(dtype in (torch.bfloat16, torch.float16), f"q: bfloat16 or float16 is wanted, not {dtype}")
-    _check("q", q, 3, dtype, device)
-    _need(device == plan.device, f"q: on {device}, the plan on {plan.device}")
-    shape = (plan.tokens, plan.q_heads, plan.head_dim)
-    _need(q.shape == shape, f"q: the plan is for {list(shape)}, not {list(q.shape)}")
-    _cache(k_cache, v_cache, dtype, device)
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError(f"q: bfloat16 or float16 is wanted, not {dtype}")
+    q_stride = _check("q", q, 3, dtype, device)
+    if device != plan.device:
+        raise ValueError(f"q: on {device}, the plan on {plan.device}")
+    shape = plan.shape
+    if q.shape != shape:
+        raise ValueError(f"q: the plan is for {list(shape)}, not {list(q.shape)}")
+    k_cache_stride, v_cache_stride = _cache(k_cache, v_cache, dtype, device)
     pages, page_size, kv_heads, dim = k_cache.shape
-    _need((kv_heads, dim) == (plan.kv_heads, plan.head_dim),
-          f"k_cache: the plan is for {plan.kv_heads} heads of {plan.head_dim}, not {kv_heads} of {dim}")
-    _check("table", table, 2, torch.int32, device)
-    _need(table.shape[0] == plan.sequences, f"table: {plan.sequences} rows are wanted, not {table.shape[0]}")
+    if kv_heads != plan.kv_heads or dim != plan.head_dim:
+        raise ValueError(f"k_cache: the plan is for {plan.kv_heads} heads of {plan.head_dim}, not {kv_heads} of {dim}")
+    table_stride = _check("table", table, 2, torch.int32, device)[0]
+    if table.shape[0] != plan.sequences:
+        raise ValueError(f"table: {plan.sequences} rows are wanted, not {table.shape[0]}")
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=device)
+        out_stride = shape[1] * dim, dim
     else:
-        _check("out", out, 3, dtype, device)
-        _need(out.shape == shape, "out: another shape than q")
+        out_stride = _check("out", out, 3, dtype, device)[:2]
+        if out.shape != shape:
+            raise ValueError("out: another shape than q")
     if lse is None:
         lse = torch.empty(shape[:2], dtype=torch.float32, device=device)
     else:
         _check("lse", lse, 2, torch.float32, device)
-        _need(lse.shape == shape[:2] and lse.is_contiguous(), f"lse: contiguous {list(shape[:2])} is wanted")
-    a = _AttentionArgs(
-        _DTYPES[dtype], pages, page_size, table.shape[1], 1 / math.sqrt(plan.head_dim) if scale is None else scale,
+        if lse.shape != shape[:2] or not lse.is_contiguous():
+            raise ValueError(f"lse: contiguous {list(shape[:2])} is wanted")
+    a = _ATTENTION_ARGS.pack(
+        _DTYPES[dtype], pages, page_size, table.shape[1], plan.head_dim ** -0.5 if scale is None else scale,
         q.data_ptr(), out.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
-        plan.words.data_ptr(), plan.scratch.data_ptr(), q.stride()[:2], out.stride()[:2], k_cache.stride()[:3],
-        v_cache.stride()[:3], table.stride(0))
-    _call(native.lib().emmy_paged_attention, device, stream, plan._h, ctypes.byref(a))
+        plan.words.data_ptr(), plan.scratch.data_ptr(), *q_stride[:2], *out_stride, *k_cache_stride, *v_cache_stride,
+        table_stride)
+    _call("emmy_paged_attention", device, stream, plan._h, a)
     return out, lse
