@@ -10,12 +10,20 @@
 // One persistent CTA an SM walks its list of units (emmy_paged.h).  Its roles:
 //   warps 0-3, 4-7  softmax of stream 0 and 1, one thread a row;
 //   warps 10, 11    issue the tensor-core products of stream 0 and 1;
-//   warp 9          loads key and value tiles, page by page, into one ring;
-//   warp 8          loads the query tiles.
+//   warps 8, 9      load key tiles, and value and query tiles; keys and values,
+//                   page by page, into one ring.
 // A unit with two query tiles gives one to each stream and both see every key
 // tile; a unit with one query tile (decode) gives it to both streams, which
 // take the key tiles in turn and are joined at the end.  Either way one
 // stream's softmax runs while the tensor cores work for the other.
+//
+// The few rows of a decoding unit (32 or less) would leave three of a stream's
+// four warps idle and one with 128 exponentials a row, 1,200 cycles, more than
+// the tile takes to arrive.  Their queries are loaded four times, into the rows
+// of each warp: every warp then has all scores of all rows, and takes a quarter
+// of the keys, with weights of 0 for the others and a maximum and a sum of its
+// own.  The eight results are joined in shared memory, where the second query
+// tile would be.
 //
 // Tensor memory: S_t at column 128 t, P_t over it (two 16-bit weights a
 // column), O_t at 256 + 128 t.  S = Q K^T and O += P V are 128 x 128 x D and
@@ -50,13 +58,13 @@ constexpr int kThreads = 384;
 // row of scores, and of the others; the shares add up to what was launched
 constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
-constexpr int kSoftmaxWarps = 8, kLoadWarp = 9, kMmaWarp = 10;
+constexpr int kSoftmaxWarps = 8, kKeyWarp = 8, kMmaWarp = 10;
 constexpr int kSmem = 227 * 1024;
 constexpr float kNoMax = -1e30f;        // exponent base of a row that has seen no key
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct alignas(64) Params {
-  CUtensorMap q, k, v;
+  CUtensorMap q, q32, k, v;            // q32: the rows of one warp
   const Unit *units;
   const int *cta_first;
   const int *table;
@@ -66,16 +74,17 @@ struct alignas(64) Params {
   void *out;
   float *lse;
   int64_t table_stride, out_stride[2];
-  int q_heads, group, per_tile, page_size, box, causal, window, aligned32;
+  int q_heads, group, per_tile, box, causal, window, aligned32;
+  int tiles_a_page;                    // of pages of a tile or more
   float scale_log2;
 };
 
 template <int D> struct Shape {
-  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kTileBytes = kTile * D * 2;       // 16 KiB or more: the joining needs them
   static constexpr int kStages = D == 128 ? 5 : 12;      // key and value tiles in flight
   static constexpr int kRing = 2 * kTileBytes;           // after two query tiles
   static constexpr int kBars = kRing + kStages * kTileBytes;
-  static constexpr int kWords = kBars + (2 * kStages + 14) * 8, kEnd = kWords + 32 + kTile * 8;
+  static constexpr int kWords = kBars + (2 * kStages + 15) * 8, kEnd = kWords + 32 + kTile * 8;
   static_assert(kEnd + 1024 <= kSmem, "shared memory");
 };
 
@@ -279,6 +288,8 @@ template <int D> struct Smem {
   __device__ uint32_t drain(int t) const { return bar(2 * Shape<D>::kStages + 10 + t); }
   // wide units: stream t may issue
   __device__ uint32_t turn(int t) const { return bar(2 * Shape<D>::kStages + 12 + t); }
+  // what a unit's end keeps in the second query tile has been used
+  __device__ uint32_t scratch_free() const { return bar(2 * Shape<D>::kStages + 14); }
   __device__ volatile int *words() const { return static_cast<volatile int *>(__cvta_shared_to_generic(base + Shape<D>::kWords)); }
   __device__ float2 *ml() const { return static_cast<float2 *>(__cvta_shared_to_generic(base + Shape<D>::kWords + 32)); }
 };
@@ -287,9 +298,10 @@ template <int D> struct Smem {
 template <int D> struct Ring {
   int stage = 0;
   uint32_t phase = 0;
-  __device__ __forceinline__ void next() {
-    if (++stage == Shape<D>::kStages) {
-      stage = 0;
+  __device__ __forceinline__ void next(int n = 1) {     // n < kStages
+    stage += n;
+    if (stage >= Shape<D>::kStages) {
+      stage -= Shape<D>::kStages;
       phase ^= 1;
     }
   }
@@ -307,102 +319,114 @@ __device__ __forceinline__ Unit read_unit(const Params &p, int i) {
   return u;
 }
 
-// Keys and values: lane b of the warp copies box b of a tile (a page, or 128
-// tokens of one).  Boxes without a key that the item sees are left out; what
-// the stage then holds in their place is masked (keys) or cleared (values).
-template <int D> __device__ void load_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last) {
-  const int lane = threadIdx.x % 32;
-  const int boxes = kTile / p.box;
+// A unit of at most 32 rows: each warp of a stream has all of them and a quarter
+// of the keys.
+__device__ __forceinline__ bool spread(const Params &p, const Unit &u) {
+  return !u.wide && u.ntiles && u.ntok * p.group <= 32;
+}
+
+// Query tiles: one 128-row tile for each stream of a wide unit, one for both of
+// a narrow one, each a box of group x tokens_per_tile rows; the rows of a spread
+// unit four times.
+template <int D> __device__ __forceinline__ void load_queries(const Params &p, const Smem<D> &sm, const Unit &u) {
+  if (spread(p, u)) {
+    bar_expect(sm.q_full(), 4 * p.group * (32 / p.group) * 128 * (D / 64));
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h)
+        load_box(sm.query(0) + h * (kTile * 128) + w * (32 * 128), &p.q32, sm.q_full(), 64 * h, 0, u.kvh, u.tok0);
+  } else {
+    const int tiles = u.wide ? 2 : 1;
+    bar_expect(sm.q_full(), tiles * p.group * p.per_tile * 128 * (D / 64));
+    for (int t = 0; t < tiles; ++t)
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h)
+        load_box(sm.query(t) + h * (kTile * 128), &p.q, sm.q_full(), 64 * h, 0, u.kvh, u.tok0 + t * p.per_tile);
+  }
+}
+
+// Key tiles, or (VALUES) value and query tiles.  Lane b of the warp copies box b
+// of a tile: a page, or 128 tokens of one.  Boxes without a key that the item
+// sees are left out; what the stage then holds in their place is masked (keys)
+// or cleared (values).  The order of the tiles in the ring is that of their use:
+// the first keys (one tile, or one for each stream), then values of tile n and
+// keys of tile n + ahead.  One warp for both took 2,400 cycles a tile pair, more
+// than a pair of 64-component heads takes to arrive.
+template <int D, bool VALUES> __device__ void load_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last) {
+  constexpr int S = Shape<D>::kStages;
+  const int lane = threadIdx.x % 32, boxes = kTile / p.box;
+  const CUtensorMap *map = VALUES ? &p.v : &p.k;
   Ring<D> ring;
-  int issued = 0;
-  bool alive = true;
+  uint32_t issued = 0, parity = 0;       // of each stage: the last copy into it
+  uint32_t q_phase = 0;
+  bool alive = true, was_spread = false;
   for (int i = first; i < last && alive; ++i) {
     const Unit u = read_unit(p, i);
     if (!u.ntiles) continue;
     if (i + 1 < last) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.units + i + 1));
     const int ahead = u.wide ? 1 : 2;
     const int *row = p.table + u.seq * p.table_stride;
-    auto page_of = [&](int tile) {           // the page of this lane's box; -1: no box
-      const int key = (u.tile0 + tile) * kTile + lane * p.box;
-      const bool wanted = tile < u.ntiles && lane < boxes && key < u.hi && key + p.box > u.lo;
-      return wanted ? max(-1, __ldg(row + key / p.page_size)) : INT_MIN;
+    struct Box { int page, token; };       // INT_MIN: no box of this lane's
+    auto box_of = [&](int n) {
+      const int tile = u.tile0 + n, key = tile * kTile + lane * p.box;
+      const bool wanted = n < u.ntiles && lane < boxes && key < u.hi && key + p.box > u.lo;
+      // pages of less than a tile, or of whole tiles
+      const int index = boxes > 1 ? tile * boxes + lane : p.tiles_a_page == 1 ? tile : tile / p.tiles_a_page;
+      return Box{wanted ? max(-1, __ldg(row + index)) : INT_MIN, boxes > 1 ? 0 : (tile - index * p.tiles_a_page) * kTile};
     };
-    auto load = [&](const CUtensorMap *map, int tile, int page) {
-      alive = alive && g.wait(sm.empty(ring.stage), ring.phase ^ 1, 1);
-      if (!alive) return;
-      const int key = (u.tile0 + tile) * kTile + lane * p.box;
-      const bool wanted = page != INT_MIN;
+    Box b0 = box_of(0), b1 = box_of(1), b2 = box_of(2);
+    if (VALUES) {
+      alive = g.wait(sm.q_empty(), q_phase ^ 1, 5);
+      // the unit before may still be joining its parts where the second tile goes
+      if (u.wide && was_spread) alive = alive && g.wait(sm.scratch_free(), q_phase ^ 1, 5);
+      if (!alive) break;
+      if (elected()) load_queries(p, sm, u);
+      __syncwarp();
+      q_phase ^= 1;
+      was_spread = spread(p, u);
+    }
+    int at = 0;                            // places of the ring behind this unit's first
+    for (int n = 0; n < u.ntiles; ++n) {
+      const int place = VALUES ? n + min(u.ntiles, n + ahead) : n < ahead ? n : 2 * n - ahead + 1;
+      ring.next(place - at);
+      at = place;
+      const Box b3 = box_of(n + 3);
+      alive = g.wait(sm.empty(ring.stage), ring.phase ^ 1, 1);
+      if (!alive) break;
+      const bool wanted = b0.page != INT_MIN;
       const uint32_t bar = sm.full(ring.stage);
-      const int n = __popc(__ballot_sync(~0u, wanted));
-      if (lane == 0) bar_expect(bar, n * p.box * D * 2);
+      const int count = __popc(__ballot_sync(~0u, wanted));
+      if (elected()) bar_expect(bar, count * p.box * D * 2);
       __syncwarp();
       if (wanted) {
         const uint32_t dst = sm.stage(ring.stage) + lane * p.box * 128;
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h)
-          load_box(dst + h * (kTile * 128), map, bar, 64 * h, key % p.page_size, u.kvh, page);
+        for (int h = 0; h < D / 64; ++h) load_box(dst + h * (kTile * 128), map, bar, 64 * h, b0.token, u.kvh, b0.page);
       }
-      ring.next();
-      ++issued;
-    };
-    int p0 = page_of(0), p1 = page_of(1), p2 = page_of(2);
-    load(&p.k, 0, p0);
-    if (ahead == 2 && u.ntiles > 1) load(&p.k, 1, p1);
-    for (int n = 0; n < u.ntiles; ++n) {
-      const int p3 = page_of(n + 3);
-      load(&p.v, n, p0);
-      if (n + ahead < u.ntiles) load(&p.k, n + ahead, ahead == 1 ? p1 : p2);
-      p0 = p1;
-      p1 = p2;
-      p2 = p3;
+      issued |= 1u << ring.stage;
+      parity = (parity & ~(1u << ring.stage)) | ring.phase << ring.stage;
+      b0 = b1;
+      b1 = b2;
+      b2 = b3;
     }
+    ring.next(2 * u.ntiles - at);
   }
-  if (!alive) {       // copies in flight land before the CTA ends
-    const int n = min(issued, Shape<D>::kStages);
-    for (int k = 0; k < n; ++k) {
-      if (ring.stage == 0) {
-        ring.stage = Shape<D>::kStages;
-        ring.phase ^= 1;
-      }
-      --ring.stage;
-      const uint64_t t0 = now_ns();
-      while (!bar_try(sm.full(ring.stage), ring.phase) && now_ns() - t0 < 100000000ull) {
-      }
-    }
-  }
-}
-
-// Query tiles: one 128-row tile for a stream of a wide unit, one for both of a
-// narrow one, each a box of group x tokens_per_tile rows.
-template <int D> __device__ void query_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last) {
-  const int bytes = p.group * p.per_tile * 128 * (D / 64);
-  uint32_t phase = 0;
-  for (int i = first; i < last; ++i) {
-    const Unit u = read_unit(p, i);
-    if (!u.ntiles) continue;
-    if (!g.wait(sm.q_empty(), phase ^ 1, 5)) break;
-    phase ^= 1;
-    const int tiles = u.wide ? 2 : 1;
-    if (elected()) {
-      bar_expect(sm.q_full(), tiles * bytes);
-      for (int t = 0; t < tiles; ++t)
-#pragma unroll
-        for (int h = 0; h < D / 64; ++h)
-          load_box(sm.query(t) + h * (kTile * 128), &p.q, sm.q_full(), 64 * h, 0, u.kvh, u.tok0 + t * p.per_tile);
-    }
-    __syncwarp();
-  }
-  // the last load lands before the CTA ends, also when its users gave up
+  // copies in flight land before the CTA ends, also when their users gave up
   const uint64_t t0 = now_ns();
-  while (!bar_try(sm.q_full(), phase ^ 1) && now_ns() - t0 < 100000000ull) {
-  }
+  if (!alive)
+    for (int k = 0; k < S; ++k)
+      while ((issued >> k & 1) && !bar_try(sm.full(k), parity >> k & 1) && now_ns() - t0 < 100000000ull) {
+      }
+  if (VALUES)
+    while (!bar_try(sm.q_full(), q_phase ^ 1) && now_ns() - t0 < 100000000ull) {
+    }
 }
 
 // The products of stream t.  In a wide unit the streams issue in turn, so that
 // one's products run while the other's softmax does; left alone they fall into
-// step and wait for the exponentials and for the tensor cores together.  Both streams' warps walk the whole ring: a stage is
-// free when both have arrived, the one that uses it by the completion of its
-// products, the other at once.
+// step and wait for the exponentials and for the tensor cores together.  Both
+// streams' warps walk the whole ring: a stage is free when both have arrived, the
+// one that uses it by the completion of its products, the other at once.
 template <int D, bool BF16> __device__ void mma_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last, uint32_t tmem, int t) {
   const int lane = threadIdx.x % 32;
   constexpr uint32_t kQk = instruction<BF16>(kTile, false), kPv = instruction<BF16>(D, true);
@@ -601,12 +625,13 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
   uint32_t s_phase = 0, f_phase = 0;
   bool alive = true;
   // this stream's tile of queries: its first token in the unit, and its rows
-  const int row_token = row / p.group, row_head = row % p.group;
+  const int row_token = row / p.group, row_head = row % p.group, lane_token = lane / p.group;
   auto first_token = [&](const Unit &u) { return u.wide ? t * p.per_tile : 0; };
   auto stream_rows = [&](const Unit &u) { return min(u.ntok - first_token(u), p.per_tile) * p.group; };
   // the keys that this thread's row sees; rows after the last take its place
   auto seen_by_row = [&](const Unit &u, int &lo, int &hi) {
-    const int pos = u.pos0 + first_token(u) + min(row_token, min(u.ntok - first_token(u), p.per_tile) - 1);
+    const int token = spread(p, u) ? lane_token : row_token;
+    const int pos = u.pos0 + first_token(u) + min(token, min(u.ntok - first_token(u), p.per_tile) - 1);
     hi = p.causal ? min(u.kv_len, pos + 1) : u.kv_len;
     lo = p.window ? max(0, pos - p.window + 1) : 0;
   };
@@ -619,10 +644,11 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
   for (int i = first; i < last; ++i) {
     int step, key0, end;           // first key of a tile, and past the last
     int min_hi, max_lo;            // every row of the warp sees the keys between
-    bool warp_active;
+    bool warp_active, quarter;     // quarter: of the keys
     {
       const Unit u = read_unit(p, i);
-      warp_active = wid * 32 < stream_rows(u);
+      quarter = spread(p, u);
+      warp_active = quarter || wid * 32 < stream_rows(u);
       int lo, hi;
       seen_by_row(u, lo, hi);
       min_hi = __reduce_min_sync(~0u, hi);
@@ -633,10 +659,77 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
     }
     float m = kNoMax, l = 0.f;
     bool begun = false;
+    // the base follows the row's maximum when that grows by more than 2^8: the
+    // running sum and output (idle, the last product is complete) come down to it
+    auto rebase = [&](float best) {
+      const bool need = best > m + (kShift + kGrow);
+      if (!__any_sync(~0u, need)) return;
+      const float to = need ? best - kShift : m;
+      const float by = need ? exp2_approx(m - to) : 1.f;
+      m = to;
+      l *= by;
+      if (!begun) return;
+      const uint64_t by2 = pair(by, by);
+#pragma unroll 1
+      for (int k = 0; k < D; k += 16) {
+        uint32_t o[16];
+        tmem_ld16(o_at + k, o);
+        tmem_ld_wait(o);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          float e, f;
+          unpair(mul2(pair(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])), by2), e, f);
+          o[2 * q] = __float_as_uint(e);
+          o[2 * q + 1] = __float_as_uint(f);
+        }
+        tmem_st16(o_at + k, o);
+      }
+    };
     for (; key0 < end; key0 += step) {
       alive = alive && g.wait(sm.s_full(t), s_phase, 3);
       s_phase ^= 1;
-      if (warp_active && alive) {
+      if (quarter && alive) {
+        fence_after();
+        uint32_t s[32], w[16], none[16];
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tmem_ld32(s_at + 32 * wid, s);
+        tmem_ld_wait(s);
+        const int base = key0 + 32 * wid;
+        if (base < max_lo || base + 32 > min_hi) {
+          int lo, hi;
+          seen_by_row(read_unit(p, i), lo, hi);
+          const int from = lo - base;
+          const unsigned span = max(0, hi - lo);
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (unsigned(k - from) >= span) s[k] = __float_as_uint(-INFINITY);
+        }
+#pragma unroll
+        for (int k = 0; k < 32; k += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) top[q] = max3(__float_as_uint(top[q]), s[k + q], s[k + 4 + q]);
+        rebase(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
+        const uint64_t c2 = pair(c, c), base2 = pair(-m, -m);
+        uint64_t part[2] = {0, 0};
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          float e, f;
+          unpair(fma2(pair(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1])), c2, base2), e, f);
+          e = exp2_approx(e);
+          f = exp2_approx(f);
+          part[q % 2] = add2(part[q % 2], pair(e, f));
+          w[q] = pack16<BF16>(e, f);
+          none[q] = 0;
+        }
+#pragma unroll
+        for (int k = 1; k < 4; ++k) tmem_st16(s_at + 16 * (wid ^ k), none);
+        tmem_st16(s_at + 16 * wid, w);
+        weights_stored(0);
+        if (lane == 0) bar_arrive(sm.p_ready(t, 1));
+        float even, odd;
+        unpair(add2(part[0], part[1]), even, odd);
+        l += even + odd;
+      } else if (warp_active && alive) {
         fence_after();
         if (key0 < max_lo || key0 + kTile > min_hi) {
           // some row of the warp does not see the whole tile: the scores are
@@ -675,32 +768,7 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
         tmem_ld_wait(s, 64, 128);
         take_in(64);
         const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-        const bool need = best > m + (kShift + kGrow);
-        if (__any_sync(~0u, need)) {
-          // a new base: the running sum and output (idle, the last product is
-          // complete) come down to it
-          const float to = need ? best - kShift : m;
-          const float by = need ? exp2_approx(m - to) : 1.f;
-          m = to;
-          l *= by;
-          if (begun) {
-            const uint64_t by2 = pair(by, by);
-#pragma unroll 1
-            for (int k = 0; k < D; k += 16) {
-              uint32_t o[16];
-              tmem_ld16(o_at + k, o);
-              tmem_ld_wait(o);
-#pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                float e, f;
-                unpair(mul2(pair(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])), by2), e, f);
-                o[2 * q] = __float_as_uint(e);
-                o[2 * q + 1] = __float_as_uint(f);
-              }
-              tmem_st16(o_at + k, o);
-            }
-          }
-        }
+        rebase(best);
         const uint64_t c2 = pair(c, c);
         const uint64_t base2 = pair(-m, -m);
         uint64_t part[4] = {0, 0, 0, 0};
@@ -761,12 +829,80 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
     }
     if (t == 0 || u.wide) {
       fence_after();
-      const bool mine = row < rows && alive, split = u.nsplit > 1;
-      const int64_t out_token = u.tok0 + first_token(u) + row_token;
-      const int head = u.kvh * p.group + row_head;
-      const int64_t part = u.part_row + int64_t(u.split) * u.ntok * p.group + row0 + row;
-      const float inv = split ? 1.f : reciprocal(l);
-      if (warp_active && alive) {
+      const bool split = u.nsplit > 1;
+      const int64_t split_row = u.part_row + int64_t(u.split) * u.ntok * p.group + row0;
+      if (quarter) {
+        // the four warps' results come down to one base and meet in shared memory,
+        // 32 columns at a time: [warp][row][8 pieces of 16 bytes], the pieces of a
+        // row in an order of its own so that neither side meets in a bank
+        const uint32_t scratch = sm.query(1);
+        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(scratch + row * 8), "f"(m), "f"(l) : "memory");
+        group_sync(1, kTile);
+        float ms[4], ls[4], top = kNoMax, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ms[w]), "=f"(ls[w]) : "r"(scratch + (32 * w + lane) * 8) : "memory");
+          top = fmaxf(top, ms[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) total += exp2_approx(ms[w] - top) * ls[w];
+        const float scale = exp2_approx(m - top) * (split ? 1.f : reciprocal(total));
+        const uint64_t f0 = pair(by0 * scale, by0 * scale), f1 = pair(by1 * scale, by1 * scale);
+        group_sync(1, kTile);
+#pragma unroll 1
+        for (int k = 0; k < D; k += 32) {
+          uint32_t o[32], o1[32];
+          tmem_ld32(o_at + k, o);
+          if (joined) tmem_ld32(o_at + kTile + k, o1);
+          tmem_ld_wait(o);
+          tmem_ld_wait(o1);
+#pragma unroll
+          for (int q = 0; q < 32; q += 4) {
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+              uint64_t x = mul2(pair(__uint_as_float(o[q + r]), __uint_as_float(o[q + r + 1])), f0);
+              if (joined) x = fma2(pair(__uint_as_float(o1[q + r]), __uint_as_float(o1[q + r + 1])), f1, x);
+              unpair(x, v[r], v[r + 1]);
+            }
+            const uint32_t at = scratch + row * 128 + ((q / 4) ^ (lane & 7)) * 16;
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
+          }
+          group_sync(1, kTile);
+          for (int r = row / 8; r < rows; r += kTile / 8) {
+            const int piece = row % 8;
+            float sum[4] = {};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              float v[4];
+              const uint32_t at = scratch + (32 * w + r) * 128 + (piece ^ (r & 7)) * 16;
+              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(at) : "memory");
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sum[e] += v[e];
+            }
+            if (!alive) continue;
+            if (split) {
+              __stcg(reinterpret_cast<float4 *>(p.part_o + (split_row + r) * D + k) + piece, make_float4(sum[0], sum[1], sum[2], sum[3]));
+            } else {
+              uint16_t *to = static_cast<uint16_t *>(p.out) + int64_t(u.tok0 + r / p.group) * p.out_stride[0] +
+                             (u.kvh * p.group + r % p.group) * p.out_stride[1] + k;
+              reinterpret_cast<uint2 *>(to)[piece] = make_uint2(pack16<BF16>(sum[0], sum[1]), pack16<BF16>(sum[2], sum[3]));
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");    // queries may come here next
+          group_sync(1, kTile);
+        }
+        if (wid == 0 && lane < rows && alive) {
+          if (split)
+            __stcg(p.part_ml + split_row + lane, make_float2(top, total));
+          else if (p.lse)
+            p.lse[int64_t(u.tok0 + lane_token) * p.q_heads + u.kvh * p.group + lane - lane_token * p.group] = log_sum(top, total);
+        }
+      } else if (warp_active && alive) {
+        const bool mine = row < rows;
+        const int64_t out_token = u.tok0 + first_token(u) + row_token, part = split_row + row;
+        const int head = u.kvh * p.group + row_head;
+        const float inv = split ? 1.f : reciprocal(l);
         const uint64_t f0 = pair(by0 * inv, by0 * inv), f1 = pair(by1 * inv, by1 * inv);
         char *to = split ? reinterpret_cast<char *>(p.part_o + part * D)
                          : static_cast<char *>(p.out) + 2 * (out_token * p.out_stride[0] + head * p.out_stride[1]);
@@ -834,6 +970,7 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
       }
     }
     if (joined) group_sync(3, 256);       // stream 1's output and sums have been read
+    if (u.ntiles && threadIdx.x == 0) bar_arrive(sm.scratch_free());
   }
 }
 
@@ -849,6 +986,7 @@ template <int D, bool BF16> __global__ void __launch_bounds__(kThreads, 1) paged
     }
     bar_init(sm.q_full(), 1);
     bar_init(sm.q_empty(), 2);
+    bar_init(sm.scratch_free(), 1);
     for (int t = 0; t < 2; ++t) {
       bar_init(sm.s_full(t), 1);
       bar_init(sm.p_ready(t, 0), 4);
@@ -883,10 +1021,10 @@ template <int D, bool BF16> __global__ void __launch_bounds__(kThreads, 1) paged
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp >= kMmaWarp)
       mma_role<D, BF16>(p, sm, g, first, last, tmem, warp - kMmaWarp);
-    else if (warp == kLoadWarp)
-      load_role<D>(p, sm, g, first, last);
+    else if (warp == kKeyWarp)
+      load_role<D, false>(p, sm, g, first, last);
     else
-      query_role<D>(p, sm, g, first, last);
+      load_role<D, true>(p, sm, g, first, last);
   }
   __syncwarp();
   fence_before();
@@ -966,7 +1104,9 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
   const uint64_t q_dims[4] = {uint64_t(d), uint64_t(group), uint64_t(plan->kv_heads), uint64_t(plan->tokens)};
   const uint64_t q_steps[3] = {step(a->q_stride[1], plan->q_heads), group * step(a->q_stride[1], plan->q_heads), step(a->q_stride[0], plan->tokens)};
   const uint32_t q_box[4] = {64, uint32_t(group), 1, uint32_t(per_tile)};
+  const uint32_t q32_box[4] = {64, uint32_t(group), 1, uint32_t(group <= 32 ? 32 / group : 1)};
   if (int e = emmy_tensormap_encode(&p.q, a->dtype, 4, a->q, q_dims, q_steps, q_box, 3)) return e;
+  if (int e = emmy_tensormap_encode(&p.q32, a->dtype, 4, a->q, q_dims, q_steps, q32_box, 3)) return e;
   const uint64_t dims[4] = {uint64_t(d), uint64_t(ps), uint64_t(plan->kv_heads), uint64_t(a->pages)};
   const uint32_t kv_box[4] = {64, box, 1, 1};
   for (int i = 0; i < 2; ++i) {
@@ -990,7 +1130,7 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
   p.q_heads = plan->q_heads;
   p.group = group;
   p.per_tile = per_tile;
-  p.page_size = ps;
+  p.tiles_a_page = ps < kTile ? 1 : ps / kTile;
   p.box = box;
   p.aligned32 = (a->out % 32 == 0) && (rows[0] == 1 || a->out_stride[0] % 16 == 0) && (rows[1] == 1 || a->out_stride[1] % 16 == 0);
   p.causal = plan->causal;
