@@ -74,7 +74,7 @@ struct alignas(64) Params {
   void *out;
   float *lse;
   int64_t table_stride, out_stride[2];
-  int q_heads, group, per_tile, box, causal, window, aligned32;
+  int q_heads, group, group_inverse, per_tile, box, causal, window, aligned32;
   int tiles_a_page;                    // of pages of a tile or more
   float scale_log2;
 };
@@ -307,15 +307,18 @@ template <int D> struct Ring {
   }
 };
 
-// Read anew where it is used (from L1): a unit kept in registers across the
+// Read anew where it is used (from L1, which keeps it): a unit kept in registers across the
 // loop over its key tiles would cost the softmax warps 16 of them.
+// row / group of a tile's rows (both under 2^8) as a product
+__device__ __forceinline__ int token_of(const Params &p, int row) { return row * p.group_inverse >> 16; }
+
 __device__ __forceinline__ Unit read_unit(const Params &p, int i) {
   Unit u;
   const Unit *at = p.units + i;
-  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.seq), "=r"(u.kvh), "=r"(u.tok0), "=r"(u.ntok) : "l"(at));
-  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4+16];" : "=r"(u.pos0), "=r"(u.tile0), "=r"(u.ntiles), "=r"(u.lo) : "l"(at));
-  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4+32];" : "=r"(u.hi), "=r"(u.kv_len), "=r"(u.wide), "=r"(u.item) : "l"(at));
-  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4+48];" : "=r"(u.split), "=r"(u.nsplit), "=r"(u.part_row), "=r"(u.pad) : "l"(at));
+  asm volatile("ld.global.nc.L1::evict_last.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.seq), "=r"(u.kvh), "=r"(u.tok0), "=r"(u.ntok) : "l"(at));
+  asm volatile("ld.global.nc.L1::evict_last.v4.b32 {%0, %1, %2, %3}, [%4+16];" : "=r"(u.pos0), "=r"(u.tile0), "=r"(u.ntiles), "=r"(u.lo) : "l"(at));
+  asm volatile("ld.global.nc.L1::evict_last.v4.b32 {%0, %1, %2, %3}, [%4+32];" : "=r"(u.hi), "=r"(u.kv_len), "=r"(u.wide), "=r"(u.item) : "l"(at));
+  asm volatile("ld.global.nc.L1::evict_last.v4.b32 {%0, %1, %2, %3}, [%4+48];" : "=r"(u.split), "=r"(u.nsplit), "=r"(u.part_row), "=r"(u.pad) : "l"(at));
   return u;
 }
 
@@ -358,7 +361,7 @@ template <int D, bool VALUES> __device__ void load_role(const Params &p, const S
   const CUtensorMap *map = VALUES ? &p.v : &p.k;
   Ring<D> ring;
   uint32_t issued = 0, parity = 0;       // of each stage: the last copy into it
-  uint32_t q_phase = 0;
+  uint32_t q_phase = 0, queries_out = 1;      // out: the last load's phase of q_full
   bool alive = true, was_spread = false;
   for (int i = first; i < last && alive; ++i) {
     const Unit u = read_unit(p, i);
@@ -375,23 +378,35 @@ template <int D, bool VALUES> __device__ void load_role(const Params &p, const S
       return Box{wanted ? max(-1, __ldg(row + index)) : INT_MIN, boxes > 1 ? 0 : (tile - index * p.tiles_a_page) * kTile};
     };
     Box b0 = box_of(0), b1 = box_of(1), b2 = box_of(2);
-    if (VALUES) {
-      alive = g.wait(sm.q_empty(), q_phase ^ 1, 5);
-      // the unit before may still be joining its parts where the second tile goes
-      if (u.wide && was_spread) alive = alive && g.wait(sm.scratch_free(), q_phase ^ 1, 5);
-      if (!alive) break;
+    // The queries go when the last unit's have been used, values meanwhile: only a
+    // full ring waits for them.  After a spread unit the second tile has to wait
+    // until the parts joined in its place have been read.
+    bool queries_due = VALUES;
+    auto queries = [&](bool now) {
+      const bool second = u.wide && was_spread;
+      if (!now) {
+        const bool free = bar_try(sm.q_empty(), q_phase ^ 1) && (!second || bar_try(sm.scratch_free(), q_phase ^ 1));
+        if (!__all_sync(~0u, free)) return;
+      } else {
+        alive = g.wait(sm.q_empty(), q_phase ^ 1, 5) && (!second || g.wait(sm.scratch_free(), q_phase ^ 1, 5));
+        if (!alive) return;
+      }
       if (elected()) load_queries(p, sm, u);
       __syncwarp();
-      q_phase ^= 1;
-      was_spread = spread(p, u);
-    }
+      queries_due = false;
+      queries_out = q_phase;
+    };
     int at = 0;                            // places of the ring behind this unit's first
     for (int n = 0; n < u.ntiles; ++n) {
       const int place = VALUES ? n + min(u.ntiles, n + ahead) : n < ahead ? n : 2 * n - ahead + 1;
       ring.next(place - at);
       at = place;
       const Box b3 = box_of(n + 3);
-      alive = g.wait(sm.empty(ring.stage), ring.phase ^ 1, 1);
+      if (VALUES && queries_due) {
+        const bool room = bar_try(sm.empty(ring.stage), ring.phase ^ 1);
+        queries(!__all_sync(~0u, room));
+      }
+      alive = alive && g.wait(sm.empty(ring.stage), ring.phase ^ 1, 1);
       if (!alive) break;
       const bool wanted = b0.page != INT_MIN;
       const uint32_t bar = sm.full(ring.stage);
@@ -409,6 +424,11 @@ template <int D, bool VALUES> __device__ void load_role(const Params &p, const S
       b1 = b2;
       b2 = b3;
     }
+    if (VALUES) {
+      if (alive && queries_due) queries(true);
+      if (alive) q_phase ^= 1;
+      was_spread = spread(p, u);
+    }
     ring.next(2 * u.ntiles - at);
   }
   // copies in flight land before the CTA ends, also when their users gave up
@@ -418,7 +438,7 @@ template <int D, bool VALUES> __device__ void load_role(const Params &p, const S
       while ((issued >> k & 1) && !bar_try(sm.full(k), parity >> k & 1) && now_ns() - t0 < 100000000ull) {
       }
   if (VALUES)
-    while (!bar_try(sm.q_full(), q_phase ^ 1) && now_ns() - t0 < 100000000ull) {
+    while (!bar_try(sm.q_full(), queries_out) && now_ns() - t0 < 100000000ull) {
     }
 }
 
@@ -603,8 +623,8 @@ template <int D, bool BF16> __device__ void join_parts(const Params &p, const Un
       }
     }
     const float inv = reciprocal(total);
-    const int64_t token = u.tok0 + first_tok + r / p.group;
-    const int head = u.kvh * p.group + r % p.group;
+    const int64_t token = u.tok0 + first_tok + token_of(p, r);
+    const int head = u.kvh * p.group + r - token_of(p, r) * p.group;
     uint2 *dst = reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + token * p.out_stride[0] + head * p.out_stride[1]) + lane % 8;
 #pragma unroll
     for (int k = 0; k < kPieces; ++k)
@@ -625,7 +645,7 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
   uint32_t s_phase = 0, f_phase = 0;
   bool alive = true;
   // this stream's tile of queries: its first token in the unit, and its rows
-  const int row_token = row / p.group, row_head = row % p.group, lane_token = lane / p.group;
+  const int row_token = token_of(p, row), row_head = row - row_token * p.group, lane_token = token_of(p, lane);
   auto first_token = [&](const Unit &u) { return u.wide ? t * p.per_tile : 0; };
   auto stream_rows = [&](const Unit &u) { return min(u.ntok - first_token(u), p.per_tile) * p.group; };
   // the keys that this thread's row sees; rows after the last take its place
@@ -833,8 +853,9 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
       const int64_t split_row = u.part_row + int64_t(u.split) * u.ntok * p.group + row0;
       if (quarter) {
         // the four warps' results come down to one base and meet in shared memory,
-        // 32 columns at a time: [warp][row][8 pieces of 16 bytes], the pieces of a
-        // row in an order of its own so that neither side meets in a bank
+        // as many columns at a time as fit for 8, 16 or 32 rows:
+        // [warp][row][pieces of 16 bytes], the pieces of a row in an order of its
+        // own so that neither side meets in a bank
         const uint32_t scratch = sm.query(1);
         asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(scratch + row * 8), "f"(m), "f"(l) : "memory");
         group_sync(1, kTile);
@@ -849,49 +870,59 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
         const float scale = exp2_approx(m - top) * (split ? 1.f : reciprocal(total));
         const uint64_t f0 = pair(by0 * scale, by0 * scale), f1 = pair(by1 * scale, by1 * scale);
         group_sync(1, kTile);
+        const int fit = rows <= 8 ? 7 : rows <= 16 ? 6 : 5;           // log2 of the columns
+        const int shift = min(fit, D == 128 ? 7 : 6) - 2, pieces = 1 << shift;
+        const uint32_t mine = scratch + ((wid << (10 - fit)) + lane) * (pieces * 16);
 #pragma unroll 1
-        for (int k = 0; k < D; k += 32) {
-          uint32_t o[32], o1[32];
-          tmem_ld32(o_at + k, o);
-          if (joined) tmem_ld32(o_at + kTile + k, o1);
-          tmem_ld_wait(o);
-          tmem_ld_wait(o1);
+        for (int first_column = 0; first_column < D; first_column += 4 * pieces) {
+          if (first_column) group_sync(1, kTile);
+#pragma unroll 1
+          for (int k = 0; k < 4 * pieces; k += 32) {
+            uint32_t o[32], o1[32];
+            tmem_ld32(o_at + first_column + k, o);
+            if (joined) tmem_ld32(o_at + kTile + first_column + k, o1);
+            tmem_ld_wait(o);
+            tmem_ld_wait(o1);
+            if (lane < rows) {
 #pragma unroll
-          for (int q = 0; q < 32; q += 4) {
-            float v[4];
+              for (int q = 0; q < 32; q += 4) {
+                float v[4];
 #pragma unroll
-            for (int r = 0; r < 4; r += 2) {
-              uint64_t x = mul2(pair(__uint_as_float(o[q + r]), __uint_as_float(o[q + r + 1])), f0);
-              if (joined) x = fma2(pair(__uint_as_float(o1[q + r]), __uint_as_float(o1[q + r + 1])), f1, x);
-              unpair(x, v[r], v[r + 1]);
+                for (int r = 0; r < 4; r += 2) {
+                  uint64_t x = mul2(pair(__uint_as_float(o[q + r]), __uint_as_float(o[q + r + 1])), f0);
+                  if (joined) x = fma2(pair(__uint_as_float(o1[q + r]), __uint_as_float(o1[q + r + 1])), f1, x);
+                  unpair(x, v[r], v[r + 1]);
+                }
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((k + q) / 4 ^ (lane & 7)) * 16), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
+              }
             }
-            const uint32_t at = scratch + row * 128 + ((q / 4) ^ (lane & 7)) * 16;
-            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
+            __syncwarp();
           }
           group_sync(1, kTile);
-          for (int r = row / 8; r < rows; r += kTile / 8) {
-            const int piece = row % 8;
+          for (int item = row; item < rows << shift; item += kTile) {
+            const int r = item >> shift, piece = item & (pieces - 1);
             float sum[4] = {};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               float v[4];
-              const uint32_t at = scratch + (32 * w + r) * 128 + (piece ^ (r & 7)) * 16;
+              const uint32_t at = scratch + (((w << (10 - fit)) + r) * pieces + (piece ^ (r & 7))) * 16;
               asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(at) : "memory");
 #pragma unroll
               for (int e = 0; e < 4; ++e) sum[e] += v[e];
             }
             if (!alive) continue;
             if (split) {
-              __stcg(reinterpret_cast<float4 *>(p.part_o + (split_row + r) * D + k) + piece, make_float4(sum[0], sum[1], sum[2], sum[3]));
+              __stcg(reinterpret_cast<float4 *>(p.part_o + (split_row + r) * D + first_column) + piece, make_float4(sum[0], sum[1], sum[2], sum[3]));
             } else {
-              uint16_t *to = static_cast<uint16_t *>(p.out) + int64_t(u.tok0 + r / p.group) * p.out_stride[0] +
-                             (u.kvh * p.group + r % p.group) * p.out_stride[1] + k;
+              const int token = token_of(p, r);
+              uint16_t *to = static_cast<uint16_t *>(p.out) + int64_t(u.tok0 + token) * p.out_stride[0] +
+                             (u.kvh * p.group + r - token * p.group) * p.out_stride[1] + first_column;
               reinterpret_cast<uint2 *>(to)[piece] = make_uint2(pack16<BF16>(sum[0], sum[1]), pack16<BF16>(sum[2], sum[3]));
             }
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");    // queries may come here next
-          group_sync(1, kTile);
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");    // queries may come here next
+        group_sync(1, kTile);
         if (wid == 0 && lane < rows && alive) {
           if (split)
             __stcg(p.part_ml + split_row + lane, make_float2(top, total));
@@ -1129,6 +1160,7 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
   p.lse = reinterpret_cast<float *>(a->lse);
   p.q_heads = plan->q_heads;
   p.group = group;
+  p.group_inverse = (65536 + group - 1) / group;
   p.per_tile = per_tile;
   p.tiles_a_page = ps < kTile ? 1 : ps / kTile;
   p.box = box;
