@@ -24,9 +24,9 @@ namespace {
 
 // Costs in units of a quarter of a one-query-tile key tile; kWidePart is what a
 // part of a cut wide unit spends on its partial result.
-constexpr int64_t kNarrowTile = 4, kNarrowUnit = 4, kWideTile = 6, kWideUnit = 12, kWidePart = 20;
+constexpr int64_t kNarrowTile = 4, kNarrowUnit = 4, kWideTile = 6, kWideUnit = 20, kWidePart = 16;
 constexpr int kMinNarrow = 2;    // tiles: the two streams of a CTA take one each
-constexpr int kMinWide = 16;     // tiles: under this a split costs more than it gives
+constexpr int kMinWide = 4;      // tiles: under this a part is all overhead
 
 int fail(const char *fmt, long a = 0, long b = 0) {
   char buf[256];
@@ -125,10 +125,13 @@ void make(const emmy_paged_plan_args &a, emmy_paged_plan_s &plan) {
     Cut best = {wide.size(), 1};
     int64_t end = deal(best, false);
     // cutting costs the parts' way through the scratch: it has to gain 3 %
-    for (const size_t waves : {1, 2, 4})
-      for (int n = 2; n <= 16; n *= 2) {
-        const size_t cut_units = std::min(wide.size(), waves * a.ctas);
-        const Cut cut = {wide.size() - cut_units, n};
+    int64_t total = 0;
+    for (const Unit &u : wide) total += kWideUnit + kWideTile * u.ntiles;
+    const bool even = end * a.ctas * 100 <= total * 103;
+    const size_t ctas = a.ctas, all = wide.size();
+    for (const size_t last : {all % ctas, ctas, ctas + all % ctas, 2 * ctas})
+      for (int n = 2; n <= 16 && !even; n *= 2) {
+        const Cut cut = {all - std::min(all, last), n};
         const int64_t e = deal(cut, false);
         if (e * 103 < end * 100) {
           end = e;

@@ -302,7 +302,8 @@ template <typename T, int N, bool WITHIN> int launch(Params &p, cudaStream_t s) 
   int resident = sms * (kBlocks * kThreads / (p.lanes * rows * tokens)) / shares;
   if (resident < 1) resident = 1;
   const dim3 grid(want < resident ? want : resident, shares), block(p.lanes, rows, tokens);
-  // angles of two turns; vectors, slots and positions on their way (N > 1)
+  // angles of two turns; vectors, slots and positions on their way (N > 1): with
+  // 256 components and 384 threads 47 KiB, under the 48 that need no asking
   const size_t smem = size_t(tokens) * 2 * a.rotary_dim * sizeof(float) +
                       (N > 1 ? size_t(kAhead) * 2 * p.lanes * rows * tokens * (16 + 4) : 0);
   rotate_append_kernel<T, N, WITHIN><<<grid, block, smem, s>>>(p);
@@ -339,10 +340,10 @@ extern "C" EMMY_API int emmy_rotate_append(const emmy_rotate_append_args *a, voi
   if (!a) return fail("emmy_rotate_append: bad argument");
   if (a->dtype != 6 && a->dtype != 7 && a->dtype != 9)
     return fail("emmy_rotate_append: dtype %ld (f16, f32 or bf16)", a->dtype);
-  if (a->tokens < 0 || a->q_heads < 0 || a->kv_heads < 0 || a->q_heads > 1024 || a->kv_heads > 1024)
+  if (a->tokens < 0 || a->tokens > (1 << 30) || a->q_heads < 0 || a->kv_heads < 0 || a->q_heads > 1024 || a->kv_heads > 1024)
     return fail("emmy_rotate_append: bad count of tokens or heads");
-  if (a->head_dim < 1 || a->head_dim > 512)
-    return fail("emmy_rotate_append: head_dim %ld outside 1..512", a->head_dim);
+  if (a->head_dim < 1 || a->head_dim > 256)
+    return fail("emmy_rotate_append: head_dim %ld outside 1..256", a->head_dim);
   if (a->rotary_dim < 0 || a->rotary_dim > a->head_dim || a->rotary_dim % 2)
     return fail("emmy_rotate_append: rotary_dim %ld must be even and at most head_dim %ld", a->rotary_dim, a->head_dim);
   if (a->axes < 1 || a->axes > 16) return fail("emmy_rotate_append: %ld position axes (1..16)", a->axes);

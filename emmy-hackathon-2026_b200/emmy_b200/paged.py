@@ -89,6 +89,13 @@ def _call(name, device, stream, *args):
         native.check(rc)
 
 
+def _made_for(stream, device, t):
+    """A tensor allocated here and written on a given stream is not reused before that is through."""
+    if stream is not None:
+        t.record_stream(torch.cuda.ExternalStream(stream, device=device))
+    return t
+
+
 class Rotation:
     """Rotary positions: ``frequencies`` (float32, on the GPU) has the radians
     per position of each pair, so its length is half of the components that
@@ -149,7 +156,7 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
     if rotation.frequencies.device != device:
         raise ValueError("rotation: on another device")
     if q_out is None:
-        q_out = torch.empty((tokens, q_heads, dim), dtype=dtype, device=device)
+        q_out = _made_for(stream, device, torch.empty((tokens, q_heads, dim), dtype=dtype, device=device))
         q_out_stride = q_heads * dim, dim
     else:
         q_out_stride = _check("q_out", q_out, 3, dtype, device)[:2]
@@ -252,14 +259,14 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     if table.shape[0] != plan.sequences:
         raise ValueError(f"table: {plan.sequences} rows are wanted, not {table.shape[0]}")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = _made_for(stream, device, torch.empty(shape, dtype=dtype, device=device))
         out_stride = shape[1] * dim, dim
     else:
         out_stride = _check("out", out, 3, dtype, device)[:2]
         if out.shape != shape:
             raise ValueError("out: another shape than q")
     if lse is None:
-        lse = torch.empty(shape[:2], dtype=torch.float32, device=device)
+        lse = _made_for(stream, device, torch.empty(shape[:2], dtype=torch.float32, device=device))
     else:
         _check("lse", lse, 2, torch.float32, device)
         if lse.shape != shape[:2] or not lse.is_contiguous():

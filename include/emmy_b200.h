@@ -216,7 +216,7 @@ typedef struct {
   int32_t tokens;        /* may be 0: nothing is launched                       */
   int32_t q_heads;       /* may be 0: no queries                                */
   int32_t kv_heads;      /* may be 0: no keys or values                         */
-  int32_t head_dim;      /* 1..512                                              */
+  int32_t head_dim;      /* 1..256                                              */
   int32_t rotary_dim;    /* leading components that turn: even, 0..head_dim     */
   int32_t axes;          /* position axes, 1..16                                */
   int32_t interleaved;   /* pairs are (2i, 2i+1), else (i, i + rotary_dim/2)    */
