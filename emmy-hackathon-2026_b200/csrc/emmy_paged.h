@@ -36,6 +36,13 @@ struct Layout {
   int n_units = 0;
 };
 
+// The few rows of a unit are spread over a stream's warps (ntiles of the unit or
+// of any part of its item).
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline bool is_spread(int wide, int ntiles, int ntok, int group) { return !wide && ntiles && ntok * group <= 32; }
+
 }  // namespace emmy_paged
 
 struct emmy_paged_plan_s {
@@ -43,5 +50,6 @@ struct emmy_paged_plan_s {
   emmy_paged::Layout at;
   int64_t tokens = 0;
   int64_t part_rows = 0;
+  bool tiled = false, spread = false;      // some unit has whole query tiles, or rows for one warp
   int32_t sequences = 0, q_heads = 0, kv_heads = 0, head_dim = 0, causal = 0, window = 0, max_kv = 0;
 };

@@ -343,7 +343,7 @@ __device__ __forceinline__ Unit read_unit(const Params &p, int i) {
 // A unit of at most 32 rows: each warp of a stream has all of them and a quarter
 // of the keys.
 __device__ __forceinline__ bool spread(const Params &p, const Unit &u) {
-  return !u.wide && u.ntiles && u.ntok * p.group <= 32;
+  return emmy_paged::is_spread(u.wide, u.ntiles, u.ntok, p.group);
 }
 
 // Query tiles: one 128-row tile for each stream of a wide unit, one for both of
@@ -1036,6 +1036,9 @@ template <int D, bool BF16> __global__ void __launch_bounds__(kThreads, 1) paged
   Smem<D> sm;
   sm.base = (smem_addr(raw) + 1023) & ~1023u;
   const int warp = threadIdx.x / 32;
+  // the first unit is on its way while the CTA sets itself up
+  const int first = __ldg(p.cta_first + blockIdx.x), last = __ldg(p.cta_first + blockIdx.x + 1);
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(p.units + first));
   if (threadIdx.x == 0) {
     for (int s = 0; s < Shape<D>::kStages; ++s) {
       bar_init(sm.full(s), 1);
@@ -1064,7 +1067,6 @@ template <int D, bool BF16> __global__ void __launch_bounds__(kThreads, 1) paged
   fence_after();
   const uint32_t tmem = __reduce_or_sync(~0u, sm.words()[1]);
   const Guard g{sm.base + Shape<D>::kWords, p};
-  const int first = p.cta_first[blockIdx.x], last = p.cta_first[blockIdx.x + 1];
   if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     softmax_role<D, BF16>(p, sm, g, first, last, tmem);
@@ -1162,8 +1164,11 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
   const uint64_t q_steps[3] = {step(a->q_stride[1], plan->q_heads), group * step(a->q_stride[1], plan->q_heads), step(a->q_stride[0], plan->tokens)};
   const uint32_t q_box[4] = {64, uint32_t(group), 1, uint32_t(per_tile)};
   const uint32_t q32_box[4] = {64, uint32_t(group), 1, uint32_t(group <= 32 ? 32 / group : 1)};
-  if (int e = emmy_tensormap_encode(&p.q, a->dtype, 4, a->q, q_dims, q_steps, q_box, 3)) return e;
-  if (int e = emmy_tensormap_encode(&p.q32, a->dtype, 4, a->q, q_dims, q_steps, q32_box, 3)) return e;
+  // (each map costs the caller half a microsecond: only those that a unit uses)
+  if (plan->tiled)
+    if (int e = emmy_tensormap_encode(&p.q, a->dtype, 4, a->q, q_dims, q_steps, q_box, 3)) return e;
+  if (plan->spread)
+    if (int e = emmy_tensormap_encode(&p.q32, a->dtype, 4, a->q, q_dims, q_steps, q32_box, 3)) return e;
   const uint64_t dims[4] = {uint64_t(d), uint64_t(ps), uint64_t(plan->kv_heads), uint64_t(a->pages)};
   const uint32_t kv_box[4] = {64, box, 1, 1};
   for (int i = 0; i < 2; ++i) {

@@ -63,6 +63,9 @@ void make(const emmy_paged_plan_args &a, emmy_paged_plan_s &plan) {
           u.tile0 = u.lo / kTile;
           u.ntiles = (u.hi - 1) / kTile + 1 - u.tile0;
         }
+        const bool spread = emmy_paged::is_spread(u.wide, u.ntiles, u.ntok, group);
+        plan.spread = plan.spread || spread;
+        plan.tiled = plan.tiled || (u.ntiles && !spread);
         (u.wide ? wide : narrow).push_back(u);
       }
     first += n;

@@ -30,6 +30,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 
@@ -294,10 +295,16 @@ template <typename T, int N, bool WITHIN> int launch(Params &p, cudaStream_t s) 
   int tokens = kThreads / 2 / (p.lanes * rows);
   tokens = tokens < 1 ? 1 : tokens > 64 ? 64 : tokens;
   if (tokens > a.tokens) tokens = a.tokens;
-  int dev = 0, sms = 0;
+  static std::atomic<int> known[64];         // SMs of each device
+  int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return failed(e);
+  int sms = dev < 64 ? known[dev].load() : 0;
+  if (!sms) {
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return failed(e);
+    if (dev < 64) known[dev].store(sms);
+  }
   const int want = (a.tokens + tokens - 1) / tokens;
   int resident = sms * (kBlocks * kThreads / (p.lanes * rows * tokens)) / shares;
   if (resident < 1) resident = 1;

@@ -45,7 +45,9 @@ def _need(ok, text):
 
 
 def _check(name, t, ndim, dtype, device):
-    """A tensor of the cache operators: on the GPU, its innermost stride 1."""
+    """A tensor of the cache operators: on the GPU, its innermost stride 1.  The
+    operators look all of theirs over in one expression first (a call of 3 us on the
+    GPU would wait for the host otherwise) and come here for the reason."""
     if not isinstance(t, torch.Tensor) or t.ndim != ndim:
         raise ValueError(f"{name}: a tensor of {ndim} dimensions is wanted")
     if t.dtype is not dtype:
@@ -64,26 +66,19 @@ def _cuda_device(name, t):
     return t.device
 
 
-def _cache(k_cache, v_cache, dtype, device):
-    strides = _check("k_cache", k_cache, 4, dtype, device)[:3], _check("v_cache", v_cache, 4, dtype, device)[:3]
-    if k_cache.shape != v_cache.shape:
-        raise ValueError("k_cache and v_cache have different shapes")
-    return strides
-
-
 _fns = {}
 
 
-def _call(name, device, stream, *args):
-    """One C-ABI call with ``device`` current, on its current stream unless one is given."""
+def _call(name, index, stream, *args):
+    """One C-ABI call with device ``index`` current, on its current stream unless one is given."""
     fn = _fns.get(name)
     if fn is None:
         fn = _fns[name] = getattr(native.lib(), name)
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _call(name, device, stream, *args)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _call(name, index, stream, *args)
     if stream is None:
-        stream = torch._C._cuda_getCurrentRawStream(device.index)
+        stream = torch._C._cuda_getCurrentRawStream(index)
     rc = fn(*args, stream)
     if rc:
         native.check(rc)
@@ -119,6 +114,7 @@ class Rotation:
                 self.axes = max(axes) + 1
                 self.pair_axis = torch.tensor(axes, dtype=torch.int32, device=device)
         self.components = 2 * self.frequencies.shape[0]
+        self.device_index = device.index
         self.pair_axis_ptr = 0 if self.pair_axis is None else self.pair_axis.data_ptr()
 
 
@@ -136,38 +132,49 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
     dtype = q.dtype
     if dtype not in _DTYPES:
         raise ValueError(f"q: bfloat16, float16 or float32 is wanted, not {dtype}")
-    q_stride = _check("q", q, 3, dtype, device)
-    k_stride = _check("k", k, 3, dtype, device)
-    v_stride = _check("v", v, 3, dtype, device)
-    k_cache_stride, v_cache_stride = _cache(k_cache, v_cache, dtype, device)
-    tokens, q_heads, dim = q.shape
-    pages, page_size, kv_heads, cache_dim = k_cache.shape
-    if k.shape != (tokens, kv_heads, dim) or v.shape != k.shape or cache_dim != dim:
-        raise ValueError("q, k, v and the caches do not fit together")
     if positions.ndim == 1:
         positions = positions[None]
-    positions_stride = _check("positions", positions, 2, torch.int32, device)[0]
-    axes = positions.shape[0]
-    if positions.shape[1] != tokens or axes < rotation.axes:
+    strides = q.stride(), k.stride(), v.stride(), k_cache.stride(), v_cache.stride(), positions.stride(), slots.stride()
+    at = q.get_device()
+    if ([len(x) for x in strides] != [3, 3, 3, 4, 4, 2, 1] or any(x[-1] != 1 for x in strides)
+            or not (dtype is k.dtype is v.dtype is k_cache.dtype is v_cache.dtype)
+            or not (positions.dtype is slots.dtype is torch.int32)
+            or not (at == k.get_device() == v.get_device() == k_cache.get_device() == v_cache.get_device()
+                    == positions.get_device() == slots.get_device())):
+        for name, t, ndim, kind in (("q", q, 3, dtype), ("k", k, 3, dtype), ("v", v, 3, dtype), ("k_cache", k_cache, 4, dtype),
+                                    ("v_cache", v_cache, 4, dtype), ("positions", positions, 2, torch.int32),
+                                    ("slots", slots, 1, torch.int32)):
+            _check(name, t, ndim, kind, device)
+    q_stride, k_stride, v_stride, k_cache_stride, v_cache_stride, positions_stride, _ = strides
+    shape = q.shape
+    tokens, q_heads, dim = shape
+    cache_shape = k_cache.shape
+    pages, page_size, kv_heads, cache_dim = cache_shape
+    if v_cache.shape != cache_shape:
+        raise ValueError("k_cache and v_cache have different shapes")
+    if k.shape != (tokens, kv_heads, dim) or v.shape != k.shape or cache_dim != dim:
+        raise ValueError("q, k, v and the caches do not fit together")
+    axes, n = positions.shape
+    if n != tokens or axes < rotation.axes:
         raise ValueError(f"positions: [{rotation.axes}, {tokens}] is wanted, not {list(positions.shape)}")
-    _check("slots", slots, 1, torch.int32, device)
     if slots.shape[0] != tokens:
         raise ValueError(f"slots: {tokens} are wanted, not {slots.shape[0]}")
-    if rotation.frequencies.device != device:
+    if rotation.device_index != at:
         raise ValueError("rotation: on another device")
     if q_out is None:
-        q_out = _made_for(stream, device, torch.empty((tokens, q_heads, dim), dtype=dtype, device=device))
+        q_out = _made_for(stream, device, torch.empty_like(q, memory_format=torch.contiguous_format))
         q_out_stride = q_heads * dim, dim
     else:
         q_out_stride = _check("q_out", q_out, 3, dtype, device)[:2]
-        if q_out.shape != q.shape:
+        if q_out.shape != shape:
             raise ValueError("q_out: another shape than q")
     a = _ROTATE_APPEND_ARGS.pack(
         _DTYPES[dtype], tokens, q_heads, kv_heads, dim, rotation.components, axes, rotation.interleaved, pages, page_size,
         q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
         positions.data_ptr(), slots.data_ptr(), rotation.frequencies.data_ptr(), rotation.pair_axis_ptr,
-        *q_stride[:2], *k_stride[:2], *v_stride[:2], *q_out_stride, *k_cache_stride, *v_cache_stride, positions_stride)
-    _call("emmy_rotate_append", device, stream, a)
+        *q_stride[:2], *k_stride[:2], *v_stride[:2], *q_out_stride, *k_cache_stride[:3], *v_cache_stride[:3],
+        positions_stride[0])
+    _call("emmy_rotate_append", at, stream, a)
     return q_out
 
 
@@ -214,6 +221,8 @@ class AttentionPlan:
         self.device, self.tokens, self.sequences = device, sum(q_lens), n
         self.q_heads, self.kv_heads, self.head_dim = int(q_heads), int(kv_heads), int(head_dim)
         self.shape = (self.tokens, self.q_heads, self.head_dim)
+        self.scale = self.head_dim ** -0.5
+        self.words_ptr, self.scratch_ptr = self.words.data_ptr(), self.scratch.data_ptr()
 
     def __del__(self):
         if self._h is not None:
@@ -224,7 +233,7 @@ class AttentionPlan:
 
     def check(self, stream=None):
         """Waits for the calls so far and raises if one of them gave up."""
-        _call("emmy_paged_plan_status", self.device, stream, self._h, self.words.data_ptr())
+        _call("emmy_paged_plan_status", self.device.index, stream, self._h, self.words.data_ptr())
 
 
 def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, stream=None):
@@ -245,36 +254,46 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     dtype = q.dtype
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError(f"q: bfloat16 or float16 is wanted, not {dtype}")
-    q_stride = _check("q", q, 3, dtype, device)
-    if device != plan.device:
+    strides = q.stride(), k_cache.stride(), v_cache.stride(), table.stride()
+    at = q.get_device()
+    if ([len(x) for x in strides] != [3, 4, 4, 2] or any(x[-1] != 1 for x in strides)
+            or not (dtype is k_cache.dtype is v_cache.dtype) or table.dtype is not torch.int32
+            or not (at == k_cache.get_device() == v_cache.get_device() == table.get_device())):
+        for name, t, ndim, kind in (("q", q, 3, dtype), ("k_cache", k_cache, 4, dtype), ("v_cache", v_cache, 4, dtype),
+                                    ("table", table, 2, torch.int32)):
+            _check(name, t, ndim, kind, device)
+    q_stride, k_cache_stride, v_cache_stride, table_stride = strides
+    if at != plan.device.index:
         raise ValueError(f"q: on {device}, the plan on {plan.device}")
     shape = plan.shape
     if q.shape != shape:
         raise ValueError(f"q: the plan is for {list(shape)}, not {list(q.shape)}")
-    k_cache_stride, v_cache_stride = _cache(k_cache, v_cache, dtype, device)
-    pages, page_size, kv_heads, dim = k_cache.shape
+    cache_shape = k_cache.shape
+    if v_cache.shape != cache_shape:
+        raise ValueError("k_cache and v_cache have different shapes")
+    pages, page_size, kv_heads, dim = cache_shape
     if kv_heads != plan.kv_heads or dim != plan.head_dim:
         raise ValueError(f"k_cache: the plan is for {plan.kv_heads} heads of {plan.head_dim}, not {kv_heads} of {dim}")
-    table_stride = _check("table", table, 2, torch.int32, device)[0]
-    if table.shape[0] != plan.sequences:
-        raise ValueError(f"table: {plan.sequences} rows are wanted, not {table.shape[0]}")
+    rows, width = table.shape
+    if rows != plan.sequences:
+        raise ValueError(f"table: {plan.sequences} rows are wanted, not {rows}")
     if out is None:
-        out = _made_for(stream, device, torch.empty(shape, dtype=dtype, device=device))
+        out = _made_for(stream, device, torch.empty_like(q, memory_format=torch.contiguous_format))
         out_stride = shape[1] * dim, dim
     else:
         out_stride = _check("out", out, 3, dtype, device)[:2]
         if out.shape != shape:
             raise ValueError("out: another shape than q")
     if lse is None:
-        lse = _made_for(stream, device, torch.empty(shape[:2], dtype=torch.float32, device=device))
+        lse = _made_for(stream, device, q.new_empty(shape[:2], dtype=torch.float32))
     else:
         _check("lse", lse, 2, torch.float32, device)
         if lse.shape != shape[:2] or not lse.is_contiguous():
             raise ValueError(f"lse: contiguous {list(shape[:2])} is wanted")
     a = _ATTENTION_ARGS.pack(
-        _DTYPES[dtype], pages, page_size, table.shape[1], plan.head_dim ** -0.5 if scale is None else scale,
+        _DTYPES[dtype], pages, page_size, width, plan.scale if scale is None else scale,
         q.data_ptr(), out.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
-        plan.words.data_ptr(), plan.scratch.data_ptr(), *q_stride[:2], *out_stride, *k_cache_stride, *v_cache_stride,
-        table_stride)
-    _call("emmy_paged_attention", device, stream, plan._h, a)
+        plan.words_ptr, plan.scratch_ptr, *q_stride[:2], *out_stride, *k_cache_stride[:3], *v_cache_stride[:3],
+        table_stride[0])
+    _call("emmy_paged_attention", at, stream, plan._h, a)
     return out, lse
