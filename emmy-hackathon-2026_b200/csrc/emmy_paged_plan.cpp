@@ -22,9 +22,13 @@ using emmy_paged::Unit;
 
 namespace {
 
-// Costs in units of a quarter of a one-query-tile key tile; kWidePart is what a
-// part of a cut wide unit spends on its partial result.
-constexpr int64_t kNarrowTile = 4, kNarrowUnit = 4, kWideTile = 6, kWideUnit = 20, kWidePart = 16;
+// What work costs, in quarters of the time of a key tile of one query tile (0.73
+// us with 64 components, 1.37 with 128, bound by memory): measured on calls of
+// 148 equal units of 64 to 256 tiles, and of 8 x 148 units of 8.  A wide tile is
+// bound by its softmax, the same for either; a unit's end drains and joins its
+// streams; a part of a cut wide unit goes through the scratch besides.
+struct Cost { int64_t narrow_tile, narrow_unit, wide_tile, wide_unit, wide_part; };
+constexpr Cost kCost64 = {4, 18, 7, 25, 22}, kCost128 = {4, 6, 4, 16, 12};
 constexpr int kMinNarrow = 2;    // tiles: the two streams of a CTA take one each
 constexpr int kMinWide = 4;      // tiles: under this a part is all overhead
 
@@ -38,6 +42,7 @@ int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 void make(const emmy_paged_plan_args &a, emmy_paged_plan_s &plan) {
   const int group = a.q_heads / a.kv_heads, per_tile = kTile / group;
+  const Cost cost = a.head_dim == 64 ? kCost64 : kCost128;
   std::vector<Unit> wide, narrow;     // one unit an item, to be cut below
   int64_t first = 0;
   for (int s = 0; s < a.sequences; ++s) {
@@ -111,7 +116,7 @@ void make(const emmy_paged_plan_args &a, emmy_paged_plan_s &plan) {
         const int b = part(wide[i], k, n), e = part(wide[i], k + 1, n);
         Slot s = least.top();
         least.pop();
-        s.first += kWideUnit + kWideTile * (e - b) + (n > 1 ? kWidePart : 0);
+        s.first += cost.wide_unit + cost.wide_tile * (e - b) + (n > 1 ? cost.wide_part : 0);
         end = std::max(end, s.first);
         least.push(s);
         if (!keep) continue;
@@ -129,7 +134,7 @@ void make(const emmy_paged_plan_args &a, emmy_paged_plan_s &plan) {
     int64_t end = deal(best, false);
     // cutting costs the parts' way through the scratch: it has to gain 3 %
     int64_t total = 0;
-    for (const Unit &u : wide) total += kWideUnit + kWideTile * u.ntiles;
+    for (const Unit &u : wide) total += cost.wide_unit + cost.wide_tile * u.ntiles;
     const bool even = end * a.ctas * 100 <= total * 103;
     const size_t ctas = a.ctas, all = wide.size();
     for (const size_t last : {all % ctas, ctas, ctas + all % ctas, 2 * ctas})
@@ -155,27 +160,27 @@ void make(const emmy_paged_plan_args &a, emmy_paged_plan_s &plan) {
       int b = 0;
       do {
         const int rest = narrow[i].ntiles - b, least_take = std::min(kMinNarrow, std::max(1, rest));
-        int64_t room = (level - filled - kNarrowUnit) / kNarrowTile;
+        int64_t room = (level - filled - cost.narrow_unit) / cost.narrow_tile;
         while (room < least_take) {
           if (++c == a.ctas) return false;
           filled = load[c];
-          room = (level - filled - kNarrowUnit) / kNarrowTile;
+          room = (level - filled - cost.narrow_unit) / cost.narrow_tile;
         }
         // a rest too small to be a piece of its own goes along
         const int take = rest - room >= kMinNarrow ? static_cast<int>(room) : rest;
         pieces.push_back({static_cast<int>(i), c, b, b + take});
-        filled += kNarrowUnit + kNarrowTile * take;
+        filled += cost.narrow_unit + cost.narrow_tile * take;
         b += take;
       } while (b < narrow[i].ntiles);
     }
     return true;
   };
   if (!narrow.empty()) {
-    int64_t high = kNarrowUnit + kNarrowTile * kMinNarrow;
+    int64_t high = cost.narrow_unit + cost.narrow_tile * kMinNarrow;
     for (const int64_t l : load) high = std::max(high, l);
     int64_t low = high;             // no CTA may stay under the level of the smallest piece
     for (const int64_t l : load) low = std::min(low, l);
-    low = std::max(low, kNarrowUnit + kNarrowTile * kMinNarrow - 1);
+    low = std::max(low, cost.narrow_unit + cost.narrow_tile * kMinNarrow - 1);
     while (!pour(high)) {
       low = high;
       high *= 2;
