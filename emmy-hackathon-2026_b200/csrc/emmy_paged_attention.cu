@@ -112,6 +112,18 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok;
 }
+// the same without the pause that a failed try takes
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
 __device__ __forceinline__ uint64_t now_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -290,7 +302,7 @@ template <bool BF16> __host__ __device__ constexpr uint32_t instruction(int n, b
 }
 
 // ---------------------------------------------------------------- roles
-template <int D> struct Smem {
+template <int D, bool SPREAD> struct Smem {
   uint32_t base;       // 1024-byte aligned
   __device__ uint32_t query(int t) const { return base + t * Shape<D>::kTileBytes; }
   __device__ uint32_t stage(int s) const { return base + Shape<D>::kRing + s * Shape<D>::kTileBytes; }
@@ -341,16 +353,20 @@ __device__ __forceinline__ Unit read_unit(const Params &p, int i) {
 }
 
 // A unit of at most 32 rows: each warp of a stream has all of them and a quarter
-// of the keys.
-__device__ __forceinline__ bool spread(const Params &p, const Unit &u) {
-  return emmy_paged::is_spread(u.wide, u.ntiles, u.ntok, p.group);
+// of the keys.  A plan without such units runs a kernel without their code
+// (!SPREAD), which in the wide units' kernel costs them 3 to 4 % though they never
+// come to it: 1,030 against 1,005 us on 8 prompts of 4,096, 165 against 158 on the
+// windowed chunks.
+template <int D, bool SPREAD> __device__ __forceinline__ bool spread(const Params &p, const Smem<D, SPREAD> &, const Unit &u) {
+  return SPREAD && emmy_paged::is_spread(u.wide, u.ntiles, u.ntok, p.group);
 }
 
 // Query tiles: one 128-row tile for each stream of a wide unit, one for both of
 // a narrow one, each a box of group x tokens_per_tile rows; the rows of a spread
 // unit four times.
-template <int D> __device__ __forceinline__ void load_queries(const Params &p, const Smem<D> &sm, const Unit &u) {
-  if (spread(p, u)) {
+template <int D, bool SPREAD>
+__device__ __forceinline__ void load_queries(const Params &p, const Smem<D, SPREAD> &sm, const Unit &u) {
+  if (spread(p, sm, u)) {
     bar_expect(sm.q_full(), 4 * p.group * (32 / p.group) * 128 * (D / 64));
     for (int w = 0; w < 4; ++w)
 #pragma unroll
@@ -373,7 +389,8 @@ template <int D> __device__ __forceinline__ void load_queries(const Params &p, c
 // the first keys (one tile, or one for each stream), then values of tile n and
 // keys of tile n + ahead.  One warp for both took 2,400 cycles a tile pair, more
 // than a pair of 64-component heads takes to arrive.
-template <int D, bool VALUES> __device__ void load_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last) {
+template <bool VALUES, int D, bool SPREAD>
+__device__ void load_role(const Params &p, const Smem<D, SPREAD> &sm, const Guard &g, int first, int last) {
   constexpr int S = Shape<D>::kStages;
   const int lane = threadIdx.x % 32, boxes = kTile / p.box;
   const CUtensorMap *map = VALUES ? &p.v : &p.k;
@@ -403,7 +420,7 @@ template <int D, bool VALUES> __device__ void load_role(const Params &p, const S
     auto queries = [&](bool now) {
       const bool second = u.wide && was_spread;
       if (!now) {
-        const bool free = bar_try(sm.q_empty(), q_phase ^ 1) && (!second || bar_try(sm.scratch_free(), q_phase ^ 1));
+        const bool free = bar_test(sm.q_empty(), q_phase ^ 1) && (!second || bar_test(sm.scratch_free(), q_phase ^ 1));
         if (!__all_sync(~0u, free)) return;
       } else {
         alive = g.wait(sm.q_empty(), q_phase ^ 1, 5) && (!second || g.wait(sm.scratch_free(), q_phase ^ 1, 5));
@@ -421,8 +438,13 @@ template <int D, bool VALUES> __device__ void load_role(const Params &p, const S
       at = place;
       const Box b3 = box_of(n + 3);
       if (VALUES && queries_due) {
-        const bool room = bar_try(sm.empty(ring.stage), ring.phase ^ 1);
-        queries(!__all_sync(~0u, room));
+        // whichever comes first: the queries' place or this tile's
+        const uint64_t t0 = now_ns();
+        for (;;) {
+          queries(false);
+          const bool room = bar_test(sm.empty(ring.stage), ring.phase ^ 1);
+          if (!queries_due || __any_sync(~0u, room || now_ns() - t0 > 1000000000ull)) break;
+        }
       }
       alive = alive && g.wait(sm.empty(ring.stage), ring.phase ^ 1, 1);
       if (!alive) break;
@@ -445,7 +467,7 @@ template <int D, bool VALUES> __device__ void load_role(const Params &p, const S
     if (VALUES) {
       if (alive && queries_due) queries(true);
       if (alive) q_phase ^= 1;
-      was_spread = spread(p, u);
+      was_spread = spread(p, sm, u);
     }
     ring.next(2 * u.ntiles - at);
   }
@@ -465,7 +487,8 @@ template <int D, bool VALUES> __device__ void load_role(const Params &p, const S
 // step and wait for the exponentials and for the tensor cores together.  Both
 // streams' warps walk the whole ring: a stage is free when both have arrived, the
 // one that uses it by the completion of its products, the other at once.
-template <int D, bool BF16> __device__ void mma_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last, uint32_t tmem, int t) {
+template <bool BF16, int D, bool SPREAD>
+__device__ void mma_role(const Params &p, const Smem<D, SPREAD> &sm, const Guard &g, int first, int last, uint32_t tmem, int t) {
   const int lane = threadIdx.x % 32;
   constexpr uint32_t kQk = instruction<BF16>(kTile, false), kPv = instruction<BF16>(D, true);
   const uint32_t s_at = tmem + kTile * t, o_at = tmem + 2 * kTile + kTile * t;
@@ -651,11 +674,15 @@ template <int D, bool BF16> __device__ void join_parts(const Params &p, const Un
   }
 }
 
-template <int D, bool BF16> __device__ void softmax_role(const Params &p, const Smem<D> &sm, const Guard &g, int first, int last, uint32_t tmem) {
+template <bool BF16, int D, bool SPREAD>
+__device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const Guard &g, int first, int last, uint32_t tmem) {
   // exponents may run 8 over the base before it moves; 16-bit floats of 5
   // exponent bits get a base 6 lower, so that small weights keep their bits
   constexpr float kShift = BF16 ? 0.f : 6.f, kGrow = 8.f;
-  constexpr int kPolyEvery = 4;       // every fourth pair's exponentials off the exponential unit
+  // every fourth pair's exponentials off the exponential unit, with 64 components:
+  // a tile pair 2,885 -> 2,605 cycles.  With 128 the tensor cores set the power, the
+  // cycles saved (3,030 -> 2,820) come back as a lower clock, and nothing is gained
+  constexpr int kPolyEvery = D == 64 ? 4 : kTile;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, t = warp / 4, wid = warp % 4;
   const int row = threadIdx.x % kTile;
   const uint32_t lanes = tmem + (uint32_t(wid * 32) << 16);
@@ -669,7 +696,7 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
   auto stream_rows = [&](const Unit &u) { return min(u.ntok - first_token(u), p.per_tile) * p.group; };
   // the keys that this thread's row sees; rows after the last take its place
   auto seen_by_row = [&](const Unit &u, int &lo, int &hi) {
-    const int token = spread(p, u) ? lane_token : row_token;
+    const int token = spread(p, sm, u) ? lane_token : row_token;
     const int pos = u.pos0 + first_token(u) + min(token, min(u.ntok - first_token(u), p.per_tile) - 1);
     hi = p.causal ? min(u.kv_len, pos + 1) : u.kv_len;
     lo = p.window ? max(0, pos - p.window + 1) : 0;
@@ -686,7 +713,7 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
     bool warp_active, quarter;     // quarter: of the keys
     {
       const Unit u = read_unit(p, i);
-      quarter = spread(p, u);
+      quarter = spread(p, sm, u);
       warp_active = quarter || wid * 32 < stream_rows(u);
       int lo, hi;
       seen_by_row(u, lo, hi);
@@ -1031,9 +1058,10 @@ template <int D, bool BF16> __device__ void softmax_role(const Params &p, const 
   }
 }
 
-template <int D, bool BF16> __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __grid_constant__ Params p) {
+template <int D, bool BF16, bool SPREAD>
+__global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __grid_constant__ Params p) {
   extern __shared__ char raw[];
-  Smem<D> sm;
+  Smem<D, SPREAD> sm;
   sm.base = (smem_addr(raw) + 1023) & ~1023u;
   const int warp = threadIdx.x / 32;
   // the first unit is on its way while the CTA sets itself up
@@ -1069,7 +1097,7 @@ template <int D, bool BF16> __global__ void __launch_bounds__(kThreads, 1) paged
   const Guard g{sm.base + Shape<D>::kWords, p};
   if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    softmax_role<D, BF16>(p, sm, g, first, last, tmem);
+    softmax_role<BF16>(p, sm, g, first, last, tmem);
     // an end of their own: code shared with the other warps would have to do
     // with their registers
     __syncwarp();
@@ -1079,11 +1107,11 @@ template <int D, bool BF16> __global__ void __launch_bounds__(kThreads, 1) paged
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp >= kMmaWarp)
-      mma_role<D, BF16>(p, sm, g, first, last, tmem, warp - kMmaWarp);
+      mma_role<BF16>(p, sm, g, first, last, tmem, warp - kMmaWarp);
     else if (warp == kKeyWarp)
-      load_role<D, false>(p, sm, g, first, last);
+      load_role<false>(p, sm, g, first, last);
     else
-      load_role<D, true>(p, sm, g, first, last);
+      load_role<true>(p, sm, g, first, last);
   }
   __syncwarp();
   fence_before();
@@ -1110,22 +1138,22 @@ int cuda_fail(const char *what, cudaError_t e) {
 uint64_t step(int64_t stride, int64_t extent) { return extent == 1 ? 16 : static_cast<uint64_t>(stride) * 2; }
 bool bad_stride(int64_t stride, int64_t extent) { return extent != 1 && (stride <= 0 || stride % 8 || stride >= (int64_t(1) << 38)); }
 
-template <int D, bool BF16> int launch(const Params &p, int ctas, cudaStream_t s) {
+template <int D, bool BF16, bool SPREAD> int launch(const Params &p, int ctas, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};     // a bit for each device
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return cuda_fail("emmy_paged_attention: cudaGetDevice", e);
   const uint64_t bit = uint64_t(1) << (dev & 63);
   if (dev > 63 || !(ready.load() & bit)) {
-    if (cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem))
+    if (cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<D, BF16, SPREAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem))
       return cuda_fail("emmy_paged_attention: shared memory", e);
     // the softmax warps wait for the registers of the split: they must exist
     cudaFuncAttributes attr;
-    if (cudaError_t e = cudaFuncGetAttributes(&attr, paged_attention_kernel<D, BF16>))
+    if (cudaError_t e = cudaFuncGetAttributes(&attr, paged_attention_kernel<D, BF16, SPREAD>))
       return cuda_fail("emmy_paged_attention: attributes", e);
     if (attr.numRegs != kLaunchRegs) return fail("emmy_paged_attention: built with %ld registers, not %ld", attr.numRegs, kLaunchRegs);
     if (dev <= 63) ready.fetch_or(bit);
   }
-  paged_attention_kernel<D, BF16><<<ctas, kThreads, kSmem, s>>>(p);
+  paged_attention_kernel<D, BF16, SPREAD><<<ctas, kThreads, kSmem, s>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : cuda_fail("emmy_paged_attention: launch", e);
 }
@@ -1201,8 +1229,12 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
   p.scale_log2 = a->scale * kLog2e;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int n = plan->at.ctas;
-  if (d == 128) return a->dtype == 9 ? launch<128, true>(p, n, s) : launch<128, false>(p, n, s);
-  return a->dtype == 9 ? launch<64, true>(p, n, s) : launch<64, false>(p, n, s);
+  if (plan->spread) {
+    if (d == 128) return a->dtype == 9 ? launch<128, true, true>(p, n, s) : launch<128, false, true>(p, n, s);
+    return a->dtype == 9 ? launch<64, true, true>(p, n, s) : launch<64, false, true>(p, n, s);
+  }
+  if (d == 128) return a->dtype == 9 ? launch<128, true, false>(p, n, s) : launch<128, false, false>(p, n, s);
+  return a->dtype == 9 ? launch<64, true, false>(p, n, s) : launch<64, false, false>(p, n, s);
 }
 
 extern "C" EMMY_API int emmy_paged_plan_status(emmy_paged_plan_t plan, uint64_t plan_words, void *stream) {
