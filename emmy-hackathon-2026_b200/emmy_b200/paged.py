@@ -84,11 +84,9 @@ def _call(name, index, stream, *args):
         native.check(rc)
 
 
-def _made_for(stream, device, t):
+def _made_for(stream, t):
     """A tensor allocated here and written on a given stream is not reused before that is through."""
-    if stream is not None:
-        t.record_stream(torch.cuda.ExternalStream(stream, device=device))
-    return t
+    t.record_stream(torch.cuda.ExternalStream(stream, device=t.device))
 
 
 class Rotation:
@@ -128,15 +126,19 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
     of page ``s // page_size``; a slot outside the cache (-1, say) stores
     nothing.  ``q_out`` may be ``q`` itself.  Rotates in 32 bits, with angles
     formed in 64, and rounds once."""
-    device = _cuda_device("q", q)
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise ValueError("q: a CUDA tensor is wanted")
     dtype = q.dtype
     if dtype not in _DTYPES:
         raise ValueError(f"q: bfloat16, float16 or float32 is wanted, not {dtype}")
     if positions.ndim == 1:
         positions = positions[None]
-    strides = q.stride(), k.stride(), v.stride(), k_cache.stride(), v_cache.stride(), positions.stride(), slots.stride()
     at = q.get_device()
-    if ([len(x) for x in strides] != [3, 3, 3, 4, 4, 2, 1] or any(x[-1] != 1 for x in strides)
+    q_stride, k_stride, v_stride = q.stride(), k.stride(), v.stride()
+    k_cache_stride, v_cache_stride, positions_stride, slots_stride = k_cache.stride(), v_cache.stride(), positions.stride(), slots.stride()
+    if (len(q_stride) != 3 or len(k_stride) != 3 or len(v_stride) != 3 or len(k_cache_stride) != 4 or len(v_cache_stride) != 4
+            or len(positions_stride) != 2 or slots_stride != (1,)
+            or not (q_stride[2] == k_stride[2] == v_stride[2] == k_cache_stride[3] == v_cache_stride[3] == positions_stride[1] == 1)
             or not (dtype is k.dtype is v.dtype is k_cache.dtype is v_cache.dtype)
             or not (positions.dtype is slots.dtype is torch.int32)
             or not (at == k.get_device() == v.get_device() == k_cache.get_device() == v_cache.get_device()
@@ -144,8 +146,7 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
         for name, t, ndim, kind in (("q", q, 3, dtype), ("k", k, 3, dtype), ("v", v, 3, dtype), ("k_cache", k_cache, 4, dtype),
                                     ("v_cache", v_cache, 4, dtype), ("positions", positions, 2, torch.int32),
                                     ("slots", slots, 1, torch.int32)):
-            _check(name, t, ndim, kind, device)
-    q_stride, k_stride, v_stride, k_cache_stride, v_cache_stride, positions_stride, _ = strides
+            _check(name, t, ndim, kind, q.device)
     shape = q.shape
     tokens, q_heads, dim = shape
     cache_shape = k_cache.shape
@@ -162,10 +163,12 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
     if rotation.device_index != at:
         raise ValueError("rotation: on another device")
     if q_out is None:
-        q_out = _made_for(stream, device, torch.empty_like(q, memory_format=torch.contiguous_format))
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if stream is not None:
+            _made_for(stream, q_out)
         q_out_stride = q_heads * dim, dim
     else:
-        q_out_stride = _check("q_out", q_out, 3, dtype, device)[:2]
+        q_out_stride = _check("q_out", q_out, 3, dtype, q.device)[:2]
         if q_out.shape != shape:
             raise ValueError("q_out: another shape than q")
     a = _ROTATE_APPEND_ARGS.pack(
@@ -222,6 +225,7 @@ class AttentionPlan:
         self.q_heads, self.kv_heads, self.head_dim = int(q_heads), int(kv_heads), int(head_dim)
         self.shape = (self.tokens, self.q_heads, self.head_dim)
         self.scale = self.head_dim ** -0.5
+        self.device_index = self.device.index
         self.words_ptr, self.scratch_ptr = self.words.data_ptr(), self.scratch.data_ptr()
 
     def __del__(self):
@@ -250,21 +254,22 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     sequence's length is never used, whatever it holds; of the keys and values
     that count, those that some tokens of a chunk see and others do not must be
     finite."""
-    device = _cuda_device("q", q)
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise ValueError("q: a CUDA tensor is wanted")
     dtype = q.dtype
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError(f"q: bfloat16 or float16 is wanted, not {dtype}")
-    strides = q.stride(), k_cache.stride(), v_cache.stride(), table.stride()
     at = q.get_device()
-    if ([len(x) for x in strides] != [3, 4, 4, 2] or any(x[-1] != 1 for x in strides)
+    q_stride, k_cache_stride, v_cache_stride, table_stride = q.stride(), k_cache.stride(), v_cache.stride(), table.stride()
+    if (len(q_stride) != 3 or len(k_cache_stride) != 4 or len(v_cache_stride) != 4 or len(table_stride) != 2
+            or not (q_stride[2] == k_cache_stride[3] == v_cache_stride[3] == table_stride[1] == 1)
             or not (dtype is k_cache.dtype is v_cache.dtype) or table.dtype is not torch.int32
             or not (at == k_cache.get_device() == v_cache.get_device() == table.get_device())):
         for name, t, ndim, kind in (("q", q, 3, dtype), ("k_cache", k_cache, 4, dtype), ("v_cache", v_cache, 4, dtype),
                                     ("table", table, 2, torch.int32)):
-            _check(name, t, ndim, kind, device)
-    q_stride, k_cache_stride, v_cache_stride, table_stride = strides
-    if at != plan.device.index:
-        raise ValueError(f"q: on {device}, the plan on {plan.device}")
+            _check(name, t, ndim, kind, q.device)
+    if at != plan.device_index:
+        raise ValueError(f"q: on {q.device}, the plan on {plan.device}")
     shape = plan.shape
     if q.shape != shape:
         raise ValueError(f"q: the plan is for {list(shape)}, not {list(q.shape)}")
@@ -278,16 +283,20 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     if rows != plan.sequences:
         raise ValueError(f"table: {plan.sequences} rows are wanted, not {rows}")
     if out is None:
-        out = _made_for(stream, device, torch.empty_like(q, memory_format=torch.contiguous_format))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if stream is not None:
+            _made_for(stream, out)
         out_stride = shape[1] * dim, dim
     else:
-        out_stride = _check("out", out, 3, dtype, device)[:2]
+        out_stride = _check("out", out, 3, dtype, q.device)[:2]
         if out.shape != shape:
             raise ValueError("out: another shape than q")
     if lse is None:
-        lse = _made_for(stream, device, q.new_empty(shape[:2], dtype=torch.float32))
+        lse = q.new_empty(shape[:2], dtype=torch.float32)
+        if stream is not None:
+            _made_for(stream, lse)
     else:
-        _check("lse", lse, 2, torch.float32, device)
+        _check("lse", lse, 2, torch.float32, q.device)
         if lse.shape != shape[:2] or not lse.is_contiguous():
             raise ValueError(f"lse: contiguous {list(shape[:2])} is wanted")
     a = _ATTENTION_ARGS.pack(
