@@ -131,3 +131,49 @@ def test_operators_need_cuda_tensors():
     plan = paged.AttentionPlan([1], [5], 8, 8, 64, device="cpu", ctas=1)
     with pytest.raises(ValueError, match="CUDA"):
         paged.attention(plan, t, None, None, None)
+
+
+def _rotate_args(**change):
+    names = ("dtype", "tokens", "q_heads", "kv_heads", "head_dim", "rotary_dim", "axes", "interleaved", "pages", "page_size",
+             "q", "k", "v", "q_out", "k_cache", "v_cache", "positions", "slots", "frequencies", "pair_axis")
+    a = dict(zip(names, [9, 3, 4, 2, 64, 64, 1, 0, 8, 16] + [4096] * 9 + [0])) | change
+    return paged._ROTATE_APPEND_ARGS.pack(*a.values(), 256, 64, 128, 64, 128, 64, 256, 64, 2048, 128, 64, 2048, 128, 64, 3)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(dtype=10), b"dtype"), (dict(tokens=-1), b"count"), (dict(q_heads=-1), b"count"), (dict(head_dim=0), b"head_dim"),
+    (dict(head_dim=257), b"head_dim"), (dict(rotary_dim=65), b"rotary_dim"), (dict(rotary_dim=66), b"rotary_dim"),
+    (dict(axes=0), b"axes"), (dict(page_size=0), b"cache"), (dict(q=0), b"null"), (dict(slots=0), b"null"),
+    (dict(positions=0), b"null"), (dict(v_cache=0), b"null"), (dict(k=4097), b"multiple"), (dict(frequencies=4098), b"multiple"),
+])
+def test_c_rotate_append_refuses(native_lib, change, words):
+    """Refused before anything of CUDA is called: no GPU is needed."""
+    assert native_lib.emmy_rotate_append(_rotate_args(**change), None) == -1
+    assert words in native_lib.emmy_last_error()
+
+
+def test_c_null_arguments(native_lib):
+    assert native_lib.emmy_rotate_append(None, None) == -1
+    assert native_lib.emmy_paged_plan_make(None, None) == -1
+    assert native_lib.emmy_paged_plan_data(None, None, None, None) == -1
+    assert native_lib.emmy_paged_attention(None, None, None) == -1
+    assert native_lib.emmy_paged_plan_status(None, 0, None) == -1
+    native_lib.emmy_paged_plan_free(None)
+    assert native_lib.emmy_rotate_append(_rotate_args(tokens=0), None) == 0
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(dtype=7), b"dtype"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(page_size=24), b"page_size"),
+    (dict(page_size=192), b"page_size"), (dict(pages=0), b"pages"), (dict(table_width=1), b"does not hold"), (dict(q=0), b"null"),
+    (dict(scratch=0), b"null"), (dict(q=4104), b"16 bytes"), (dict(scratch=4112), b"16 bytes"), (dict(table=4098), b"16 bytes"),
+    (dict(q_token=100), b"stride"), (dict(k_page=-2048), b"stride"), (dict(v_token=0), b"stride"),
+])
+def test_c_attention_refuses(native_lib, change, words):
+    plan = paged.AttentionPlan([2], [5000], 8, 2, 64, device="cpu", ctas=148)
+    assert plan.scratch.numel()
+    names = ("dtype", "pages", "page_size", "table_width", "scale", "q", "out", "lse", "k_cache", "v_cache", "table",
+             "plan_words", "scratch", "q_token", "q_head", "out_token", "out_head", "k_page", "k_token", "k_head",
+             "v_page", "v_token", "v_head", "table_stride")
+    a = dict(zip(names, [9, 400, 16, 400, 0.125] + [4096] * 8 + [512, 64, 512, 64, 2048, 128, 64, 2048, 128, 64, 400])) | change
+    assert native_lib.emmy_paged_attention(plan._h, paged._ATTENTION_ARGS.pack(*a.values()), None) == -1
+    assert words in native_lib.emmy_last_error(), native_lib.emmy_last_error()
