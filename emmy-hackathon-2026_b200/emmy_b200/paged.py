@@ -9,7 +9,8 @@ A cache is two tensors, keys and values, of shape [pages, page_size, kv_heads,
 head_dim] with any strides of the outer dimensions, so ``[pages, kv_heads,
 page_size, head_dim]`` storage is passed as its ``transpose(1, 2)``.  Both
 operators run on the current stream of their tensors' device, or on the CUDA
-stream ``stream`` (its address), and return without waiting.  They are thin over
+stream ``stream`` (its address; it has to last as long as what was allocated for
+calls on it: returned tensors, plans, rotations), and return without waiting.  They are thin over
 the C ABI (``emmy_rotate_append``, ``emmy_paged_attention`` in
 ``include/emmy_b200.h``) and raise :class:`~.native.EmmyError` with its message
 on arguments it refuses, ``ValueError`` on what only Python can see.
@@ -70,26 +71,37 @@ _fns = {}
 
 
 def _call(name, index, stream, *args):
-    """One C-ABI call with device ``index`` current, on its current stream unless one is given."""
+    """One C-ABI call on ``stream`` with its device ``index`` current."""
     fn = _fns.get(name)
     if fn is None:
         fn = _fns[name] = getattr(native.lib(), name)
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
             return _call(name, index, stream, *args)
-    if stream is None:
-        stream = torch._C._cuda_getCurrentRawStream(index)
     rc = fn(*args, stream)
     if rc:
         native.check(rc)
 
 
 def _made_for(stream, t):
-    """A tensor allocated here and written on a given stream is not reused before that is through."""
+    """Memory allocated here and used on another stream is not reused before that stream is through."""
     t.record_stream(torch.cuda.ExternalStream(stream, device=t.device))
 
 
-class Rotation:
+class _Kept:
+    """Device memory that calls on any stream use and that may be dropped while they run."""
+
+    def _keep(self, index, *tensors):
+        self._tensors = [t for t in tensors if t is not None]
+        self._streams = {torch._C._cuda_getCurrentRawStream(index)}
+
+    def _used_on(self, stream):
+        for t in self._tensors:
+            _made_for(stream, t)
+        self._streams.add(stream)
+
+
+class Rotation(_Kept):
     """Rotary positions: ``frequencies`` (float32, on the GPU) has the radians
     per position of each pair, so its length is half of the components that
     turn, the leading ones of a head.  ``axes[i]`` (host integers; default 0) is
@@ -114,6 +126,7 @@ class Rotation:
         self.components = 2 * self.frequencies.shape[0]
         self.device_index = device.index
         self.pair_axis_ptr = 0 if self.pair_axis is None else self.pair_axis.data_ptr()
+        self._keep(device.index, self.frequencies, self.pair_axis)
 
 
 def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=None, stream=None):
@@ -177,11 +190,15 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
         positions.data_ptr(), slots.data_ptr(), rotation.frequencies.data_ptr(), rotation.pair_axis_ptr,
         *q_stride[:2], *k_stride[:2], *v_stride[:2], *q_out_stride, *k_cache_stride[:3], *v_cache_stride[:3],
         positions_stride[0])
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(at)
+    if stream not in rotation._streams:
+        rotation._used_on(stream)
     _call("emmy_rotate_append", at, stream, a)
     return q_out
 
 
-class AttentionPlan:
+class AttentionPlan(_Kept):
     """How the attention of one batch is cut into units of work: made once from
     the host's lengths, used by every layer's call.
 
@@ -194,7 +211,8 @@ class AttentionPlan:
 
     A plan holds device memory (``words``, ``scratch``) that its calls write:
     they must not overlap on the GPU, so calls on several streams need a plan
-    each."""
+    each.  It may be dropped while a call runs, on whichever stream, but not
+    before a CUDA graph that holds its calls."""
 
     def __init__(self, q_lens, kv_lens, q_heads, kv_heads, head_dim, causal=True, window=None, device=None,
                  ctas=None):
@@ -227,6 +245,8 @@ class AttentionPlan:
         self.scale = self.head_dim ** -0.5
         self.device_index = self.device.index
         self.words_ptr, self.scratch_ptr = self.words.data_ptr(), self.scratch.data_ptr()
+        if device.type == "cuda":
+            self._keep(device.index, self.words, self.scratch)
 
     def __del__(self):
         if self._h is not None:
@@ -237,7 +257,10 @@ class AttentionPlan:
 
     def check(self, stream=None):
         """Waits for the calls so far and raises if one of them gave up."""
-        _call("emmy_paged_plan_status", self.device.index, stream, self._h, self.words.data_ptr())
+        index = self.device.index
+        if stream is None:
+            stream = torch._C._cuda_getCurrentRawStream(index)
+        _call("emmy_paged_plan_status", index, stream, self._h, self.words.data_ptr())
 
 
 def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, stream=None):
@@ -304,5 +327,9 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
         q.data_ptr(), out.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
         plan.words_ptr, plan.scratch_ptr, *q_stride[:2], *out_stride, *k_cache_stride[:3], *v_cache_stride[:3],
         table_stride[0])
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(at)
+    if stream not in plan._streams:
+        plan._used_on(stream)
     _call("emmy_paged_attention", at, stream, plan._h, a)
     return out, lse

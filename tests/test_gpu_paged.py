@@ -239,6 +239,35 @@ def test_streams_and_graphs():
     plan.check()
 
 
+@pytest.mark.parametrize("given", [False, True])
+def test_memory_of_a_dropped_plan_waits_for_its_stream(given):
+    """The allocator's own list says so: nothing is written to memory that a kernel may still use."""
+    made = make([1], [20000], 8, 2, 128, 16)
+    side = torch.cuda.Stream()
+    plan = paged.AttentionPlan([1], [20000], 8, 2, 128)
+    rotation = paged.Rotation(torch.ones(32, device="cuda") * 0.5, axes=[0] * 16 + [1] * 16)
+    assert plan.scratch.numel()
+    used = {t.data_ptr() for t in (plan.scratch, plan.words, rotation.frequencies, rotation.pair_axis)}
+    at = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    out, lse = torch.empty_like(made[0]), torch.empty(1, 8, device="cuda")
+    turned = torch.empty_like(made[0])
+    kv = torch.zeros(1, 2, 128, dtype=made[0].dtype, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.current_stream() if given else side):
+        how = dict(stream=side.cuda_stream) if given else {}
+        paged.rotate_append(rotation, made[0], kv, kv, at, at[0], made[1], made[2], q_out=turned, **how)
+        paged.attention(plan, *made, out=out, lse=lse, **how)
+    del plan, rotation
+    states = {}
+    for segment in torch.cuda.memory_snapshot():
+        address = segment["address"]
+        for block in segment["blocks"]:
+            states[address] = block["state"]
+            address += block["size"]
+    side.synchronize()
+    assert [states.get(a) for a in used] == ["active_pending_free"] * 4
+
+
 def test_pages_outside_the_cache_read_as_zeros():
     q, k, v, table = make([1], [64], 4, 2, 64, 16)
     bad = table.clone()
