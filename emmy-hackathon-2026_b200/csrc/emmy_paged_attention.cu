@@ -267,10 +267,11 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^x of a pair on the multiply-add pipe, for x <= 128: n = x rounded, a cubic in
-// x - n on [-1/2, 1/2] (minimising the largest relative error, 7.5e-5: under a
-// fiftieth of the rounding to bfloat16 that follows), times 2^n, exactly 0 from
-// -127 down.  NaN stays.
+// 2^x of a pair on the multiply-add pipe, for x <= 128: n = x rounded, a quintic in
+// x - n on [-1/2, 1/2] (minimising the largest relative error: 2.2e-7 evaluated in 32
+// bits, what the exponential unit has too), times 2^n, exactly 0 from -127 down.  NaN
+// stays.  A cubic's 7.5e-5 would do for the weights, which are rounded to 16 bits, but
+// shows in their sum: the lse of rows of few keys came out up to 7e-5 off.
 __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
   float a, b;
   unpair(x, a, b);
@@ -279,9 +280,11 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
   x = pair(a, b);
   const uint64_t t = add2(x, pair(12582912.f, 12582912.f));     // 1.5 * 2^23: n in the low bits
   const uint64_t f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x);
-  uint64_t p = fma2(pair(0.05517221987247467f, 0.05517221987247467f), f, pair(0.24261115491390228f, 0.24261115491390228f));
-  p = fma2(p, f, pair(0.6932608485221863f, 0.6932608485221863f));
-  p = fma2(p, f, pair(0.9999280571937561f, 0.9999280571937561f));
+  uint64_t p = fma2(pair(0.0013276472454890609f, 0.0013276472454890609f), f, pair(0.0096755409613251686f, 0.0096755409613251686f));
+  p = fma2(p, f, pair(0.055507130920886993f, 0.055507130920886993f));
+  p = fma2(p, f, pair(0.24022120237350464f, 0.24022120237350464f));
+  p = fma2(p, f, pair(0.69314694404602051f, 0.69314694404602051f));
+  p = fma2(p, f, pair(1.f, 1.f));
   unpair(t, a, b);
   return mul2(p, pair(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
 }
@@ -687,10 +690,13 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
   // exponents may run 8 over the base before it moves; 16-bit floats of 5
   // exponent bits get a base 6 lower, so that small weights keep their bits
   constexpr float kShift = BF16 ? 0.f : 6.f, kGrow = 8.f;
-  // every fourth pair's exponentials off the exponential unit, with 64 components:
-  // a tile pair 2,885 -> 2,605 cycles.  With 128 the tensor cores set the power, the
-  // cycles saved (3,030 -> 2,820) come back as a lower clock, and nothing is gained
-  constexpr int kPolyEvery = D == 64 ? 4 : kTile;
+  // with 64 components every fourth pair's exponentials off the exponential unit, every
+  // eighth where the decoding units' code is in the kernel too and registers are short:
+  // 4 prompts of 4,096 tokens, 32 + 8 heads, 374 us against 387 with every eighth and 392
+  // with none; 8 chunks of 1 to 511 over 12,288, 32 + 4 heads, 155 us against 159 with
+  // every fourth and 163 with none.  With 128 components the tensor cores set the power:
+  // cycles saved (3,030 -> 2,820 a tile pair) come back as a lower clock, nothing is gained
+  constexpr int kPolyEvery = D == 128 ? kTile : SPREAD ? 8 : 4;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, t = warp / 4, wid = warp % 4;
   const int row = threadIdx.x % kTile;
   const uint32_t lanes = tmem + (uint32_t(wid * 32) << 16);

@@ -213,6 +213,25 @@ def test_strided_views_and_given_outputs():
     assert bool((frame == 7.0).all())
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("q_lens,kv_lens,heads,kv_heads", [
+    ([40, 1, 7, 18], [40, 33, 9, 18], 8, 2), ([1, 1, 2, 4], [3, 8, 16, 40], 4, 4), ([40, 40], [40, 40], 10, 2),
+])
+def test_lse_to_the_last_bits(q_lens, kv_lens, heads, kv_heads, dim, dtype):
+    """Components of -2..2, so products and their sums are exact and a row's largest
+    weights can stand at any key.  What is left: the exponentials (2^-22 from the unit,
+    at most 2.7e-6 where a polynomial forms them), the sum's n roundings, and a few of
+    2^-24 of the scores and the result."""
+    q, k, v, table = make(q_lens, kv_lens, heads, kv_heads, dim, 16, dtype)
+    q, k = (torch.nan_to_num(x).clamp(-2, 2).round() for x in (q, k))
+    plan = paged.AttentionPlan(q_lens, kv_lens, heads, kv_heads, dim)
+    lse = paged.attention(plan, q, k, v, table)[1]
+    want = definition(q, k, torch.nan_to_num(v), table, q_lens, kv_lens, dim ** -0.5)[1]
+    most = 4.0 * dim * dim ** -0.5
+    assert bool(((lse.double() - want).abs() <= 2.7e-6 + 2.0 ** -22 + (max(kv_lens) + 4 * most + 8) * 2.0 ** -24).all())
+
+
 def test_streams_and_graphs():
     q_lens, kv_lens = [1, 1, 5], [5000, 77, 640]
     made = make(q_lens, kv_lens, 8, 2, 128, 16)
