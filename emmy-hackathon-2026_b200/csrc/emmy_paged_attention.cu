@@ -21,9 +21,10 @@
 // four warps idle and one with 128 exponentials a row, 1,200 cycles, more than
 // the tile takes to arrive.  Their queries are loaded four times, into the rows
 // of each warp: every warp then has all scores of all rows, and takes a quarter
-// of the keys, with weights of 0 for the others and a maximum and a sum of its
-// own.  The eight results are joined in shared memory, where the second query
-// tile would be.
+// of the keys, with a maximum and a sum of its own.  The products with a quarter's
+// values write that warp's rows only: weights of 0 in the other rows would come to
+// the same, but for values that are infinite.  The eight results are joined in
+// shared memory, where the second query tile would be.
 //
 // Tensor memory: S_t at column 128 t, P_t over it (two 16-bit weights a
 // column), O_t at 256 + 128 t.  S = Q K^T and O += P V are 128 x 128 x D and
@@ -199,6 +200,16 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       "mov.b64 b, {%2, %3};\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
       "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(static_cast<uint32_t>(acc))
+      : "memory");
+}
+// the same, into the rows of warp `w` (lanes 32 w to 32 w + 31 of D) only
+__device__ __forceinline__ void mma_ts_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, bool acc, int w) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, {%6, %7, %8, %9}, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(static_cast<uint32_t>(acc)), "r"(w == 0 ? 0u : ~0u), "r"(w == 1 ? 0u : ~0u),
+      "r"(w == 2 ? 0u : ~0u), "r"(w == 3 ? 0u : ~0u)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t *r) {
@@ -518,8 +529,14 @@ __device__ void mma_role(const Params &p, const Smem<D, SPREAD> &sm, const Guard
       commit(sm.empty(stage));
     }
   };
-  auto issue_pv = [&](uint32_t b, int half, bool acc) {      // O_t (+)= P_t V over 64 keys
-    if (alive && elected()) {
+  // O_t (+)= P_t V over 64 keys; quarters: 32 keys into the rows of one warp each
+  auto issue_pv = [&](uint32_t b, int half, bool acc, bool quarters) {
+    if (!alive || !elected()) return;
+    if (quarters) {
+#pragma unroll
+      for (int k = 4 * half; k < 4 * half + 4; ++k)
+        mma_ts_rows(o_at, s_at + 8 * k, b + k * (16 * 128 / 16), kOperandHigh, kPv, acc || k % 2, k / 2);
+    } else {
 #pragma unroll
       for (int k = 4 * half; k < 4 * half + 4; ++k)
         mma_ts(o_at, s_at + 8 * k, b + k * (16 * 128 / 16), kOperandHigh, kPv, acc || k > 0);
@@ -558,6 +575,7 @@ __device__ void mma_role(const Params &p, const Smem<D, SPREAD> &sm, const Guard
     const Unit u = read_unit(p, i);
     if (!u.ntiles) continue;
     const int ahead = u.wide ? 1 : 2;
+    const bool quarters = spread(p, sm, u);
     const uint32_t q_op = operand(sm.query(u.wide ? t : 0), 16);
     wait(sm.q_full(), q_phase);
     q_phase ^= 1;
@@ -599,11 +617,11 @@ __device__ void mma_role(const Params &p, const Smem<D, SPREAD> &sm, const Guard
         take_turn(u.wide);
         wait(sm.p_ready(t, 0), p_phase);
         fence_after();
-        issue_pv(v_op, 0, n >= ahead);
+        issue_pv(v_op, 0, n >= ahead, quarters);
         wait(sm.p_ready(t, 1), p_phase);
         p_phase ^= 1;
         fence_after();
-        issue_pv(v_op, 1, true);
+        issue_pv(v_op, 1, quarters ? n >= ahead : true, quarters);
         if (more) issue_qk(q_op, k_op, k_stage);
         give_turn(u.wide);
         if (more) {
@@ -770,7 +788,7 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
       s_phase ^= 1;
       if (quarter && alive) {
         fence_after();
-        uint32_t s[32], w[16], none[16];
+        uint32_t s[32], w[16];
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         tmem_ld32(s_at + 32 * wid, s);
         tmem_ld_wait(s);
@@ -799,10 +817,7 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
           f = exp2_approx(f);
           part[q % 2] = add2(part[q % 2], pair(e, f));
           w[q] = pack16<BF16>(e, f);
-          none[q] = 0;
         }
-#pragma unroll
-        for (int k = 1; k < 4; ++k) tmem_st16(s_at + 16 * (wid ^ k), none);
         tmem_st16(s_at + 16 * wid, w);
         weights_stored(0);
         if (lane == 0) bar_arrive(sm.p_ready(t, 1));

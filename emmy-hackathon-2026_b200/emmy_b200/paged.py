@@ -276,7 +276,8 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     that sees no key gets 0, and -inf.  What lies in the cache beyond a
     sequence's length is never used, whatever it holds; of the keys and values
     that count, those that some tokens of a chunk see and others do not must be
-    finite."""
+    finite.  An infinite value that all of them see makes its component infinite
+    (NaN, where its weight rounds to 0 in the cache's type)."""
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError("q: a CUDA tensor is wanted")
     dtype = q.dtype

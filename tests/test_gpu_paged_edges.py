@@ -1,0 +1,55 @@
+"""The paged-cache operators on the GPU where their values or arguments are unusual."""
+import math
+
+import pytest
+import torch
+
+from emmy_b200 import paged
+from test_gpu_paged import UNIT, close, definition, make
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------- infinite values
+@pytest.mark.parametrize("dim,dtype", [(64, torch.bfloat16), (64, torch.float16), (128, torch.bfloat16), (128, torch.float16)])
+@pytest.mark.parametrize("q_lens,kv_lens,heads,kv_heads", [
+    ([1], [40], 8, 2), ([1, 1, 1, 1], [129, 300, 1000, 64], 8, 2), ([3, 2], [300, 500], 4, 4), ([20], [400], 8, 2),
+    ([90], [700], 8, 2), ([1], [9000], 8, 1), ([1, 300], [640, 900], 6, 2)])
+def test_infinite_values(dim, dtype, q_lens, kv_lens, heads, kv_heads):
+    """An infinite value that every token of a chunk sees gives an infinite component,
+    both signs of it NaN, and no other component, head or sequence is touched.  (Scores
+    are within +-8 or so: no weight rounds to 0 in 16 bits.)"""
+    q, k, v, table = make(q_lens, kv_lens, heads, kv_heads, dim, 16, dtype)
+    for s, (n, length) in enumerate(zip(q_lens, kv_lens)):
+        # each value of a component of its own, at keys all over a tile, in the last
+        # head of keys; two meet in the last component
+        seen = length - n + 1
+        for i, j in enumerate(j for j in (0, 5, 33, 37, 64, 70, 96, 127, 128, 250, 299, 639, 8999) if j < seen):
+            v[table[s, j // 16].long(), j % 16, -1, 3 * i] = math.inf if i % 2 else -math.inf
+        for j, x in ((0, math.inf), (seen - 1, -math.inf)):
+            v[table[s, j // 16].long(), j % 16, -1, dim - 1] = x
+    plan = paged.AttentionPlan(q_lens, kv_lens, heads, kv_heads, dim)
+    out, lse = paged.attention(plan, q, k, v, table)
+    plan.check()
+    o, ls, size = definition(q, k, v, table, q_lens, kv_lens, dim ** -0.5)
+    special = ~o.isfinite()
+    assert special.any()
+    assert torch.equal(torch.nan_to_num(out.double(), nan=1.0, posinf=2.0, neginf=3.0)[special],
+                       torch.nan_to_num(o, nan=1.0, posinf=2.0, neginf=3.0)[special])
+    close(out.masked_fill(special, 0.0), lse, (o.masked_fill(special, 0.0), ls, size.masked_fill(special, 0.0)), UNIT[dtype])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_infinite_values_outside_the_window(dim):
+    """A decoding token's window hides them, whatever tile or page they share with it."""
+    q_lens, kv_lens = [1, 1, 1], [300, 129, 1000]
+    q, k, v, table = make(q_lens, kv_lens, 8, 2, dim, 16)
+    for s, n in enumerate(kv_lens):
+        for j in range(n - 100):
+            for c, x in ((k, math.nan), (v, math.inf)):
+                c[table[s, j // 16].long(), j % 16] = x
+    plan = paged.AttentionPlan(q_lens, kv_lens, 8, 2, dim, window=100)
+    out, lse = paged.attention(plan, q, k, v, table)
+    plan.check()
+    clean = [torch.nan_to_num(c, nan=0.0, posinf=0.0, neginf=0.0) for c in (k, v)]
+    close(out, lse, definition(q, *clean, table, q_lens, kv_lens, dim ** -0.5, window=100), UNIT[q.dtype])
