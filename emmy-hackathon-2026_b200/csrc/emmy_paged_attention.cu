@@ -48,7 +48,9 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -69,7 +71,7 @@ constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
 constexpr int kSoftmaxWarps = 8, kKeyWarp = 8, kMmaWarp = 10;
 constexpr int kSmem = 227 * 1024;
-constexpr float kNoMax = -1e30f;        // exponent base of a row that has seen no key
+constexpr float kNoMax = -FLT_MAX;      // exponent base of a row that has seen no key
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct alignas(64) Params {
@@ -85,7 +87,7 @@ struct alignas(64) Params {
   int64_t table_stride, out_stride[2];
   int q_heads, group, group_inverse, per_tile, box, causal, window, aligned32;
   int tiles_a_page;                    // of pages of a tile or more
-  float scale_log2;
+  float scale_log2, scale_power;       // c, and the power of two next to it
 };
 
 template <int D> struct Shape {
@@ -708,18 +710,19 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
   // exponents may run 8 over the base before it moves; 16-bit floats of 5
   // exponent bits get a base 6 lower, so that small weights keep their bits
   constexpr float kShift = BF16 ? 0.f : 6.f, kGrow = 8.f;
-  // with 64 components every fourth pair's exponentials off the exponential unit, every
-  // eighth where the decoding units' code is in the kernel too and registers are short:
-  // 4 prompts of 4,096 tokens, 32 + 8 heads, 374 us against 387 with every eighth and 392
-  // with none; 8 chunks of 1 to 511 over 12,288, 32 + 4 heads, 155 us against 159 with
-  // every fourth and 163 with none.  With 128 components the tensor cores set the power:
-  // cycles saved (3,030 -> 2,820 a tile pair) come back as a lower clock, nothing is gained
-  constexpr int kPolyEvery = D == 128 ? kTile : SPREAD ? 8 : 4;
+  // with 64 components every fourth pair's exponentials off the exponential unit: 4
+  // prompts of 4,096 tokens, 32 + 8 heads, 377 us against 387 with every eighth and 392
+  // with none; 8 chunks of 1 to 511 over 12,288, 32 + 4 heads, 163 us against 166 with
+  // every eighth.  With 128 components the tensor cores set the power: cycles saved
+  // (3,030 -> 2,820 a tile pair) come back as a lower clock, nothing is gained
+  constexpr int kPolyEvery = D == 128 ? kTile : 4;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, t = warp / 4, wid = warp % 4;
   const int row = threadIdx.x % kTile;
   const uint32_t lanes = tmem + (uint32_t(wid * 32) << 16);
   const uint32_t s_at = lanes + kTile * t, o_at = lanes + 2 * kTile + kTile * t;
   const float c = p.scale_log2;
+  // a base of this size is off by 2^5 at most (the sums take that) or 1 (weights of 5 exponent bits)
+  constexpr float kLarge = BF16 ? 0x1p29f : 0x1p24f;
   uint32_t s_phase = 0, f_phase = 0;
   bool alive = true;
   // this stream's tile of queries: its first token in the unit, and its rows
@@ -755,16 +758,29 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
       key0 = (u.tile0 + (u.wide ? 0 : t)) * kTile;
       end = (u.tile0 + u.ntiles) * kTile;
     }
-    float m = kNoMax, l = 0.f;
+    // A base stands away from the product of score and c that it was rounded from, and
+    // the multiply-add of the exponents, exact until its end, raises 2 to that: nothing
+    // to a small base, 0 or infinity to a large one.  A row whose base is kLarge or more
+    // multiplies by the power of two next to c instead, which is exact.  What that does
+    // to scores a rounding apart is within the rounding of scores as large in 32 bits;
+    // from 2^29 up different ones are 32 and more apart, and only the largest counts.
+    float m = kNoMax, l = 0.f, by_c = c;
     bool begun = false;
     // the base follows the row's maximum when that grows by more than 2^8: the
     // running sum and output (idle, the last product is complete) come down to it
-    auto rebase = [&](float best) {
-      const bool need = best > m + (kShift + kGrow);
+    auto rebase = [&](float top) {
+      const float best = __fmul_rn(top, by_c);
+      const bool need = best - m > kShift + kGrow;      // (a large m + 14 would be rounded)
       if (!__any_sync(~0u, need)) return;
-      const float to = need ? best - kShift : m;
-      const float by = need ? exp2_approx(m - to) : 1.f;
-      m = to;
+      float by = 1.f;
+      if (need) {
+        const float scaled = __fmul_rn(top, c), was = by_c;
+        const bool large = fabsf(scaled) >= kLarge;
+        by_c = large ? p.scale_power : c;
+        const float to = large ? __fmul_rn(top, by_c) : scaled - kShift;
+        by = exp2_approx(was == by_c ? m - to : m * (c / was) - (large ? scaled : to));
+        m = to;
+      }
       l *= by;
       if (!begun) return;
       const uint64_t by2 = pair(by, by);
@@ -806,8 +822,8 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
         for (int k = 0; k < 32; k += 8)
 #pragma unroll
           for (int q = 0; q < 4; ++q) top[q] = max3(__float_as_uint(top[q]), s[k + q], s[k + 4 + q]);
-        rebase(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
-        const uint64_t c2 = pair(c, c), base2 = pair(-m, -m);
+        rebase(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        const uint64_t c2 = pair(by_c, by_c), base2 = pair(-m, -m);
         uint64_t part[2] = {0, 0};
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
@@ -862,9 +878,8 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
         take_in(0);
         tmem_ld_wait(s, 64, 128);
         take_in(64);
-        const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-        rebase(best);
-        const uint64_t c2 = pair(c, c);
+        rebase(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        const uint64_t c2 = pair(by_c, by_c);
         const uint64_t base2 = pair(-m, -m);
         uint64_t part[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -915,6 +930,7 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
       f_phase ^= 1;
       fence_after();
     }
+    if (by_c != c) m *= c / by_c;        // from here on every row's base is one of c
     float by0 = 1.f, by1 = 0.f;
     if (joined) {
       if (t == 1) sm.ml()[row] = make_float2(m, l);
@@ -1256,6 +1272,9 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
   p.causal = plan->causal;
   p.window = plan->window;
   p.scale_log2 = a->scale * kLog2e;
+  int exponent = 0;
+  const float mantissa = std::frexp(p.scale_log2, &exponent);      // 1/2 to 1
+  p.scale_power = std::ldexp(1.f, std::min(127, mantissa * mantissa < 0.5f ? exponent - 1 : exponent));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int n = plan->at.ctas;
   if (plan->spread) {

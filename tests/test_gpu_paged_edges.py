@@ -53,3 +53,38 @@ def test_infinite_values_outside_the_window(dim):
     plan.check()
     clean = [torch.nan_to_num(c, nan=0.0, posinf=0.0, neginf=0.0) for c in (k, v)]
     close(out, lse, definition(q, *clean, table, q_lens, kv_lens, dim ** -0.5, window=100), UNIT[q.dtype])
+
+
+# ---------------------------------------------------------------- large scores
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype,size", [(torch.bfloat16, n) for n in (20, 24, 27, 29, 33, 60, 112)] +
+                         [(torch.float16, n) for n in (20, 24, 27, 29, 33)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 3, 20, 300, 9], [300, 40, 170, 900, 4]), ([1], [20000])])
+@pytest.mark.parametrize("factor", [1.0, 181 / 128])
+def test_scores_of_any_size(factor, q_lens, kv_lens, dim, dtype, size, sign):
+    """Scores of +-factor * 2^size and half of that before they are scaled: exact, as
+    every product of components has 8 bits, so a row's weights are equal over its largest
+    ones.  Odd heads have scores of +-8 and so on in the same tiles.
+
+    The logarithm carries the rounding of the scale, of its conversion to base 2, of the
+    scaled score and of the way back: 8 roundings of 2^-24 of it."""
+    heads, kv_heads = 8, 2
+    q, k, v, table = make(q_lens, kv_lens, heads, kv_heads, dim, 16, dtype)
+    b = min(12, size // 2)
+    q[:, 0::2], q[:, 1::2] = 2.0 ** (size - b) / dim, 2.0 ** (3 - b) / dim
+    g = torch.Generator(device="cuda").manual_seed(5)
+    half = torch.rand(k.shape[:3], generator=g, device="cuda") < 0.5
+    keys = torch.where(half, 2.0 ** (b - 1), 2.0 ** b) * (factor * sign)
+    k.copy_(torch.where(k.isnan(), k.float(), keys[..., None]).to(dtype))
+    assert q.isfinite().all() and (q > 0).all()
+    plan = paged.AttentionPlan(q_lens, kv_lens, heads, kv_heads, dim)
+    out, lse = paged.attention(plan, q, k, v, table)
+    plan.check()
+    o, ls, weighed = definition(q, k, v, table, q_lens, kv_lens, dim ** -0.5)
+    assert torch.isfinite(out).all()
+    u = UNIT[dtype]
+    assert bool(((out.double() - o).abs() <= u * (o.abs() + weighed) * 1.01 + 1e-4 * weighed).all())
+    empty = ls == -math.inf
+    assert torch.equal(lse == -math.inf, empty)
+    assert bool(((lse.double() - ls).abs() <= 8 * 2.0 ** -24 * ls.abs() + 1e-4)[~empty].all())
