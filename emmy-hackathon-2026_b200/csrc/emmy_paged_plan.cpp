@@ -242,11 +242,17 @@ extern "C" EMMY_API int emmy_paged_plan_make(const emmy_paged_plan_args *a, emmy
     return fail("emmy_paged_plan_make: window %ld (a window is causal)", a->window);
   if (a->ctas < 1 || a->ctas > 65536) return fail("emmy_paged_plan_make: %ld CTAs", a->ctas);
   int64_t tokens = 0;
+  int32_t longest = 0;
   for (int s = 0; s < a->sequences; ++s) {
     if (a->q_lens[s] < 0 || a->kv_lens[s] < 0 || a->q_lens[s] > (1 << 30) || a->kv_lens[s] > (1 << 30))
       return fail("emmy_paged_plan_make: sequence %ld has a length outside 0..2^30", s);
     tokens += a->q_lens[s];
+    longest = std::max(longest, a->kv_lens[s]);
   }
+  // A window that hides no key is none; others, and the positions that they are taken
+  // from, down to -2^30, are small enough for 32 bits here and in the kernel.
+  emmy_paged_plan_args args = *a;
+  if (args.window >= longest) args.window = 0;
   if (tokens * a->q_heads > (int64_t(1) << 30)) return fail("emmy_paged_plan_make: too many tokens");
   try {
     emmy_paged_plan_s *plan = new emmy_paged_plan_s;
@@ -255,9 +261,9 @@ extern "C" EMMY_API int emmy_paged_plan_make(const emmy_paged_plan_args *a, emmy
     plan->kv_heads = a->kv_heads;
     plan->head_dim = a->head_dim;
     plan->causal = a->causal != 0;
-    plan->window = a->window;
+    plan->window = args.window;
     try {
-      make(*a, *plan);
+      make(args, *plan);
     } catch (...) {
       delete plan;
       throw;

@@ -227,7 +227,8 @@ class AttentionPlan(_Kept):
         if ctas is None:
             ctas = torch.cuda.get_device_properties(device).multi_processor_count
         n = len(q_lens)
-        a = _PlanArgs(n, None, None, q_heads, kv_heads, head_dim, bool(causal), window or 0, ctas)
+        # (2^30: more than any length, and so no window)
+        a = _PlanArgs(n, None, None, q_heads, kv_heads, head_dim, bool(causal), min(window or 0, 1 << 30), ctas)
         lens = (_i32 * (2 * n))(*q_lens, *kv_lens)
         a.q_lens, a.kv_lens = ctypes.addressof(lens), ctypes.addressof(lens) + 4 * n
         L = native.lib()

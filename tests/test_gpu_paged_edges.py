@@ -88,3 +88,18 @@ def test_scores_of_any_size(factor, q_lens, kv_lens, dim, dtype, size, sign):
     empty = ls == -math.inf
     assert torch.equal(lse == -math.inf, empty)
     assert bool(((lse.double() - ls).abs() <= 8 * 2.0 ** -24 * ls.abs() + 1e-4)[~empty].all())
+
+
+# --------------------------------------------------------------------- windows
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31 - 1, 2 ** 32 + 5, 2 ** 63])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_windows_beyond_every_length(window, dim):
+    q_lens, kv_lens = [10, 1, 300, 40], [4, 1000, 100, 640]
+    made = make(q_lens, kv_lens, 8, 2, dim, 16)
+    got = []
+    for w in (None, window):
+        plan = paged.AttentionPlan(q_lens, kv_lens, 8, 2, dim, window=w)
+        got.append(paged.attention(plan, *made))
+        plan.check()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    close(*got[1], definition(*made, q_lens, kv_lens, dim ** -0.5), UNIT[torch.bfloat16])

@@ -1,0 +1,48 @@
+"""Paged-cache operators on the CPU: arguments at the ends of their ranges, and the
+order and streams that the kernels and their memory rely on."""
+import sys
+
+import pytest
+import torch
+
+from emmy_b200 import native, paged
+from test_paged_plan import units_of
+
+pytestmark = pytest.mark.usefixtures("native_lib")
+
+
+# --------------------------------------------------------------------- windows
+def c_plan_words(q_lens, kv_lens, window):
+    """Words of a plan made through the C ABI, where a window has 32 bits."""
+    import ctypes
+    lens = (ctypes.c_int32 * (2 * len(q_lens)))(*q_lens, *kv_lens)
+    a = paged._PlanArgs(len(q_lens), ctypes.addressof(lens), ctypes.addressof(lens) + 4 * len(q_lens), 8, 2, 64, 1, window, 148)
+    L, h = native.lib(), ctypes.c_void_p()
+    native.check(L.emmy_paged_plan_make(ctypes.byref(a), ctypes.byref(h)))
+    words, count, scratch = ctypes.c_void_p(), ctypes.c_size_t(), ctypes.c_size_t()
+    native.check(L.emmy_paged_plan_data(h, ctypes.byref(words), ctypes.byref(count), ctypes.byref(scratch)))
+    got = list((ctypes.c_int32 * count.value).from_address(words.value))
+    L.emmy_paged_plan_free(h)
+    return got
+
+
+LENGTHS = [([10], [4]), ([40, 1], [30, 1000]), ([1], [1]), ([2 ** 20], [0]), ([300, 7], [5000, 2])]
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", LENGTHS)
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30])
+def test_windows_of_31_bits_hide_nothing(q_lens, kv_lens, window):
+    assert c_plan_words(q_lens, kv_lens, window) == c_plan_words(q_lens, kv_lens, 0)
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", LENGTHS)
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, sys.maxsize, 2 ** 64])
+def test_windows_beyond_every_length(q_lens, kv_lens, window):
+    plans = [paged.AttentionPlan(q_lens, kv_lens, 8, 2, 64, window=w, device="cpu", ctas=148) for w in (window, None)]
+    assert plans[0].words.tolist() == plans[1].words.tolist()
+
+
+def test_the_longest_window_that_hides_a_key():
+    """One position less than the longest sequence has: its last token does not see the first."""
+    plan = paged.AttentionPlan([1, 1], [100, 1000], 8, 2, 64, window=999, device="cpu", ctas=148)
+    assert {(u["seq"], u["lo"]) for u in units_of(plan)[0]} == {(0, 0), (1, 1)}
