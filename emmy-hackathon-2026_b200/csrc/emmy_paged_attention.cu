@@ -1208,7 +1208,7 @@ template <int D, bool BF16, bool SPREAD> int launch(const Params &p, int ctas, c
 extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, void *stream) {
   if (!plan || !a) return fail("emmy_paged_attention: bad argument");
   if (a->dtype != 6 && a->dtype != 9) return fail("emmy_paged_attention: dtype %ld (f16 or bf16)", a->dtype);
-  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail("emmy_paged_attention: scale must be positive and finite");
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale * kLog2e)) return fail("emmy_paged_attention: scale must be positive and finite");
   if (plan->tokens == 0) return 0;
   const int ps = a->page_size;
   if (ps < 8 || (ps < kTile ? (ps & (ps - 1)) != 0 : ps % kTile != 0))

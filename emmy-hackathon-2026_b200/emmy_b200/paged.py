@@ -61,6 +61,10 @@ def _check(name, t, ndim, dtype, device):
     return stride
 
 
+def _unfit(e):
+    return ValueError(f"an argument does not fit its field of the C ABI: {e}")
+
+
 def _cuda_device(name, t):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name}: a CUDA tensor is wanted")
@@ -184,12 +188,15 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
         q_out_stride = _check("q_out", q_out, 3, dtype, q.device)[:2]
         if q_out.shape != shape:
             raise ValueError("q_out: another shape than q")
-    a = _ROTATE_APPEND_ARGS.pack(
-        _DTYPES[dtype], tokens, q_heads, kv_heads, dim, rotation.components, axes, rotation.interleaved, pages, page_size,
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        positions.data_ptr(), slots.data_ptr(), rotation.frequencies.data_ptr(), rotation.pair_axis_ptr,
-        *q_stride[:2], *k_stride[:2], *v_stride[:2], *q_out_stride, *k_cache_stride[:3], *v_cache_stride[:3],
-        positions_stride[0])
+    try:
+        a = _ROTATE_APPEND_ARGS.pack(
+            _DTYPES[dtype], tokens, q_heads, kv_heads, dim, rotation.components, axes, rotation.interleaved, pages, page_size,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            positions.data_ptr(), slots.data_ptr(), rotation.frequencies.data_ptr(), rotation.pair_axis_ptr,
+            *q_stride[:2], *k_stride[:2], *v_stride[:2], *q_out_stride, *k_cache_stride[:3], *v_cache_stride[:3],
+            positions_stride[0])
+    except (struct.error, OverflowError) as e:
+        raise _unfit(e) from None
     if stream is None:
         stream = torch._C._cuda_getCurrentRawStream(at)
     if stream not in rotation._streams:
@@ -221,6 +228,7 @@ class AttentionPlan(_Kept):
         _need(len(q_lens) == len(kv_lens), "q_lens and kv_lens have different lengths")
         _need(all(0 <= x <= 1 << 30 for x in q_lens + kv_lens), "lengths must be 0..2^30")
         _need(window is None or window >= 1, "window: at least 1, or None")
+        _need(all(x is None or -1 << 31 <= x < 1 << 31 for x in (q_heads, kv_heads, head_dim, ctas)), "counts have to fit 32 bits")
         device = torch.device("cuda" if device is None else device)
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
@@ -324,11 +332,14 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
         _check("lse", lse, 2, torch.float32, q.device)
         if lse.shape != shape[:2] or not lse.is_contiguous():
             raise ValueError(f"lse: contiguous {list(shape[:2])} is wanted")
-    a = _ATTENTION_ARGS.pack(
-        _DTYPES[dtype], pages, page_size, width, plan.scale if scale is None else scale,
-        q.data_ptr(), out.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
-        plan.words_ptr, plan.scratch_ptr, *q_stride[:2], *out_stride, *k_cache_stride[:3], *v_cache_stride[:3],
-        table_stride[0])
+    try:
+        a = _ATTENTION_ARGS.pack(
+            _DTYPES[dtype], pages, page_size, width, plan.scale if scale is None else scale,
+            q.data_ptr(), out.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
+            plan.words_ptr, plan.scratch_ptr, *q_stride[:2], *out_stride, *k_cache_stride[:3], *v_cache_stride[:3],
+            table_stride[0])
+    except (struct.error, OverflowError) as e:
+        raise _unfit(e) from None
     if stream is None:
         stream = torch._C._cuda_getCurrentRawStream(at)
     if stream not in plan._streams:

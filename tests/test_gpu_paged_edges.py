@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from emmy_b200 import paged
+from emmy_b200 import native, paged
 from test_gpu_paged import UNIT, close, definition, make
 
 pytestmark = pytest.mark.gpu
@@ -103,3 +103,14 @@ def test_windows_beyond_every_length(window, dim):
         plan.check()
     assert all(torch.equal(a, b) for a, b in zip(*got))
     close(*got[1], definition(*made, q_lens, kv_lens, dim ** -0.5), UNIT[torch.bfloat16])
+
+
+# --------------------------------------------------------------------- numbers
+def test_scales_out_of_range():
+    made = make([2], [64], 4, 2, 64, 16)
+    plan = paged.AttentionPlan([2], [64], 4, 2, 64)
+    for scale in (1e39, 3e38, 1e-60, math.nan):
+        with pytest.raises(native.EmmyError, match="scale"):
+            paged.attention(plan, *made, scale=scale)
+    with pytest.raises(ValueError, match="fit"):
+        paged.attention(plan, *made, scale="1")

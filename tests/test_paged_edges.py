@@ -46,3 +46,22 @@ def test_the_longest_window_that_hides_a_key():
     """One position less than the longest sequence has: its last token does not see the first."""
     plan = paged.AttentionPlan([1, 1], [100, 1000], 8, 2, 64, window=999, device="cpu", ctas=148)
     assert {(u["seq"], u["lo"]) for u in units_of(plan)[0]} == {(0, 0), (1, 1)}
+
+
+# --------------------------------------------------------------------- numbers
+@pytest.mark.parametrize("change", [dict(q_heads=2 ** 32 + 32), dict(kv_heads=2 ** 32 + 8), dict(head_dim=2 ** 32 + 128), dict(ctas=2 ** 32 + 1),
+                                    dict(ctas=-2 ** 32 + 1), dict(q_heads=2 ** 31)])
+def test_counts_beyond_32_bits_are_refused(change):
+    """Not taken as their lowest 32 bits."""
+    a = dict(q_lens=[1], kv_lens=[5], q_heads=32, kv_heads=8, head_dim=128, device="cpu", ctas=148) | change
+    with pytest.raises(ValueError, match="32 bits"):
+        paged.AttentionPlan(**a)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_c_attention_refuses_scales_without_a_base_of_2(native_lib, scale):
+    """scale x log2(e) has to be finite as well."""
+    plan = paged.AttentionPlan([2], [5000], 8, 2, 64, device="cpu", ctas=148)
+    a = paged._ATTENTION_ARGS.pack(9, 400, 16, 400, scale, *[4096] * 8, 512, 64, 512, 64, 2048, 128, 64, 2048, 128, 64, 400)
+    assert native_lib.emmy_paged_attention(plan._h, a, None) == -1
+    assert b"scale" in native_lib.emmy_last_error(), native_lib.emmy_last_error()
