@@ -1211,18 +1211,19 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
   if (!(a->scale > 0.f) || !std::isfinite(a->scale * kLog2e)) return fail("emmy_paged_attention: scale must be positive and finite");
   if (plan->tokens == 0) return 0;
   const int ps = a->page_size;
+  const bool reads = plan->tiled || plan->spread;     // some unit sees a key
   if (ps < 8 || (ps < kTile ? (ps & (ps - 1)) != 0 : ps % kTile != 0))
     return fail("emmy_paged_attention: page_size %ld (8, 16, 32, 64 or a multiple of 128)", ps);
-  if (a->pages < 1) return fail("emmy_paged_attention: a cache of %ld pages", a->pages);
+  if (a->pages < (reads ? 1 : 0)) return fail("emmy_paged_attention: a cache of %ld pages", a->pages);
   if (a->table_width < 0 || int64_t(a->table_width) * ps < plan->max_kv)
     return fail("emmy_paged_attention: a table of %ld pages a sequence does not hold %ld tokens", a->table_width, plan->max_kv);
-  if (!a->q || !a->out || !a->k_cache || !a->v_cache || !a->table || !a->plan_words || (plan->part_rows && !a->scratch))
+  if (!a->q || !a->out || (reads && (!a->k_cache || !a->v_cache || !a->table)) || !a->plan_words || (plan->part_rows && !a->scratch))
     return fail("emmy_paged_attention: null address");
   if ((a->q | a->out | a->k_cache | a->v_cache | a->plan_words) % 16 || a->scratch % 32 || (a->table | a->lse) % 4)
     return fail("emmy_paged_attention: address not a multiple of 16 bytes (scratch: 32)");
   const int group = plan->q_heads / plan->kv_heads, d = plan->head_dim;
   const int64_t extent[3] = {a->pages, ps, plan->kv_heads};
-  for (int i = 0; i < 3; ++i)
+  for (int i = 0; i < 3 && reads; ++i)
     if (bad_stride(a->k_cache_stride[i], extent[i]) || bad_stride(a->v_cache_stride[i], extent[i]))
       return fail("emmy_paged_attention: cache stride %ld not a positive multiple of 8 elements", i);
   const int64_t rows[2] = {plan->tokens, plan->q_heads};
@@ -1244,7 +1245,7 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
     if (int e = emmy_tensormap_encode(&p.q32, a->dtype, 4, a->q, q_dims, q_steps, q32_box, 3)) return e;
   const uint64_t dims[4] = {uint64_t(d), uint64_t(ps), uint64_t(plan->kv_heads), uint64_t(a->pages)};
   const uint32_t kv_box[4] = {64, box, 1, 1};
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 2 && reads; ++i) {
     const int64_t *st = i ? a->v_cache_stride : a->k_cache_stride;
     const uint64_t steps[3] = {step(st[1], ps), step(st[2], plan->kv_heads), step(st[0], a->pages)};
     if (int e = emmy_tensormap_encode(i ? &p.v : &p.k, a->dtype, 4, i ? a->v_cache : a->k_cache, dims, steps, kv_box, 3)) return e;

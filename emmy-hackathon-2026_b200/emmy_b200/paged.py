@@ -282,7 +282,8 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     the pages of each sequence in order (entries after its last page are not
     read; a page outside the cache reads as zeros).  page_size is 8, 16, 32, 64
     or a multiple of 128.  ``scale`` defaults to 1/sqrt(head_dim).  A token
-    that sees no key gets 0, and -inf.  What lies in the cache beyond a
+    that sees no key gets 0, and -inf; where none sees any, cache and table may
+    be empty.  What lies in the cache beyond a
     sequence's length is never used, whatever it holds; of the keys and values
     that count, those that some tokens of a chunk see and others do not must be
     finite.  An infinite value that all of them see makes its component infinite

@@ -279,8 +279,9 @@ typedef struct {
 
 /* out = softmax(scale q k^T) v of each new token over the cached tokens that it */
 /* sees, lse the natural logarithm of the sum; a token that sees none gets 0 and */
-/* -inf.  A page number outside the cache reads as zeros.  q and the caches need */
-/* 16-byte aligned addresses and strides.                                       */
+/* -inf (where no token sees any, cache and table may be empty, at address 0).   */
+/* A page number outside the cache reads as zeros.  q and the caches need        */
+/* 16-byte aligned addresses and strides.                                        */
 EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_paged_attention_args *a,
                                   void *stream);
 /* Reads the plan's status word (waits for `stream`): EMMY_EKERNEL when a call   */

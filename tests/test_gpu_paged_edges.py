@@ -114,3 +114,17 @@ def test_scales_out_of_range():
             paged.attention(plan, *made, scale=scale)
     with pytest.raises(ValueError, match="fit"):
         paged.attention(plan, *made, scale="1")
+
+
+# ------------------------------------------------------------- nothing to read
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_batch_without_keys_needs_no_cache(causal):
+    q = torch.randn(5, 8, 64, device="cuda").bfloat16()
+    plan = paged.AttentionPlan([2, 3], [0, 0], 8, 2, 64, causal=causal)
+    for pages in (0, 3):
+        cache = torch.zeros(pages, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+        for width in (0, 2):
+            out, lse = paged.attention(plan, q, cache, cache, torch.zeros(2, width, dtype=torch.int32, device="cuda"),
+                                       out=torch.full_like(q, 7.0))
+            plan.check()
+            assert not out.any() and bool((lse == -math.inf).all())

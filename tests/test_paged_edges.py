@@ -65,3 +65,19 @@ def test_c_attention_refuses_scales_without_a_base_of_2(native_lib, scale):
     a = paged._ATTENTION_ARGS.pack(9, 400, 16, 400, scale, *[4096] * 8, 512, 64, 512, 64, 2048, 128, 64, 2048, 128, 64, 400)
     assert native_lib.emmy_paged_attention(plan._h, a, None) == -1
     assert b"scale" in native_lib.emmy_last_error(), native_lib.emmy_last_error()
+
+
+# ------------------------------------------------------------- nothing to read
+@pytest.mark.parametrize("change", [dict(table=0, table_width=0), dict(pages=0, k_cache=0, v_cache=0), dict(pages=0, table=0, table_width=0)])
+@pytest.mark.parametrize("kv_lens,refused", [([0, 0], False), ([0, 1], True), ([3, 0], True)])
+def test_a_cache_is_needed_where_a_token_sees_a_key(native_lib, change, kv_lens, refused):
+    """Refused for its arguments (before any CUDA call), or not."""
+    plan = paged.AttentionPlan([2, 3], kv_lens, 8, 2, 64, causal=False, device="cpu", ctas=148)
+    names = ("dtype", "pages", "page_size", "table_width", "scale", "q", "out", "lse", "k_cache", "v_cache", "table")
+    a = dict(zip(names, [9, 400, 16, 400, 0.125] + [4096] * 6)) | change
+    a = paged._ATTENTION_ARGS.pack(*a.values(), 4096, 4096, 512, 64, 512, 64, 2048, 128, 64, 2048, 128, 64, 400)
+    if not refused and torch.cuda.is_available():
+        pytest.skip("would run")
+    native_lib.emmy_paged_attention(plan._h, a, None)
+    said = any(word in native_lib.emmy_last_error() for word in (b"null", b"does not hold", b"a cache of"))
+    assert said == refused, native_lib.emmy_last_error()
