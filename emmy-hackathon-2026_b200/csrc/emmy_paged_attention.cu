@@ -40,7 +40,7 @@
 // heads of 128 in 1.0 ms (1,100 TFLOP/s of what causal attention needs).
 //
 // Every wait is bounded; one that runs out sets the plan's status word, and
-// from then on nothing more is issued.
+// from then on its CTA issues nothing more, and later calls do nothing.
 #include "emmy_paged.h"
 
 #include <cuda.h>
@@ -1110,6 +1110,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
   sm.base = (smem_addr(raw) + 1023) & ~1023u;
   const int warp = threadIdx.x / 32;
   // the first unit is on its way while the CTA sets itself up
+  const unsigned status = threadIdx.x == 0 ? __ldcg(p.status) : 0;
   const int first = __ldg(p.cta_first + blockIdx.x), last = __ldg(p.cta_first + blockIdx.x + 1);
   asm volatile("prefetch.global.L1 [%0];" ::"l"(p.units + first));
   if (threadIdx.x == 0) {
@@ -1136,9 +1137,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   fence_before();
-  __syncthreads();
+  // an earlier call that gave up left counters and parts as they were: nothing is started over them
+  const bool gave_up = __syncthreads_or(status);
   fence_after();
   const uint32_t tmem = __reduce_or_sync(~0u, sm.words()[1]);
+  if (gave_up) {
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    return;
+  }
   const Guard g{sm.base + Shape<D>::kWords, p};
   if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));

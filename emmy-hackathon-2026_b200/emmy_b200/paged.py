@@ -265,7 +265,8 @@ class AttentionPlan(_Kept):
                 pass
 
     def check(self, stream=None):
-        """Waits for the calls so far and raises if one of them gave up."""
+        """Waits for the calls so far and raises if one of them gave up: its outputs
+        are void, and later calls with this plan do nothing."""
         index = self.device.index
         if stream is None:
             stream = torch._C._cuda_getCurrentRawStream(index)

@@ -285,7 +285,8 @@ typedef struct {
 EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_paged_attention_args *a,
                                   void *stream);
 /* Reads the plan's status word (waits for `stream`): EMMY_EKERNEL when a call   */
-/* that used these device words gave up on a wait, and its outputs are void.     */
+/* that used these device words gave up on a wait.  Its outputs are void; later   */
+/* calls with these words do nothing, until the plan's words are copied anew.     */
 EMMY_API int emmy_paged_plan_status(emmy_paged_plan_t plan, uint64_t plan_words, void *stream);
 
 #ifdef __cplusplus

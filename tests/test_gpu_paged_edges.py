@@ -128,3 +128,23 @@ def test_a_batch_without_keys_needs_no_cache(causal):
                                        out=torch.full_like(q, 7.0))
             plan.check()
             assert not out.any() and bool((lse == -math.inf).all())
+
+
+# ------------------------------------------------------------------- gave up
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 3], [9000, 70]), ([1, 300], [9000, 900]), ([300], [900])])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_plan_that_gave_up_stays_so(dim, q_lens, kv_lens):
+    """Once a wait ran out (here: the word that says so is set), later calls with the plan write nothing."""
+    made = make(q_lens, kv_lens, 8, 2, dim, 16)
+    plan = paged.AttentionPlan(q_lens, kv_lens, 8, 2, dim)
+    plan.words[0] = 2
+    words = plan.words.clone()
+    out, lse = torch.full_like(made[0], 7.0), torch.full(made[0].shape[:2], 7.0, device="cuda")
+    paged.attention(plan, *made, out=out, lse=lse)
+    with pytest.raises(native.EmmyError, match="ran out"):
+        plan.check()
+    assert bool((out == 7.0).all()) and bool((lse == 7.0).all()) and torch.equal(plan.words, words)
+    plan.words[0] = 0
+    paged.attention(plan, *made, out=out, lse=lse)
+    plan.check()
+    close(out, lse, definition(*made, q_lens, kv_lens, dim ** -0.5), UNIT[torch.bfloat16])
