@@ -87,9 +87,14 @@ def _call(name, index, stream, *args):
         native.check(rc)
 
 
+def _stream_at(handle, device):
+    # 0 and 1 are the default stream; ExternalStream(0) is one of PyTorch's pool
+    return torch.cuda.default_stream(device) if handle in (0, 1) else torch.cuda.ExternalStream(handle, device=device)
+
+
 def _made_for(stream, t):
     """Memory allocated here and used on another stream is not reused before that stream is through."""
-    t.record_stream(torch.cuda.ExternalStream(stream, device=t.device))
+    t.record_stream(_stream_at(stream, t.device))
 
 
 class _Kept:

@@ -81,3 +81,19 @@ def test_a_cache_is_needed_where_a_token_sees_a_key(native_lib, change, kv_lens,
     native_lib.emmy_paged_attention(plan._h, a, None)
     said = any(word in native_lib.emmy_last_error() for word in (b"null", b"does not hold", b"a cache of"))
     assert said == refused, native_lib.emmy_last_error()
+
+
+# --------------------------------------------------------------------- streams
+@pytest.mark.parametrize("handle,name", [(0, "default"), (1, "default"), (2, "external 2"), (4096, "external 4096")])
+def test_memory_is_recorded_on_the_stream_that_a_handle_names(monkeypatch, handle, name):
+    """0 and 1 are the default stream; as an external one, 0 would be a stream of PyTorch's own."""
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda at, device=None: f"external {at}")
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: "default")
+    recorded = []
+
+    class Memory:
+        device = torch.device("cuda", 0)
+        record_stream = recorded.append
+
+    paged._made_for(handle, Memory())
+    assert recorded == [name]
