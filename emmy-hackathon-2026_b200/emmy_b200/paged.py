@@ -100,9 +100,11 @@ def _made_for(stream, t):
 class _Kept:
     """Device memory that calls on any stream use and that may be dropped while they run."""
 
-    def _keep(self, index, *tensors):
+    def _keep(self, *tensors):
+        # (recorded on the current stream too when that is first used: the tensors may be
+        # another's; on their own it does nothing)
         self._tensors = [t for t in tensors if t is not None]
-        self._streams = {torch._C._cuda_getCurrentRawStream(index)}
+        self._streams = set()
 
     def _used_on(self, stream):
         for t in self._tensors:
@@ -121,7 +123,7 @@ class Rotation(_Kept):
     def __init__(self, frequencies, axes=None, interleaved=False):
         device = _cuda_device("frequencies", frequencies)
         _check("frequencies", frequencies, 1, torch.float32, device)
-        self.frequencies = frequencies.contiguous()
+        self.frequencies = frequencies
         self.interleaved = bool(interleaved)
         self.axes = 1
         self.pair_axis = None
@@ -135,7 +137,7 @@ class Rotation(_Kept):
         self.components = 2 * self.frequencies.shape[0]
         self.device_index = device.index
         self.pair_axis_ptr = 0 if self.pair_axis is None else self.pair_axis.data_ptr()
-        self._keep(device.index, self.frequencies, self.pair_axis)
+        self._keep(self.frequencies, self.pair_axis)
 
 
 def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=None, stream=None):
@@ -260,7 +262,7 @@ class AttentionPlan(_Kept):
         self.device_index = self.device.index
         self.words_ptr, self.scratch_ptr = self.words.data_ptr(), self.scratch.data_ptr()
         if device.type == "cuda":
-            self._keep(device.index, self.words, self.scratch)
+            self._keep(self.words, self.scratch)
 
     def __del__(self):
         if self._h is not None:

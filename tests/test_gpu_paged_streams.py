@@ -84,3 +84,20 @@ def test_memory_of_one_stream_is_free_at_once():
     got = states()
     torch.cuda.synchronize()
     assert PENDING not in [got.get(a) for a in used]
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_frequencies_of_another_stream(given):
+    """Allocated on one stream; the rotation made and used under another, both dropped."""
+    case, side = Case(), torch.cuda.Stream()
+    frequencies = case.frequencies.clone()
+    address = frequencies.data_ptr()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        rotation = paged.Rotation(frequencies)
+        paged.rotate_append(rotation, case.q, case.kv, case.kv, case.at[0], case.slots, *case.caches, q_out=case.turned,
+                            **(dict(stream=side.cuda_stream) if given else {}))
+    del rotation, frequencies
+    got = states()
+    torch.cuda.synchronize()
+    assert got.get(address) == PENDING

@@ -97,3 +97,21 @@ def test_memory_is_recorded_on_the_stream_that_a_handle_names(monkeypatch, handl
 
     paged._made_for(handle, Memory())
     assert recorded == [name]
+
+
+def test_memory_that_others_allocated_is_recorded_on_every_stream(monkeypatch):
+    """Also on the stream that was current when it was handed over: it need not be from there."""
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 4096, raising=False)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda at, device=None: at)
+    recorded = []
+
+    class Memory:
+        device = torch.device("cuda", 0)
+        record_stream = recorded.append
+
+    kept = paged._Kept()
+    kept._keep(Memory(), None)
+    for stream in (4096, 8192, 4096, 8192):
+        if stream not in kept._streams:
+            kept._used_on(stream)
+    assert recorded == [4096, 8192]
