@@ -10,10 +10,13 @@ head_dim] with any strides of the outer dimensions, so ``[pages, kv_heads,
 page_size, head_dim]`` storage is passed as its ``transpose(1, 2)``.  Both
 operators run on the current stream of their tensors' device, or on the CUDA
 stream ``stream`` (its address; it has to last as long as what was allocated for
-calls on it: returned tensors, plans, rotations), and return without waiting.  They are thin over
-the C ABI (``emmy_rotate_append``, ``emmy_paged_attention`` in
-``include/emmy_b200.h``) and raise :class:`~.native.EmmyError` with its message
-on arguments it refuses, ``ValueError`` on what only Python can see.
+calls on it: returned tensors, plans, rotations), and return without waiting.
+Tensors that they return may be used on that stream and on the current one;
+those that they are given are the caller's to keep until a ``stream`` is through
+with them.  They are thin over the C ABI (``emmy_rotate_append``,
+``emmy_paged_attention`` in ``include/emmy_b200.h``) and raise
+:class:`~.native.EmmyError` with its message on arguments it refuses,
+``ValueError`` on what only Python can see.
 """
 from __future__ import annotations
 
@@ -95,6 +98,18 @@ def _stream_at(handle, device):
 def _made_for(stream, t):
     """Memory allocated here and used on another stream is not reused before that stream is through."""
     t.record_stream(_stream_at(stream, t.device))
+
+
+def _new(stream, like, shape, dtype):
+    """Memory for a result that the stream writes: its own, for what the current stream
+    had there before may still run; the caller's, on the current stream, as well."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    current = torch.cuda.current_stream(like.device)
+    with torch.cuda.stream(_stream_at(stream, like.device)):
+        t = like.new_empty(shape, dtype=dtype)
+    t.record_stream(current)
+    return t
 
 
 class _Kept:
@@ -187,9 +202,7 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
     if rotation.device_index != at:
         raise ValueError("rotation: on another device")
     if q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        if stream is not None:
-            _made_for(stream, q_out)
+        q_out = _new(stream, q, shape, dtype)
         q_out_stride = q_heads * dim, dim
     else:
         q_out_stride = _check("q_out", q_out, 3, dtype, q.device)[:2]
@@ -325,18 +338,14 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     if rows != plan.sequences:
         raise ValueError(f"table: {plan.sequences} rows are wanted, not {rows}")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        if stream is not None:
-            _made_for(stream, out)
+        out = _new(stream, q, shape, dtype)
         out_stride = shape[1] * dim, dim
     else:
         out_stride = _check("out", out, 3, dtype, q.device)[:2]
         if out.shape != shape:
             raise ValueError("out: another shape than q")
     if lse is None:
-        lse = q.new_empty(shape[:2], dtype=torch.float32)
-        if stream is not None:
-            _made_for(stream, lse)
+        lse = _new(stream, q, shape[:2], torch.float32)
     else:
         _check("lse", lse, 2, torch.float32, q.device)
         if lse.shape != shape[:2] or not lse.is_contiguous():

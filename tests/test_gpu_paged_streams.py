@@ -101,3 +101,31 @@ def test_frequencies_of_another_stream(given):
     got = states()
     torch.cuda.synchronize()
     assert got.get(address) == PENDING
+
+
+@pytest.mark.parametrize("side_is_current", [False, True])
+def test_results_for_a_given_stream_are_of_its_memory(side_is_current):
+    """What the current stream has let go of, and may still use, is not written by another;
+    results that are dropped wait for the current stream, which may have read them."""
+    case, side = Case(), torch.cuda.Stream()
+    current, user = (side, torch.cuda.default_stream()) if side_is_current else (torch.cuda.default_stream(), side)
+    with torch.cuda.stream(current):
+        plan, rotation = case.made()
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        held = [torch.empty_like(t) for t in (case.turned, case.out, case.lse)]
+        torch.cuda._sleep(1_000_000)
+        for t in held:
+            t.zero_()
+        freed = {t.data_ptr() for t in held}
+        del held, t
+        got = case.call(plan, rotation, given=False, stream=user.cuda_stream)
+        mine = {t.data_ptr() for t in got}
+        assert not mine & freed
+        current.wait_stream(user)
+        want = case.call(plan, rotation)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del got
+        now = states()
+        torch.cuda.synchronize()
+        assert [now.get(a) for a in mine] == [PENDING] * 3
