@@ -285,11 +285,14 @@ class AttentionPlan(_Kept):
                 pass
 
     def check(self, stream=None):
-        """Waits for the calls so far and raises if one of them gave up: its outputs
-        are void, and later calls with this plan do nothing."""
+        """Waits for the calls so far (with ``stream``, for those on it only) and raises
+        if one of them gave up: its outputs are void, and later calls with this
+        plan do nothing."""
         index = self.device.index
         if stream is None:
             stream = torch._C._cuda_getCurrentRawStream(index)
+            if not self._streams <= {stream}:
+                torch.cuda.synchronize(index)
         _call("emmy_paged_plan_status", index, stream, self._h, self.words.data_ptr())
 
 

@@ -129,3 +129,18 @@ def test_results_for_a_given_stream_are_of_its_memory(side_is_current):
         now = states()
         torch.cuda.synchronize()
         assert [now.get(a) for a in mine] == [PENDING] * 3
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_check_waits_for_calls_on_other_streams(given):
+    case, side = Case(), torch.cuda.Stream()
+    plan, rotation = case.made()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        if not given:
+            case.call(plan, rotation)
+    if given:
+        case.call(plan, rotation, stream=side.cuda_stream)
+    plan.check()
+    assert side.query()

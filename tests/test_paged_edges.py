@@ -115,3 +115,17 @@ def test_memory_that_others_allocated_is_recorded_on_every_stream(monkeypatch):
         if stream not in kept._streams:
             kept._used_on(stream)
     assert recorded == [4096, 8192]
+
+
+@pytest.mark.parametrize("used,given,waits", [({7}, None, False), ({8}, None, True), ({7, 8}, None, True), (set(), None, False),
+                                              ({7, 8}, 8, False)])
+def test_check_waits_for_every_stream_that_calls_ran_on(monkeypatch, used, given, waits):
+    """On the current one (7) alone its status is read in order; others are waited for first."""
+    plan = paged.AttentionPlan([1], [5], 8, 8, 64, device="cpu", ctas=1)
+    did = []
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 7, raising=False)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: did.append("all"))
+    monkeypatch.setattr(paged, "_call", lambda name, index, stream, *args: did.append(stream))
+    plan._streams = used
+    plan.check(given)
+    assert did == ["all"] * waits + [given or 7]
