@@ -12,7 +12,9 @@ constexpr int kTile = 128;          // keys of a tile, and rows of a tile of que
 // new token t * tokens_per_tile + r / G of the unit, query head r % G of the
 // group) against `ntiles` key tiles.  More than one tile of queries is a `wide`
 // unit.  An item is the same queries against all their keys; `nsplit` units
-// share one, each leaving a partial result in its rows of the scratch.
+// share one, each leaving a partial result in its rows of the scratch.  A CTA's
+// wide units come before its others: the kernel relies on that (a unit of few rows
+// joins its results where the second tile of queries of a wide unit would lie).
 struct Unit {
   int32_t seq, kvh;
   int32_t tok0, ntok;       // first row of q, new tokens

@@ -95,7 +95,7 @@ template <int D> struct Shape {
   static constexpr int kStages = D == 128 ? 5 : 12;      // key and value tiles in flight
   static constexpr int kRing = 2 * kTileBytes;           // after two query tiles
   static constexpr int kBars = kRing + kStages * kTileBytes;
-  static constexpr int kWords = kBars + (2 * kStages + 15) * 8, kEnd = kWords + 32 + kTile * 8;
+  static constexpr int kWords = kBars + (2 * kStages + 14) * 8, kEnd = kWords + 32 + kTile * 8;
   static_assert(kEnd + 1024 <= kSmem, "shared memory");
 };
 
@@ -342,8 +342,6 @@ template <int D, bool SPREAD> struct Smem {
   __device__ uint32_t drain(int t) const { return bar(2 * Shape<D>::kStages + 10 + t); }
   // wide units: stream t may issue
   __device__ uint32_t turn(int t) const { return bar(2 * Shape<D>::kStages + 12 + t); }
-  // what a unit's end keeps in the second query tile has been used
-  __device__ uint32_t scratch_free() const { return bar(2 * Shape<D>::kStages + 14); }
   __device__ volatile int *words() const { return static_cast<volatile int *>(__cvta_shared_to_generic(base + Shape<D>::kWords)); }
   __device__ float2 *ml() const { return static_cast<float2 *>(__cvta_shared_to_generic(base + Shape<D>::kWords + 32)); }
 };
@@ -421,7 +419,7 @@ __device__ void load_role(const Params &p, const Smem<D, SPREAD> &sm, const Guar
   Ring<D> ring;
   uint32_t issued = 0, parity = 0;       // of each stage: the last copy into it
   uint32_t q_phase = 0, queries_out = 1;      // out: the last load's phase of q_full
-  bool alive = true, was_spread = false;
+  bool alive = true;
   for (int i = first; i < last && alive; ++i) {
     const Unit u = read_unit(p, i);
     if (!u.ntiles) continue;
@@ -438,16 +436,14 @@ __device__ void load_role(const Params &p, const Smem<D, SPREAD> &sm, const Guar
     };
     Box b0 = box_of(0), b1 = box_of(1), b2 = box_of(2);
     // The queries go when the last unit's have been used, values meanwhile: only a
-    // full ring waits for them.  After a spread unit the second tile has to wait
-    // until the parts joined in its place have been read.
+    // full ring waits for them.  (What spread units join in the second tile's place is
+    // never in their way: a CTA's wide units come before its others.)
     bool queries_due = VALUES;
     auto queries = [&](bool now) {
-      const bool second = u.wide && was_spread;
       if (!now) {
-        const bool free = bar_test(sm.q_empty(), q_phase ^ 1) && (!second || bar_test(sm.scratch_free(), q_phase ^ 1));
-        if (!__all_sync(~0u, free)) return;
+        if (!__all_sync(~0u, bar_test(sm.q_empty(), q_phase ^ 1))) return;
       } else {
-        alive = g.wait(sm.q_empty(), q_phase ^ 1, 5) && (!second || g.wait(sm.scratch_free(), q_phase ^ 1, 5));
+        alive = g.wait(sm.q_empty(), q_phase ^ 1, 5);
         if (!alive) return;
       }
       if (elected()) load_queries(p, sm, u);
@@ -491,7 +487,6 @@ __device__ void load_role(const Params &p, const Smem<D, SPREAD> &sm, const Guar
     if (VALUES) {
       if (alive && queries_due) queries(true);
       if (alive) q_phase ^= 1;
-      was_spread = spread(p, sm, u);
     }
     ring.next(2 * u.ntiles - at);
   }
@@ -1019,7 +1014,6 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
             }
           }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");    // queries may come here next
         group_sync(1, kTile);
         if (wid == 0 && lane < rows && alive) {
           if (split)
@@ -1099,7 +1093,6 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
       }
     }
     if (joined) group_sync(3, 256);       // stream 1's output and sums have been read
-    if (u.ntiles && threadIdx.x == 0) bar_arrive(sm.scratch_free());
   }
 }
 
@@ -1120,7 +1113,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
     }
     bar_init(sm.q_full(), 1);
     bar_init(sm.q_empty(), 2);
-    bar_init(sm.scratch_free(), 1);
     for (int t = 0; t < 2; ++t) {
       bar_init(sm.s_full(t), 1);
       bar_init(sm.p_ready(t, 0), 4);

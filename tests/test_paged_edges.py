@@ -1,5 +1,6 @@
 """Paged-cache operators on the CPU: arguments at the ends of their ranges, and the
 order and streams that the kernels and their memory rely on."""
+import random
 import sys
 
 import pytest
@@ -129,3 +130,20 @@ def test_check_waits_for_every_stream_that_calls_ran_on(monkeypatch, used, given
     plan._streams = used
     plan.check(given)
     assert did == ["all"] * waits + [given or 7]
+
+
+# ----------------------------------------------------------------------- order
+@pytest.mark.parametrize("seed", range(40))
+def test_wide_units_of_a_cta_come_first(seed):
+    """The kernel gives what a unit of few rows joins the place of a wide unit's queries."""
+    r = random.Random(seed)
+    n = r.randint(1, 12)
+    q_lens = [r.choice((0, 1, 1, 2, 17, 64, 300, 1000)) for _ in range(n)]
+    kv_lens = [r.choice((0, 5, 130, 1000, 9000)) for _ in range(n)]
+    kv_heads = r.choice((1, 2, 8))
+    plan = paged.AttentionPlan(q_lens, kv_lens, kv_heads * r.choice((1, 3, 4, 32)), kv_heads, r.choice((64, 128)),
+                               window=r.choice((None, 100)), device="cpu", ctas=r.choice((1, 2, 7, 148)))
+    units, first, _ = units_of(plan)
+    for a, b in zip(first, first[1:]):
+        wide = [u["wide"] for u in units[a:b]]
+        assert wide == sorted(wide, reverse=True)
