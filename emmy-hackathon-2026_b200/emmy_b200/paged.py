@@ -16,7 +16,8 @@ those that they are given are the caller's to keep until a ``stream`` is through
 with them.  They are thin over the C ABI (``emmy_rotate_append``,
 ``emmy_paged_attention`` in ``include/emmy_b200.h``) and raise
 :class:`~.native.EmmyError` with its message on arguments it refuses,
-``ValueError`` on what only Python can see.
+``ValueError`` on what only Python can see.  They have no backward pass, and
+refuse tensors that require grad unless gradients are off.
 """
 from __future__ import annotations
 
@@ -62,6 +63,12 @@ def _check(name, t, ndim, dtype, device):
     if stride[-1] != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: the innermost stride must be 1")
     return stride
+
+
+def _no_backward(*tensors):
+    """For serving: the results would be cut off from what made them without a word."""
+    if any(getattr(t, "requires_grad", False) for t in tensors):
+        raise ValueError("a tensor requires grad, and this operator has no backward pass: call it under torch.no_grad()")
 
 
 def _unfit(e):
@@ -163,7 +170,8 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
     float16 or float32.  ``positions`` int32 [tokens], or [axes, tokens] for a
     rotation of several axes.  ``slots`` int32 [tokens]: token ``s % page_size``
     of page ``s // page_size``; a slot outside the cache (-1, say) stores
-    nothing.  ``q_out`` may be ``q`` itself.  Rotates in 32 bits, with angles
+    nothing; of two tokens with one slot, each component is one or the other's.
+    ``q_out`` may be ``q`` itself.  Rotates in 32 bits, with angles
     formed in 64, and rounds once."""
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError("q: a CUDA tensor is wanted")
@@ -186,6 +194,8 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
                                     ("v_cache", v_cache, 4, dtype), ("positions", positions, 2, torch.int32),
                                     ("slots", slots, 1, torch.int32)):
             _check(name, t, ndim, kind, q.device)
+    if torch.is_grad_enabled():
+        _no_backward(q, k, v, k_cache, v_cache, q_out, rotation.frequencies)
     shape = q.shape
     tokens, q_heads, dim = shape
     cache_shape = k_cache.shape
@@ -326,6 +336,8 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
         for name, t, ndim, kind in (("q", q, 3, dtype), ("k_cache", k_cache, 4, dtype), ("v_cache", v_cache, 4, dtype),
                                     ("table", table, 2, torch.int32)):
             _check(name, t, ndim, kind, q.device)
+    if torch.is_grad_enabled():
+        _no_backward(q, k_cache, v_cache, out, lse)
     if at != plan.device_index:
         raise ValueError(f"q: on {q.device}, the plan on {plan.device}")
     shape = plan.shape

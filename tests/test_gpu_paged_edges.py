@@ -148,3 +148,41 @@ def test_a_plan_that_gave_up_stays_so(dim, q_lens, kv_lens):
     paged.attention(plan, *made, out=out, lse=lse)
     plan.check()
     close(out, lse, definition(*made, q_lens, kv_lens, dim ** -0.5), UNIT[torch.bfloat16])
+
+
+# ------------------------------------------------------------------ gradients
+def _rotate_inputs():
+    cache = [torch.zeros(4, 16, 2, 64, device="cuda") for _ in range(2)]
+    q, k, v = (torch.randn(5, n, 64, device="cuda") for n in (4, 2, 2))
+    at = torch.arange(5, dtype=torch.int32, device="cuda")
+    return paged.Rotation(torch.ones(32, device="cuda")), q, k, v, at, at, *cache
+
+
+@pytest.mark.parametrize("which", [1, 2, 3, 6, 7, "q_out", "frequencies"])
+def test_rotate_append_has_no_backward(which):
+    args, kw = list(_rotate_inputs()), {}
+    if which == "q_out":
+        kw["q_out"] = torch.zeros_like(args[1], requires_grad=True)
+    elif which == "frequencies":
+        args[0].frequencies.requires_grad_()
+    else:
+        args[which].requires_grad_()
+    with pytest.raises(ValueError, match="backward"):
+        paged.rotate_append(*args, **kw)
+    with torch.no_grad():
+        paged.rotate_append(*args, **kw)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2, "out", "lse"])
+def test_attention_has_no_backward(which):
+    args, kw = list(make([2], [64], 4, 2, 64, 16, poison=0.0)), {}
+    plan = paged.AttentionPlan([2], [64], 4, 2, 64)
+    if isinstance(which, str):
+        kw[which] = torch.zeros((2, 4, 64) if which == "out" else (2, 4), device="cuda",
+                                dtype=torch.bfloat16 if which == "out" else torch.float32, requires_grad=True)
+    else:
+        args[which].requires_grad_()
+    with pytest.raises(ValueError, match="backward"):
+        paged.attention(plan, *args, **kw)
+    with torch.inference_mode():
+        paged.attention(plan, *args, **kw)
