@@ -36,6 +36,7 @@ _ROTATE_APPEND_ARGS = struct.Struct("@10i10Q15q")
 _ATTENTION_ARGS = struct.Struct("@4if8Q11q")
 
 _i32 = ctypes.c_int32
+_CONTIGUOUS = torch.contiguous_format
 
 
 class _PlanArgs(ctypes.Structure):
@@ -65,10 +66,16 @@ def _check(name, t, ndim, dtype, device):
     return stride
 
 
-def _no_backward(*tensors):
+def _no_backward():
     """For serving: the results would be cut off from what made them without a word."""
-    if any(getattr(t, "requires_grad", False) for t in tensors):
-        raise ValueError("a tensor requires grad, and this operator has no backward pass: call it under torch.no_grad()")
+    raise ValueError("a tensor requires grad, and this operator has no backward pass: call it under torch.no_grad()")
+
+
+# what every call asks (of a device that is up: its tensors are there)
+_grads_on, _empty_like = torch.is_grad_enabled, torch.empty_like
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# as any operation in place does: autograd checks what it keeps by it
+_written_to = torch.autograd.graph.increment_version
 
 
 def _unfit(e):
@@ -89,7 +96,7 @@ def _call(name, index, stream, *args):
     fn = _fns.get(name)
     if fn is None:
         fn = _fns[name] = getattr(native.lib(), name)
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         with torch.cuda.device(index):
             return _call(name, index, stream, *args)
     rc = fn(*args, stream)
@@ -110,8 +117,6 @@ def _made_for(stream, t):
 def _new(stream, like, shape, dtype):
     """Memory for a result that the stream writes: its own, for what the current stream
     had there before may still run; the caller's, on the current stream, as well."""
-    if stream is None:
-        return like.new_empty(shape, dtype=dtype)
     current = torch.cuda.current_stream(like.device)
     with torch.cuda.stream(_stream_at(stream, like.device)):
         t = like.new_empty(shape, dtype=dtype)
@@ -158,6 +163,7 @@ class Rotation(_Kept):
                 self.pair_axis = torch.tensor(axes, dtype=torch.int32, device=device)
         self.components = 2 * self.frequencies.shape[0]
         self.device_index = device.index
+        self.frequencies_ptr = frequencies.data_ptr()
         self.pair_axis_ptr = 0 if self.pair_axis is None else self.pair_axis.data_ptr()
         self._keep(self.frequencies, self.pair_axis)
 
@@ -194,8 +200,10 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
                                     ("v_cache", v_cache, 4, dtype), ("positions", positions, 2, torch.int32),
                                     ("slots", slots, 1, torch.int32)):
             _check(name, t, ndim, kind, q.device)
-    if torch.is_grad_enabled():
-        _no_backward(q, k, v, k_cache, v_cache, q_out, rotation.frequencies)
+    grads = _grads_on()
+    if grads and (q.requires_grad or k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+                  or rotation.frequencies.requires_grad):
+        _no_backward()
     shape = q.shape
     tokens, q_heads, dim = shape
     cache_shape = k_cache.shape
@@ -212,26 +220,29 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
     if rotation.device_index != at:
         raise ValueError("rotation: on another device")
     if q_out is None:
-        q_out = _new(stream, q, shape, dtype)
+        q_out = _empty_like(q, memory_format=_CONTIGUOUS) if stream is None else _new(stream, q, shape, dtype)
         q_out_stride = q_heads * dim, dim
     else:
         q_out_stride = _check("q_out", q_out, 3, dtype, q.device)[:2]
         if q_out.shape != shape:
             raise ValueError("q_out: another shape than q")
+        if grads and q_out.requires_grad:
+            _no_backward()
     try:
         a = _ROTATE_APPEND_ARGS.pack(
             _DTYPES[dtype], tokens, q_heads, kv_heads, dim, rotation.components, axes, rotation.interleaved, pages, page_size,
             q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            positions.data_ptr(), slots.data_ptr(), rotation.frequencies.data_ptr(), rotation.pair_axis_ptr,
+            positions.data_ptr(), slots.data_ptr(), rotation.frequencies_ptr, rotation.pair_axis_ptr,
             *q_stride[:2], *k_stride[:2], *v_stride[:2], *q_out_stride, *k_cache_stride[:3], *v_cache_stride[:3],
             positions_stride[0])
     except (struct.error, OverflowError) as e:
         raise _unfit(e) from None
     if stream is None:
-        stream = torch._C._cuda_getCurrentRawStream(at)
+        stream = _current_stream(at)
     if stream not in rotation._streams:
         rotation._used_on(stream)
     _call("emmy_rotate_append", at, stream, a)
+    _written_to((k_cache, v_cache, q_out))
     return q_out
 
 
@@ -336,8 +347,9 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
         for name, t, ndim, kind in (("q", q, 3, dtype), ("k_cache", k_cache, 4, dtype), ("v_cache", v_cache, 4, dtype),
                                     ("table", table, 2, torch.int32)):
             _check(name, t, ndim, kind, q.device)
-    if torch.is_grad_enabled():
-        _no_backward(q, k_cache, v_cache, out, lse)
+    grads = _grads_on()
+    if grads and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        _no_backward()
     if at != plan.device_index:
         raise ValueError(f"q: on {q.device}, the plan on {plan.device}")
     shape = plan.shape
@@ -352,19 +364,24 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     rows, width = table.shape
     if rows != plan.sequences:
         raise ValueError(f"table: {plan.sequences} rows are wanted, not {rows}")
+    given = out is not None or lse is not None
     if out is None:
-        out = _new(stream, q, shape, dtype)
+        out = _empty_like(q, memory_format=_CONTIGUOUS) if stream is None else _new(stream, q, shape, dtype)
         out_stride = shape[1] * dim, dim
     else:
         out_stride = _check("out", out, 3, dtype, q.device)[:2]
         if out.shape != shape:
             raise ValueError("out: another shape than q")
+        if grads and out.requires_grad:
+            _no_backward()
     if lse is None:
-        lse = _new(stream, q, shape[:2], torch.float32)
+        lse = q.new_empty(shape[:2], dtype=torch.float32) if stream is None else _new(stream, q, shape[:2], torch.float32)
     else:
         _check("lse", lse, 2, torch.float32, q.device)
         if lse.shape != shape[:2] or not lse.is_contiguous():
             raise ValueError(f"lse: contiguous {list(shape[:2])} is wanted")
+        if grads and lse.requires_grad:
+            _no_backward()
     try:
         a = _ATTENTION_ARGS.pack(
             _DTYPES[dtype], pages, page_size, width, plan.scale if scale is None else scale,
@@ -374,8 +391,10 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     except (struct.error, OverflowError) as e:
         raise _unfit(e) from None
     if stream is None:
-        stream = torch._C._cuda_getCurrentRawStream(at)
+        stream = _current_stream(at)
     if stream not in plan._streams:
         plan._used_on(stream)
     _call("emmy_paged_attention", at, stream, plan._h, a)
+    if given:
+        _written_to((out, lse))
     return out, lse

@@ -235,7 +235,8 @@ typedef struct {
 
 /* Turns every pair of the leading rotary_dim components of q and k by          */
 /* position x frequency, writes the queries to q_out and the keys and values    */
-/* to the cache slots of their tokens.  Two tokens with one slot: either stays. */
+/* to the cache slots of their tokens.  Two tokens with one slot: each component */
+/* is one or the other's.                                                       */
 EMMY_API int emmy_rotate_append(const emmy_rotate_append_args *a, void *stream);
 
 typedef struct emmy_paged_plan_s *emmy_paged_plan_t;

@@ -186,3 +186,27 @@ def test_attention_has_no_backward(which):
         paged.attention(plan, *args, **kw)
     with torch.inference_mode():
         paged.attention(plan, *args, **kw)
+
+
+# ------------------------------------------------------------------- versions
+def test_what_is_written_is_known_to_autograd():
+    """A tensor that another operation keeps for its gradient and that is then written here."""
+    rotation, q, k, v, at, _, kc, vc = _rotate_inputs()
+    for kept in (q, kc, vc):
+        w = torch.ones_like(kept, requires_grad=True)
+        y = (w * kept).sum()
+        paged.rotate_append(rotation, q, k, v, at, at, kc, vc, q_out=q)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    made = make([2], [64], 4, 2, 64, 16, poison=0.0)
+    plan = paged.AttentionPlan([2], [64], 4, 2, 64)
+    out, lse = torch.zeros_like(made[0]), torch.zeros(2, 4, device="cuda")
+    for kept in (out, lse):
+        w = torch.ones_like(kept, requires_grad=True)
+        y = (w * kept).sum()
+        paged.attention(plan, *made, out=out, lse=lse)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    with torch.inference_mode():                   # tensors without a version counter
+        out = torch.empty_like(made[0])
+        paged.attention(plan, *made, out=out)
