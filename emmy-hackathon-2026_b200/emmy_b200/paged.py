@@ -127,11 +127,15 @@ def _new(stream, like, shape, dtype):
 class _Kept:
     """Device memory that calls on any stream use and that may be dropped while they run."""
 
-    def _keep(self, *tensors):
-        # (recorded on the current stream too when that is first used: the tensors may be
-        # another's; on their own it does nothing)
+    def _keep(self, *tensors, own=False):
+        # own: allocated on the current stream just now; others may come from any
         self._tensors = [t for t in tensors if t is not None]
         self._streams = set()
+        current = torch._C._cuda_getCurrentRawStream(tensors[0].device.index)
+        if own:
+            self._streams.add(current)
+        else:
+            self._used_on(current)
 
     def _used_on(self, stream):
         for t in self._tensors:
@@ -233,7 +237,8 @@ def rotate_append(rotation, q, k, v, positions, slots, k_cache, v_cache, q_out=N
             _DTYPES[dtype], tokens, q_heads, kv_heads, dim, rotation.components, axes, rotation.interleaved, pages, page_size,
             q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
             positions.data_ptr(), slots.data_ptr(), rotation.frequencies_ptr, rotation.pair_axis_ptr,
-            *q_stride[:2], *k_stride[:2], *v_stride[:2], *q_out_stride, *k_cache_stride[:3], *v_cache_stride[:3],
+            q_stride[0], q_stride[1], k_stride[0], k_stride[1], v_stride[0], v_stride[1], q_out_stride[0], q_out_stride[1],
+            k_cache_stride[0], k_cache_stride[1], k_cache_stride[2], v_cache_stride[0], v_cache_stride[1], v_cache_stride[2],
             positions_stride[0])
     except (struct.error, OverflowError) as e:
         raise _unfit(e) from None
@@ -296,7 +301,7 @@ class AttentionPlan(_Kept):
         self.device_index = self.device.index
         self.words_ptr, self.scratch_ptr = self.words.data_ptr(), self.scratch.data_ptr()
         if device.type == "cuda":
-            self._keep(self.words, self.scratch)
+            self._keep(self.words, self.scratch, own=True)
 
     def __del__(self):
         if self._h is not None:
@@ -386,7 +391,8 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
         a = _ATTENTION_ARGS.pack(
             _DTYPES[dtype], pages, page_size, width, plan.scale if scale is None else scale,
             q.data_ptr(), out.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
-            plan.words_ptr, plan.scratch_ptr, *q_stride[:2], *out_stride, *k_cache_stride[:3], *v_cache_stride[:3],
+            plan.words_ptr, plan.scratch_ptr, q_stride[0], q_stride[1], out_stride[0], out_stride[1],
+            k_cache_stride[0], k_cache_stride[1], k_cache_stride[2], v_cache_stride[0], v_cache_stride[1], v_cache_stride[2],
             table_stride[0])
     except (struct.error, OverflowError) as e:
         raise _unfit(e) from None
