@@ -37,7 +37,8 @@
 // exponentials 1,340), P V and Q K^T (1,100), 3,030 cycles for both streams where
 // the tensor cores alone take 2,048 and the exponential unit as much: 1,180 to
 // 1,280 TFLOP/s at units of 64 and 128 tiles, 8 prompts of 4,096 tokens with 32 + 8
-// heads of 128 in 1.0 ms (1,100 TFLOP/s of what causal attention needs).
+// heads of 128 in 0.99 ms replayed from a graph (1,105 TFLOP/s of what causal attention
+// needs) and 1.08 ms called again and again, where the power limit lowers the clock.
 //
 // Every wait is bounded; one that runs out sets the plan's status word, and
 // from then on its CTA issues nothing more, and later calls do nothing.
@@ -706,7 +707,7 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
   // exponent bits get a base 6 lower, so that small weights keep their bits
   constexpr float kShift = BF16 ? 0.f : 6.f, kGrow = 8.f;
   // with 64 components every fourth pair's exponentials off the exponential unit: 4
-  // prompts of 4,096 tokens, 32 + 8 heads, 377 us against 387 with every eighth and 392
+  // prompts of 4,096 tokens, 32 + 8 heads, 374 us against 387 with every eighth and 392
   // with none; 8 chunks of 1 to 511 over 12,288, 32 + 4 heads, 163 us against 166 with
   // every eighth.  With 128 components the tensor cores set the power: cycles saved
   // (3,030 -> 2,820 a tile pair) come back as a lower clock, nothing is gained

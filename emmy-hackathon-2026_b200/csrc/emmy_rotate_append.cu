@@ -18,7 +18,8 @@
 // is turned: with one token ahead in registers 1,024 threads an SM kept too few
 // bytes in flight (4,700 GB/s).  Blocks of 384 threads take the 48 heads of the
 // video case in one share, with its angles formed once: 65 us, 6,150 GB/s, against
-// 70 us of 256 in two; 4,095 tokens of 32 + 32 heads 35 us, 5,700 GB/s.
+// 70 us of 256 in two; 4,095 tokens of 32 + 32 heads 35 us, 5,700 GB/s (replayed from a
+// graph; called again and again 71 and 37 us).
 //
 // The angle is formed in 64 bits as a count of half turns and reduced there:
 // at position 2^17 a 32-bit product is already off by 0.008 radians, and the

@@ -55,6 +55,29 @@ def test_infinite_values_outside_the_window(dim):
     close(out, lse, definition(q, *clean, table, q_lens, kv_lens, dim ** -0.5, window=100), UNIT[q.dtype])
 
 
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_keys_that_later_tokens_see(what, dim):
+    """A key that is not finite spoils the tokens that see it only (their score is NaN
+    or infinite), not the others of the chunk."""
+    q_lens, kv_lens = [3, 20, 300, 1], [300, 171, 640, 77]
+    q, k, v, table = make(q_lens, kv_lens, 8, 2, dim, 16)
+    want = definition(q, k, v, table, q_lens, kv_lens, dim ** -0.5)
+    clean = torch.ones(len(q), dtype=torch.bool, device="cuda")
+    start = 0
+    for s, (n, length) in enumerate(zip(q_lens, kv_lens)):
+        j = length - 1 - n // 3                                # the last n // 3 + 1 tokens see it
+        k[table[s, j // 16].long(), j % 16] = what
+        start += n
+        clean[start - n // 3 - 1:start] = False
+    plan = paged.AttentionPlan(q_lens, kv_lens, 8, 2, dim)
+    out, lse = paged.attention(plan, q, k, v, table)
+    plan.check()
+    close(out[clean], lse[clean], tuple(w[clean] for w in want), UNIT[q.dtype])
+    if math.isnan(what):
+        assert out[~clean].isnan().all() and lse[~clean].isnan().all()
+
+
 # ---------------------------------------------------------------- large scores
 @pytest.mark.parametrize("sign", [1, -1])
 @pytest.mark.parametrize("dtype,size", [(torch.bfloat16, n) for n in (20, 24, 27, 29, 33, 60, 112)] +
