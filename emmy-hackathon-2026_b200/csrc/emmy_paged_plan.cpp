@@ -7,7 +7,7 @@
 // CTAs that run at the same time share a head's keys in L2.  Units of one query
 // tile are bound by reading their keys and leave a small partial result, so
 // they are poured over the CTAs up to a common level, cut where a CTA is full.
-#include "emmy_paged.h"
+#include "emmy_quantised.h"
 
 #include <algorithm>
 #include <cstdio>
@@ -40,13 +40,17 @@ int fail(const char *fmt, long a = 0, long b = 0) {
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-void make(const emmy_paged_plan_args &a, emmy_paged_plan_s &plan) {
+void make(const emmy_paged_plan_args &a, const uint8_t *left_out, emmy_paged_plan_s &plan) {
   const int group = a.q_heads / a.kv_heads, per_tile = kTile / group;
   const Cost cost = a.head_dim == 64 ? kCost64 : kCost128;
   std::vector<Unit> wide, narrow;     // one unit an item, to be cut below
   int64_t first = 0;
   for (int s = 0; s < a.sequences; ++s) {
     const int n = a.q_lens[s], len = a.kv_lens[s];
+    if (left_out && left_out[s]) {
+      first += n;
+      continue;
+    }
     plan.max_kv = std::max(plan.max_kv, len);
     const int blocks = static_cast<int>(div_up(n, 2 * per_tile));
     for (int h = 0; h < a.kv_heads; ++h)
@@ -231,7 +235,7 @@ void make(const emmy_paged_plan_args &a, emmy_paged_plan_s &plan) {
 
 }  // namespace
 
-extern "C" EMMY_API int emmy_paged_plan_make(const emmy_paged_plan_args *a, emmy_paged_plan_t *out) {
+int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_out, emmy_paged_plan_t *out) {
   if (!a || !out || a->sequences < 0 || (a->sequences && (!a->q_lens || !a->kv_lens)))
     return fail("emmy_paged_plan_make: bad argument");
   *out = nullptr;
@@ -263,7 +267,7 @@ extern "C" EMMY_API int emmy_paged_plan_make(const emmy_paged_plan_args *a, emmy
     plan->causal = a->causal != 0;
     plan->window = args.window;
     try {
-      make(args, *plan);
+      make(args, left_out, *plan);
     } catch (...) {
       delete plan;
       throw;
@@ -279,6 +283,10 @@ extern "C" EMMY_API int emmy_paged_plan_make(const emmy_paged_plan_args *a, emmy
   } catch (...) {
     return emmy_internal_fail(EMMY_EINVAL, "emmy_paged_plan_make: failed");
   }
+}
+
+extern "C" EMMY_API int emmy_paged_plan_make(const emmy_paged_plan_args *a, emmy_paged_plan_t *out) {
+  return emmy_internal_paged_plan(a, nullptr, out);
 }
 
 extern "C" EMMY_API int emmy_paged_plan_data(emmy_paged_plan_t plan, const int32_t **words, size_t *n_words,

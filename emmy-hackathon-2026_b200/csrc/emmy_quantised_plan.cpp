@@ -1,0 +1,255 @@
+// emmy_quantised_plan.cpp -- cuts the attention over an 8-bit cache into work.
+//
+// A sequence whose query rows of a key head are few (kFewRows) is bound by reading
+// its keys, which a kernel of its own takes as they lie: its slices of 16 keys are
+// poured over the CTAs up to a common level, an item being cut where a CTA is full.
+// The others are bound by the tensor cores: their keys are read back to 16 bits once,
+// in pages of 128 tokens, and go through the 16-bit cache's attention.
+#include "emmy_quantised.h"
+
+#include <algorithm>
+#include <cstdio>
+#include <cstring>
+#include <memory>
+#include <new>
+
+int emmy_internal_fail(int code, const char *msg);   // emmy_runtime.cpp
+
+using namespace emmy_quantised;
+
+namespace {
+
+// What a piece costs beside its slices, in slices of its CTA (0.19 us where all CTAs
+// read), and the fewest that are worth a piece of their own.
+constexpr int kPieceCost = 6, kMinPiece = 16;
+constexpr int kCtasAnSm = 2;
+
+int fail(const char *fmt, long a = 0, long b = 0) {
+  char buf[256];
+  snprintf(buf, sizeof buf, fmt, a, b);
+  return emmy_internal_fail(EMMY_EINVAL, buf);
+}
+
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
+  const int group = a.q_heads / a.kv_heads;
+  std::vector<uint8_t> few(a.sequences);
+  bool any_others = false;
+  int most = 0;
+  for (int s = 0; s < a.sequences; ++s) {
+    const int64_t rows = int64_t(a.q_lens[s]) * group;
+    few[s] = rows <= kFewRows;
+    any_others = any_others || !few[s];
+    if (few[s]) most = std::max(most, static_cast<int>(rows));
+    plan.max_kv = std::max(plan.max_kv, a.kv_lens[s]);
+  }
+  plan.tiles = most <= 8 ? 1 : 4;
+  const int at_once = 8 * plan.tiles;
+
+  std::vector<Piece> items;
+  std::vector<Job> jobs;
+  std::vector<int32_t> table;
+  int64_t first = 0;
+  for (int s = 0; s < a.sequences; ++s) {
+    const int n = a.q_lens[s], len = a.kv_lens[s], pos0 = len - n;
+    // keys that new tokens from..to-1 see between them
+    auto lowest = [&](int from) { return a.window ? std::max(0, pos0 + from - a.window + 1) : 0; };
+    auto highest = [&](int to) { return a.causal ? std::max(0, std::min(len, pos0 + to)) : len; };
+    if (few[s]) {
+      for (int h = 0; h < a.kv_heads; ++h)
+        for (int r = 0; r < n * group; r += at_once) {
+          Piece p;
+          memset(&p, 0, sizeof p);
+          p.seq = s;
+          p.kvh = h;
+          p.tok0 = static_cast<int32_t>(first);
+          p.row0 = r;
+          p.rows = std::min(at_once, n * group - r);
+          p.pos0 = pos0;
+          p.kv_len = len;
+          p.lo = lowest(r / group);
+          p.hi = highest((r + p.rows - 1) / group + 1);
+          p.nsplit = 1;
+          if (p.hi > p.lo) {
+            p.slice0 = p.lo / kSlice;
+            p.nslices = (p.hi - 1) / kSlice + 1 - p.slice0;
+            plan.reads = true;
+          }
+          items.push_back(p);
+        }
+    } else if (highest(n) > lowest(0)) {
+      plan.reads = true;
+      for (int b = lowest(0) / kBlock; b * kBlock < highest(n); ++b) {
+        // (a token that no row sees is not used, but lies in a page that is)
+        jobs.push_back({s, b * kBlock, std::min(kBlock, len - b * kBlock), static_cast<int32_t>(plan.workspace_pages++)});
+      }
+    }
+    first += n;
+  }
+  plan.tokens = first;
+
+  // the lowest level up to which the items fit on the CTAs
+  const int slots = kCtasAnSm * a.ctas;
+  struct Part { int item, cta, b, e; };
+  std::vector<Part> parts;
+  auto pour = [&](int64_t level) {
+    parts.clear();
+    int c = 0;
+    int64_t filled = 0;
+    for (size_t i = 0; i < items.size(); ++i) {
+      int b = 0;
+      do {
+        const int rest = items[i].nslices - b, least = std::min(kMinPiece, std::max(1, rest));
+        while (level - filled - kPieceCost < least) {
+          if (++c == slots) return false;
+          filled = 0;
+        }
+        const int64_t room = level - filled - kPieceCost;
+        // a rest too small to be a piece of its own goes along
+        const int take = rest - room >= kMinPiece ? static_cast<int>(room) : rest;
+        parts.push_back({static_cast<int>(i), c, b, b + take});
+        filled += kPieceCost + take;
+        b += take;
+      } while (b < items[i].nslices);
+    }
+    return true;
+  };
+  std::vector<std::vector<Piece>> dealt(slots);
+  int counters = 0;
+  if (!items.empty()) {
+    int64_t low = kPieceCost, high = kPieceCost + kMinPiece;
+    while (!pour(high)) {
+      low = high;
+      high *= 2;
+    }
+    while (high - low > 1) {
+      const int64_t mid = low + (high - low) / 2;
+      (pour(mid) ? high : low) = mid;
+    }
+    pour(high);
+    for (size_t i = 0; i < parts.size();) {
+      size_t e = i + 1;
+      while (e < parts.size() && parts[e].item == parts[i].item) ++e;
+      Piece p = items[parts[i].item];
+      p.nsplit = static_cast<int32_t>(e - i);
+      if (p.nsplit > 1) {
+        p.item = counters++;
+        if (plan.part_rows > (int64_t(1) << 30)) throw 1;
+        p.part_row = static_cast<int32_t>(plan.part_rows);
+        plan.part_rows += int64_t(p.nsplit) * p.rows;
+      }
+      const int slice0 = p.slice0;
+      for (size_t k = i; k < e; ++k) {
+        p.slice0 = slice0 + parts[k].b;
+        p.nslices = parts[k].e - parts[k].b;
+        p.split = static_cast<int32_t>(k - i);
+        dealt[parts[k].cta].push_back(p);
+      }
+      i = e;
+    }
+  }
+  std::stable_partition(dealt.begin(), dealt.end(), [](const std::vector<Piece> &d) { return !d.empty(); });
+  int used = 0;
+  while (used < slots && !dealt[used].empty()) ++used;
+  size_t n_pieces = 0;
+  for (const auto &d : dealt) n_pieces += d.size();
+
+  if (any_others) {
+    emmy_paged_plan_t others = nullptr;
+    if (emmy_internal_paged_plan(&a, few.data(), &others)) throw 2;
+    plan.others = others;
+    for (const Job &j : jobs) plan.table_width = std::max(plan.table_width, j.first / kBlock + 1);
+    plan.table_width = std::max<int32_t>(plan.table_width, static_cast<int32_t>(div_up(others->max_kv, kBlock)));
+    table.assign(int64_t(a.sequences) * plan.table_width, 0);
+    for (const Job &j : jobs) table[int64_t(j.seq) * plan.table_width + j.first / kBlock] = j.page;
+    plan.n_jobs = static_cast<int32_t>(jobs.size());
+  }
+
+  Layout &at = plan.at;
+  int64_t words = used + 1;
+  auto place = [&](int64_t count, int64_t grid) {
+    const int64_t begin = div_up(words, grid) * grid;
+    words = begin + count;
+    return begin;
+  };
+  const int64_t at_counters = place(counters, 1), at_pieces = place(16 * int64_t(n_pieces), 16),
+                at_others = place(plan.others ? int64_t(plan.others->words.size()) : 0, 16),
+                at_table = place(int64_t(table.size()), 4), at_jobs = place(4 * int64_t(jobs.size()), 4);
+  if (words > (int64_t(1) << 30)) throw 1;
+  at.ctas = used;
+  at.counters = static_cast<int>(at_counters);
+  at.pieces = static_cast<int>(at_pieces);
+  at.others = static_cast<int>(at_others);
+  at.table = static_cast<int>(at_table);
+  at.jobs = static_cast<int>(at_jobs);
+  plan.words.assign(words, 0);
+  size_t k = 0;
+  for (int i = 0; i < used; ++i) {
+    plan.words[i] = static_cast<int32_t>(k);
+    memcpy(&plan.words[at.pieces + 16 * k], dealt[i].data(), dealt[i].size() * sizeof(Piece));
+    k += dealt[i].size();
+  }
+  plan.words[used] = static_cast<int32_t>(k);
+  if (plan.others) memcpy(&plan.words[at.others], plan.others->words.data(), 4 * plan.others->words.size());
+  if (!table.empty()) memcpy(&plan.words[at.table], table.data(), 4 * table.size());
+  if (!jobs.empty()) memcpy(&plan.words[at.jobs], jobs.data(), sizeof(Job) * jobs.size());
+}
+
+}  // namespace
+
+extern "C" EMMY_API int emmy_quantised_plan_make(const emmy_paged_plan_args *a, emmy_quantised_plan_t *out) {
+  if (!a || !out || a->sequences < 0 || (a->sequences && (!a->q_lens || !a->kv_lens)))
+    return fail("emmy_quantised_plan_make: bad argument");
+  *out = nullptr;
+  if (a->kv_heads < 1 || a->q_heads < 1 || a->q_heads % a->kv_heads || a->q_heads / a->kv_heads > kFewRows)
+    return fail("emmy_quantised_plan_make: %ld query heads for %ld key heads (1 to 128 times as many)", a->q_heads, a->kv_heads);
+  if (a->head_dim != 64 && a->head_dim != 128) return fail("emmy_quantised_plan_make: head_dim %ld (64 or 128)", a->head_dim);
+  if (a->window < 0 || (a->window && !a->causal))
+    return fail("emmy_quantised_plan_make: window %ld (a window is causal)", a->window);
+  if (a->ctas < 1 || a->ctas > 65536) return fail("emmy_quantised_plan_make: %ld CTAs", a->ctas);
+  int64_t tokens = 0;
+  int32_t longest = 0;
+  for (int s = 0; s < a->sequences; ++s) {
+    if (a->q_lens[s] < 0 || a->kv_lens[s] < 0 || a->q_lens[s] > (1 << 30) || a->kv_lens[s] > (1 << 30))
+      return fail("emmy_quantised_plan_make: sequence %ld has a length outside 0..2^30", s);
+    tokens += a->q_lens[s];
+    longest = std::max(longest, a->kv_lens[s]);
+  }
+  emmy_paged_plan_args args = *a;
+  if (args.window >= longest) args.window = 0;      // (hides no key)
+  if (tokens * a->q_heads > (int64_t(1) << 30)) return fail("emmy_quantised_plan_make: too many tokens");
+  try {
+    std::unique_ptr<emmy_quantised_plan_s> plan(new emmy_quantised_plan_s);
+    plan->sequences = a->sequences;
+    plan->q_heads = a->q_heads;
+    plan->kv_heads = a->kv_heads;
+    plan->head_dim = a->head_dim;
+    plan->causal = a->causal != 0;
+    plan->window = args.window;
+    make(args, *plan);
+    *out = plan.release();
+    return 0;
+  } catch (const std::bad_alloc &) {
+    return emmy_internal_fail(EMMY_ENOMEM, "emmy_quantised_plan_make: out of host memory");
+  } catch (int) {
+    return emmy_internal_fail(EMMY_EINVAL, "emmy_quantised_plan_make: too much work for one plan");
+  } catch (...) {
+    return emmy_internal_fail(EMMY_EINVAL, "emmy_quantised_plan_make: failed");
+  }
+}
+
+extern "C" EMMY_API int emmy_quantised_plan_data(emmy_quantised_plan_t plan, const int32_t **words, size_t *n_words, size_t *scratch) {
+  if (!plan || !words || !n_words || !scratch) return fail("emmy_quantised_plan_data: bad argument");
+  *words = plan->words.data();
+  *n_words = plan->words.size();
+  // partial rows of head_dim floats with (base, sum) of each; those of the others'
+  // plan; 16-bit keys and values read back: each from a multiple of 128 bytes on
+  const size_t row = (plan->head_dim + 2) * sizeof(float);
+  auto whole = [](size_t bytes) { return (bytes + 127) / 128 * 128; };
+  *scratch = whole(plan->part_rows * row) + (plan->others ? whole(plan->others->part_rows * row) : 0) +
+             size_t(plan->workspace_pages) * kBlock * plan->kv_heads * plan->head_dim * 2 * 2;
+  return 0;
+}
+
+extern "C" EMMY_API void emmy_quantised_plan_free(emmy_quantised_plan_t plan) { delete plan; }

@@ -25,6 +25,12 @@
 // at position 2^17 a 32-bit product is already off by 0.008 radians, and the
 // reduction of a large 32-bit angle would cost a slow path besides.  Rotation
 // is in 32 bits; the one rounding is to the cache's or q_out's type.
+//
+// With norms (queries and keys of each head times the reciprocal of their root mean
+// square and a weight) and a cache of 8-bit floats it is the same walk: the squares'
+// sums of a head's threads meet in shared memory at the barrier that the angles have
+// anyway, the weights of a thread's two vectors stay in registers, and keys and values
+// are multiplied by a power of two -- exactly -- and rounded once.
 #include "../../include/emmy_b200.h"
 
 #include <cuda_bf16.h>
@@ -34,18 +40,24 @@
 #include <atomic>
 #include <cstdint>
 #include <cstdio>
+#include <type_traits>
 
 int emmy_internal_fail(int code, const char *msg);   // emmy_runtime.cpp
 
 namespace {
 
 constexpr int kThreads = 384, kBlocks = 3;      // at most a block; at least an SM
+constexpr int kNormBlocks = 2;                  // with norms, whose weights take registers
 constexpr int kAhead = 3;                       // tokens in flight or being turned
 
 struct Params {
   emmy_rotate_append_args a;
   int lanes;                       // threads of a row: a head's vectors by two
+  uint64_t q_weight, k_weight, exponents;
+  float eps;
 };
+
+struct E4M3 { uint8_t bits; };     // an 8-bit float: 4 exponent bits, largest 448
 
 // N elements moved as one access: 16 bytes, or one element
 template <typename T, int N> struct alignas(N * sizeof(T)) Vec { T e[N]; };
@@ -97,6 +109,28 @@ template <int N> __device__ __forceinline__ void round_to(const float *f, Vec<__
   }
 }
 
+// the largest 8-bit float for what is larger; NaN stays
+template <int N> __device__ __forceinline__ void round_to(const float *f, Vec<E4M3, N> &v) {
+  uint16_t two;
+  if constexpr (N == 1) {
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(f[0]));
+    v.e[0].bits = static_cast<uint8_t>(two);
+  } else {
+    uint32_t words[N / 4];
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+      uint16_t more;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(f[e + 1]), "f"(f[e]));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(more) : "f"(f[e + 3]), "f"(f[e + 2]));
+      words[e / 4] = two | uint32_t(more) << 16;
+    }
+    if constexpr (N == 8)
+      *reinterpret_cast<uint2 *>(&v) = make_uint2(words[0], words[1]);
+    else
+      *reinterpret_cast<uint32_t *>(&v) = words[0];
+  }
+}
+
 template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const void *from) {
   const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
   if constexpr (BYTES == 16)
@@ -108,10 +142,11 @@ template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const 
 // blockDim = (lanes, heads, tokens); blockIdx.y: the block's share of the heads
 // of queries, keys and values.  WITHIN: the pairs lie inside a vector
 // (interleaved, N > 1); otherwise a pair is one element of each of the thread's
-// two vectors.
-template <typename T, int N, bool WITHIN>
-__global__ void __launch_bounds__(kThreads, kBlocks) rotate_append_kernel(const __grid_constant__ Params p) {
+// two vectors.  C: the cache's elements, T or 8-bit floats.
+template <typename T, typename C, int N, bool WITHIN, bool NORM>
+__global__ void __launch_bounds__(kThreads, NORM ? kNormBlocks : kBlocks) rotate_append_kernel(const __grid_constant__ Params p) {
   using V = Vec<T, N>;
+  constexpr bool SMALL = !std::is_same<T, C>::value;
   extern __shared__ __align__(16) float angles[];
   const emmy_rotate_append_args &a = p.a;
   const int half = a.rotary_dim / 2, heads = a.q_heads + 2 * a.kv_heads;
@@ -122,6 +157,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_append_kernel(const 
   const bool query = head < a.q_heads, turns = head < a.q_heads + a.kv_heads, moves = head < heads;
   const T *src;
   T *dst;
+  [[maybe_unused]] C *small = nullptr;         // a cache of another type
+  [[maybe_unused]] float small_scale = 1.f;
   int64_t src_token, dst_page, dst_token;      // queries: dst_token of q_out, no pages
   if (query) {
     src = reinterpret_cast<const T *>(a.q) + head * a.q_stride[1];
@@ -136,6 +173,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_append_kernel(const 
     dst = reinterpret_cast<T *>(a.v_cache) + (head - a.q_heads - a.kv_heads) * a.v_cache_stride[2];
     src_token = a.v_stride[0], dst_page = a.v_cache_stride[0], dst_token = a.v_cache_stride[1];
   }
+  [[maybe_unused]] V weight_one{}, weight_two{};
   // its two vectors, `apart` elements from one another
   bool turn_one, turn_two;
   int apart, first_pair, second_pair;         // pairs of the first and (WITHIN) the second
@@ -158,6 +196,22 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_append_kernel(const 
     turn_one = turn_one && turns;
     turn_two = turn_two && turns;
     apart = two < a.head_dim ? two - one : 0;   // an odd head ends with one: moved twice
+    if constexpr (SMALL) {
+      if (!query && moves) {
+        const int kv_head = head - a.q_heads - (turns ? 0 : a.kv_heads);
+        small = (turns ? reinterpret_cast<C *>(a.k_cache) + kv_head * a.k_cache_stride[2]
+                       : reinterpret_cast<C *>(a.v_cache) + kv_head * a.v_cache_stride[2]) + one;
+        const int e = p.exponents ? reinterpret_cast<const int *>(p.exponents)[kv_head + (turns ? 0 : a.kv_heads)] : 0;
+        small_scale = exp2f(float(-min(max(e, EMMY_MIN_EXPONENT), EMMY_MAX_EXPONENT)));      // (exact)
+      }
+    }
+    if constexpr (NORM) {
+      if (turns) {
+        const T *w = reinterpret_cast<const T *>(query ? p.q_weight : p.k_weight) + one;
+        weight_one = *reinterpret_cast<const V *>(w);
+        weight_two = *reinterpret_cast<const V *>(w + apart);
+      }
+    }
     src += one;
     dst += one;
   }
@@ -184,6 +238,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_append_kernel(const 
   const int threads = blockDim.x * blockDim.y * blockDim.z, me = (threadIdx.z * blockDim.y + threadIdx.y) * blockDim.x + lane;
   V *const vectors = reinterpret_cast<V *>(angles + blockDim.z * 2 * a.rotary_dim) + me;       // [kAhead][2][threads]
   int *const numbers = reinterpret_cast<int *>(vectors - me + (COPIED ? kAhead * 2 * threads : 0)) + me;   // [kAhead][2][threads]
+  // sums of squares of this token and the next in turn, [2][threads]
+  [[maybe_unused]] float *const squares = reinterpret_cast<float *>(numbers - me + (COPIED ? kAhead * 2 * threads : 0)) + me;
+  [[maybe_unused]] int odd = 0;
   auto fetch = [&](int token, int stage) {
     if (COPIED && token < a.tokens) {
       if (moves) {
@@ -205,6 +262,25 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_append_kernel(const 
   for (int base = blockIdx.x * blockDim.z; base < a.tokens; base += step) {
     fetch(token + (kAhead - 1) * step, (stage + kAhead - 1) % kAhead);
     asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+    [[maybe_unused]] V read_one{}, read_two{};   // (q_out may be q: read before any of the head is written)
+    if constexpr (NORM) {
+      float sum = 0.f;
+      if (token < a.tokens && moves) {
+        const T *at = src + token * src_token;
+        read_one = COPIED ? vectors[stage * 2 * threads] : *reinterpret_cast<const V *>(at);
+        read_two = COPIED ? vectors[(stage * 2 + 1) * threads] : *reinterpret_cast<const V *>(at + apart);
+        float f[N], g[N];
+        widen(read_one, f);
+        widen(read_two, g);
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum += f[e] * f[e];
+        if (apart) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) sum += g[e] * g[e];
+        }
+      }
+      squares[odd] = sum;
+    }
     if (turning) {
       if (token < a.tokens && pair < half) {
         turn(angle, pair, COPIED ? numbers[(stage * 2 + 1) * threads] : positions[token], frequency);
@@ -215,14 +291,49 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_append_kernel(const 
       __syncthreads();
     }
     if (token < a.tokens && moves) {
-      const T *at = src + token * src_token;
-      V u = COPIED ? vectors[stage * 2 * threads] : *reinterpret_cast<const V *>(at);
-      V v = COPIED ? vectors[(stage * 2 + 1) * threads] : *reinterpret_cast<const V *>(at + apart);
+      V u, v;
+      if constexpr (NORM) {
+        u = read_one;
+        v = read_two;
+      } else {
+        const T *at = src + token * src_token;
+        u = COPIED ? vectors[stage * 2 * threads] : *reinterpret_cast<const V *>(at);
+        v = COPIED ? vectors[(stage * 2 + 1) * threads] : *reinterpret_cast<const V *>(at + apart);
+      }
       const int slot = query ? 0 : COPIED ? numbers[stage * 2 * threads] : slots[token];
-      if (turn_one) {
-        float f[N], g[N], c[N], s[N];
+      float f[N], g[N];
+      if constexpr (NORM || SMALL) {
         widen(u, f);
         widen(v, g);
+      }
+      if constexpr (NORM) {
+        if (turns) {
+          const float *of_head = squares - lane + odd;
+          float sum = 0.f;
+          if (p.lanes % 4 == 0) {
+            for (int i = 0; i < p.lanes; i += 4) {
+              const float4 x = *reinterpret_cast<const float4 *>(of_head + i);
+              sum += (x.x + x.y) + (x.z + x.w);
+            }
+          } else {
+            for (int i = 0; i < p.lanes; ++i) sum += of_head[i];
+          }
+          const float by = __frsqrt_rn(sum / float(a.head_dim) + p.eps);
+          float w[N];
+          widen(weight_one, w);
+#pragma unroll
+          for (int e = 0; e < N; ++e) f[e] = f[e] * by * w[e];
+          widen(weight_two, w);
+#pragma unroll
+          for (int e = 0; e < N; ++e) g[e] = g[e] * by * w[e];
+        }
+      }
+      if (turn_one) {
+        float c[N], s[N];
+        if constexpr (!NORM && !SMALL) {
+          widen(u, f);
+          widen(v, g);
+        }
         constexpr int M = N == 1 ? 1 : WITHIN ? N / 2 : 4;
         using Angles = Vec<float, M>;
 #pragma unroll
@@ -242,8 +353,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_append_kernel(const 
                         cg = c[N / 2 + e / 2], sg = s[N / 2 + e / 2];
             f[e] = f0 * ce - f1 * se;
             f[e + 1] = f1 * ce + f0 * se;
-            g[e] = g0 * cg - g1 * sg;
-            g[e + 1] = g1 * cg + g0 * sg;
+            if (!(NORM || SMALL) || turn_two) {      // (otherwise left out below)
+              g[e] = g0 * cg - g1 * sg;
+              g[e + 1] = g1 * cg + g0 * sg;
+            }
           }
         } else {
 #pragma unroll
@@ -253,10 +366,32 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_append_kernel(const 
             g[e] = ge * c[e] + fe * s[e];
           }
         }
-        round_to(f, u);
-        if (turn_two) round_to(g, v);
+        if constexpr (!NORM) {
+          round_to(f, u);
+          if (turn_two) round_to(g, v);
+        }
       }
-      if (query || (slot >= 0 && slot < n_slots)) {
+      if constexpr (NORM) {
+        if (turns) {
+          round_to(f, u);
+          round_to(g, v);
+        }
+      }
+      if (SMALL && !query) {
+        if constexpr (SMALL) {
+          if (slot >= 0 && slot < n_slots) {
+            const int page = slot / a.page_size;
+            C *to = small + page * dst_page + (slot - page * a.page_size) * dst_token;
+            Vec<C, N> r;
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] *= small_scale, g[e] *= small_scale;
+            round_to(f, r);
+            *reinterpret_cast<Vec<C, N> *>(to) = r;
+            round_to(g, r);
+            *reinterpret_cast<Vec<C, N> *>(to + apart) = r;
+          }
+        }
+      } else if (query || (slot >= 0 && slot < n_slots)) {
         T *to;
         if (query) {
           to = dst + token * dst_token;
@@ -268,6 +403,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_append_kernel(const 
         *reinterpret_cast<V *>(to + apart) = v;
       }
     }
+    if constexpr (NORM) odd = threads - odd;
     token += step;
     stage = (stage + 1) % kAhead;
     angle += flip;
@@ -287,7 +423,7 @@ int failed(cudaError_t e) {
   return emmy_internal_fail(static_cast<int>(e), buf);
 }
 
-template <typename T, int N, bool WITHIN> int launch(Params &p, cudaStream_t s) {
+template <typename T, typename C, int N, bool WITHIN, bool NORM> int launch(Params &p, cudaStream_t s) {
   const emmy_rotate_append_args &a = p.a;
   p.lanes = (a.head_dim / N + 1) / 2;
   // heads in shares of equal size, and a few tokens a block where one is small
@@ -307,21 +443,32 @@ template <typename T, int N, bool WITHIN> int launch(Params &p, cudaStream_t s) 
     if (dev < 64) known[dev].store(sms);
   }
   const int want = (a.tokens + tokens - 1) / tokens;
-  int resident = sms * (kBlocks * kThreads / (p.lanes * rows * tokens)) / shares;
+  int resident = sms * ((NORM ? kNormBlocks : kBlocks) * kThreads / (p.lanes * rows * tokens)) / shares;
   if (resident < 1) resident = 1;
   const dim3 grid(want < resident ? want : resident, shares), block(p.lanes, rows, tokens);
   // angles of two turns; vectors, slots and positions on their way (N > 1): with
   // 256 components and 384 threads 47 KiB, under the 48 that need no asking
   const size_t smem = size_t(tokens) * 2 * a.rotary_dim * sizeof(float) +
-                      (N > 1 ? size_t(kAhead) * 2 * p.lanes * rows * tokens * (16 + 4) : 0);
-  rotate_append_kernel<T, N, WITHIN><<<grid, block, smem, s>>>(p);
+                      (N > 1 ? size_t(kAhead) * 2 * p.lanes * rows * tokens * (16 + 4) : 0) +
+                      (NORM ? size_t(2) * p.lanes * rows * tokens * sizeof(float) : 0);
+  if constexpr (NORM) {
+    // up to 51 KiB with the squares
+    static std::atomic<uint64_t> ready{0};   // a bit for each device
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (smem > 48 * 1024 && (dev > 63 || !(ready.load() & bit))) {
+      e = cudaFuncSetAttribute(rotate_append_kernel<T, C, N, WITHIN, NORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
+      if (e != cudaSuccess) return failed(e);
+      if (dev <= 63) ready.fetch_or(bit);
+    }
+  }
+  rotate_append_kernel<T, C, N, WITHIN, NORM><<<grid, block, smem, s>>>(p);
   e = cudaGetLastError();
   return e == cudaSuccess ? 0 : failed(e);
 }
 
 // 16-byte accesses need every address and stride to be a multiple of 16 bytes
 // and heads, halves and the part that stays to be whole vectors.
-template <typename T> int dispatch(Params &p, cudaStream_t s) {
+template <typename T, typename C, bool NORM> int dispatch(Params &p, cudaStream_t s) {
   constexpr int N = 16 / sizeof(T);
   const emmy_rotate_append_args &a = p.a;
   uint64_t addr = 0;
@@ -331,46 +478,75 @@ template <typename T> int dispatch(Params &p, cudaStream_t s) {
     for (int i = 0; i < 2; ++i) strides |= a.q_stride[i] | a.q_out_stride[i];
   }
   if (a.kv_heads) {
-    addr |= a.k | a.v | a.k_cache | a.v_cache;
+    addr |= a.k | a.v | (a.k_cache | a.v_cache) * (sizeof(T) / sizeof(C));     // (N elements of 8 bits are N bytes)
     for (int i = 0; i < 2; ++i) strides |= a.k_stride[i] | a.v_stride[i];
     for (int i = 0; i < 3; ++i) strides |= a.k_cache_stride[i] | a.v_cache_stride[i];
   }
+  if (NORM) addr |= (a.q_heads ? p.q_weight : 0) | (a.kv_heads ? p.k_weight : 0);
   const bool whole = addr % 16 == 0 && strides % N == 0 && a.head_dim % (2 * N) == 0;
   // (vectors of angles: 16 bytes of shared memory hold the cosines of 4 pairs)
-  if (whole && a.interleaved && a.rotary_dim % N == 0 && a.rotary_dim % 8 == 0) return launch<T, N, true>(p, s);
-  if (whole && !a.interleaved && a.rotary_dim / 2 % N == 0) return launch<T, N, false>(p, s);
-  return launch<T, 1, false>(p, s);
+  if (whole && a.interleaved && a.rotary_dim % N == 0 && a.rotary_dim % 8 == 0) return launch<T, C, N, true, NORM>(p, s);
+  if (whole && !a.interleaved && a.rotary_dim / 2 % N == 0) return launch<T, C, N, false, NORM>(p, s);
+  return launch<T, C, 1, false, NORM>(p, s);
+}
+
+template <typename T> int dispatch(Params &p, bool small, bool norm, cudaStream_t s) {
+  if (small) return norm ? dispatch<T, E4M3, true>(p, s) : dispatch<T, E4M3, false>(p, s);
+  return norm ? dispatch<T, T, true>(p, s) : dispatch<T, T, false>(p, s);
+}
+
+// `name`: the entry's, for messages
+int run(const char *name, Params &p, bool small, bool norm, void *stream) {
+  const emmy_rotate_append_args *const a = &p.a;
+  auto bad = [&](const char *fmt, long x = 0, long y = 0) {
+    char with[256];
+    snprintf(with, sizeof with, "%s: %s", name, fmt);
+    return fail(with, x, y);
+  };
+  if (a->dtype != 6 && a->dtype != 7 && a->dtype != 9) return bad("dtype %ld (f16, f32 or bf16)", a->dtype);
+  if (a->tokens < 0 || a->tokens > (1 << 30) || a->q_heads < 0 || a->kv_heads < 0 || a->q_heads > 1024 || a->kv_heads > 1024)
+    return bad("bad count of tokens or heads");
+  if (a->head_dim < 1 || a->head_dim > 256) return bad("head_dim %ld outside 1..256", a->head_dim);
+  if (a->rotary_dim < 0 || a->rotary_dim > a->head_dim || a->rotary_dim % 2)
+    return bad("rotary_dim %ld must be even and at most head_dim %ld", a->rotary_dim, a->head_dim);
+  if (a->axes < 1 || a->axes > 16) return bad("%ld position axes (1..16)", a->axes);
+  if (a->kv_heads && (a->pages < 0 || a->page_size < 1)) return bad("a cache of %ld pages of %ld tokens", a->pages, a->page_size);
+  if (norm && !(p.eps >= 0.f)) return bad("eps must not be negative");
+  if (a->tokens == 0 || (a->q_heads == 0 && a->kv_heads == 0)) return 0;
+  if ((a->q_heads && (!a->q || !a->q_out)) ||
+      (a->kv_heads && (!a->k || !a->v || !a->slots || (a->pages && (!a->k_cache || !a->v_cache)))) ||
+      (a->rotary_dim && (!a->positions || !a->frequencies)) ||
+      (norm && ((a->q_heads && !p.q_weight) || (a->kv_heads && !p.k_weight))))
+    return bad("null address");
+  const uint64_t elements = (a->q_heads ? a->q | a->q_out : 0) | (a->kv_heads ? a->k | a->v : 0) |
+                            (a->kv_heads && !small ? a->k_cache | a->v_cache : 0) |
+                            (norm ? (a->q_heads ? p.q_weight : 0) | (a->kv_heads ? p.k_weight : 0) : 0);
+  if (elements % (a->dtype == 7 ? 4 : 2) || (a->kv_heads ? (a->slots | p.exponents) % 4 : 0) ||
+      (a->rotary_dim ? (a->positions | a->frequencies | a->pair_axis) % 4 : 0))
+    return bad("address not a multiple of its element's size");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->dtype == 6) return dispatch<__half>(p, small, norm, s);
+  if (a->dtype == 7) return dispatch<float>(p, small, norm, s);
+  return dispatch<__nv_bfloat16>(p, small, norm, s);
 }
 
 }  // namespace
 
 extern "C" EMMY_API int emmy_rotate_append(const emmy_rotate_append_args *a, void *stream) {
   if (!a) return fail("emmy_rotate_append: bad argument");
-  if (a->dtype != 6 && a->dtype != 7 && a->dtype != 9)
-    return fail("emmy_rotate_append: dtype %ld (f16, f32 or bf16)", a->dtype);
-  if (a->tokens < 0 || a->tokens > (1 << 30) || a->q_heads < 0 || a->kv_heads < 0 || a->q_heads > 1024 || a->kv_heads > 1024)
-    return fail("emmy_rotate_append: bad count of tokens or heads");
-  if (a->head_dim < 1 || a->head_dim > 256)
-    return fail("emmy_rotate_append: head_dim %ld outside 1..256", a->head_dim);
-  if (a->rotary_dim < 0 || a->rotary_dim > a->head_dim || a->rotary_dim % 2)
-    return fail("emmy_rotate_append: rotary_dim %ld must be even and at most head_dim %ld", a->rotary_dim, a->head_dim);
-  if (a->axes < 1 || a->axes > 16) return fail("emmy_rotate_append: %ld position axes (1..16)", a->axes);
-  if (a->kv_heads && (a->pages < 0 || a->page_size < 1))
-    return fail("emmy_rotate_append: a cache of %ld pages of %ld tokens", a->pages, a->page_size);
-  if (a->tokens == 0 || (a->q_heads == 0 && a->kv_heads == 0)) return 0;
-  if ((a->q_heads && (!a->q || !a->q_out)) ||
-      (a->kv_heads && (!a->k || !a->v || !a->slots || (a->pages && (!a->k_cache || !a->v_cache)))) ||
-      (a->rotary_dim && (!a->positions || !a->frequencies)))
-    return fail("emmy_rotate_append: null address");
-  const uint64_t elements = (a->q_heads ? a->q | a->q_out : 0) |
-                            (a->kv_heads ? a->k | a->v | a->k_cache | a->v_cache : 0);
-  if (elements % (a->dtype == 7 ? 4 : 2) || (a->kv_heads ? a->slots % 4 : 0) ||
-      (a->rotary_dim ? (a->positions | a->frequencies | a->pair_axis) % 4 : 0))
-    return fail("emmy_rotate_append: address not a multiple of its element's size");
-  Params p;
+  Params p{};
   p.a = *a;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == 6) return dispatch<__half>(p, s);
-  if (a->dtype == 7) return dispatch<float>(p, s);
-  return dispatch<__nv_bfloat16>(p, s);
+  return run("emmy_rotate_append", p, false, false, stream);
+}
+
+extern "C" EMMY_API int emmy_norm_rotate_append(const emmy_norm_rotate_append_args *a, void *stream) {
+  if (!a) return fail("emmy_norm_rotate_append: bad argument");
+  if (a->cache_bits8 != 0 && a->cache_bits8 != 1) return fail("emmy_norm_rotate_append: cache_bits8 %ld (0 or 1)", a->cache_bits8);
+  Params p{};
+  p.a = a->a;
+  p.q_weight = a->q_weight;
+  p.k_weight = a->k_weight;
+  p.eps = a->eps;
+  p.exponents = a->cache_bits8 ? a->exponents : 0;
+  return run("emmy_norm_rotate_append", p, a->cache_bits8 != 0, a->q_weight || a->k_weight, stream);
 }

@@ -19,9 +19,9 @@ REPO = ROOT.parent
 LIB_PATH = PKG / "libemmy_b200.so"
 SRC = ROOT / "csrc" / "emmy_runtime.cpp"
 NOALLOC_SRC = ROOT / "csrc" / "emmy_noalloc.cu"
-PLAN_SRC = ROOT / "csrc" / "emmy_paged_plan.cpp"
-PAGED_SRCS = [ROOT / "csrc" / "emmy_rotate_append.cu", ROOT / "csrc" / "emmy_paged_attention.cu"]
-PAGED_HEADER = ROOT / "csrc" / "emmy_paged.h"
+PLAN_SRCS = [ROOT / "csrc" / f"emmy_{name}_plan.cpp" for name in ("paged", "quantised")]
+PAGED_SRCS = [ROOT / "csrc" / f"emmy_{name}.cu" for name in ("rotate_append", "paged_attention", "quantised_attention", "verify")]
+PAGED_HEADERS = [ROOT / "csrc" / f"emmy_{name}.h" for name in ("paged", "quantised")]
 HEADER = REPO / "include" / "emmy_b200.h"
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 
@@ -34,8 +34,10 @@ EXPORTS = [
     "emmy_memcpy_htod_async", "emmy_memcpy_dtoh_async", "emmy_stream_sync", "emmy_mem_alloc",
     "emmy_mem_free", "emmy_ipc_handle", "emmy_ipc_open", "emmy_ipc_close",
     "emmy_time_launches", "emmy_run_host", "emmy_rmsnorm_noalloc",
-    "emmy_rotate_append", "emmy_paged_plan_make", "emmy_paged_plan_data", "emmy_paged_plan_free",
-    "emmy_paged_attention", "emmy_paged_plan_status",
+    "emmy_rotate_append", "emmy_norm_rotate_append", "emmy_paged_plan_make", "emmy_paged_plan_data",
+    "emmy_paged_plan_free", "emmy_paged_attention", "emmy_paged_plan_status",
+    "emmy_quantised_plan_make", "emmy_quantised_plan_data", "emmy_quantised_plan_free",
+    "emmy_quantised_attention", "emmy_quantised_plan_status", "emmy_verify",
 ]
 
 
@@ -49,7 +51,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile the runtime library in-tree: host C++, and by nvcc the entry
     points that carry GPU code of their own (the GPU code of an IR is the PTX
     it compiles to)."""
-    deps = [SRC, NOALLOC_SRC, HEADER, PLAN_SRC, *PAGED_SRCS, PAGED_HEADER]
+    deps = [SRC, NOALLOC_SRC, HEADER, *PLAN_SRCS, *PAGED_SRCS, *PAGED_HEADERS]
     if LIB_PATH.exists() and not force and all(
             LIB_PATH.stat().st_mtime >= d.stat().st_mtime for d in deps):
         return LIB_PATH
@@ -72,7 +74,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             print(*(ln for ln in r.stderr.splitlines() if "spill" in ln or "Used" in ln), sep="\n")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wextra",
            "-fvisibility=hidden", "-Wl,--exclude-libs,ALL", "-s",
-           f"-I{inc}", str(SRC), str(PLAN_SRC), *map(str, objs), "-o", str(tmp), str(ptxc),
+           f"-I{inc}", str(SRC), *map(str, PLAN_SRCS), *map(str, objs), "-o", str(tmp), str(ptxc),
            f"-L{CUDA_HOME / 'lib64'}", "-lcudart_static", "-ldl", "-lpthread", "-lrt"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     for obj in objs:
@@ -151,13 +153,17 @@ def lib() -> ctypes.CDLL:
                                            c_u32p, c_u32p] + [ctypes.c_uint64] * 5 + [
                                            ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
         L.emmy_rotate_append.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
-        L.emmy_paged_plan_make.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p)]
-        L.emmy_paged_plan_data.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p)] + [
-            ctypes.POINTER(ctypes.c_size_t)] * 2
-        L.emmy_paged_plan_free.argtypes = [ctypes.c_void_p]
-        L.emmy_paged_plan_free.restype = None
-        L.emmy_paged_attention.argtypes = [ctypes.c_void_p] * 3
-        L.emmy_paged_plan_status.argtypes = [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]
+        L.emmy_norm_rotate_append.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        L.emmy_verify.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        for kind in ("paged", "quantised"):
+            make, data, free, attention, status = (getattr(L, f"emmy_{kind}_{name}") for name in (
+                "plan_make", "plan_data", "plan_free", "attention", "plan_status"))
+            make.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p)]
+            data.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p)] + [ctypes.POINTER(ctypes.c_size_t)] * 2
+            free.argtypes = [ctypes.c_void_p]
+            free.restype = None
+            attention.argtypes = [ctypes.c_void_p] * 3
+            status.argtypes = [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]
         _LIB = L
     return _LIB
 

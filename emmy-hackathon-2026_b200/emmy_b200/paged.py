@@ -1,20 +1,31 @@
-"""A paged key/value cache and the two operators of a serving step around it.
+"""A paged key/value cache and the operators of a serving step around it.
 
 * :func:`rotate_append` turns new queries and keys by their positions (rotary
   positions of one or several axes) and writes keys and values to the cache;
+  :func:`norm_rotate_append` does so with norms of the queries and keys of each
+  head before, or with a cache of 8-bit floats, at half the bytes;
 * :func:`attention` is the attention of a ragged chunk of new tokens, one token
-  a sequence (decoding) upwards, over that cache.
+  a sequence (decoding) upwards, over that cache, :func:`quantised_attention`
+  the same over a cache of 8-bit floats;
+* :func:`verify` keeps or rejects drafted tokens by the target's probabilities
+  and draws the next one, from given random numbers.
 
 A cache is two tensors, keys and values, of shape [pages, page_size, kv_heads,
 head_dim] with any strides of the outer dimensions, so ``[pages, kv_heads,
-page_size, head_dim]`` storage is passed as its ``transpose(1, 2)``.  Both
+page_size, head_dim]`` storage is passed as its ``transpose(1, 2)``.  What an
+8-bit cache (torch.float8_e4m3fn) holds stands for its value times 2^e, with an
+exponent e from -15 to 7 for the keys and one for the values of each head: the
+``exponents`` (int32 [2, kv_heads]) that every call is given.  Powers of two
+quantise with one rounding and are exact in either 16-bit type; a float has the
+same relative precision over its whole range, so an exponent only has to bring
+the largest magnitude to 448 or less: 2^e at least that over 448.  All
 operators run on the current stream of their tensors' device, or on the CUDA
 stream ``stream`` (its address; it has to last as long as what was allocated for
 calls on it: returned tensors, plans, rotations), and return without waiting.
 Tensors that they return may be used on that stream and on the current one;
 those that they are given are the caller's to keep until a ``stream`` is through
 with them.  They are thin over the C ABI (``emmy_rotate_append``,
-``emmy_paged_attention`` in ``include/emmy_b200.h``) and raise
+``emmy_paged_attention`` and so on in ``include/emmy_b200.h``) and raise
 :class:`~.native.EmmyError` with its message on arguments it refuses,
 ``ValueError`` on what only Python can see.  They have no backward pass, and
 refuse tensors that require grad unless gradients are off.
@@ -34,6 +45,11 @@ _DTYPES = {torch.float16: 6, torch.float32: 7, torch.bfloat16: 9}
 # ctypes structure of as many fields, on calls of 3 us on the GPU
 _ROTATE_APPEND_ARGS = struct.Struct("@10i10Q15q")
 _ATTENTION_ARGS = struct.Struct("@4if8Q11q")
+_NORM_ROTATE_APPEND_ARGS = struct.Struct("@10i10Q15q3Qfi")
+_QUANTISED_ATTENTION_ARGS = struct.Struct("@4if8Q11qQ")
+_VERIFY_ARGS = struct.Struct("@6i8Q2q")
+
+E4M3 = torch.float8_e4m3fn
 
 _i32 = ctypes.c_int32
 _CONTIGUOUS = torch.contiguous_format
@@ -271,6 +287,8 @@ class AttentionPlan(_Kept):
     each.  It may be dropped while a call runs, on whichever stream, but not
     before a CUDA graph that holds its calls."""
 
+    _kind = "paged"
+
     def __init__(self, q_lens, kv_lens, q_heads, kv_heads, head_dim, causal=True, window=None, device=None,
                  ctas=None):
         self._h = None
@@ -289,12 +307,11 @@ class AttentionPlan(_Kept):
         a = _PlanArgs(n, None, None, q_heads, kv_heads, head_dim, bool(causal), min(window or 0, 1 << 30), ctas)
         lens = (_i32 * (2 * n))(*q_lens, *kv_lens)
         a.q_lens, a.kv_lens = ctypes.addressof(lens), ctypes.addressof(lens) + 4 * n
-        L = native.lib()
         h = ctypes.c_void_p()
-        native.check(L.emmy_paged_plan_make(ctypes.byref(a), ctypes.byref(h)))
+        native.check(self._entry("make")(ctypes.byref(a), ctypes.byref(h)))
         self._h = h
         words, count, scratch = ctypes.c_void_p(), ctypes.c_size_t(), ctypes.c_size_t()
-        native.check(L.emmy_paged_plan_data(h, ctypes.byref(words), ctypes.byref(count), ctypes.byref(scratch)))
+        native.check(self._entry("data")(h, ctypes.byref(words), ctypes.byref(count), ctypes.byref(scratch)))
         host = torch.frombuffer((_i32 * count.value).from_address(words.value), dtype=torch.int32)
         self.words = host.to(device, copy=True)
         self.scratch = torch.empty(scratch.value, dtype=torch.uint8, device=device)
@@ -310,9 +327,12 @@ class AttentionPlan(_Kept):
     def __del__(self):
         if self._h is not None:
             try:
-                native.lib().emmy_paged_plan_free(self._h)
+                self._entry("free")(self._h)
             except Exception:
                 pass
+
+    def _entry(self, name):
+        return getattr(native.lib(), f"emmy_{self._kind}_plan_{name}")
 
     def check(self, stream=None):
         """Waits for the calls so far (with ``stream``, for those on it only) and raises
@@ -323,7 +343,7 @@ class AttentionPlan(_Kept):
             stream = torch._C._cuda_getCurrentRawStream(index)
             if not self._streams <= {stream}:
                 torch.cuda.synchronize(index)
-        _call("emmy_paged_plan_status", index, stream, self._h, self.words.data_ptr())
+        _call(f"emmy_{self._kind}_plan_status", index, stream, self._h, self.words.data_ptr())
 
 
 def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, stream=None):
@@ -360,6 +380,8 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     grads = _grads_on()
     if grads and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         _no_backward()
+    if plan._kind != "paged":
+        raise ValueError("plan: an AttentionPlan is wanted")
     if at != plan.device_index:
         raise ValueError(f"q: on {q.device}, the plan on {plan.device}")
     shape = plan.shape
@@ -409,3 +431,250 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     if given:
         _written_to((out, lse))
     return out, lse
+
+
+def _exponents(exponents, kv_heads, device):
+    """Their address; 0 for none."""
+    if exponents is None:
+        return 0
+    _check("exponents", exponents, 2, torch.int32, device)
+    if exponents.shape != (2, kv_heads) or not exponents.is_contiguous():
+        raise ValueError(f"exponents: contiguous [2, {kv_heads}] is wanted, not {list(exponents.shape)}")
+    return exponents.data_ptr()
+
+
+class Norm(_Kept):
+    """Norms of queries and keys: a head x becomes x / sqrt(mean(x^2) + eps) *
+    weight, with weights [head_dim] of the tensors' type for all heads of
+    queries and all of keys."""
+
+    def __init__(self, q_weight, k_weight, eps=1e-6):
+        device = _cuda_device("q_weight", q_weight)
+        _need(q_weight.dtype in _DTYPES, f"q_weight: bfloat16, float16 or float32 is wanted, not {q_weight.dtype}")
+        for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+            _check(name, t, 1, q_weight.dtype, device)
+        _need(q_weight.shape == k_weight.shape, "q_weight and k_weight have different shapes")
+        _need(float(eps) >= 0, "eps: 0 or more")
+        self.q_weight, self.k_weight, self.eps = q_weight, k_weight, float(eps)
+        self.dtype, self.dim, self.device_index = q_weight.dtype, q_weight.shape[0], device.index
+        self._keep(q_weight, k_weight)
+
+
+def norm_rotate_append(rotation, norm, q, k, v, positions, slots, k_cache, v_cache, exponents=None, q_out=None, stream=None):
+    """:func:`rotate_append` with norms, a cache of 8-bit floats, or both.
+
+    ``norm``, a :class:`Norm` or None, applies to the queries and keys of each
+    head before they turn.  ``k_cache`` and ``v_cache`` are of the type of ``q``,
+    or float8_e4m3fn: keys and values are then multiplied by 2^-exponent of their
+    head (``exponents``, see the module; None: all 0) and rounded, to 448 where
+    they are larger.  All in 32 bits, with one rounding for what is written."""
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise ValueError("q: a CUDA tensor is wanted")
+    dtype, device = q.dtype, q.device
+    if dtype not in _DTYPES:
+        raise ValueError(f"q: bfloat16, float16 or float32 is wanted, not {dtype}")
+    if isinstance(positions, torch.Tensor) and positions.ndim == 1:
+        positions = positions[None]
+    kind = E4M3 if isinstance(k_cache, torch.Tensor) and k_cache.dtype is E4M3 else dtype
+    q_stride, k_stride, v_stride, k_cache_stride, v_cache_stride, positions_stride, slots_stride = (
+        _check(name, t, ndim, of, device) for name, t, ndim, of in (
+            ("q", q, 3, dtype), ("k", k, 3, dtype), ("v", v, 3, dtype), ("k_cache", k_cache, 4, kind), ("v_cache", v_cache, 4, kind),
+            ("positions", positions, 2, torch.int32), ("slots", slots, 1, torch.int32)))
+    grads = _grads_on()
+    if grads and (q.requires_grad or k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+                  or rotation.frequencies.requires_grad or (norm is not None and (norm.q_weight.requires_grad or norm.k_weight.requires_grad))):
+        _no_backward()
+    shape = q.shape
+    tokens, q_heads, dim = shape
+    pages, page_size, kv_heads, cache_dim = k_cache.shape
+    if v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache and v_cache have different shapes")
+    if k.shape != (tokens, kv_heads, dim) or v.shape != k.shape or cache_dim != dim:
+        raise ValueError("q, k, v and the caches do not fit together")
+    axes, n = positions.shape
+    if n != tokens or axes < rotation.axes:
+        raise ValueError(f"positions: [{rotation.axes}, {tokens}] is wanted, not {list(positions.shape)}")
+    if slots.shape[0] != tokens:
+        raise ValueError(f"slots: {tokens} are wanted, not {slots.shape[0]}")
+    at = q.get_device()
+    if rotation.device_index != at:
+        raise ValueError("rotation: on another device")
+    weights, eps = (0, 0), 0.0
+    if norm is not None:
+        if norm.device_index != at:
+            raise ValueError("norm: on another device")
+        if norm.dtype is not dtype or norm.dim != dim:
+            raise ValueError(f"norm: weights of {dim} components of {dtype} are wanted, not {norm.dim} of {norm.dtype}")
+        weights, eps = (norm.q_weight.data_ptr(), norm.k_weight.data_ptr()), norm.eps
+    if exponents is not None and kind is not E4M3:
+        raise ValueError("exponents: for a cache of 8-bit floats only")
+    exponents_ptr = _exponents(exponents, kv_heads, device)
+    if q_out is None:
+        q_out = _empty_like(q, memory_format=_CONTIGUOUS) if stream is None else _new(stream, q, shape, dtype)
+        q_out_stride = q_heads * dim, dim
+    else:
+        q_out_stride = _check("q_out", q_out, 3, dtype, device)[:2]
+        if q_out.shape != shape:
+            raise ValueError("q_out: another shape than q")
+        if grads and q_out.requires_grad:
+            _no_backward()
+    try:
+        a = _NORM_ROTATE_APPEND_ARGS.pack(
+            _DTYPES[dtype], tokens, q_heads, kv_heads, dim, rotation.components, axes, rotation.interleaved, pages, page_size,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            positions.data_ptr(), slots.data_ptr(), rotation.frequencies_ptr, rotation.pair_axis_ptr,
+            q_stride[0], q_stride[1], k_stride[0], k_stride[1], v_stride[0], v_stride[1], q_out_stride[0], q_out_stride[1],
+            k_cache_stride[0], k_cache_stride[1], k_cache_stride[2], v_cache_stride[0], v_cache_stride[1], v_cache_stride[2],
+            positions_stride[0], *weights, exponents_ptr, eps, kind is E4M3)
+    except (struct.error, OverflowError) as e:
+        raise _unfit(e) from None
+    if stream is None:
+        stream = _current_stream(at)
+    for kept in (rotation, norm):
+        if kept is not None and stream not in kept._streams:
+            kept._used_on(stream)
+    _call("emmy_norm_rotate_append", at, stream, a)
+    _written_to((k_cache, v_cache, q_out))
+    return q_out
+
+
+class QuantisedPlan(AttentionPlan):
+    """An :class:`AttentionPlan` for :func:`quantised_attention`.
+
+    Sequences with at most 128 query rows a key head (new tokens times
+    ``q_heads / kv_heads``) read the 8-bit cache as it lies.  The keys and values
+    of the others, which see them with the tensor cores, are read back to 16 bits
+    once a call, into ``scratch``: 4 bytes x kv_heads x head_dim for each of
+    their cached tokens."""
+
+    _kind = "quantised"
+
+
+def quantised_attention(plan, q, k_cache, v_cache, exponents, table, scale=None, out=None, lse=None, stream=None):
+    """:func:`attention` over a cache of 8-bit floats, with a :class:`QuantisedPlan`.
+
+    ``k_cache`` and ``v_cache`` are float8_e4m3fn, of any page_size; ``q`` is
+    bfloat16 or float16, of 64 or 128 components.  ``exponents``: int32 [2, kv_heads] (see the module;
+    None: all 0).  All else is as for :func:`attention`, what it says of keys and
+    values that are not finite included (an 8-bit float can be NaN)."""
+    if not isinstance(plan, QuantisedPlan):
+        raise ValueError("plan: a QuantisedPlan is wanted")
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise ValueError("q: a CUDA tensor is wanted")
+    dtype, device = q.dtype, q.device
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError(f"q: bfloat16 or float16 is wanted, not {dtype}")
+    q_stride, k_cache_stride, v_cache_stride, table_stride = (_check(name, t, ndim, kind, device) for name, t, ndim, kind in (
+        ("q", q, 3, dtype), ("k_cache", k_cache, 4, E4M3), ("v_cache", v_cache, 4, E4M3), ("table", table, 2, torch.int32)))
+    grads = _grads_on()
+    if grads and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        _no_backward()
+    at, shape = q.get_device(), plan.shape
+    if at != plan.device_index:
+        raise ValueError(f"q: on {device}, the plan on {plan.device}")
+    if q.shape != shape:
+        raise ValueError(f"q: the plan is for {list(shape)}, not {list(q.shape)}")
+    pages, page_size, kv_heads, dim = k_cache.shape
+    if v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache and v_cache have different shapes")
+    if kv_heads != plan.kv_heads or dim != plan.head_dim:
+        raise ValueError(f"k_cache: the plan is for {plan.kv_heads} heads of {plan.head_dim}, not {kv_heads} of {dim}")
+    rows, width = table.shape
+    if rows != plan.sequences:
+        raise ValueError(f"table: {plan.sequences} rows are wanted, not {rows}")
+    exponents_ptr = _exponents(exponents, kv_heads, device)
+    given = out is not None or lse is not None
+    if out is None:
+        out = _empty_like(q, memory_format=_CONTIGUOUS) if stream is None else _new(stream, q, shape, dtype)
+        out_stride = shape[1] * dim, dim
+    else:
+        out_stride = _check("out", out, 3, dtype, device)[:2]
+        if out.shape != shape:
+            raise ValueError("out: another shape than q")
+        if grads and out.requires_grad:
+            _no_backward()
+    if lse is None:
+        lse = q.new_empty(shape[:2], dtype=torch.float32) if stream is None else _new(stream, q, shape[:2], torch.float32)
+    else:
+        _check("lse", lse, 2, torch.float32, device)
+        if lse.shape != shape[:2] or not lse.is_contiguous():
+            raise ValueError(f"lse: contiguous {list(shape[:2])} is wanted")
+        if grads and lse.requires_grad:
+            _no_backward()
+    try:
+        a = _QUANTISED_ATTENTION_ARGS.pack(
+            _DTYPES[dtype], pages, page_size, width, plan.scale if scale is None else scale,
+            q.data_ptr(), out.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
+            plan.words_ptr, plan.scratch_ptr, q_stride[0], q_stride[1], out_stride[0], out_stride[1],
+            k_cache_stride[0], k_cache_stride[1], k_cache_stride[2], v_cache_stride[0], v_cache_stride[1], v_cache_stride[2],
+            table_stride[0], exponents_ptr)
+    except (struct.error, OverflowError) as e:
+        raise _unfit(e) from None
+    if stream is None:
+        stream = _current_stream(at)
+    if stream not in plan._streams:
+        plan._used_on(stream)
+    _call("emmy_quantised_attention", at, stream, plan._h, a)
+    if given:
+        _written_to((out, lse))
+    return out, lse
+
+
+def verify(target, proposal, drafted, uniforms, finals, first, stream=None):
+    """``(accepted, tokens)``: how many drafted tokens of each sequence are kept, and
+    each sequence's tokens: those, the one drawn after them, then -1.
+
+    Sequence s has rows ``first[s]`` to ``first[s + 1] - 1`` of ``target``
+    [rows, vocabulary], the target's probabilities after each of its n drafted
+    tokens and before the first: n + 1 of them, as its logits come from a step
+    with the token before the drafts and the drafts.  ``first``: int32
+    [sequences + 1], from 0 to rows.  ``proposal`` [rows - sequences, vocabulary],
+    the probabilities that the drafts were drawn with, ``drafted`` (int32) and
+    ``uniforms`` (float32, in [0, 1)) have an entry for each draft, in order;
+    ``finals`` (float32, in [0, 1)) one for each sequence.  ``proposal`` None: the
+    drafts were certain.  ``target`` and ``proposal``: float32, bfloat16 or float16.
+
+    Draft x is kept, and those before it, while uniform * proposal[x] < target[x].
+    The next token is the first whose running sum exceeds final times the whole
+    sum: of max(target - proposal, 0) at the first draft that is not kept, of
+    target where nothing is left of that, and after the last draft.  So each token
+    is distributed as the target's.  Products, differences and sums are in 64 bits.
+    A draft outside the vocabulary is not kept.  What is not a number counts as 0;
+    a sequence without anything to draw from gets -1 for that token.  Where ``first`` does
+    not say rows (it is not read on the host), ``accepted`` is -1 and the tokens are not written.
+
+    ``accepted`` int32 [sequences], ``tokens`` int32 [rows]."""
+    if not isinstance(target, torch.Tensor) or not target.is_cuda:
+        raise ValueError("target: a CUDA tensor is wanted")
+    dtype, device = target.dtype, target.device
+    if dtype not in _DTYPES:
+        raise ValueError(f"target: float32, bfloat16 or float16 is wanted, not {dtype}")
+    for name, t, ndim, kind in (("target", target, 2, dtype), ("drafted", drafted, 1, torch.int32), ("uniforms", uniforms, 1, torch.float32),
+                                ("finals", finals, 1, torch.float32), ("first", first, 1, torch.int32)):
+        _check(name, t, ndim, kind, device)
+    rows, vocabulary = target.shape
+    sequences, drafts = finals.shape[0], drafted.shape[0]
+    if first.shape[0] != sequences + 1:
+        raise ValueError(f"first: {sequences + 1} entries are wanted, not {first.shape[0]}")
+    if drafts != rows - sequences or uniforms.shape[0] != drafts:
+        raise ValueError(f"drafted and uniforms: {rows - sequences} entries are wanted, one less a sequence than rows of target")
+    if proposal is not None:
+        _check("proposal", proposal, 2, dtype, device)
+        if proposal.shape != (drafts, vocabulary):
+            raise ValueError(f"proposal: {[drafts, vocabulary]} is wanted, not {list(proposal.shape)}")
+    if _grads_on() and (target.requires_grad or uniforms.requires_grad or finals.requires_grad or (proposal is not None and proposal.requires_grad)):
+        _no_backward()
+    if stream is None:
+        accepted, tokens = first.new_empty(sequences), first.new_empty(rows)
+    else:
+        accepted, tokens = _new(stream, first, (sequences,), torch.int32), _new(stream, first, (rows,), torch.int32)
+    try:
+        a = _VERIFY_ARGS.pack(
+            _DTYPES[dtype], sequences, rows, drafts, vocabulary, 0, target.data_ptr(), 0 if proposal is None else proposal.data_ptr(),
+            drafted.data_ptr(), uniforms.data_ptr(), finals.data_ptr(), first.data_ptr(), accepted.data_ptr(), tokens.data_ptr(),
+            target.stride(0), 0 if proposal is None else proposal.stride(0))
+    except (struct.error, OverflowError) as e:
+        raise _unfit(e) from None
+    at = target.get_device()
+    _call("emmy_verify", at, _current_stream(at) if stream is None else stream, a)
+    return accepted, tokens

@@ -239,6 +239,23 @@ typedef struct {
 /* is one or the other's.                                                       */
 EMMY_API int emmy_rotate_append(const emmy_rotate_append_args *a, void *stream);
 
+/* The same with norms and with a cache of 8-bit floats (e4m3: 4 exponent bits,  */
+/* largest 448).  Before they turn, q and k of each head become                  */
+/* x * rsqrt(mean(x^2) + eps) * weight; what an 8-bit cache holds stands for its */
+/* value times 2^exponent of its head: keys and values are multiplied by          */
+/* 2^-exponent, rounded once, and saturate.  With exponents from -15 to 7 (others  */
+/* count as the nearest of them) every value is a number of f16 and bf16 too.      */
+#define EMMY_MIN_EXPONENT (-15)
+#define EMMY_MAX_EXPONENT 7
+typedef struct {
+  emmy_rotate_append_args a;   /* dtype: of q, k, v, q_out (and the caches)         */
+  uint64_t q_weight, k_weight; /* [head_dim], dense, of dtype; both 0: no norms      */
+  uint64_t exponents;          /* int32 [2][kv_heads]: of keys, of values; 0: all 0  */
+  float eps;                   /* >= 0                                               */
+  int32_t cache_bits8;         /* 1: the caches hold 8-bit floats; 0: dtype          */
+} emmy_norm_rotate_append_args;
+EMMY_API int emmy_norm_rotate_append(const emmy_norm_rotate_append_args *a, void *stream);
+
 typedef struct emmy_paged_plan_s *emmy_paged_plan_t;
 
 typedef struct {
@@ -289,6 +306,54 @@ EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_paged_atten
 /* that used these device words gave up on a wait.  Its outputs are void; later   */
 /* calls with these words do nothing, until the plan's words are copied anew.     */
 EMMY_API int emmy_paged_plan_status(emmy_paged_plan_t plan, uint64_t plan_words, void *stream);
+
+/* Attention over a cache of 8-bit floats as emmy_norm_rotate_append writes it.  */
+/* The plan is of the same arguments as emmy_paged_plan_make's; its words and      */
+/* `scratch` bytes (128-byte aligned; partial results, and 16-bit keys and values  */
+/* of the sequences that bring many tokens, read back) are kept as there.          */
+typedef struct emmy_quantised_plan_s *emmy_quantised_plan_t;
+EMMY_API int emmy_quantised_plan_make(const emmy_paged_plan_args *a, emmy_quantised_plan_t *out);
+EMMY_API int emmy_quantised_plan_data(emmy_quantised_plan_t plan, const int32_t **words, size_t *n_words,
+                                      size_t *scratch);
+EMMY_API void emmy_quantised_plan_free(emmy_quantised_plan_t plan);
+
+typedef struct {
+  emmy_paged_attention_args a; /* dtype: of q and out; page_size: any, >= 1          */
+  uint64_t exponents;          /* int32 [2][kv_heads]: of keys, of values; 0: all 0  */
+} emmy_quantised_attention_args;
+EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, const emmy_quantised_attention_args *a,
+                                      void *stream);
+/* As emmy_paged_plan_status. */
+EMMY_API int emmy_quantised_plan_status(emmy_quantised_plan_t plan, uint64_t plan_words, void *stream);
+
+/* Drafted tokens against the target's probabilities.  Sequence s has rows          */
+/* first[s]..first[s+1]-1 of `target`, one more than it has drafts; its draft i is  */
+/* drafted[first[s]-s+i], with that row of `proposal`.  Draft x is kept, and those   */
+/* before it, while uniform * proposal[x] < target[x] in its row; the next token is  */
+/* the first whose running sum exceeds final * the whole sum, of max(target -        */
+/* proposal, 0) at the first draft that is not kept (of target where nothing is left */
+/* of that, and after the last draft).  Products, differences and sums in 64 bits.   */
+/* tokens: of the sequence's rows, the drafts kept, the next token, then -1; the     */
+/* next token is -1 where the whole sum is not above 0.  A draft outside the          */
+/* vocabulary is not kept.  A sequence whose entries of `first` are not rows gets -1  */
+/* as accepted, and nothing else is read or written for it.                          */
+typedef struct {
+  int32_t dtype;            /* of target and proposal: 6, 7 or 9                 */
+  int32_t sequences, rows;  /* rows: of target                                   */
+  int32_t drafts;           /* rows of proposal, entries of drafted and uniforms */
+  int32_t vocabulary;
+  int32_t reserved;         /* 0                                                 */
+  uint64_t target;          /* [rows][vocabulary]                                */
+  uint64_t proposal;        /* [drafts][vocabulary]; 0: the drafts were certain  */
+  uint64_t drafted;         /* int32 [drafts]                                    */
+  uint64_t uniforms;        /* f32 [drafts], in [0, 1)                           */
+  uint64_t finals;          /* f32 [sequences], in [0, 1)                        */
+  uint64_t first;           /* int32 [sequences + 1], from 0 to rows             */
+  uint64_t accepted;        /* int32 [sequences]: drafts kept                    */
+  uint64_t tokens;          /* int32 [rows]                                      */
+  int64_t target_stride, proposal_stride;   /* of a row, in elements             */
+} emmy_verify_args;
+EMMY_API int emmy_verify(const emmy_verify_args *a, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,208 @@
+"""The plan of attention over an 8-bit cache on the CPU: its pieces and read-back jobs
+cover every query row and every key that the row sees exactly once, parts own scratch
+rows and counters of their own, work is even, and what the operators of an 8-bit cache
+and of drafted tokens cannot take is refused before any CUDA call."""
+import random
+
+import pytest
+import torch
+
+from emmy_b200 import native, paged
+
+pytestmark = pytest.mark.usefixtures("native_lib")
+
+FIELDS = ("seq", "kvh", "tok0", "row0", "rows", "pos0", "lo", "hi", "kv_len", "slice0", "nslices", "item", "split", "nsplit",
+          "part_row", "pad")
+FEW = 128
+
+
+def parts_of(plan, q_lens, q_heads, kv_heads):
+    """(pieces, cta_first): the words begin with cta_first, whose length is known from the last entry on."""
+    w = plan.words.tolist()
+    # the first entry is 0 and they grow; the pieces begin at a multiple of 16 words
+    n = sum(bool(q) and q * (q_heads // kv_heads) <= FEW for q in q_lens)
+    if not n:
+        return [], [0]
+    ctas = next(k for k in range(1, len(w)) if w[k] <= w[k - 1]) - 1
+    first = w[:ctas + 1]
+    # counters lie between, all 0: the first piece is the first record whose rows are not 0
+    at = next(k for k in range((ctas + 1 + 15) // 16 * 16, len(w), 16) if w[k + 4])
+    assert not any(w[ctas + 1:at])
+    return [dict(zip(FIELDS, w[at + 16 * i:at + 16 * i + 16])) for i in range(first[-1])], first
+
+
+CASES = [
+    ([1], [301], 32, 8, True, 0),
+    ([1], [131071], 32, 8, True, 0),
+    ([1] * 64, [random.Random(s).randint(1, 8191) for s in range(64)], 32, 8, True, 0),
+    ([3, 9, 0, 30, 1], [3000, 12288, 0, 77, 900], 32, 8, True, 0),
+    ([9, 2, 64], [20, 2, 640], 6, 2, True, 5),
+    ([33], [1000], 40, 8, False, 0),
+    ([1], [16384], 128, 1, True, 0),
+    ([2, 5], [9, 2], 4, 4, True, 0),
+    ([7, 25], [65536, 5000], 5, 1, True, 333),
+    ([500, 1, 300], [700, 9000, 200], 8, 2, True, 0),
+    ([0, 0], [10, 0], 4, 4, True, 0),
+    ([], [], 4, 4, True, 0),
+]
+
+
+@pytest.mark.parametrize("q_lens,kv_lens,hq,hkv,causal,window", CASES)
+@pytest.mark.parametrize("ctas", [1, 7, 148])
+def test_pieces_cover_the_work_once(q_lens, kv_lens, hq, hkv, causal, window, ctas):
+    plan = paged.QuantisedPlan(q_lens, kv_lens, hq, hkv, 64, causal, window or None, device="cpu", ctas=ctas)
+    pieces, first = parts_of(plan, q_lens, hq, hkv)
+    group = hq // hkv
+    few = [q * group <= FEW for q in q_lens]
+    most = max([8] + [q * group for q, f in zip(q_lens, few) if f])
+    at_once = 8 if most <= 8 else 32
+    assert len(first) - 1 <= 2 * ctas
+    items = {}
+    for u in pieces:
+        assert few[u["seq"]] and 0 < u["rows"] <= at_once and 0 <= u["kvh"] < hkv
+        assert u["tok0"] == sum(q_lens[:u["seq"]]) and u["pos0"] == kv_lens[u["seq"]] - q_lens[u["seq"]] and u["kv_len"] == kv_lens[u["seq"]]
+        items.setdefault((u["seq"], u["kvh"], u["row0"]), []).append(u)
+    covered, scratch, numbers = set(), set(), set()
+    for (s, h, row0), us in items.items():
+        rows = range(row0, row0 + us[0]["rows"])
+        assert rows.stop <= q_lens[s] * group
+        mine = {(s, h, r) for r in rows}
+        assert not mine & covered
+        covered |= mine
+        lows = [max(0, us[0]["pos0"] + r // group - window + 1) if window else 0 for r in rows]
+        highs = [min(kv_lens[s], us[0]["pos0"] + r // group + 1) if causal else kv_lens[s] for r in rows]
+        lo, hi = min(lows), max(highs + [0])
+        if hi <= lo:
+            assert [u["nslices"] for u in us] == [0]
+        else:
+            at = lo // 16
+            for k, u in enumerate(sorted(us, key=lambda u: u["split"])):
+                assert (u["slice0"], u["split"], u["lo"], u["hi"]) == (at, k, lo, hi) and u["nslices"] > 0
+                at += u["nslices"]
+            assert at == -(-hi // 16)
+        assert all((u["nsplit"], u["item"], u["part_row"], u["rows"]) == (len(us), us[0]["item"], us[0]["part_row"], us[0]["rows"]) for u in us)
+        if len(us) > 1:
+            assert us[0]["item"] not in numbers
+            numbers.add(us[0]["item"])
+            mine = set(range(us[0]["part_row"], us[0]["part_row"] + len(us) * us[0]["rows"]))
+            assert not mine & scratch
+            scratch |= mine
+    assert len(covered) == sum(q * hq for q, f in zip(q_lens, few) if f)
+    assert numbers == set(range(len(numbers))) and scratch == set(range(len(scratch)))
+    # the others' keys: 4 bytes a component of whole pages of 128 tokens that some row sees, and parts
+    blocks = 0
+    for q, kv, f in zip(q_lens, kv_lens, few):
+        hi, lo = kv, max(0, kv - q - window + 1) if window else 0
+        blocks += 0 if f or hi <= 0 else -(-hi // 128) - lo // 128
+    assert plan.scratch.numel() >= len(scratch) * 66 * 4 + blocks * 128 * hkv * 64 * 4
+    if all(few):
+        assert plan.scratch.numel() == -(-len(scratch) * 66 * 4 // 128) * 128
+
+
+@pytest.mark.parametrize("q_lens,kv_lens,most", [
+    ([1] * 64, [random.Random(s).randint(517, 8191) for s in range(64)], 1.03),
+    ([1], [131071], 1.03),
+    ([5] * 24, [random.Random(s).randint(65, 4095) for s in range(24)], 1.1),
+])
+def test_work_is_even(q_lens, kv_lens, most):
+    plan = paged.QuantisedPlan(q_lens, kv_lens, 32, 8, 128, device="cpu", ctas=148)
+    pieces, first = parts_of(plan, q_lens, 32, 8)
+    load = [sum(u["nslices"] for u in pieces[a:b]) for a, b in zip(first, first[1:])]
+    assert max(load) <= most * sum(load) / 296 + 16, (max(load), sum(load) / 296)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(q_heads=33), "query heads"), (dict(kv_heads=0), "query heads"), (dict(q_heads=8 * 129), "query heads"),
+    (dict(head_dim=96), "head_dim"), (dict(causal=False, window=4), "window"), (dict(ctas=0), "CTAs"),
+])
+def test_plan_refuses(change, words):
+    a = dict(q_lens=[1], kv_lens=[5], q_heads=32, kv_heads=8, head_dim=128, device="cpu", ctas=148) | change
+    with pytest.raises(native.EmmyError, match=words) as e:
+        paged.QuantisedPlan(**a)
+    assert e.value.code == -1
+
+
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31, 2 ** 64, 1000])
+def test_windows_beyond_every_length(window):
+    plans = [paged.QuantisedPlan([1, 200], [999, 1000], 8, 2, 64, window=w, device="cpu", ctas=148) for w in (window, None)]
+    assert plans[0].words.tolist() == plans[1].words.tolist()
+
+
+def test_plans_of_one_operator_are_not_the_others():
+    q = torch.zeros(1, 8, 64)
+    for plan, call in ((paged.AttentionPlan, paged.quantised_attention),):
+        with pytest.raises(ValueError, match="QuantisedPlan"):
+            call(plan([1], [5], 8, 8, 64, device="cpu", ctas=1), q, q, q, None, q)
+
+
+def test_operators_need_cuda_tensors():
+    t = torch.zeros(1, 8, 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        paged.norm_rotate_append(None, None, t, t, t, None, None, None, None)
+    with pytest.raises(ValueError, match="CUDA"):
+        paged.quantised_attention(paged.QuantisedPlan([1], [5], 8, 8, 64, device="cpu", ctas=1), t, None, None, None, None)
+    with pytest.raises(ValueError, match="CUDA"):
+        paged.verify(t[0], None, None, None, None, None)
+    with pytest.raises(ValueError, match="CUDA"):
+        paged.Norm(t[0, 0], t[0, 0])
+
+
+def test_c_null_arguments(native_lib):
+    assert native_lib.emmy_norm_rotate_append(None, None) == -1
+    assert native_lib.emmy_quantised_plan_make(None, None) == -1
+    assert native_lib.emmy_quantised_plan_data(None, None, None, None) == -1
+    assert native_lib.emmy_quantised_attention(None, None, None) == -1
+    assert native_lib.emmy_quantised_plan_status(None, 0, None) == -1
+    assert native_lib.emmy_verify(None, None) == -1
+    native_lib.emmy_quantised_plan_free(None)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(dtype=10), b"dtype"), (dict(tokens=-1), b"count"), (dict(head_dim=257), b"head_dim"), (dict(rotary_dim=65), b"rotary_dim"),
+    (dict(axes=0), b"axes"), (dict(page_size=0), b"cache"), (dict(q=0), b"null"), (dict(v_cache=0), b"null"), (dict(k=4097), b"multiple"),
+    (dict(q_weight=0), b"null"), (dict(k_weight=0), b"null"), (dict(k_weight=4097), b"multiple"), (dict(exponents=4098), b"multiple"),
+    (dict(eps=-1.0), b"eps"), (dict(eps=float("nan")), b"eps"), (dict(bits8=2), b"cache_bits8"), (dict(bits8=0, k_cache=4097), b"multiple"),
+])
+def test_c_norm_rotate_append_refuses(native_lib, change, words):
+    names = ("dtype", "tokens", "q_heads", "kv_heads", "head_dim", "rotary_dim", "axes", "interleaved", "pages", "page_size",
+             "q", "k", "v", "q_out", "k_cache", "v_cache", "positions", "slots", "frequencies", "pair_axis")
+    more = ("q_weight", "k_weight", "exponents", "eps", "bits8")
+    a = dict(zip(names + more, [9, 3, 4, 2, 64, 64, 1, 0, 8, 16] + [4096] * 9 + [0] + [4096] * 3 + [1e-6, 1])) | change
+    packed = paged._NORM_ROTATE_APPEND_ARGS.pack(*(a[n] for n in names), 256, 64, 128, 64, 128, 64, 256, 64, 2048, 128, 64, 2048, 128, 64, 3,
+                                                 *(a[n] for n in more))
+    assert native_lib.emmy_norm_rotate_append(packed, None) == -1
+    said = native_lib.emmy_last_error()
+    assert words in said and b"norm_rotate_append" in said, said
+
+
+@pytest.mark.parametrize("q_lens", [[2], [300]])
+@pytest.mark.parametrize("change,words", [
+    (dict(dtype=7), b"dtype"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=3.4e38), b"scale"),
+    (dict(page_size=0), b"page_size"), (dict(pages=0), b"pages"), (dict(table_width=1), b"does not hold"), (dict(q=0), b"null"),
+    (dict(scratch=0), b"null"), (dict(q=4104), b"16 bytes"), (dict(scratch=4112), b"16 bytes"), (dict(table=4098), b"16 bytes"),
+    (dict(exponents=4098), b"16 bytes"), (dict(k_cache=4104), b"16 bytes"), (dict(q_token=100), b"stride"), (dict(k_page=-2048), b"stride"),
+    (dict(v_token=136), b"stride"), (dict(v_token=0), b"stride"),
+])
+def test_c_attention_refuses(native_lib, q_lens, change, words):
+    plan = paged.QuantisedPlan(q_lens, [5000], 8, 2, 64, device="cpu", ctas=148)
+    assert plan.scratch.numel()
+    names = ("dtype", "pages", "page_size", "table_width", "scale", "q", "out", "lse", "k_cache", "v_cache", "table",
+             "plan_words", "scratch", "q_token", "q_head", "out_token", "out_head", "k_page", "k_token", "k_head",
+             "v_page", "v_token", "v_head", "table_stride", "exponents")
+    a = dict(zip(names, [9, 400, 16, 400, 0.125] + [4096] * 8 + [512, 64, 512, 64, 2048, 128, 64, 2048, 128, 64, 400, 4096])) | change
+    assert native_lib.emmy_quantised_attention(plan._h, paged._QUANTISED_ATTENTION_ARGS.pack(*a.values()), None) == -1
+    assert words in native_lib.emmy_last_error(), native_lib.emmy_last_error()
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(dtype=8), b"dtype"), (dict(sequences=-1), b"count"), (dict(rows=-1), b"count"), (dict(drafts=-1), b"count"), (dict(drafts=9), b"count"),
+    (dict(vocabulary=0), b"vocabulary"), (dict(target=0), b"null"), (dict(drafted=0), b"null"), (dict(tokens=0), b"null"),
+    (dict(target=4098), b"multiple"), (dict(first=4098), b"multiple"), (dict(target_stride=-5), b"stride"),
+])
+def test_c_verify_refuses(native_lib, change, words):
+    names = ("dtype", "sequences", "rows", "drafts", "vocabulary", "reserved", "target", "proposal", "drafted", "uniforms", "finals", "first",
+             "accepted", "tokens", "target_stride", "proposal_stride")
+    a = dict(zip(names, [7, 2, 8, 6, 100, 0] + [4096] * 8 + [100, 100])) | change
+    assert native_lib.emmy_verify(paged._VERIFY_ARGS.pack(*a.values()), None) == -1
+    assert words in native_lib.emmy_last_error(), native_lib.emmy_last_error()
+    assert native_lib.emmy_verify(paged._VERIFY_ARGS.pack(*(a | dict(zip(names, [7, 0, 0, 0, 5]))).values()), None) == 0
