@@ -7,15 +7,20 @@
 
 namespace emmy_quantised {
 
-constexpr int kSlice = 16;          // keys that a warp takes at once
+constexpr int slice_keys(int head_dim) { return 2048 / head_dim; }      // that a warp takes at once: 2 KiB of 8-bit keys
 constexpr int kFewRows = 128;       // query rows of a sequence and key head up to which they are few
 constexpr int kBlock = 128;         // tokens of a page of the workspace, which the others' keys are read back to
 
-// A piece of work of one CTA: up to 8 or 32 query rows of one sequence and key head
-// (row r is new token (row0 + r) / G of the sequence, query head (row0 + r) % G of
-// the group) against some of the key slices that they see between them.  `nsplit`
-// pieces share an item: each leaves a partial result in its rows of the scratch, and
-// the last to arrive joins them.
+// Warps of a CTA whose pieces have up to `tiles` tiles of 8 query rows: as many as the
+// registers of their sums allow twice an SM (128, 168 or 255 a thread).
+constexpr int warps_of(int tiles) { return tiles == 1 ? 8 : tiles == 2 ? 6 : 4; }
+
+// A piece of work: up to 8, 16 or 32 query rows of one sequence and key head (row r is
+// new token (row0 + r) / G of the sequence, query head (row0 + r) % G of the group)
+// against some of the key slices that they see between them.  The warps of a CTA share
+// its `shared` pieces, slice by slice in turn, and have others of their own after
+// them.  `nsplit` pieces share an item: each leaves a partial result in its rows of the
+// scratch, which a kernel of its own joins.
 struct Piece {
   int32_t seq, kvh;
   int32_t tok0;             // the sequence's first row of q
@@ -24,20 +29,28 @@ struct Piece {
   int32_t lo, hi;           // keys that the item's rows see between them
   int32_t kv_len;
   int32_t slice0, nslices;
-  int32_t item, split, nsplit;   // item: its arrival counter
+  int32_t split, nsplit;
   int32_t part_row;         // first scratch row of the item
-  int32_t pad;
+  int32_t pad[2];
 };
 static_assert(sizeof(Piece) == 64, "pieces are read as 64-byte records");
+
+// A row of an item of several parts: where the first part's is, how many rows one
+// part is from the next, and where the result goes.
+struct Joined { int32_t part_row, step, nsplit, token, head, pad[3]; };
+static_assert(sizeof(Joined) == 32, "rows are read as two 16-byte records");
 
 struct Job { int32_t seq, first, count, page; };      // read back: tokens first..first+count of a sequence, to a page
 static_assert(sizeof(Job) == 16, "jobs are read as 16-byte records");
 
-// The plan's words on the device, by their offsets: cta_first[ctas + 1], the items'
-// counters, pieces, the words of the plan of the others (emmy_paged.h), their page
-// table [sequences][width] in the workspace, and the jobs that fill it.
+// The plan's words on the device, by their offsets: CTAs, warps of one, offset of the
+// pieces, the status; from 4 on where the pieces of each CTA begin that its warps share
+// and then those of each warp (ctas x (warps + 1) + 1); pieces, rows to join, the words
+// of the plan of the others (emmy_paged.h), their page table [sequences][width] in the
+// workspace, and the jobs that fill it.  The kernel writes the status only.
 struct Layout {
-  int ctas = 0, counters = 0, pieces = 0, others = 0, table = 0, jobs = 0;
+  static constexpr int status = 3;
+  int ctas = 0, pieces = 0, joined = 0, others = 0, table = 0, jobs = 0;
 };
 
 }  // namespace emmy_quantised
@@ -48,8 +61,8 @@ struct emmy_quantised_plan_s {
   emmy_paged_plan_s *others = nullptr;       // of the sequences with many rows; null: none
   int64_t tokens = 0, part_rows = 0, workspace_pages = 0;
   int32_t sequences = 0, q_heads = 0, kv_heads = 0, head_dim = 0, causal = 0, window = 0, max_kv = 0;
-  int32_t tiles = 1;                         // tiles of 8 rows that a piece may have: 1 or 4
-  int32_t table_width = 0, n_jobs = 0;
+  int32_t tiles = 1;                         // tiles of 8 rows that a piece may have: 1, 2 or 4
+  int32_t table_width = 0, n_jobs = 0, n_joined = 0;
   bool reads = false;                        // some row sees a key
   ~emmy_quantised_plan_s() { delete others; }
 };

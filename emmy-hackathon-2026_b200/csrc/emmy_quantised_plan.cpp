@@ -1,8 +1,9 @@
 // emmy_quantised_plan.cpp -- cuts the attention over an 8-bit cache into work.
 //
 // A sequence whose query rows of a key head are few (kFewRows) is bound by reading
-// its keys, which a kernel of its own takes as they lie: its slices of 16 keys are
+// its keys, which a kernel of its own takes as they lie: its slices of keys are
 // poured over the CTAs up to a common level, an item being cut where a CTA is full.
+// The pieces go to the CTA's warps together or to each on its own (below).
 // The others are bound by the tensor cores: their keys are read back to 16 bits once,
 // in pages of 128 tokens, and go through the 16-bit cache's attention.
 #include "emmy_quantised.h"
@@ -19,9 +20,11 @@ using namespace emmy_quantised;
 
 namespace {
 
-// What a piece costs beside its slices, in slices of its CTA (0.19 us where all CTAs
-// read), and the fewest that are worth a piece of their own.
-constexpr int kPieceCost = 6, kMinPiece = 16;
+// What a piece costs beside its slices, in slices of a warp (1.5 us where all warps of
+// the GPU read): one that a CTA's warps share, for their waiting for one another and
+// joining, and one of a warp.  Slices that are worth a shared piece or one of a warp;
+// parts up to which an item is left to its warps, the last of which joins them.
+constexpr int kSharedCost = 3, kOwnCost = 1, kMinShared = 16, kMinOwn = 4, kMostParts = 16;
 constexpr int kCtasAnSm = 2;
 
 int fail(const char *fmt, long a = 0, long b = 0) {
@@ -44,9 +47,13 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
     if (few[s]) most = std::max(most, static_cast<int>(rows));
     plan.max_kv = std::max(plan.max_kv, a.kv_lens[s]);
   }
-  plan.tiles = most <= 8 ? 1 : 4;
+  plan.tiles = most <= 8 ? 1 : most <= 16 ? 2 : 4;
+  const int keys = slice_keys(a.head_dim);
   const int at_once = 8 * plan.tiles;
 
+  // the items of a sequence and a block of its rows, one for each key head
+  struct Rows { int seq, row0, nslices; size_t first; bool own; };
+  std::vector<Rows> blocks;
   std::vector<Piece> items;
   std::vector<Job> jobs;
   std::vector<int32_t> table;
@@ -57,27 +64,26 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
     auto lowest = [&](int from) { return a.window ? std::max(0, pos0 + from - a.window + 1) : 0; };
     auto highest = [&](int to) { return a.causal ? std::max(0, std::min(len, pos0 + to)) : len; };
     if (few[s]) {
-      for (int h = 0; h < a.kv_heads; ++h)
-        for (int r = 0; r < n * group; r += at_once) {
-          Piece p;
-          memset(&p, 0, sizeof p);
-          p.seq = s;
-          p.kvh = h;
-          p.tok0 = static_cast<int32_t>(first);
-          p.row0 = r;
-          p.rows = std::min(at_once, n * group - r);
-          p.pos0 = pos0;
-          p.kv_len = len;
-          p.lo = lowest(r / group);
-          p.hi = highest((r + p.rows - 1) / group + 1);
-          p.nsplit = 1;
-          if (p.hi > p.lo) {
-            p.slice0 = p.lo / kSlice;
-            p.nslices = (p.hi - 1) / kSlice + 1 - p.slice0;
-            plan.reads = true;
-          }
-          items.push_back(p);
+      for (int r = 0; r < n * group; r += at_once) {
+        Piece p;
+        memset(&p, 0, sizeof p);
+        p.seq = s;
+        p.tok0 = static_cast<int32_t>(first);
+        p.row0 = r;
+        p.rows = std::min(at_once, n * group - r);
+        p.pos0 = pos0;
+        p.kv_len = len;
+        p.lo = lowest(r / group);
+        p.hi = highest((r + p.rows - 1) / group + 1);
+        p.nsplit = 1;
+        if (p.hi > p.lo) {
+          p.slice0 = p.lo / keys;
+          p.nslices = (p.hi - 1) / keys + 1 - p.slice0;
+          plan.reads = true;
         }
+        blocks.push_back({s, r, p.nslices, items.size(), false});
+        for (p.kvh = 0; p.kvh < a.kv_heads; ++p.kvh) items.push_back(p);
+      }
     } else if (highest(n) > lowest(0)) {
       plan.reads = true;
       for (int b = lowest(0) / kBlock; b * kBlock < highest(n); ++b) {
@@ -89,36 +95,62 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
   }
   plan.tokens = first;
 
+  // A CTA's warps either share a piece, or take a head each of some slices (`heads` of
+  // them, and the slices in `ways` where there are more warps than heads): then nothing
+  // waits for anything, and the heads of a token, which lie together, are read at about
+  // the same time.  That is for work enough for all warps, and for sequences short
+  // enough to be cut into few parts.
+  const int warps = warps_of(plan.tiles), slots = kCtasAnSm * a.ctas;
+  int heads = 1;
+  for (int h = 2; h <= warps; ++h)
+    if (warps % h == 0 && a.kv_heads % h == 0) heads = h;
+  const int ways = warps / heads;
+  int64_t total = 0;
+  for (const Piece &p : items) total += p.nslices;
+  const int64_t level0 = div_up(total, int64_t(slots) * warps);        // slices of a warp
+  for (Rows &b : blocks) b.own = level0 >= 2 * kMinOwn && (b.nslices / (level0 * ways) + 2) * ways <= kMostParts;
+  std::stable_partition(blocks.begin(), blocks.end(), [](const Rows &b) { return !b.own; });
+
   // the lowest level up to which the items fit on the CTAs
-  const int slots = kCtasAnSm * a.ctas;
-  struct Part { int item, cta, b, e; };
+  struct Part { size_t item; int cta, warp, b, e; };      // warp -1: shared
   std::vector<Part> parts;
   auto pour = [&](int64_t level) {
     parts.clear();
     int c = 0;
     int64_t filled = 0;
-    for (size_t i = 0; i < items.size(); ++i) {
-      int b = 0;
-      do {
-        const int rest = items[i].nslices - b, least = std::min(kMinPiece, std::max(1, rest));
-        while (level - filled - kPieceCost < least) {
-          if (++c == slots) return false;
-          filled = 0;
-        }
-        const int64_t room = level - filled - kPieceCost;
-        // a rest too small to be a piece of its own goes along
-        const int take = rest - room >= kMinPiece ? static_cast<int>(room) : rest;
-        parts.push_back({static_cast<int>(i), c, b, b + take});
-        filled += kPieceCost + take;
-        b += take;
-      } while (b < items[i].nslices);
-    }
+    for (const Rows &rows : blocks)
+      for (int h = 0; h < a.kv_heads; h += rows.own ? heads : 1) {
+        const int per = rows.own ? ways : warps, cost = rows.own ? kOwnCost : kSharedCost;
+        const int worth = rows.own ? kMinOwn * ways : kMinShared;
+        int b = 0;
+        do {
+          const int rest = rows.nslices - b, least = std::min(worth, std::max(1, rest));
+          while ((level - filled - cost) * per < least) {
+            if (++c == slots) return false;
+            filled = 0;
+          }
+          const int64_t room = (level - filled - cost) * per;
+          // a rest too small to be a piece of its own goes along
+          const int take = rest - room >= worth ? static_cast<int>(room) : rest;
+          if (rows.own) {
+            for (int k = 0; k < ways; ++k) {
+              const int from = b + static_cast<int>(int64_t(take) * k / ways), to = b + static_cast<int>(int64_t(take) * (k + 1) / ways);
+              if (to > from || (take == 0 && k == 0))
+                for (int i = 0; i < heads; ++i) parts.push_back({rows.first + h + i, c, k * heads + i, from, to});
+            }
+          } else {
+            parts.push_back({rows.first + h, c, -1, b, b + take});
+          }
+          filled += cost + div_up(take, per);
+          b += take;
+        } while (b < rows.nslices);
+      }
     return true;
   };
-  std::vector<std::vector<Piece>> dealt(slots);
-  int counters = 0;
+  std::vector<std::vector<Piece>> dealt(slots * (warps + 1));
+  std::vector<Joined> joined;
   if (!items.empty()) {
-    int64_t low = kPieceCost, high = kPieceCost + kMinPiece;
+    int64_t low = 0, high = kSharedCost + kMinShared;
     while (!pour(high)) {
       low = high;
       high *= 2;
@@ -128,15 +160,18 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
       (pour(mid) ? high : low) = mid;
     }
     pour(high);
+    // the parts of an item in the order of their slices
+    std::stable_sort(parts.begin(), parts.end(), [](const Part &x, const Part &y) { return x.item != y.item ? x.item < y.item : x.b < y.b; });
     for (size_t i = 0; i < parts.size();) {
       size_t e = i + 1;
       while (e < parts.size() && parts[e].item == parts[i].item) ++e;
       Piece p = items[parts[i].item];
       p.nsplit = static_cast<int32_t>(e - i);
       if (p.nsplit > 1) {
-        p.item = counters++;
         if (plan.part_rows > (int64_t(1) << 30)) throw 1;
         p.part_row = static_cast<int32_t>(plan.part_rows);
+        for (int r = 0; r < p.rows; ++r)
+          joined.push_back({p.part_row + r, p.rows, p.nsplit, p.tok0 + (p.row0 + r) / group, p.kvh * group + (p.row0 + r) % group, {0, 0, 0}});
         plan.part_rows += int64_t(p.nsplit) * p.rows;
       }
       const int slice0 = p.slice0;
@@ -144,14 +179,16 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
         p.slice0 = slice0 + parts[k].b;
         p.nslices = parts[k].e - parts[k].b;
         p.split = static_cast<int32_t>(k - i);
-        dealt[parts[k].cta].push_back(p);
+        dealt[parts[k].cta * (warps + 1) + parts[k].warp + 1].push_back(p);
       }
       i = e;
     }
   }
-  std::stable_partition(dealt.begin(), dealt.end(), [](const std::vector<Piece> &d) { return !d.empty(); });
+  // (CTAs are filled in their order: those with work come first, and the others are not launched)
   int used = 0;
-  while (used < slots && !dealt[used].empty()) ++used;
+  for (int c = 0; c < slots; ++c)
+    for (int w = 0; w <= warps; ++w)
+      if (!dealt[c * (warps + 1) + w].empty()) used = c + 1;
   size_t n_pieces = 0;
   for (const auto &d : dealt) n_pieces += d.size();
 
@@ -167,30 +204,36 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
   }
 
   Layout &at = plan.at;
-  int64_t words = used + 1;
+  int64_t words = 4 + int64_t(used) * (warps + 1) + 1;
   auto place = [&](int64_t count, int64_t grid) {
     const int64_t begin = div_up(words, grid) * grid;
     words = begin + count;
     return begin;
   };
-  const int64_t at_counters = place(counters, 1), at_pieces = place(16 * int64_t(n_pieces), 16),
+  const int64_t at_pieces = place(16 * int64_t(n_pieces), 16), at_joined = place(8 * int64_t(joined.size()), 8),
                 at_others = place(plan.others ? int64_t(plan.others->words.size()) : 0, 16),
                 at_table = place(int64_t(table.size()), 4), at_jobs = place(4 * int64_t(jobs.size()), 4);
   if (words > (int64_t(1) << 30)) throw 1;
   at.ctas = used;
-  at.counters = static_cast<int>(at_counters);
   at.pieces = static_cast<int>(at_pieces);
+  at.joined = static_cast<int>(at_joined);
+  plan.n_joined = static_cast<int32_t>(joined.size());
   at.others = static_cast<int>(at_others);
   at.table = static_cast<int>(at_table);
   at.jobs = static_cast<int>(at_jobs);
   plan.words.assign(words, 0);
   size_t k = 0;
-  for (int i = 0; i < used; ++i) {
-    plan.words[i] = static_cast<int32_t>(k);
-    memcpy(&plan.words[at.pieces + 16 * k], dealt[i].data(), dealt[i].size() * sizeof(Piece));
+  const int lists = used * (warps + 1);
+  for (int i = 0; i < lists; ++i) {
+    plan.words[4 + i] = static_cast<int32_t>(k);
+    if (!dealt[i].empty()) memcpy(&plan.words[at.pieces + 16 * k], dealt[i].data(), dealt[i].size() * sizeof(Piece));
     k += dealt[i].size();
   }
-  plan.words[used] = static_cast<int32_t>(k);
+  plan.words[4 + lists] = static_cast<int32_t>(k);
+  plan.words[0] = used;
+  plan.words[1] = warps;
+  plan.words[2] = at.pieces;
+  if (!joined.empty()) memcpy(&plan.words[at.joined], joined.data(), sizeof(Joined) * joined.size());
   if (plan.others) memcpy(&plan.words[at.others], plan.others->words.data(), 4 * plan.others->words.size());
   if (!table.empty()) memcpy(&plan.words[at.table], table.data(), 4 * table.size());
   if (!jobs.empty()) memcpy(&plan.words[at.jobs], jobs.data(), sizeof(Job) * jobs.size());
@@ -243,11 +286,11 @@ extern "C" EMMY_API int emmy_quantised_plan_data(emmy_quantised_plan_t plan, con
   if (!plan || !words || !n_words || !scratch) return fail("emmy_quantised_plan_data: bad argument");
   *words = plan->words.data();
   *n_words = plan->words.size();
-  // partial rows of head_dim floats with (base, sum) of each; those of the others'
+  // partial rows of head_dim floats with (base, sum, c) of each; those of the others'
   // plan; 16-bit keys and values read back: each from a multiple of 128 bytes on
-  const size_t row = (plan->head_dim + 2) * sizeof(float);
+  const size_t row = (plan->head_dim + 4) * sizeof(float), others_row = (plan->head_dim + 2) * sizeof(float);
   auto whole = [](size_t bytes) { return (bytes + 127) / 128 * 128; };
-  *scratch = whole(plan->part_rows * row) + (plan->others ? whole(plan->others->part_rows * row) : 0) +
+  *scratch = whole(plan->part_rows * row) + (plan->others ? whole(plan->others->part_rows * others_row) : 0) +
              size_t(plan->workspace_pages) * kBlock * plan->kv_heads * plan->head_dim * 2 * 2;
   return 0;
 }

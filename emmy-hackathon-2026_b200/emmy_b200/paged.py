@@ -553,9 +553,8 @@ class QuantisedPlan(AttentionPlan):
 def quantised_attention(plan, q, k_cache, v_cache, exponents, table, scale=None, out=None, lse=None, stream=None):
     """:func:`attention` over a cache of 8-bit floats, with a :class:`QuantisedPlan`.
 
-    ``k_cache`` and ``v_cache`` are float8_e4m3fn, of any page_size; ``q`` is
-    bfloat16 or float16, of 64 or 128 components.  ``exponents``: int32 [2, kv_heads] (see the module;
-    None: all 0).  All else is as for :func:`attention`, what it says of keys and
+    ``k_cache`` and ``v_cache`` are float8_e4m3fn, with a page_size of 8 or a
+    multiple of it.  ``exponents``: int32 [2, kv_heads] (see the module; None: all 0).  All else is as for :func:`attention`, what it says of keys and
     values that are not finite included (an 8-bit float can be NaN)."""
     if not isinstance(plan, QuantisedPlan):
         raise ValueError("plan: a QuantisedPlan is wanted")

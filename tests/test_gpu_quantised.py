@@ -269,7 +269,7 @@ def check(q_lens, kv_lens, heads, kv_heads, dim, page, dtype=BF16, layout="token
 
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("layout,page", [("token", 16), ("head", 64), ("token", 8), ("head", 128), ("token", 384), ("head", 1), ("token", 7)])
+@pytest.mark.parametrize("layout,page", [("token", 16), ("head", 64), ("token", 8), ("head", 128), ("token", 384), ("head", 8), ("token", 24)])
 def test_decode_types_pages_layouts(dim, dtype, layout, page):
     check([1] * 10, [1, 15, 16, 17, 31, 32, 33, 257, 640, 1000], 16, 4, dim, page, dtype, layout)
 
@@ -327,6 +327,19 @@ def test_split_over_keys(dim, dtype, q_lens, kv_lens, heads, kv_heads):
     words = plan.words.clone()
     assert plan.scratch.numel() > 0
     for _ in range(5):
+        again = paged.quantised_attention(plan, *made)
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+    assert torch.equal(plan.words, words)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("heads,kv_heads,tokens", [(32, 8, 1), (6, 6, 2), (20, 4, 3), (8, 1, 4), (5, 5, 9), (3, 3, 24), (64, 16, 1)])
+def test_pieces_of_a_warp(heads, kv_heads, tokens, dim, dtype):
+    """Work enough that each warp takes a head of its own, in parts that their last joins."""
+    kv_lens = [(331 * s) % 1500 + tokens for s in range(60)]
+    plan, made, out, lse = check([tokens] * 60, kv_lens, heads, kv_heads, dim, 16, dtype, ctas=3)
+    words = plan.words.clone()
+    for _ in range(3):
         again = paged.quantised_attention(plan, *made)
         assert torch.equal(again[0], out) and torch.equal(again[1], lse)
     assert torch.equal(plan.words, words)

@@ -11,24 +11,25 @@ from emmy_b200 import native, paged
 
 pytestmark = pytest.mark.usefixtures("native_lib")
 
-FIELDS = ("seq", "kvh", "tok0", "row0", "rows", "pos0", "lo", "hi", "kv_len", "slice0", "nslices", "item", "split", "nsplit",
-          "part_row", "pad")
+FIELDS = ("seq", "kvh", "tok0", "row0", "rows", "pos0", "lo", "hi", "kv_len", "slice0", "nslices", "split", "nsplit", "part_row")
 FEW = 128
 
 
-def parts_of(plan, q_lens, q_heads, kv_heads):
-    """(pieces, cta_first): the words begin with cta_first, whose length is known from the last entry on."""
+def parts_of(plan):
+    """(pieces, where the lists of each CTA and warp begin, warps)"""
     w = plan.words.tolist()
-    # the first entry is 0 and they grow; the pieces begin at a multiple of 16 words
-    n = sum(bool(q) and q * (q_heads // kv_heads) <= FEW for q in q_lens)
-    if not n:
-        return [], [0]
-    ctas = next(k for k in range(1, len(w)) if w[k] <= w[k - 1]) - 1
-    first = w[:ctas + 1]
-    # counters lie between, all 0: the first piece is the first record whose rows are not 0
-    at = next(k for k in range((ctas + 1 + 15) // 16 * 16, len(w), 16) if w[k + 4])
-    assert not any(w[ctas + 1:at])
-    return [dict(zip(FIELDS, w[at + 16 * i:at + 16 * i + 16])) for i in range(first[-1])], first
+    ctas, warps, at, status = w[:4]
+    first = w[4:4 + ctas * (warps + 1) + 1]
+    assert status == 0 and first[0] == 0 and all(a <= b for a, b in zip(first, first[1:])) and at % 16 == 0
+    assert not any(w[4 + len(first):at])
+    return [dict(zip(FIELDS, w[at + 16 * i:at + 16 * i + 14])) for i in range(first[-1])], first, warps
+
+
+def rows_to_join(plan, pieces, group):
+    """Behind the pieces: (part_row, step, nsplit, token, head) of each row of an item of several parts."""
+    w, at = plan.words.tolist(), plan.words.tolist()[2] + 16 * len(pieces)
+    n = sum(u["rows"] for u in pieces if u["nsplit"] > 1 and u["split"] == 0)
+    return [tuple(w[at + 8 * i:at + 8 * i + 5]) for i in range(n)]
 
 
 CASES = [
@@ -51,18 +52,18 @@ CASES = [
 @pytest.mark.parametrize("ctas", [1, 7, 148])
 def test_pieces_cover_the_work_once(q_lens, kv_lens, hq, hkv, causal, window, ctas):
     plan = paged.QuantisedPlan(q_lens, kv_lens, hq, hkv, 64, causal, window or None, device="cpu", ctas=ctas)
-    pieces, first = parts_of(plan, q_lens, hq, hkv)
+    pieces, first, warps = parts_of(plan)
     group = hq // hkv
     few = [q * group <= FEW for q in q_lens]
     most = max([8] + [q * group for q, f in zip(q_lens, few) if f])
-    at_once = 8 if most <= 8 else 32
-    assert len(first) - 1 <= 2 * ctas
+    at_once = 8 if most <= 8 else 16 if most <= 16 else 32
+    assert warps == {8: 8, 16: 6, 32: 4}[at_once] and len(first) - 1 <= 2 * ctas * (warps + 1)
     items = {}
     for u in pieces:
         assert few[u["seq"]] and 0 < u["rows"] <= at_once and 0 <= u["kvh"] < hkv
         assert u["tok0"] == sum(q_lens[:u["seq"]]) and u["pos0"] == kv_lens[u["seq"]] - q_lens[u["seq"]] and u["kv_len"] == kv_lens[u["seq"]]
         items.setdefault((u["seq"], u["kvh"], u["row0"]), []).append(u)
-    covered, scratch, numbers = set(), set(), set()
+    covered, scratch, joined = set(), set(), set()
     for (s, h, row0), us in items.items():
         rows = range(row0, row0 + us[0]["rows"])
         assert rows.stop <= q_lens[s] * group
@@ -75,28 +76,27 @@ def test_pieces_cover_the_work_once(q_lens, kv_lens, hq, hkv, causal, window, ct
         if hi <= lo:
             assert [u["nslices"] for u in us] == [0]
         else:
-            at = lo // 16
+            at = lo // 32                # slices of 32 keys of 64 components
             for k, u in enumerate(sorted(us, key=lambda u: u["split"])):
                 assert (u["slice0"], u["split"], u["lo"], u["hi"]) == (at, k, lo, hi) and u["nslices"] > 0
                 at += u["nslices"]
-            assert at == -(-hi // 16)
-        assert all((u["nsplit"], u["item"], u["part_row"], u["rows"]) == (len(us), us[0]["item"], us[0]["part_row"], us[0]["rows"]) for u in us)
+            assert at == -(-hi // 32)
+        assert all((u["nsplit"], u["part_row"], u["rows"]) == (len(us), us[0]["part_row"], us[0]["rows"]) for u in us)
         if len(us) > 1:
-            assert us[0]["item"] not in numbers
-            numbers.add(us[0]["item"])
+            joined |= {(us[0]["part_row"] + r - row0, len(rows), len(us), us[0]["tok0"] + r // group, h * group + r % group) for r in rows}
             mine = set(range(us[0]["part_row"], us[0]["part_row"] + len(us) * us[0]["rows"]))
             assert not mine & scratch
             scratch |= mine
     assert len(covered) == sum(q * hq for q, f in zip(q_lens, few) if f)
-    assert numbers == set(range(len(numbers))) and scratch == set(range(len(scratch)))
+    assert scratch == set(range(len(scratch))) and joined == set(rows_to_join(plan, pieces, group))
     # the others' keys: 4 bytes a component of whole pages of 128 tokens that some row sees, and parts
     blocks = 0
     for q, kv, f in zip(q_lens, kv_lens, few):
         hi, lo = kv, max(0, kv - q - window + 1) if window else 0
         blocks += 0 if f or hi <= 0 else -(-hi // 128) - lo // 128
-    assert plan.scratch.numel() >= len(scratch) * 66 * 4 + blocks * 128 * hkv * 64 * 4
+    assert plan.scratch.numel() >= len(scratch) * 68 * 4 + blocks * 128 * hkv * 64 * 4
     if all(few):
-        assert plan.scratch.numel() == -(-len(scratch) * 66 * 4 // 128) * 128
+        assert plan.scratch.numel() == -(-len(scratch) * 68 * 4 // 128) * 128
 
 
 @pytest.mark.parametrize("q_lens,kv_lens,most", [
@@ -106,9 +106,23 @@ def test_pieces_cover_the_work_once(q_lens, kv_lens, hq, hkv, causal, window, ct
 ])
 def test_work_is_even(q_lens, kv_lens, most):
     plan = paged.QuantisedPlan(q_lens, kv_lens, 32, 8, 128, device="cpu", ctas=148)
-    pieces, first = parts_of(plan, q_lens, 32, 8)
-    load = [sum(u["nslices"] for u in pieces[a:b]) for a, b in zip(first, first[1:])]
-    assert max(load) <= most * sum(load) / 296 + 16, (max(load), sum(load) / 296)
+    pieces, first, warps = parts_of(plan)
+    load = []
+    for c in range(0, len(first) - 1, warps + 1):
+        shared, *own = (sum(u["nslices"] for u in pieces[a:b]) for a, b in zip(first[c:], first[c + 1:c + warps + 2]))
+        load.append(-(-shared // warps) + max(own))
+    even = sum(u["nslices"] for u in pieces) / 296 / warps
+    assert max(load) <= most * even + 4, (max(load), even)
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_parts_of_random_plans(seed):
+    """Whatever is shared or a warp's own: each item's slices once, in order of its parts."""
+    r = random.Random(seed)
+    n, kv_heads, group = r.randint(1, 70), r.choice((1, 2, 3, 4, 6, 8, 32)), r.choice((1, 2, 4, 5, 8, 16))
+    q_lens = [r.choice((1, 1, 1, r.randint(0, 9), r.randint(0, 40))) for _ in range(n)]
+    kv_lens = [r.choice((0, r.randint(1, 300), r.randint(1, 9000))) for _ in range(n)]
+    test_pieces_cover_the_work_once(q_lens, kv_lens, group * kv_heads, kv_heads, r.random() < 0.8, 0, r.choice((1, 5, 148)))
 
 
 @pytest.mark.parametrize("change,words", [
@@ -178,7 +192,7 @@ def test_c_norm_rotate_append_refuses(native_lib, change, words):
 @pytest.mark.parametrize("q_lens", [[2], [300]])
 @pytest.mark.parametrize("change,words", [
     (dict(dtype=7), b"dtype"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=3.4e38), b"scale"),
-    (dict(page_size=0), b"page_size"), (dict(pages=0), b"pages"), (dict(table_width=1), b"does not hold"), (dict(q=0), b"null"),
+    (dict(page_size=0), b"page_size"), (dict(page_size=12), b"page_size"), (dict(pages=0), b"pages"), (dict(table_width=1), b"does not hold"), (dict(q=0), b"null"),
     (dict(scratch=0), b"null"), (dict(q=4104), b"16 bytes"), (dict(scratch=4112), b"16 bytes"), (dict(table=4098), b"16 bytes"),
     (dict(exponents=4098), b"16 bytes"), (dict(k_cache=4104), b"16 bytes"), (dict(q_token=100), b"stride"), (dict(k_page=-2048), b"stride"),
     (dict(v_token=136), b"stride"), (dict(v_token=0), b"stride"),
