@@ -80,7 +80,7 @@ template <int D, int NT> struct Shape {
   static constexpr int kHalf = 16 * D, kStage = kSubs * 2 * kHalf;         // bytes: 16 keys, then their values
   static constexpr int kSteps = D / 16;                                    // products of 16 components
   static constexpr int kRounds = D / 32;                                   // of 4 of a thread's components, at a unit's end
-  static constexpr bool kQueryRegs = NT == 1;                              // queries in registers
+  static constexpr bool kQueryRegs = NT * D <= 128;                        // queries in registers
   static constexpr int kStages = NT == 4 && D == 128 ? 4 : NT == 4 ? 5 : 3;        // slices of a warp in flight or in use
   static constexpr int kRing = kStages * kStage, kQueryBytes = kQueryRegs ? 0 : NT * kSteps * 256;
   static constexpr int kQuery = kWarps * kRing;
@@ -316,7 +316,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 2) few_rows_kernel(con
     }
     if (alone && i >= last) break;
     const Piece u = read_piece(p, i);
-    const int tiles = NT == 1 ? 1 : (u.rows + 7) / 8;
     // ------------------------------------------------------------ queries
     uint32_t q[S::kQueryRegs ? NT * 2 * S::kSteps : 1];
     float c[S::kQueryRegs ? 2 * NT : 1];
@@ -354,14 +353,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 2) few_rows_kernel(con
     if (S::kQueryRegs) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if (NT > 1 && nt >= tiles) break;
         const float of_row = take_row(nt, q + (S::kQueryRegs ? nt * 2 * S::kSteps : 0));
         c[S::kQueryRegs ? 2 * nt : 0] = __shfl_sync(~0u, of_row, 8 * t);
         c[S::kQueryRegs ? 2 * nt + 1 : 0] = __shfl_sync(~0u, of_row, 8 * t + 4);
         if (t == 0) scales[8 * nt + g] = of_row;
       }
     } else {
-      for (int nt = 0; nt < tiles; ++nt) {
+#pragma unroll 1
+      for (int nt = 0; nt < NT; ++nt) {
         uint32_t w[2 * S::kSteps];
         const float of_row = take_row(nt, w);
 #pragma unroll
@@ -451,7 +450,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 2) few_rows_kernel(con
             const uint32_t a[4] = {widen_low(x[k]), widen_low(y[k]), widen_high(x[k]), widen_high(y[k])};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              if (NT > 1 && nt >= tiles) break;
               uint32_t b[2];
               if (S::kQueryRegs)
                 b[0] = q[S::kQueryRegs ? 2 * (nt * S::kSteps + 4 * d + k) : 0], b[1] = q[S::kQueryRegs ? 2 * (nt * S::kSteps + 4 * d + k) + 1 : 0];
@@ -471,7 +469,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 2) few_rows_kernel(con
         const int key = key0 + key_of<D>(g);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          if (NT > 1 && nt >= tiles) break;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             int lo, hi;
@@ -489,7 +486,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 2) few_rows_kernel(con
       auto exponents = [&] {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          if (NT > 1 && nt >= tiles) break;
           const float by[2] = {scale_of(nt, 0), scale_of(nt, 1)};
 #pragma unroll
           for (int h = 0; h < S::kSubs; ++h)
@@ -504,7 +500,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 2) few_rows_kernel(con
       if (__any_sync(~0u, most > kShift + kGrow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          if (NT > 1 && nt >= tiles) break;
           float by[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -526,7 +521,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 2) few_rows_kernel(con
       uint32_t w[NT][S::kSubs][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if (NT > 1 && nt >= tiles) break;
 #pragma unroll
         for (int h = 0; h < S::kSubs; ++h) {
 #pragma unroll
@@ -559,7 +553,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 2) few_rows_kernel(con
           const uint32_t b[4] = {widen_low(p1), widen_high(p1), widen_low(p3), widen_high(p3)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            if (NT > 1 && nt >= tiles) break;
             mma(o[nt][2 * k], a, w[nt][h][0], w[nt][h][1]);
             mma(o[nt][2 * k + 1], b, w[nt][h][0], w[nt][h][1]);
           }
@@ -589,7 +582,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 2) few_rows_kernel(con
     if (alone) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if (NT > 1 && nt >= tiles) break;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = 8 * nt + 2 * t + e;
@@ -643,7 +635,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 2) few_rows_kernel(con
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      if (NT > 1 && nt >= tiles) break;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = 8 * nt + 2 * t + e;
@@ -656,7 +647,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 2) few_rows_kernel(con
     const uint32_t join = base + S::kJoin;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      if (NT > 1 && nt >= tiles) break;
 #pragma unroll
       for (int from = 0; from < S::kRounds; ++from) {
         if (nt || from) __syncthreads();
