@@ -53,5 +53,6 @@ struct emmy_paged_plan_s {
   int64_t tokens = 0;
   int64_t part_rows = 0;
   bool tiled = false, spread = false;      // some unit has whole query tiles, or rows for one warp
+  bool narrow = false;                     // made without wide units
   int32_t sequences = 0, q_heads = 0, kv_heads = 0, head_dim = 0, causal = 0, window = 0, max_kv = 0;
 };

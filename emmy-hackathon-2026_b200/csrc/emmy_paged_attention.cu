@@ -65,12 +65,15 @@ namespace {
 using emmy_paged::kTile;
 using emmy_paged::Unit;
 
-constexpr int kThreads = 384;
-// registers a thread: at launch, then those of the softmax warps, which hold a
-// row of scores, and of the others; the shares add up to what was launched
-constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
-static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
-constexpr int kSoftmaxWarps = 8, kKeyWarp = 8, kMmaWarp = 10;
+// Registers a thread: at launch, then those of the softmax warps, which hold a
+// row of scores, and of the others; the shares add up to what was launched.
+// BITS8: a cache of 8-bit floats, which four more warps widen.
+template <bool BITS8> struct Warps {
+  static constexpr int kThreads = BITS8 ? 512 : 384;
+  static constexpr int kLaunchRegs = BITS8 ? 128 : 168, kSoftmaxRegs = BITS8 ? 200 : 216, kOtherRegs = BITS8 ? 56 : 72;
+  static_assert(256 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs <= kThreads * kLaunchRegs, "register split");
+};
+constexpr int kSoftmaxWarps = 8, kKeyWarp = 8, kMmaWarp = 10, kWideningWarp = 12;
 constexpr int kSmem = 227 * 1024;
 constexpr float kNoMax = -FLT_MAX;      // exponent base of a row that has seen no key
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -89,14 +92,22 @@ struct alignas(64) Params {
   int q_heads, group, group_inverse, per_tile, box, causal, window, aligned32;
   int tiles_a_page;                    // of pages of a tile or more
   float scale_log2, scale_power;       // c, and the power of two next to it
+  const int *exponents;                // of an 8-bit cache's keys and values, [2][kv_heads]; null: 0
+  int kv_heads;
 };
 
-template <int D> struct Shape {
+template <int D, bool BITS8> struct Shape {
   static constexpr int kTileBytes = kTile * D * 2;       // 16 KiB or more: the joining needs them
-  static constexpr int kStages = D == 128 ? 5 : 12;      // key and value tiles in flight
-  static constexpr int kRing = 2 * kTileBytes;           // after two query tiles
-  static constexpr int kBars = kRing + kStages * kTileBytes;
-  static constexpr int kWords = kBars + (2 * kStages + 14) * 8, kEnd = kWords + 32 + kTile * 8;
+  static constexpr int kStages = BITS8 ? (D == 128 ? 4 : 8) : D == 128 ? 5 : 12;      // key and value tiles in flight
+  // after two query tiles (BITS8, where no unit is wide: one, and 16 KiB for the joining)
+  static constexpr int kRing = kTileBytes + (BITS8 ? 16384 : kTileBytes);
+  // BITS8: the tiles as they arrive, of 8-bit floats; the others are widened
+  static constexpr int kRawStages = BITS8 ? (D == 128 ? 3 : 8) : 0, kRaw = kRing + kStages * kTileBytes;
+  static constexpr int kBars = kRaw + kRawStages * (kTileBytes / 2);
+  static constexpr int kWords = kBars + (2 * kStages + 14 + 2 * kRawStages + (BITS8 ? 1 : 0)) * 8, kPowers = kWords + 32 + kTile * 8;
+  static constexpr int kEnd = kPowers + (BITS8 ? 2 * kTile : 0);
+  // tiles that are copied ahead, and bytes of an element there
+  static constexpr int kCopied = BITS8 ? kRawStages : kStages, kElement = BITS8 ? 1 : 2;
   static_assert(kEnd + 1024 <= kSmem, "shared memory");
 };
 
@@ -327,34 +338,43 @@ template <bool BF16> __host__ __device__ constexpr uint32_t instruction(int n, b
 }
 
 // ---------------------------------------------------------------- roles
-template <int D, bool SPREAD> struct Smem {
+template <int D, bool SPREAD, bool BITS8> struct Smem {
+  using S = Shape<D, BITS8>;
   uint32_t base;       // 1024-byte aligned
-  __device__ uint32_t query(int t) const { return base + t * Shape<D>::kTileBytes; }
-  __device__ uint32_t stage(int s) const { return base + Shape<D>::kRing + s * Shape<D>::kTileBytes; }
-  __device__ uint32_t bar(int i) const { return base + Shape<D>::kBars + 8 * i; }
+  __device__ uint32_t query(int t) const { return base + t * S::kTileBytes; }
+  __device__ uint32_t stage(int s) const { return base + S::kRing + s * S::kTileBytes; }
+  __device__ uint32_t bar(int i) const { return base + S::kBars + 8 * i; }
   __device__ uint32_t full(int s) const { return bar(s); }
-  __device__ uint32_t empty(int s) const { return bar(Shape<D>::kStages + s); }
-  __device__ uint32_t q_full() const { return bar(2 * Shape<D>::kStages); }
-  __device__ uint32_t q_empty() const { return bar(2 * Shape<D>::kStages + 1); }
-  __device__ uint32_t s_full(int t) const { return bar(2 * Shape<D>::kStages + 2 + t); }
+  __device__ uint32_t empty(int s) const { return bar(S::kStages + s); }
+  __device__ uint32_t q_full() const { return bar(2 * S::kStages); }
+  __device__ uint32_t q_empty() const { return bar(2 * S::kStages + 1); }
+  __device__ uint32_t s_full(int t) const { return bar(2 * S::kStages + 2 + t); }
   // the weights of a tile's first and last 64 keys
-  __device__ uint32_t p_ready(int t, int half) const { return bar(2 * Shape<D>::kStages + 4 + 2 * t + half); }
-  __device__ uint32_t final(int t) const { return bar(2 * Shape<D>::kStages + 8 + t); }
-  __device__ uint32_t drain(int t) const { return bar(2 * Shape<D>::kStages + 10 + t); }
+  __device__ uint32_t p_ready(int t, int half) const { return bar(2 * S::kStages + 4 + 2 * t + half); }
+  __device__ uint32_t final(int t) const { return bar(2 * S::kStages + 8 + t); }
+  __device__ uint32_t drain(int t) const { return bar(2 * S::kStages + 10 + t); }
   // wide units: stream t may issue
-  __device__ uint32_t turn(int t) const { return bar(2 * Shape<D>::kStages + 12 + t); }
-  __device__ volatile int *words() const { return static_cast<volatile int *>(__cvta_shared_to_generic(base + Shape<D>::kWords)); }
-  __device__ float2 *ml() const { return static_cast<float2 *>(__cvta_shared_to_generic(base + Shape<D>::kWords + 32)); }
+  __device__ uint32_t turn(int t) const { return bar(2 * S::kStages + 12 + t); }
+  // where queries are known to have been copied, and by which power of two a row of
+  // them was multiplied, of even and odd units
+  __device__ uint32_t q_copied() const { return BITS8 ? bar(2 * S::kStages + 14 + 2 * S::kRawStages) : q_full(); }
+  __device__ volatile int8_t *powers(int odd) const { return static_cast<volatile int8_t *>(__cvta_shared_to_generic(base + S::kPowers)) + odd * kTile; }
+  // where tiles are copied to, and their barriers
+  __device__ uint32_t copied(int s) const { return BITS8 ? base + S::kRaw + s * (S::kTileBytes / 2) : stage(s); }
+  __device__ uint32_t copied_full(int s) const { return BITS8 ? bar(2 * S::kStages + 14 + s) : full(s); }
+  __device__ uint32_t copied_empty(int s) const { return BITS8 ? bar(2 * S::kStages + 14 + S::kRawStages + s) : empty(s); }
+  __device__ volatile int *words() const { return static_cast<volatile int *>(__cvta_shared_to_generic(base + S::kWords)); }
+  __device__ float2 *ml() const { return static_cast<float2 *>(__cvta_shared_to_generic(base + S::kWords + 32)); }
 };
 // words(): 0 dead, 1 tensor memory address, 2 + t "last to arrive" of stream t
 
-template <int D> struct Ring {
+template <int STAGES> struct Ring {
   int stage = 0;
   uint32_t phase = 0;
-  __device__ __forceinline__ void next(int n = 1) {     // n < kStages
+  __device__ __forceinline__ void next(int n = 1) {     // n <= STAGES
     stage += n;
-    if (stage >= Shape<D>::kStages) {
-      stage -= Shape<D>::kStages;
+    if (stage >= STAGES) {
+      stage -= STAGES;
       phase ^= 1;
     }
   }
@@ -380,28 +400,28 @@ __device__ __forceinline__ Unit read_unit(const Params &p, int i) {
 // (!SPREAD), which in the wide units' kernel costs them 3 to 4 % though they never
 // come to it: 1,030 against 1,005 us on 8 prompts of 4,096, 165 against 158 on the
 // windowed chunks.
-template <int D, bool SPREAD> __device__ __forceinline__ bool spread(const Params &p, const Smem<D, SPREAD> &, const Unit &u) {
+template <int D, bool SPREAD, bool BITS8> __device__ __forceinline__ bool spread(const Params &p, const Smem<D, SPREAD, BITS8> &, const Unit &u) {
   return SPREAD && emmy_paged::is_spread(u.wide, u.ntiles, u.ntok, p.group);
 }
 
 // Query tiles: one 128-row tile for each stream of a wide unit, one for both of
 // a narrow one, each a box of group x tokens_per_tile rows; the rows of a spread
 // unit four times.
-template <int D, bool SPREAD>
-__device__ __forceinline__ void load_queries(const Params &p, const Smem<D, SPREAD> &sm, const Unit &u) {
+template <int D, bool SPREAD, bool BITS8>
+__device__ __forceinline__ void load_queries(const Params &p, const Smem<D, SPREAD, BITS8> &sm, const Unit &u) {
   if (spread(p, sm, u)) {
-    bar_expect(sm.q_full(), 4 * p.group * (32 / p.group) * 128 * (D / 64));
+    bar_expect(sm.q_copied(), 4 * p.group * (32 / p.group) * 128 * (D / 64));
     for (int w = 0; w < 4; ++w)
 #pragma unroll
       for (int h = 0; h < D / 64; ++h)
-        load_box(sm.query(0) + h * (kTile * 128) + w * (32 * 128), &p.q32, sm.q_full(), 64 * h, 0, u.kvh, u.tok0);
+        load_box(sm.query(0) + h * (kTile * 128) + w * (32 * 128), &p.q32, sm.q_copied(), 64 * h, 0, u.kvh, u.tok0);
   } else {
     const int tiles = u.wide ? 2 : 1;
-    bar_expect(sm.q_full(), tiles * p.group * p.per_tile * 128 * (D / 64));
+    bar_expect(sm.q_copied(), tiles * p.group * p.per_tile * 128 * (D / 64));
     for (int t = 0; t < tiles; ++t)
 #pragma unroll
       for (int h = 0; h < D / 64; ++h)
-        load_box(sm.query(t) + h * (kTile * 128), &p.q, sm.q_full(), 64 * h, 0, u.kvh, u.tok0 + t * p.per_tile);
+        load_box(sm.query(t) + h * (kTile * 128), &p.q, sm.q_copied(), 64 * h, 0, u.kvh, u.tok0 + t * p.per_tile);
   }
 }
 
@@ -412,12 +432,12 @@ __device__ __forceinline__ void load_queries(const Params &p, const Smem<D, SPRE
 // the first keys (one tile, or one for each stream), then values of tile n and
 // keys of tile n + ahead.  One warp for both took 2,400 cycles a tile pair, more
 // than a pair of 64-component heads takes to arrive.
-template <bool VALUES, int D, bool SPREAD>
-__device__ void load_role(const Params &p, const Smem<D, SPREAD> &sm, const Guard &g, int first, int last) {
-  constexpr int S = Shape<D>::kStages;
+template <bool VALUES, int D, bool SPREAD, bool BITS8>
+__device__ void load_role(const Params &p, const Smem<D, SPREAD, BITS8> &sm, const Guard &g, int first, int last) {
+  constexpr int S = Shape<D, BITS8>::kCopied, kElement = Shape<D, BITS8>::kElement;
   const int lane = threadIdx.x % 32, boxes = kTile / p.box;
   const CUtensorMap *map = VALUES ? &p.v : &p.k;
-  Ring<D> ring;
+  Ring<S> ring;
   uint32_t issued = 0, parity = 0;       // of each stage: the last copy into it
   uint32_t q_phase = 0, queries_out = 1;      // out: the last load's phase of q_full
   bool alive = true;
@@ -463,21 +483,25 @@ __device__ void load_role(const Params &p, const Smem<D, SPREAD> &sm, const Guar
         const uint64_t t0 = now_ns();
         for (;;) {
           queries(false);
-          const bool room = bar_test(sm.empty(ring.stage), ring.phase ^ 1);
+          const bool room = bar_test(sm.copied_empty(ring.stage), ring.phase ^ 1);
           if (!queries_due || __any_sync(~0u, room || now_ns() - t0 > 1000000000ull)) break;
         }
       }
-      alive = alive && g.wait(sm.empty(ring.stage), ring.phase ^ 1, 1);
+      alive = alive && g.wait(sm.copied_empty(ring.stage), ring.phase ^ 1, 1);
       if (!alive) break;
       const bool wanted = b0.page != INT_MIN;
-      const uint32_t bar = sm.full(ring.stage);
+      const uint32_t bar = sm.copied_full(ring.stage);
       const int count = __popc(__ballot_sync(~0u, wanted));
-      if (elected()) bar_expect(bar, count * p.box * D * 2);
+      if (elected()) bar_expect(bar, count * p.box * D * kElement);
       __syncwarp();
       if (wanted) {
-        const uint32_t dst = sm.stage(ring.stage) + lane * p.box * 128;
+        if (BITS8) {
+          load_box(sm.copied(ring.stage) + lane * p.box * D, map, bar, 0, b0.token, u.kvh, b0.page);
+        } else {
+          const uint32_t dst = sm.stage(ring.stage) + lane * p.box * 128;
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h) load_box(dst + h * (kTile * 128), map, bar, 64 * h, b0.token, u.kvh, b0.page);
+          for (int h = 0; h < D / 64; ++h) load_box(dst + h * (kTile * 128), map, bar, 64 * h, b0.token, u.kvh, b0.page);
+        }
       }
       issued |= 1u << ring.stage;
       parity = (parity & ~(1u << ring.stage)) | ring.phase << ring.stage;
@@ -495,11 +519,135 @@ __device__ void load_role(const Params &p, const Smem<D, SPREAD> &sm, const Guar
   const uint64_t t0 = now_ns();
   if (!alive)
     for (int k = 0; k < S; ++k)
-      while ((issued >> k & 1) && !bar_try(sm.full(k), parity >> k & 1) && now_ns() - t0 < 100000000ull) {
+      while ((issued >> k & 1) && !bar_try(sm.copied_full(k), parity >> k & 1) && now_ns() - t0 < 100000000ull) {
       }
   if (VALUES)
-    while (!bar_try(sm.q_full(), queries_out) && now_ns() - t0 < 100000000ull) {
+    while (!bar_try(sm.q_copied(), queries_out) && now_ns() - t0 < 100000000ull) {
     }
+}
+
+__device__ __forceinline__ void load16(uint32_t at, uint32_t *r) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void store16(uint32_t at, const uint32_t *r) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ uint32_t widened(uint32_t word, bool upper) {
+  uint32_t r;
+  if (upper)
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(word));
+  else
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(word));
+  return r;
+}
+
+// BITS8: 32 rows a warp, and 32 keys of each tile.
+//
+// Tiles go from where they arrive to f16 tiles for the products, in the ring's order;
+// every 8-bit float is an f16.  A lane has 8 components of every second or fourth of
+// its warp's keys, so that 16 lanes read 128 bytes in a row and 8 write a row's pieces,
+// whose order is the 128-byte swizzle's.
+//
+// Queries (BF16: of bfloat16) become f16 where they lie, a row a lane, times the power of
+// two that brings the row's largest to 2^14..2^15: exact for components down to 2^-29
+// of it, and within 2^-40 of it below.  The softmax takes it back.
+template <bool BF16, int D, bool SPREAD>
+__device__ void widen_role(const Params &p, const Smem<D, SPREAD, true> &sm, const Guard &g, int first, int last) {
+  using S = Shape<D, true>;
+  constexpr int kOfRow = D / 8, kAtOnce = 32 / kOfRow;       // lanes of a row, rows at once
+  const int warp = threadIdx.x / 32 - kWideningWarp, lane = threadIdx.x % 32;
+  const int key = 32 * warp + lane / kOfRow, piece = lane % kOfRow;
+  const uint32_t from = key * D + piece * 8, to = (piece / 8) * (kTile * 128) + key * 128 + ((piece % 8) ^ (key & 7)) * 16;
+  Ring<S::kRawStages> raw;
+  Ring<S::kStages> ring;
+  uint32_t q_phase = 0;
+  bool alive = true;
+  auto tile = [&] {
+    alive = alive && g.wait(sm.copied_full(raw.stage), raw.phase, 6) && g.wait(sm.empty(ring.stage), ring.phase ^ 1, 7);
+    if (alive) {
+      const uint32_t src = sm.copied(raw.stage) + from, dst = sm.stage(ring.stage) + to;
+#pragma unroll
+      for (int k0 = 0; k0 < 32 / kAtOnce; k0 += 8) {
+        uint32_t in[8][2];         // (reads under way together)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(in[k][0]), "=r"(in[k][1]) : "r"(src + (k0 + k) * kAtOnce * D) : "memory");
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t out[4] = {widened(in[k][0], false), widened(in[k][0], true), widened(in[k][1], false), widened(in[k][1], true)};
+          store16((dst ^ ((k0 + k) * kAtOnce & 7) * 16) + (k0 + k) * kAtOnce * 128, out);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        bar_arrive(sm.full(ring.stage));
+        bar_arrive(sm.copied_empty(raw.stage));
+      }
+    }
+    raw.next();
+    ring.next();
+  };
+  auto queries = [&](const Unit &u) {
+    alive = alive && g.wait(sm.q_copied(), q_phase, 8);
+    const int row = 32 * warp + lane, rows = u.ntok * p.group;
+    if (alive && (spread(p, sm, u) ? lane < rows : row < rows)) {
+      const uint32_t at = sm.query(0) + row * 128;
+      auto both = [&](uint32_t x) {
+        if (BF16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+        return __half22float2(*reinterpret_cast<__half2 *>(&x));
+      };
+      float top = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < D / 8; ++k) {
+        uint32_t in[4];
+        load16(at + k / 8 * (kTile * 128) + ((k % 8) ^ (row & 7)) * 16, in);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = both(in[e]);
+          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+      const int up = top == 0.f ? 0 : min(14 - (int(__float_as_uint(top) >> 23) - 127), 120);
+      const float by = __uint_as_float(uint32_t(up + 127) << 23);
+#pragma unroll 4
+      for (int k = 0; k < D / 8; ++k) {
+        const uint32_t where = at + k / 8 * (kTile * 128) + ((k % 8) ^ (row & 7)) * 16;
+        uint32_t x[4];
+        load16(where, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = both(x[e]);
+          x[e] = pack16<false>(f.x * by, f.y * by);
+        }
+        store16(where, x);
+      }
+      sm.powers(q_phase)[row] = static_cast<int8_t>(up);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0 && alive) bar_arrive(sm.q_full());
+    q_phase ^= 1;
+  };
+  for (int i = first; i < last; ++i) {
+    const Unit u = read_unit(p, i);
+    if (!u.ntiles) continue;
+    // the queries' place may be in use until the unit before is through with its keys
+    for (int n = 0; n < min(2, u.ntiles); ++n) tile();
+    queries(u);
+    for (int n = 0; n < u.ntiles; ++n) {
+      tile();
+      if (n + 2 < u.ntiles) tile();
+    }
+  }
+}
+
+// 2^exponent of a head's keys (0) or values (1)
+__device__ __forceinline__ int exponent_of(const Params &p, int which, int head) {
+  return p.exponents ? min(max(__ldg(p.exponents + which * p.kv_heads + head), EMMY_MIN_EXPONENT), EMMY_MAX_EXPONENT) : 0;
+}
+template <bool BITS8> __device__ __forceinline__ float unscaled(const Params &p, const Unit &u) {
+  return BITS8 ? __uint_as_float(uint32_t(exponent_of(p, 1, u.kvh) + 127) << 23) : 1.f;
 }
 
 // The products of stream t.  In a wide unit the streams issue in turn, so that
@@ -507,12 +655,12 @@ __device__ void load_role(const Params &p, const Smem<D, SPREAD> &sm, const Guar
 // step and wait for the exponentials and for the tensor cores together.  Both
 // streams' warps walk the whole ring: a stage is free when both have arrived, the
 // one that uses it by the completion of its products, the other at once.
-template <bool BF16, int D, bool SPREAD>
-__device__ void mma_role(const Params &p, const Smem<D, SPREAD> &sm, const Guard &g, int first, int last, uint32_t tmem, int t) {
+template <bool BF16, int D, bool SPREAD, bool BITS8>
+__device__ void mma_role(const Params &p, const Smem<D, SPREAD, BITS8> &sm, const Guard &g, int first, int last, uint32_t tmem, int t) {
   const int lane = threadIdx.x % 32;
   constexpr uint32_t kQk = instruction<BF16>(kTile, false), kPv = instruction<BF16>(D, true);
   const uint32_t s_at = tmem + kTile * t, o_at = tmem + 2 * kTile + kTile * t;
-  Ring<D> ring;
+  Ring<Shape<D, BITS8>::kStages> ring;
   uint32_t q_phase = 0, p_phase = 0, turn_phase = t ^ 1;
   bool alive = true;
   auto wait = [&](uint32_t bar, uint32_t parity) { alive = alive && g.wait(bar, parity, 2); };
@@ -670,7 +818,7 @@ __device__ __forceinline__ float log_sum(float m, float l) { return l > 0.f ? (m
 
 // The parts of `rows` rows, joined in their order: weights 2^(m - top), eight
 // lanes a row and four rows a warp at once, so that 16 loads are in flight.
-template <int D, bool BF16> __device__ void join_parts(const Params &p, const Unit &u, int rows, int row0, int first_tok, int wid, int lane) {
+template <int D, bool BF16, bool BITS8> __device__ void join_parts(const Params &p, const Unit &u, int rows, int row0, int first_tok, int wid, int lane) {
   constexpr int kPieces = D / 32;           // of 4 components a lane
   const int64_t stride = int64_t(u.ntok) * p.group;
   for (int r = wid * 4 + lane / 8; r < rows; r += 16) {
@@ -690,7 +838,7 @@ template <int D, bool BF16> __device__ void join_parts(const Params &p, const Un
         acc[k][0] += by * v.x, acc[k][1] += by * v.y, acc[k][2] += by * v.z, acc[k][3] += by * v.w;
       }
     }
-    const float inv = reciprocal(total);
+    const float inv = reciprocal(total) * unscaled<BITS8>(p, u);
     const int64_t token = u.tok0 + first_tok + token_of(p, r);
     const int head = u.kvh * p.group + r - token_of(p, r) * p.group;
     uint2 *dst = reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + token * p.out_stride[0] + head * p.out_stride[1]) + lane % 8;
@@ -701,11 +849,13 @@ template <int D, bool BF16> __device__ void join_parts(const Params &p, const Un
   }
 }
 
-template <bool BF16, int D, bool SPREAD>
-__device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const Guard &g, int first, int last, uint32_t tmem) {
+template <bool BF16, int D, bool SPREAD, bool BITS8>
+__device__ void softmax_role(const Params &p, const Smem<D, SPREAD, BITS8> &sm, const Guard &g, int first, int last, uint32_t tmem) {
   // exponents may run 8 over the base before it moves; 16-bit floats of 5
   // exponent bits get a base 6 lower, so that small weights keep their bits
-  constexpr float kShift = BF16 ? 0.f : 6.f, kGrow = 8.f;
+  // BITS8: all products are of f16, whatever the queries and results are
+  constexpr bool kBrain = BF16 && !BITS8;
+  constexpr float kShift = kBrain ? 0.f : 6.f, kGrow = 8.f;
   // with 64 components every fourth pair's exponentials off the exponential unit: 4
   // prompts of 4,096 tokens, 32 + 8 heads, 374 us against 387 with every eighth and 392
   // with none; 8 chunks of 1 to 511 over 12,288, 32 + 4 heads, 163 us against 166 with
@@ -716,10 +866,11 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
   const int row = threadIdx.x % kTile;
   const uint32_t lanes = tmem + (uint32_t(wid * 32) << 16);
   const uint32_t s_at = lanes + kTile * t, o_at = lanes + 2 * kTile + kTile * t;
-  const float c = p.scale_log2;
+  float c = p.scale_log2, c_power = p.scale_power;     // (BITS8: of a row)
   // a base of this size is off by 2^5 at most (the sums take that) or 1 (weights of 5 exponent bits)
-  constexpr float kLarge = BF16 ? 0x1p29f : 0x1p24f;
+  constexpr float kLarge = kBrain ? 0x1p29f : 0x1p24f;
   uint32_t s_phase = 0, f_phase = 0;
+  [[maybe_unused]] int odd = 0;        // of the units with tiles
   bool alive = true;
   // this stream's tile of queries: its first token in the unit, and its rows
   const int row_token = token_of(p, row), row_head = row - row_token * p.group, lane_token = token_of(p, lane);
@@ -760,6 +911,7 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
     // multiplies by the power of two next to c instead, which is exact.  What that does
     // to scores a rounding apart is within the rounding of scores as large in 32 bits;
     // from 2^29 up different ones are 32 and more apart, and only the largest counts.
+    if (BITS8) c = p.scale_log2;
     float m = kNoMax, l = 0.f, by_c = c;
     bool begun = false;
     // the base follows the row's maximum when that grows by more than 2^8: the
@@ -772,7 +924,7 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
       if (need) {
         const float scaled = __fmul_rn(top, c), was = by_c;
         const bool large = fabsf(scaled) >= kLarge;
-        by_c = large ? p.scale_power : c;
+        by_c = large ? c_power : c;
         const float to = large ? __fmul_rn(top, by_c) : scaled - kShift;
         by = exp2_approx(was == by_c ? m - to : m * (c / was) - (large ? scaled : to));
         m = to;
@@ -798,6 +950,12 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
     for (; key0 < end; key0 += step) {
       alive = alive && g.wait(sm.s_full(t), s_phase, 3);
       s_phase ^= 1;
+      if (BITS8 && !begun) {
+        const int power = exponent_of(p, 0, read_unit(p, i).kvh) - sm.powers(odd)[row];
+        auto of_row = [&](float x) { return fminf(fmaxf(ldexpf(x, power), FLT_MIN), FLT_MAX); };
+        by_c = c = of_row(p.scale_log2);
+        c_power = of_row(p.scale_power);
+      }
       if (quarter && alive) {
         fence_after();
         uint32_t s[32], w[16];
@@ -828,7 +986,7 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
           e = exp2_approx(e);
           f = exp2_approx(f);
           part[q % 2] = add2(part[q % 2], pair(e, f));
-          w[q] = pack16<BF16>(e, f);
+          w[q] = pack16<kBrain>(e, f);
         }
         tmem_st16(s_at + 16 * wid, w);
         weights_stored(0);
@@ -898,7 +1056,7 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
               x = pair(e, f);
             }
             part[q % 4] = add2(part[q % 4], x);
-            w[q] = pack16<BF16>(e, f);
+            w[q] = pack16<kBrain>(e, f);
           }
           if (h == 2) weights_stored(0);      // of the first 64 keys
           tmem_st16(s_at + 16 * h, w);
@@ -919,6 +1077,7 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
 
     // ------------------------------------------------------------ the unit's end
     const Unit u = read_unit(p, i);
+    if (BITS8 && u.ntiles) odd ^= 1;
     const int rows = stream_rows(u), row0 = first_token(u) * p.group;
     const bool joined = !u.wide && u.ntiles > 1;      // stream 1 saw keys too
     if (begun) {
@@ -961,7 +1120,7 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
         }
 #pragma unroll
         for (int w = 0; w < 4; ++w) total += exp2_approx(ms[w] - top) * ls[w];
-        const float scale = exp2_approx(m - top) * (split ? 1.f : reciprocal(total));
+        const float scale = exp2_approx(m - top) * (split ? 1.f : reciprocal(total) * unscaled<BITS8>(p, u));
         const uint64_t f0 = pair(by0 * scale, by0 * scale), f1 = pair(by1 * scale, by1 * scale);
         group_sync(1, kTile);
         const int fit = rows <= 8 ? 7 : rows <= 16 ? 6 : 5;           // log2 of the columns
@@ -1026,7 +1185,7 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
         const bool mine = row < rows;
         const int64_t out_token = u.tok0 + first_token(u) + row_token, part = split_row + row;
         const int head = u.kvh * p.group + row_head;
-        const float inv = split ? 1.f : reciprocal(l);
+        const float inv = split ? 1.f : reciprocal(l) * unscaled<BITS8>(p, u);
         const uint64_t f0 = pair(by0 * inv, by0 * inv), f1 = pair(by1 * inv, by1 * inv);
         char *to = split ? reinterpret_cast<char *>(p.part_o + part * D)
                          : static_cast<char *>(p.out) + 2 * (out_token * p.out_stride[0] + head * p.out_stride[1]);
@@ -1090,17 +1249,18 @@ __device__ void softmax_role(const Params &p, const Smem<D, SPREAD> &sm, const G
           sm.words()[2 + t] = is_last;
         }
         group_sync(1 + t, kTile);
-        if (sm.words()[2 + t]) join_parts<D, BF16>(p, u, rows, row0, first_token(u), wid, lane);
+        if (sm.words()[2 + t]) join_parts<D, BF16, BITS8>(p, u, rows, row0, first_token(u), wid, lane);
       }
     }
     if (joined) group_sync(3, 256);       // stream 1's output and sums have been read
   }
 }
 
-template <int D, bool BF16, bool SPREAD>
-__global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __grid_constant__ Params p) {
+template <int D, bool BF16, bool SPREAD, bool BITS8>
+__global__ void __launch_bounds__(Warps<BITS8>::kThreads, 1) paged_attention_kernel(const __grid_constant__ Params p) {
+  using S = Shape<D, BITS8>;
   extern __shared__ char raw[];
-  Smem<D, SPREAD> sm;
+  Smem<D, SPREAD, BITS8> sm;
   sm.base = (smem_addr(raw) + 1023) & ~1023u;
   const int warp = threadIdx.x / 32;
   // the first unit is on its way while the CTA sets itself up
@@ -1108,11 +1268,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
   const int first = __ldg(p.cta_first + blockIdx.x), last = __ldg(p.cta_first + blockIdx.x + 1);
   asm volatile("prefetch.global.L1 [%0];" ::"l"(p.units + first));
   if (threadIdx.x == 0) {
-    for (int s = 0; s < Shape<D>::kStages; ++s) {
-      bar_init(sm.full(s), 1);
+    for (int s = 0; s < S::kStages; ++s) {
+      bar_init(sm.full(s), BITS8 ? 4 : 1);
       bar_init(sm.empty(s), 2);
     }
-    bar_init(sm.q_full(), 1);
+    for (int s = 0; s < S::kRawStages; ++s) {
+      bar_init(sm.copied_full(s), 1);
+      bar_init(sm.copied_empty(s), 4);
+    }
+    if (BITS8) bar_init(sm.q_copied(), 1);
+    bar_init(sm.q_full(), BITS8 ? 4 : 1);
     bar_init(sm.q_empty(), 2);
     for (int t = 0; t < 2; ++t) {
       bar_init(sm.s_full(t), 1);
@@ -1138,9 +1303,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     return;
   }
-  const Guard g{sm.base + Shape<D>::kWords, p};
+  const Guard g{sm.base + S::kWords, p};
   if (warp < kSoftmaxWarps) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Warps<BITS8>::kSoftmaxRegs));
     softmax_role<BF16>(p, sm, g, first, last, tmem);
     // an end of their own: code shared with the other warps would have to do
     // with their registers
@@ -1149,9 +1314,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
     asm volatile("barrier.cta.sync 0;" ::: "memory");
     return;
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp >= kMmaWarp)
-      mma_role<BF16>(p, sm, g, first, last, tmem, warp - kMmaWarp);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Warps<BITS8>::kOtherRegs));
+    if (BITS8 && warp >= kWideningWarp) {
+      if constexpr (BITS8) widen_role<BF16>(p, sm, g, first, last);
+    } else if (warp >= kMmaWarp)
+      mma_role<BF16 && !BITS8>(p, sm, g, first, last, tmem, warp - kMmaWarp);
     else if (warp == kKeyWarp)
       load_role<false>(p, sm, g, first, last);
     else
@@ -1179,33 +1346,36 @@ int cuda_fail(const char *what, cudaError_t e) {
 }
 
 // A stride in bytes; that of an extent of 1 is never used, whatever it says.
-uint64_t step(int64_t stride, int64_t extent) { return extent == 1 ? 16 : static_cast<uint64_t>(stride) * 2; }
-bool bad_stride(int64_t stride, int64_t extent) { return extent != 1 && (stride <= 0 || stride % 8 || stride >= (int64_t(1) << 38)); }
+uint64_t step(int64_t stride, int64_t extent, int element = 2) { return extent == 1 ? 16 : static_cast<uint64_t>(stride) * element; }
+bool bad_stride(int64_t stride, int64_t extent, int grid = 8) {
+  return extent != 1 && (stride <= 0 || stride % grid || stride >= (int64_t(1) << 38));
+}
 
-template <int D, bool BF16, bool SPREAD> int launch(const Params &p, int ctas, cudaStream_t s) {
+template <int D, bool BF16, bool SPREAD, bool BITS8> int launch(const Params &p, int ctas, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};     // a bit for each device
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return cuda_fail("emmy_paged_attention: cudaGetDevice", e);
   const uint64_t bit = uint64_t(1) << (dev & 63);
   if (dev > 63 || !(ready.load() & bit)) {
-    if (cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<D, BF16, SPREAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem))
+    if (cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<D, BF16, SPREAD, BITS8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem))
       return cuda_fail("emmy_paged_attention: shared memory", e);
     // the softmax warps wait for the registers of the split: they must exist
     cudaFuncAttributes attr;
-    if (cudaError_t e = cudaFuncGetAttributes(&attr, paged_attention_kernel<D, BF16, SPREAD>))
+    if (cudaError_t e = cudaFuncGetAttributes(&attr, paged_attention_kernel<D, BF16, SPREAD, BITS8>))
       return cuda_fail("emmy_paged_attention: attributes", e);
-    if (attr.numRegs != kLaunchRegs) return fail("emmy_paged_attention: built with %ld registers, not %ld", attr.numRegs, kLaunchRegs);
+    if (attr.numRegs != Warps<BITS8>::kLaunchRegs)
+      return fail("emmy_paged_attention: built with %ld registers, not %ld", attr.numRegs, Warps<BITS8>::kLaunchRegs);
     if (dev <= 63) ready.fetch_or(bit);
   }
-  paged_attention_kernel<D, BF16, SPREAD><<<ctas, kThreads, kSmem, s>>>(p);
+  paged_attention_kernel<D, BF16, SPREAD, BITS8><<<ctas, Warps<BITS8>::kThreads, kSmem, s>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : cuda_fail("emmy_paged_attention: launch", e);
 }
 
-}  // namespace
-
-extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, void *stream) {
+// bits8: the caches hold 8-bit floats, with `exponents`
+int run(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, bool bits8, uint64_t exponents, void *stream) {
   if (!plan || !a) return fail("emmy_paged_attention: bad argument");
+  if (bits8 && !plan->narrow) return fail("emmy_paged_attention: a plan with wide units");
   if (a->dtype != 6 && a->dtype != 9) return fail("emmy_paged_attention: dtype %ld (f16 or bf16)", a->dtype);
   if (!(a->scale > 0.f) || !std::isfinite(a->scale * kLog2e)) return fail("emmy_paged_attention: scale must be positive and finite");
   if (plan->tokens == 0) return 0;
@@ -1223,8 +1393,8 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
   const int group = plan->q_heads / plan->kv_heads, d = plan->head_dim;
   const int64_t extent[3] = {a->pages, ps, plan->kv_heads};
   for (int i = 0; i < 3 && reads; ++i)
-    if (bad_stride(a->k_cache_stride[i], extent[i]) || bad_stride(a->v_cache_stride[i], extent[i]))
-      return fail("emmy_paged_attention: cache stride %ld not a positive multiple of 8 elements", i);
+    if (bad_stride(a->k_cache_stride[i], extent[i], bits8 ? 16 : 8) || bad_stride(a->v_cache_stride[i], extent[i], bits8 ? 16 : 8))
+      return fail("emmy_paged_attention: cache stride %ld not a positive multiple of %ld elements", i, bits8 ? 16 : 8);
   const int64_t rows[2] = {plan->tokens, plan->q_heads};
   for (int i = 0; i < 2; ++i)
     if (bad_stride(a->q_stride[i], rows[i]) || bad_stride(a->out_stride[i], rows[i]))
@@ -1243,11 +1413,13 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
   if (plan->spread)
     if (int e = emmy_tensormap_encode(&p.q32, a->dtype, 4, a->q, q_dims, q_steps, q32_box, 3)) return e;
   const uint64_t dims[4] = {uint64_t(d), uint64_t(ps), uint64_t(plan->kv_heads), uint64_t(a->pages)};
-  const uint32_t kv_box[4] = {64, box, 1, 1};
+  const uint32_t kv_box[4] = {bits8 ? uint32_t(d) : 64, box, 1, 1};
+  const int element = bits8 ? 1 : 2;
   for (int i = 0; i < 2 && reads; ++i) {
     const int64_t *st = i ? a->v_cache_stride : a->k_cache_stride;
-    const uint64_t steps[3] = {step(st[1], ps), step(st[2], plan->kv_heads), step(st[0], a->pages)};
-    if (int e = emmy_tensormap_encode(i ? &p.v : &p.k, a->dtype, 4, i ? a->v_cache : a->k_cache, dims, steps, kv_box, 3)) return e;
+    const uint64_t steps[3] = {step(st[1], ps, element), step(st[2], plan->kv_heads, element), step(st[0], a->pages, element)};
+    // (8-bit tiles, type 0 and without a swizzle, are read and written on by threads)
+    if (int e = emmy_tensormap_encode(i ? &p.v : &p.k, bits8 ? 0 : a->dtype, 4, i ? a->v_cache : a->k_cache, dims, steps, kv_box, bits8 ? 0 : 3)) return e;
   }
   int *words = reinterpret_cast<int *>(a->plan_words);
   p.status = reinterpret_cast<unsigned *>(words);
@@ -1276,13 +1448,29 @@ extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_
   const float mantissa = std::frexp(p.scale_log2, &exponent);      // 1/2 to 1
   p.scale_power = std::ldexp(1.f, std::min(127, mantissa * mantissa < 0.5f ? exponent - 1 : exponent));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  p.exponents = reinterpret_cast<const int *>(exponents);
+  p.kv_heads = plan->kv_heads;
   const int n = plan->at.ctas;
-  if (plan->spread) {
-    if (d == 128) return a->dtype == 9 ? launch<128, true, true>(p, n, s) : launch<128, false, true>(p, n, s);
-    return a->dtype == 9 ? launch<64, true, true>(p, n, s) : launch<64, false, true>(p, n, s);
+  if (bits8) {
+    if (d == 128) return a->dtype == 9 ? launch<128, true, true, true>(p, n, s) : launch<128, false, true, true>(p, n, s);
+    return a->dtype == 9 ? launch<64, true, true, true>(p, n, s) : launch<64, false, true, true>(p, n, s);
   }
-  if (d == 128) return a->dtype == 9 ? launch<128, true, false>(p, n, s) : launch<128, false, false>(p, n, s);
-  return a->dtype == 9 ? launch<64, true, false>(p, n, s) : launch<64, false, false>(p, n, s);
+  if (plan->spread) {
+    if (d == 128) return a->dtype == 9 ? launch<128, true, true, false>(p, n, s) : launch<128, false, true, false>(p, n, s);
+    return a->dtype == 9 ? launch<64, true, true, false>(p, n, s) : launch<64, false, true, false>(p, n, s);
+  }
+  if (d == 128) return a->dtype == 9 ? launch<128, true, false, false>(p, n, s) : launch<128, false, false, false>(p, n, s);
+  return a->dtype == 9 ? launch<64, true, false, false>(p, n, s) : launch<64, false, false, false>(p, n, s);
+}
+
+}  // namespace
+
+extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, void *stream) {
+  return run(plan, a, false, 0, stream);
+}
+
+int emmy_internal_paged_attention8(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, uint64_t exponents, void *stream) {
+  return run(plan, a, true, exponents, stream);
 }
 
 extern "C" EMMY_API int emmy_paged_plan_status(emmy_paged_plan_t plan, uint64_t plan_words, void *stream) {

@@ -41,7 +41,7 @@ int fail(const char *fmt, long a = 0, long b = 0) {
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 void make(const emmy_paged_plan_args &a, const uint8_t *left_out, emmy_paged_plan_s &plan) {
-  const int group = a.q_heads / a.kv_heads, per_tile = kTile / group;
+  const int group = a.q_heads / a.kv_heads, per_tile = kTile / group, per_unit = plan.narrow ? per_tile : 2 * per_tile;
   const Cost cost = a.head_dim == 64 ? kCost64 : kCost128;
   std::vector<Unit> wide, narrow;     // one unit an item, to be cut below
   int64_t first = 0;
@@ -52,16 +52,16 @@ void make(const emmy_paged_plan_args &a, const uint8_t *left_out, emmy_paged_pla
       continue;
     }
     plan.max_kv = std::max(plan.max_kv, len);
-    const int blocks = static_cast<int>(div_up(n, 2 * per_tile));
+    const int blocks = static_cast<int>(div_up(n, per_unit));
     for (int h = 0; h < a.kv_heads; ++h)
       for (int b = blocks - 1; b >= 0; --b) {
         Unit u;
         memset(&u, 0, sizeof u);
-        const int t0 = b * 2 * per_tile;
+        const int t0 = b * per_unit;
         u.seq = s;
         u.kvh = h;
         u.tok0 = static_cast<int32_t>(first + t0);
-        u.ntok = std::min(2 * per_tile, n - t0);
+        u.ntok = std::min(per_unit, n - t0);
         u.pos0 = len - n + t0;
         u.kv_len = len;
         u.hi = a.causal ? std::min(len, u.pos0 + u.ntok) : len;
@@ -235,7 +235,7 @@ void make(const emmy_paged_plan_args &a, const uint8_t *left_out, emmy_paged_pla
 
 }  // namespace
 
-int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_out, emmy_paged_plan_t *out) {
+int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_out, bool narrow, emmy_paged_plan_t *out) {
   if (!a || !out || a->sequences < 0 || (a->sequences && (!a->q_lens || !a->kv_lens)))
     return fail("emmy_paged_plan_make: bad argument");
   *out = nullptr;
@@ -266,6 +266,7 @@ int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_
     plan->head_dim = a->head_dim;
     plan->causal = a->causal != 0;
     plan->window = args.window;
+    plan->narrow = narrow;
     try {
       make(args, left_out, *plan);
     } catch (...) {
@@ -286,7 +287,7 @@ int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_
 }
 
 extern "C" EMMY_API int emmy_paged_plan_make(const emmy_paged_plan_args *a, emmy_paged_plan_t *out) {
-  return emmy_internal_paged_plan(a, nullptr, out);
+  return emmy_internal_paged_plan(a, nullptr, false, out);
 }
 
 extern "C" EMMY_API int emmy_paged_plan_data(emmy_paged_plan_t plan, const int32_t **words, size_t *n_words,

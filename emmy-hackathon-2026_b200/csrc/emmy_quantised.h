@@ -8,8 +8,13 @@
 namespace emmy_quantised {
 
 constexpr int slice_keys(int head_dim) { return 2048 / head_dim; }      // that a warp takes at once: 2 KiB of 8-bit keys
-constexpr int kFewRows = 128;       // query rows of a sequence and key head up to which they are few
-constexpr int kBlock = 128;         // tokens of a page of the workspace, which the others' keys are read back to
+// Query rows of a sequence and key head up to which they are few, and up to which the
+// tensor-core kernel widens its keys itself (128 rows at a time) instead of reading them
+// back.  32 sequences of up to 8,191 keys, 8 heads of 128: 256 rows 284 us against 332;
+// 24 of up to 4,095, 32 heads of 64: 128 rows 199 us against 268, 160 rows 334 against 268.
+constexpr int kFewRows = 16;
+constexpr int middle_rows(int head_dim) { return head_dim == 128 ? 256 : 128; }
+constexpr int kBlock = 128;         // tokens of a page of the workspace, which keys are read back to
 
 // Warps of a CTA whose pieces have up to `tiles` tiles of 8 query rows: as many as the
 // registers of their sums allow twice an SM (128, 168 or 255 a thread).
@@ -46,11 +51,11 @@ static_assert(sizeof(Job) == 16, "jobs are read as 16-byte records");
 // The plan's words on the device, by their offsets: CTAs, warps of one, offset of the
 // pieces, the status; from 4 on where the pieces of each CTA begin that its warps share
 // and then those of each warp (ctas x (warps + 1) + 1); pieces, rows to join, the words
-// of the plan of the others (emmy_paged.h), their page table [sequences][width] in the
-// workspace, and the jobs that fill it.  The kernel writes the status only.
+// of the plans of the sequences with more rows, middle and many (emmy_paged.h), the page
+// table [sequences][width] of the latter in the workspace, and the jobs that fill it.  The kernel writes the status only.
 struct Layout {
   static constexpr int status = 3;
-  int ctas = 0, pieces = 0, joined = 0, others = 0, table = 0, jobs = 0;
+  int ctas = 0, pieces = 0, joined = 0, middle = 0, many = 0, table = 0, jobs = 0;
 };
 
 }  // namespace emmy_quantised
@@ -58,14 +63,38 @@ struct Layout {
 struct emmy_quantised_plan_s {
   std::vector<int32_t> words;
   emmy_quantised::Layout at;
-  emmy_paged_plan_s *others = nullptr;       // of the sequences with many rows; null: none
+  emmy_paged_plan_s *middle = nullptr, *many = nullptr;       // of the sequences with more rows; null: none
   int64_t tokens = 0, part_rows = 0, workspace_pages = 0;
   int32_t sequences = 0, q_heads = 0, kv_heads = 0, head_dim = 0, causal = 0, window = 0, max_kv = 0;
   int32_t tiles = 1;                         // tiles of 8 rows that a piece may have: 1, 2 or 4
   int32_t table_width = 0, n_jobs = 0, n_joined = 0;
   bool reads = false;                        // some row sees a key
-  ~emmy_quantised_plan_s() { delete others; }
+  ~emmy_quantised_plan_s() {
+    delete middle;
+    delete many;
+  }
 };
 
-// emmy_paged_plan.cpp: a plan without the sequences that left_out marks, whose rows it leaves alone
-int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_out, emmy_paged_plan_t *out);
+namespace emmy_quantised {
+
+// The scratch by its offsets, multiples of 128 bytes: partial rows of head_dim floats
+// with (base, sum, c) of each; those of the other plans; 16-bit keys and values read back.
+struct Scratch { size_t middle, many, workspace, end; };
+inline Scratch scratch_of(const emmy_quantised_plan_s &plan) {
+  auto whole = [](size_t bytes) { return (bytes + 127) / 128 * 128; };
+  auto others = [&](const emmy_paged_plan_s *p) { return p ? whole(size_t(p->part_rows) * (plan.head_dim + 2) * sizeof(float)) : 0; };
+  Scratch at;
+  at.middle = whole(size_t(plan.part_rows) * (plan.head_dim + 4) * sizeof(float));
+  at.many = at.middle + others(plan.middle);
+  at.workspace = at.many + others(plan.many);
+  at.end = at.workspace + size_t(plan.workspace_pages) * kBlock * plan.kv_heads * plan.head_dim * 2 * 2;
+  return at;
+}
+
+}  // namespace emmy_quantised
+
+// emmy_paged_plan.cpp: a plan without the sequences that left_out marks, whose rows it
+// leaves alone; `narrow`: without wide units
+int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_out, bool narrow, emmy_paged_plan_t *out);
+// emmy_paged_attention.cu: over a cache of 8-bit floats
+int emmy_internal_paged_attention8(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, uint64_t exponents, void *stream);

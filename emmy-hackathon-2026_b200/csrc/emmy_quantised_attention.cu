@@ -834,12 +834,14 @@ extern "C" EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, con
   if (!(a->scale > 0.f) || !std::isfinite(a->scale * kLog2e)) return fail("emmy_quantised_attention: scale must be positive and finite");
   if (plan->tokens == 0) return 0;
   const bool reads = plan->reads;
-  if (a->page_size < 8 || a->page_size % 8) return fail("emmy_quantised_attention: page_size %ld (a multiple of 8)", a->page_size);
+  const int ps = a->page_size;
+  if (ps < 8 || (ps < kBlock ? (ps & (ps - 1)) != 0 : ps % kBlock != 0))
+    return fail("emmy_quantised_attention: page_size %ld (8, 16, 32, 64 or a multiple of 128)", ps);
   if (a->pages < (reads ? 1 : 0)) return fail("emmy_quantised_attention: a cache of %ld pages", a->pages);
   if (a->table_width < 0 || int64_t(a->table_width) * a->page_size < plan->max_kv)
     return fail("emmy_quantised_attention: a table of %ld pages a sequence does not hold %ld tokens", a->table_width, plan->max_kv);
-  const bool scratch = plan->part_rows || (plan->others && (plan->others->part_rows || plan->workspace_pages));
-  if (!a->q || !a->out || (reads && (!a->k_cache || !a->v_cache || !a->table)) || !a->plan_words || (scratch && !a->scratch))
+  const Scratch scratch = scratch_of(*plan);
+  if (!a->q || !a->out || (reads && (!a->k_cache || !a->v_cache || !a->table)) || !a->plan_words || (scratch.end && !a->scratch))
     return fail("emmy_quantised_attention: null address");
   if ((a->q | a->out | a->k_cache | a->v_cache | a->plan_words) % 16 || a->scratch % 128 || (a->table | a->lse | args->exponents) % 4)
     return fail("emmy_quantised_attention: address not a multiple of 16 bytes (scratch: 128)");
@@ -855,8 +857,6 @@ extern "C" EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, con
   const int d = plan->head_dim;
   int *words = reinterpret_cast<int *>(a->plan_words);
   char *scratch_at = reinterpret_cast<char *>(a->scratch);
-  auto whole = [](size_t bytes) { return (bytes + 127) / 128 * 128; };
-  const size_t row = (d + 4) * sizeof(float), others_row = (d + 2) * sizeof(float);
   // key * inverse >> shift is key / page_size for keys up to 2^30: 2^shift / page_size
   // rounded up is too large by less than 1, which key times that, under 2^shift, forgives
   int log = 0;
@@ -903,8 +903,8 @@ extern "C" EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, con
     p.bf16 = a->dtype == 9;
     p.scale_log2 = a->scale * kLog2e;
     const int n = plan->at.ctas;
-    const int e = d == 128 ? (plan->tiles == 1 ? launch<128, 1>(p, n, s) : plan->tiles == 2 ? launch<128, 2>(p, n, s) : launch<128, 4>(p, n, s))
-                           : (plan->tiles == 1 ? launch<64, 1>(p, n, s) : plan->tiles == 2 ? launch<64, 2>(p, n, s) : launch<64, 4>(p, n, s));
+    const int e = d == 128 ? (plan->tiles == 1 ? launch<128, 1>(p, n, s) : launch<128, 2>(p, n, s))
+                           : (plan->tiles == 1 ? launch<64, 1>(p, n, s) : launch<64, 2>(p, n, s));
     if (e) return e;
     if (plan->n_joined) {
       JoinParams join{};
@@ -933,18 +933,22 @@ extern "C" EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, con
         return cuda_fail("emmy_quantised_attention: launch", e);
     }
   }
-  if (!plan->others) return 0;
   emmy_paged_attention_args b = *a;
-  const size_t at_others = whole(plan->part_rows * row), at_workspace = at_others + whole(plan->others->part_rows * others_row);
+  if (plan->middle) {
+    b.plan_words = reinterpret_cast<uint64_t>(words + plan->at.middle);
+    b.scratch = a->scratch + scratch.middle;
+    if (int e = emmy_internal_paged_attention8(plan->middle, &b, args->exponents, stream)) return e;
+  }
+  if (!plan->many) return 0;
   const int64_t page = int64_t(kBlock) * plan->kv_heads * d;
   b.page_size = kBlock;
   b.pages = static_cast<int32_t>(plan->workspace_pages);
   b.table_width = plan->table_width;
   b.table = reinterpret_cast<uint64_t>(words + plan->at.table);
   b.table_stride = plan->table_width;
-  b.plan_words = reinterpret_cast<uint64_t>(words + plan->at.others);
-  b.scratch = a->scratch + at_others;
-  b.k_cache = a->scratch + at_workspace;
+  b.plan_words = reinterpret_cast<uint64_t>(words + plan->at.many);
+  b.scratch = a->scratch + scratch.many;
+  b.k_cache = a->scratch + scratch.workspace;
   b.v_cache = b.k_cache + plan->workspace_pages * page * 2;
   const int64_t strides[3] = {page, d, int64_t(kBlock) * d};
   for (int i = 0; i < 3; ++i) b.k_cache_stride[i] = b.v_cache_stride[i] = strides[i];
@@ -972,7 +976,7 @@ extern "C" EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, con
       read_back_kernel<64><<<grid, 256, 0, s>>>(p);
     if (const cudaError_t e = cudaGetLastError()) return cuda_fail("emmy_quantised_attention: launch", e);
   }
-  return emmy_paged_attention(plan->others, &b, stream);
+  return emmy_paged_attention(plan->many, &b, stream);
 }
 
 extern "C" EMMY_API int emmy_quantised_plan_status(emmy_quantised_plan_t plan, uint64_t plan_words, void *stream) {
@@ -981,5 +985,7 @@ extern "C" EMMY_API int emmy_quantised_plan_status(emmy_quantised_plan_t plan, u
   if (int e = emmy_memcpy_dtoh_async(&status, plan_words + 4 * uint64_t(plan->at.status), sizeof status, stream)) return e;
   if (int e = emmy_stream_sync(stream)) return e;
   if (status) return emmy_internal_fail(EMMY_EKERNEL, "emmy_quantised_attention: a wait ran out");
-  return plan->others ? emmy_paged_plan_status(plan->others, plan_words + 4 * uint64_t(plan->at.others), stream) : 0;
+  if (plan->middle)
+    if (int e = emmy_paged_plan_status(plan->middle, plan_words + 4 * uint64_t(plan->at.middle), stream)) return e;
+  return plan->many ? emmy_paged_plan_status(plan->many, plan_words + 4 * uint64_t(plan->at.many), stream) : 0;
 }

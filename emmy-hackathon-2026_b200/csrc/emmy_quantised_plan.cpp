@@ -4,8 +4,9 @@
 // its keys, which a kernel of its own takes as they lie: its slices of keys are
 // poured over the CTAs up to a common level, an item being cut where a CTA is full.
 // The pieces go to the CTA's warps together or to each on its own (below).
-// The others are bound by the tensor cores: their keys are read back to 16 bits once,
-// in pages of 128 tokens, and go through the 16-bit cache's attention.
+// With more rows, which the tensor-core kernel takes, the keys are widened within it
+// (middle), or read back to 16 bits once, in pages of 128 tokens, where many tiles of
+// rows use them (many).
 #include "emmy_quantised.h"
 
 #include <algorithm>
@@ -23,8 +24,9 @@ namespace {
 // What a piece costs beside its slices, in slices of a warp (1.5 us where all warps of
 // the GPU read): one that a CTA's warps share, for their waiting for one another and
 // joining, and one of a warp.  Slices that are worth a shared piece or one of a warp;
-// parts up to which an item is left to its warps, the last of which joins them.
-constexpr int kSharedCost = 3, kOwnCost = 1, kMinShared = 16, kMinOwn = 4, kMostParts = 16;
+// parts up to which an item is left to its warps (131,071 keys of one sequence: 53 us
+// shared in 37 parts, 69 in 296; 8 sequences of 8,191: 36 us shared, 33 in 48 parts).
+constexpr int kSharedCost = 5, kOwnCost = 2, kMinShared = 16, kMinOwn = 4, kMostParts = 64;
 constexpr int kCtasAnSm = 2;
 
 int fail(const char *fmt, long a = 0, long b = 0) {
@@ -35,19 +37,34 @@ int fail(const char *fmt, long a = 0, long b = 0) {
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Tiles of 8 query rows that the kernel for few rows computes, 1 or 2: more of them
+// take a slice of keys longer, fewer read some keys twice.  Measured on 32 and 24
+// sequences of up to 8,191 and 4,095 keys: 16 rows of 128 components take 1.17 of the
+// time of 8, of 64 components 1.35.
+int few_tiles(const emmy_paged_plan_args &a, const std::vector<uint8_t> &kind) {
+  int64_t one = 0, two = 0;
+  for (int s = 0; s < a.sequences; ++s) {
+    const int64_t rows = int64_t(a.q_lens[s]) * (a.q_heads / a.kv_heads);
+    if (kind[s]) continue;
+    one += a.kv_lens[s] * div_up(rows, 8) * 100;
+    two += a.kv_lens[s] * div_up(rows, 16) * (a.head_dim == 128 ? 117 : 135);
+  }
+  return one <= two ? 1 : 2;
+}
+
 void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
   const int group = a.q_heads / a.kv_heads;
-  std::vector<uint8_t> few(a.sequences);
-  bool any_others = false;
-  int most = 0;
+  // which kernels a sequence goes to
+  enum { kFew, kMiddle, kMany };
+  std::vector<uint8_t> kind(a.sequences);
+  bool any[3] = {};
   for (int s = 0; s < a.sequences; ++s) {
     const int64_t rows = int64_t(a.q_lens[s]) * group;
-    few[s] = rows <= kFewRows;
-    any_others = any_others || !few[s];
-    if (few[s]) most = std::max(most, static_cast<int>(rows));
+    kind[s] = rows <= kFewRows ? kFew : rows <= middle_rows(a.head_dim) ? kMiddle : kMany;
+    any[kind[s]] = true;
     plan.max_kv = std::max(plan.max_kv, a.kv_lens[s]);
   }
-  plan.tiles = most <= 8 ? 1 : most <= 16 ? 2 : 4;
+  plan.tiles = few_tiles(a, kind);
   const int keys = slice_keys(a.head_dim);
   const int at_once = 8 * plan.tiles;
 
@@ -63,7 +80,7 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
     // keys that new tokens from..to-1 see between them
     auto lowest = [&](int from) { return a.window ? std::max(0, pos0 + from - a.window + 1) : 0; };
     auto highest = [&](int to) { return a.causal ? std::max(0, std::min(len, pos0 + to)) : len; };
-    if (few[s]) {
+    if (kind[s] == kFew) {
       for (int r = 0; r < n * group; r += at_once) {
         Piece p;
         memset(&p, 0, sizeof p);
@@ -86,7 +103,7 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
       }
     } else if (highest(n) > lowest(0)) {
       plan.reads = true;
-      for (int b = lowest(0) / kBlock; b * kBlock < highest(n); ++b) {
+      for (int b = lowest(0) / kBlock; kind[s] == kMany && b * kBlock < highest(n); ++b) {
         // (a token that no row sees is not used, but lies in a page that is)
         jobs.push_back({s, b * kBlock, std::min(kBlock, len - b * kBlock), static_cast<int32_t>(plan.workspace_pages++)});
       }
@@ -192,12 +209,17 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
   size_t n_pieces = 0;
   for (const auto &d : dealt) n_pieces += d.size();
 
-  if (any_others) {
-    emmy_paged_plan_t others = nullptr;
-    if (emmy_internal_paged_plan(&a, few.data(), &others)) throw 2;
-    plan.others = others;
-    for (const Job &j : jobs) plan.table_width = std::max(plan.table_width, j.first / kBlock + 1);
-    plan.table_width = std::max<int32_t>(plan.table_width, static_cast<int32_t>(div_up(others->max_kv, kBlock)));
+  auto plan_of = [&](int which) {
+    std::vector<uint8_t> left_out(a.sequences);
+    for (int s = 0; s < a.sequences; ++s) left_out[s] = kind[s] != which;
+    emmy_paged_plan_t made = nullptr;
+    if (any[which] && emmy_internal_paged_plan(&a, left_out.data(), which == kMiddle, &made)) throw 2;
+    return made;
+  };
+  plan.middle = plan_of(kMiddle);
+  plan.many = plan_of(kMany);
+  if (plan.many) {
+    plan.table_width = static_cast<int32_t>(div_up(plan.many->max_kv, kBlock));
     table.assign(int64_t(a.sequences) * plan.table_width, 0);
     for (const Job &j : jobs) table[int64_t(j.seq) * plan.table_width + j.first / kBlock] = j.page;
     plan.n_jobs = static_cast<int32_t>(jobs.size());
@@ -211,14 +233,16 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
     return begin;
   };
   const int64_t at_pieces = place(16 * int64_t(n_pieces), 16), at_joined = place(8 * int64_t(joined.size()), 8),
-                at_others = place(plan.others ? int64_t(plan.others->words.size()) : 0, 16),
+                at_middle = place(plan.middle ? int64_t(plan.middle->words.size()) : 0, 16),
+                at_many = place(plan.many ? int64_t(plan.many->words.size()) : 0, 16),
                 at_table = place(int64_t(table.size()), 4), at_jobs = place(4 * int64_t(jobs.size()), 4);
   if (words > (int64_t(1) << 30)) throw 1;
   at.ctas = used;
   at.pieces = static_cast<int>(at_pieces);
   at.joined = static_cast<int>(at_joined);
   plan.n_joined = static_cast<int32_t>(joined.size());
-  at.others = static_cast<int>(at_others);
+  at.middle = static_cast<int>(at_middle);
+  at.many = static_cast<int>(at_many);
   at.table = static_cast<int>(at_table);
   at.jobs = static_cast<int>(at_jobs);
   plan.words.assign(words, 0);
@@ -234,7 +258,8 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
   plan.words[1] = warps;
   plan.words[2] = at.pieces;
   if (!joined.empty()) memcpy(&plan.words[at.joined], joined.data(), sizeof(Joined) * joined.size());
-  if (plan.others) memcpy(&plan.words[at.others], plan.others->words.data(), 4 * plan.others->words.size());
+  if (plan.middle) memcpy(&plan.words[at.middle], plan.middle->words.data(), 4 * plan.middle->words.size());
+  if (plan.many) memcpy(&plan.words[at.many], plan.many->words.data(), 4 * plan.many->words.size());
   if (!table.empty()) memcpy(&plan.words[at.table], table.data(), 4 * table.size());
   if (!jobs.empty()) memcpy(&plan.words[at.jobs], jobs.data(), sizeof(Job) * jobs.size());
 }
@@ -245,7 +270,7 @@ extern "C" EMMY_API int emmy_quantised_plan_make(const emmy_paged_plan_args *a, 
   if (!a || !out || a->sequences < 0 || (a->sequences && (!a->q_lens || !a->kv_lens)))
     return fail("emmy_quantised_plan_make: bad argument");
   *out = nullptr;
-  if (a->kv_heads < 1 || a->q_heads < 1 || a->q_heads % a->kv_heads || a->q_heads / a->kv_heads > kFewRows)
+  if (a->kv_heads < 1 || a->q_heads < 1 || a->q_heads % a->kv_heads || a->q_heads / a->kv_heads > 128)
     return fail("emmy_quantised_plan_make: %ld query heads for %ld key heads (1 to 128 times as many)", a->q_heads, a->kv_heads);
   if (a->head_dim != 64 && a->head_dim != 128) return fail("emmy_quantised_plan_make: head_dim %ld (64 or 128)", a->head_dim);
   if (a->window < 0 || (a->window && !a->causal))
@@ -286,12 +311,7 @@ extern "C" EMMY_API int emmy_quantised_plan_data(emmy_quantised_plan_t plan, con
   if (!plan || !words || !n_words || !scratch) return fail("emmy_quantised_plan_data: bad argument");
   *words = plan->words.data();
   *n_words = plan->words.size();
-  // partial rows of head_dim floats with (base, sum, c) of each; those of the others'
-  // plan; 16-bit keys and values read back: each from a multiple of 128 bytes on
-  const size_t row = (plan->head_dim + 4) * sizeof(float), others_row = (plan->head_dim + 2) * sizeof(float);
-  auto whole = [](size_t bytes) { return (bytes + 127) / 128 * 128; };
-  *scratch = whole(plan->part_rows * row) + (plan->others ? whole(plan->others->part_rows * others_row) : 0) +
-             size_t(plan->workspace_pages) * kBlock * plan->kv_heads * plan->head_dim * 2 * 2;
+  *scratch = emmy_quantised::scratch_of(*plan).end;
   return 0;
 }
 

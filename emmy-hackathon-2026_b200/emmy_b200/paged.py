@@ -433,13 +433,11 @@ def attention(plan, q, k_cache, v_cache, table, scale=None, out=None, lse=None, 
     return out, lse
 
 
-def _exponents(exponents, kv_heads, device):
-    """Their address; 0 for none."""
-    if exponents is None:
-        return 0
-    _check("exponents", exponents, 2, torch.int32, device)
-    if exponents.shape != (2, kv_heads) or not exponents.is_contiguous():
-        raise ValueError(f"exponents: contiguous [2, {kv_heads}] is wanted, not {list(exponents.shape)}")
+def _exponents(exponents, kv_heads, at):
+    """Their address."""
+    if (not isinstance(exponents, torch.Tensor) or exponents.dtype is not torch.int32 or exponents.get_device() != at
+            or exponents.shape != (2, kv_heads) or not exponents.is_contiguous()):
+        raise ValueError(f"exponents: a contiguous tensor of {torch.int32}, of [2, {kv_heads}], on the others' device is wanted")
     return exponents.data_ptr()
 
 
@@ -456,6 +454,7 @@ class Norm(_Kept):
         _need(q_weight.shape == k_weight.shape, "q_weight and k_weight have different shapes")
         _need(float(eps) >= 0, "eps: 0 or more")
         self.q_weight, self.k_weight, self.eps = q_weight, k_weight, float(eps)
+        self.q_weight_ptr, self.k_weight_ptr = q_weight.data_ptr(), k_weight.data_ptr()
         self.dtype, self.dim, self.device_index = q_weight.dtype, q_weight.shape[0], device.index
         self._keep(q_weight, k_weight)
 
@@ -470,24 +469,35 @@ def norm_rotate_append(rotation, norm, q, k, v, positions, slots, k_cache, v_cac
     they are larger.  All in 32 bits, with one rounding for what is written."""
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError("q: a CUDA tensor is wanted")
-    dtype, device = q.dtype, q.device
+    dtype = q.dtype
     if dtype not in _DTYPES:
         raise ValueError(f"q: bfloat16, float16 or float32 is wanted, not {dtype}")
-    if isinstance(positions, torch.Tensor) and positions.ndim == 1:
+    if positions.ndim == 1:
         positions = positions[None]
-    kind = E4M3 if isinstance(k_cache, torch.Tensor) and k_cache.dtype is E4M3 else dtype
-    q_stride, k_stride, v_stride, k_cache_stride, v_cache_stride, positions_stride, slots_stride = (
-        _check(name, t, ndim, of, device) for name, t, ndim, of in (
-            ("q", q, 3, dtype), ("k", k, 3, dtype), ("v", v, 3, dtype), ("k_cache", k_cache, 4, kind), ("v_cache", v_cache, 4, kind),
-            ("positions", positions, 2, torch.int32), ("slots", slots, 1, torch.int32)))
+    at, kind = q.get_device(), k_cache.dtype
+    q_stride, k_stride, v_stride = q.stride(), k.stride(), v.stride()
+    k_cache_stride, v_cache_stride, positions_stride, slots_stride = k_cache.stride(), v_cache.stride(), positions.stride(), slots.stride()
+    if (len(q_stride) != 3 or len(k_stride) != 3 or len(v_stride) != 3 or len(k_cache_stride) != 4 or len(v_cache_stride) != 4
+            or len(positions_stride) != 2 or slots_stride != (1,)
+            or not (q_stride[2] == k_stride[2] == v_stride[2] == k_cache_stride[3] == v_cache_stride[3] == positions_stride[1] == 1)
+            or not (dtype is k.dtype is v.dtype) or not (kind is dtype or kind is E4M3) or kind is not v_cache.dtype
+            or not (positions.dtype is slots.dtype is torch.int32)
+            or not (at == k.get_device() == v.get_device() == k_cache.get_device() == v_cache.get_device()
+                    == positions.get_device() == slots.get_device())):
+        if kind is not E4M3:
+            kind = dtype
+        for name, t, ndim, of in (("q", q, 3, dtype), ("k", k, 3, dtype), ("v", v, 3, dtype), ("k_cache", k_cache, 4, kind),
+                                  ("v_cache", v_cache, 4, kind), ("positions", positions, 2, torch.int32), ("slots", slots, 1, torch.int32)):
+            _check(name, t, ndim, of, q.device)
     grads = _grads_on()
     if grads and (q.requires_grad or k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad
                   or rotation.frequencies.requires_grad or (norm is not None and (norm.q_weight.requires_grad or norm.k_weight.requires_grad))):
         _no_backward()
     shape = q.shape
     tokens, q_heads, dim = shape
-    pages, page_size, kv_heads, cache_dim = k_cache.shape
-    if v_cache.shape != k_cache.shape:
+    cache_shape = k_cache.shape
+    pages, page_size, kv_heads, cache_dim = cache_shape
+    if v_cache.shape != cache_shape:
         raise ValueError("k_cache and v_cache have different shapes")
     if k.shape != (tokens, kv_heads, dim) or v.shape != k.shape or cache_dim != dim:
         raise ValueError("q, k, v and the caches do not fit together")
@@ -496,24 +506,25 @@ def norm_rotate_append(rotation, norm, q, k, v, positions, slots, k_cache, v_cac
         raise ValueError(f"positions: [{rotation.axes}, {tokens}] is wanted, not {list(positions.shape)}")
     if slots.shape[0] != tokens:
         raise ValueError(f"slots: {tokens} are wanted, not {slots.shape[0]}")
-    at = q.get_device()
     if rotation.device_index != at:
         raise ValueError("rotation: on another device")
-    weights, eps = (0, 0), 0.0
+    q_weight, k_weight, eps = 0, 0, 0.0
     if norm is not None:
         if norm.device_index != at:
             raise ValueError("norm: on another device")
         if norm.dtype is not dtype or norm.dim != dim:
             raise ValueError(f"norm: weights of {dim} components of {dtype} are wanted, not {norm.dim} of {norm.dtype}")
-        weights, eps = (norm.q_weight.data_ptr(), norm.k_weight.data_ptr()), norm.eps
-    if exponents is not None and kind is not E4M3:
-        raise ValueError("exponents: for a cache of 8-bit floats only")
-    exponents_ptr = _exponents(exponents, kv_heads, device)
+        q_weight, k_weight, eps = norm.q_weight_ptr, norm.k_weight_ptr, norm.eps
+    exponents_ptr = 0
+    if exponents is not None:
+        if kind is not E4M3:
+            raise ValueError("exponents: for a cache of 8-bit floats only")
+        exponents_ptr = _exponents(exponents, kv_heads, at)
     if q_out is None:
         q_out = _empty_like(q, memory_format=_CONTIGUOUS) if stream is None else _new(stream, q, shape, dtype)
         q_out_stride = q_heads * dim, dim
     else:
-        q_out_stride = _check("q_out", q_out, 3, dtype, device)[:2]
+        q_out_stride = _check("q_out", q_out, 3, dtype, q.device)[:2]
         if q_out.shape != shape:
             raise ValueError("q_out: another shape than q")
         if grads and q_out.requires_grad:
@@ -525,14 +536,15 @@ def norm_rotate_append(rotation, norm, q, k, v, positions, slots, k_cache, v_cac
             positions.data_ptr(), slots.data_ptr(), rotation.frequencies_ptr, rotation.pair_axis_ptr,
             q_stride[0], q_stride[1], k_stride[0], k_stride[1], v_stride[0], v_stride[1], q_out_stride[0], q_out_stride[1],
             k_cache_stride[0], k_cache_stride[1], k_cache_stride[2], v_cache_stride[0], v_cache_stride[1], v_cache_stride[2],
-            positions_stride[0], *weights, exponents_ptr, eps, kind is E4M3)
+            positions_stride[0], q_weight, k_weight, exponents_ptr, eps, kind is E4M3)
     except (struct.error, OverflowError) as e:
         raise _unfit(e) from None
     if stream is None:
         stream = _current_stream(at)
-    for kept in (rotation, norm):
-        if kept is not None and stream not in kept._streams:
-            kept._used_on(stream)
+    if stream not in rotation._streams:
+        rotation._used_on(stream)
+    if norm is not None and stream not in norm._streams:
+        norm._used_on(stream)
     _call("emmy_norm_rotate_append", at, stream, a)
     _written_to((k_cache, v_cache, q_out))
     return q_out
@@ -541,11 +553,10 @@ def norm_rotate_append(rotation, norm, q, k, v, positions, slots, k_cache, v_cac
 class QuantisedPlan(AttentionPlan):
     """An :class:`AttentionPlan` for :func:`quantised_attention`.
 
-    Sequences with at most 128 query rows a key head (new tokens times
-    ``q_heads / kv_heads``) read the 8-bit cache as it lies.  The keys and values
-    of the others, which see them with the tensor cores, are read back to 16 bits
-    once a call, into ``scratch``: 4 bytes x kv_heads x head_dim for each of
-    their cached tokens."""
+    Sequences with many new tokens, of over 256 query rows a key head (tokens
+    times ``q_heads / kv_heads``; 128 with a head_dim of 64), have their keys and values read back to 16
+    bits once a call, into ``scratch``: 4 bytes x kv_heads x head_dim for each of
+    the cached tokens that they see.  The others read the 8-bit cache as it lies."""
 
     _kind = "quantised"
 
@@ -553,41 +564,49 @@ class QuantisedPlan(AttentionPlan):
 def quantised_attention(plan, q, k_cache, v_cache, exponents, table, scale=None, out=None, lse=None, stream=None):
     """:func:`attention` over a cache of 8-bit floats, with a :class:`QuantisedPlan`.
 
-    ``k_cache`` and ``v_cache`` are float8_e4m3fn, with a page_size of 8 or a
-    multiple of it.  ``exponents``: int32 [2, kv_heads] (see the module; None: all 0).  All else is as for :func:`attention`, what it says of keys and
+    ``k_cache`` and ``v_cache`` are float8_e4m3fn; ``exponents``: int32
+    [2, kv_heads] (see the module; None: all 0).  All else is as for :func:`attention`, what it says of keys and
     values that are not finite included (an 8-bit float can be NaN)."""
     if not isinstance(plan, QuantisedPlan):
         raise ValueError("plan: a QuantisedPlan is wanted")
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError("q: a CUDA tensor is wanted")
-    dtype, device = q.dtype, q.device
+    dtype = q.dtype
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError(f"q: bfloat16 or float16 is wanted, not {dtype}")
-    q_stride, k_cache_stride, v_cache_stride, table_stride = (_check(name, t, ndim, kind, device) for name, t, ndim, kind in (
-        ("q", q, 3, dtype), ("k_cache", k_cache, 4, E4M3), ("v_cache", v_cache, 4, E4M3), ("table", table, 2, torch.int32)))
+    at = q.get_device()
+    q_stride, k_cache_stride, v_cache_stride, table_stride = q.stride(), k_cache.stride(), v_cache.stride(), table.stride()
+    if (len(q_stride) != 3 or len(k_cache_stride) != 4 or len(v_cache_stride) != 4 or len(table_stride) != 2
+            or not (q_stride[2] == k_cache_stride[3] == v_cache_stride[3] == table_stride[1] == 1)
+            or not (k_cache.dtype is v_cache.dtype is E4M3) or table.dtype is not torch.int32
+            or not (at == k_cache.get_device() == v_cache.get_device() == table.get_device())):
+        for name, t, ndim, kind in (("q", q, 3, dtype), ("k_cache", k_cache, 4, E4M3), ("v_cache", v_cache, 4, E4M3),
+                                    ("table", table, 2, torch.int32)):
+            _check(name, t, ndim, kind, q.device)
     grads = _grads_on()
     if grads and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         _no_backward()
-    at, shape = q.get_device(), plan.shape
+    shape = plan.shape
     if at != plan.device_index:
-        raise ValueError(f"q: on {device}, the plan on {plan.device}")
+        raise ValueError(f"q: on {q.device}, the plan on {plan.device}")
     if q.shape != shape:
         raise ValueError(f"q: the plan is for {list(shape)}, not {list(q.shape)}")
-    pages, page_size, kv_heads, dim = k_cache.shape
-    if v_cache.shape != k_cache.shape:
+    cache_shape = k_cache.shape
+    pages, page_size, kv_heads, dim = cache_shape
+    if v_cache.shape != cache_shape:
         raise ValueError("k_cache and v_cache have different shapes")
     if kv_heads != plan.kv_heads or dim != plan.head_dim:
         raise ValueError(f"k_cache: the plan is for {plan.kv_heads} heads of {plan.head_dim}, not {kv_heads} of {dim}")
     rows, width = table.shape
     if rows != plan.sequences:
         raise ValueError(f"table: {plan.sequences} rows are wanted, not {rows}")
-    exponents_ptr = _exponents(exponents, kv_heads, device)
+    exponents_ptr = 0 if exponents is None else _exponents(exponents, kv_heads, at)
     given = out is not None or lse is not None
     if out is None:
         out = _empty_like(q, memory_format=_CONTIGUOUS) if stream is None else _new(stream, q, shape, dtype)
         out_stride = shape[1] * dim, dim
     else:
-        out_stride = _check("out", out, 3, dtype, device)[:2]
+        out_stride = _check("out", out, 3, dtype, q.device)[:2]
         if out.shape != shape:
             raise ValueError("out: another shape than q")
         if grads and out.requires_grad:
@@ -595,7 +614,7 @@ def quantised_attention(plan, q, k_cache, v_cache, exponents, table, scale=None,
     if lse is None:
         lse = q.new_empty(shape[:2], dtype=torch.float32) if stream is None else _new(stream, q, shape[:2], torch.float32)
     else:
-        _check("lse", lse, 2, torch.float32, device)
+        _check("lse", lse, 2, torch.float32, q.device)
         if lse.shape != shape[:2] or not lse.is_contiguous():
             raise ValueError(f"lse: contiguous {list(shape[:2])} is wanted")
         if grads and lse.requires_grad:
@@ -645,25 +664,31 @@ def verify(target, proposal, drafted, uniforms, finals, first, stream=None):
     ``accepted`` int32 [sequences], ``tokens`` int32 [rows]."""
     if not isinstance(target, torch.Tensor) or not target.is_cuda:
         raise ValueError("target: a CUDA tensor is wanted")
-    dtype, device = target.dtype, target.device
+    dtype, at = target.dtype, target.get_device()
     if dtype not in _DTYPES:
         raise ValueError(f"target: float32, bfloat16 or float16 is wanted, not {dtype}")
-    for name, t, ndim, kind in (("target", target, 2, dtype), ("drafted", drafted, 1, torch.int32), ("uniforms", uniforms, 1, torch.float32),
-                                ("finals", finals, 1, torch.float32), ("first", first, 1, torch.int32)):
-        _check(name, t, ndim, kind, device)
+    target_stride, proposal_stride = target.stride(), (0, 1) if proposal is None else proposal.stride()
+    if (len(target_stride) != 2 or len(proposal_stride) != 2 or target_stride[1] != 1 or proposal_stride[1] != 1
+            or not (drafted.stride() == uniforms.stride() == finals.stride() == first.stride() == (1,))
+            or not (drafted.dtype is first.dtype is torch.int32) or not (uniforms.dtype is finals.dtype is torch.float32)
+            or not (at == drafted.get_device() == uniforms.get_device() == finals.get_device() == first.get_device())
+            or (proposal is not None and (proposal.dtype is not dtype or proposal.get_device() != at))):
+        for name, t, ndim, kind in (("target", target, 2, dtype), ("drafted", drafted, 1, torch.int32), ("uniforms", uniforms, 1, torch.float32),
+                                    ("finals", finals, 1, torch.float32), ("first", first, 1, torch.int32), ("proposal", proposal, 2, dtype)):
+            if t is not None or name != "proposal":
+                _check(name, t, ndim, kind, target.device)
     rows, vocabulary = target.shape
     sequences, drafts = finals.shape[0], drafted.shape[0]
     if first.shape[0] != sequences + 1:
         raise ValueError(f"first: {sequences + 1} entries are wanted, not {first.shape[0]}")
     if drafts != rows - sequences or uniforms.shape[0] != drafts:
         raise ValueError(f"drafted and uniforms: {rows - sequences} entries are wanted, one less a sequence than rows of target")
-    if proposal is not None:
-        _check("proposal", proposal, 2, dtype, device)
-        if proposal.shape != (drafts, vocabulary):
-            raise ValueError(f"proposal: {[drafts, vocabulary]} is wanted, not {list(proposal.shape)}")
+    if proposal is not None and proposal.shape != (drafts, vocabulary):
+        raise ValueError(f"proposal: {[drafts, vocabulary]} is wanted, not {list(proposal.shape)}")
     if _grads_on() and (target.requires_grad or uniforms.requires_grad or finals.requires_grad or (proposal is not None and proposal.requires_grad)):
         _no_backward()
     if stream is None:
+        stream = _current_stream(at)
         accepted, tokens = first.new_empty(sequences), first.new_empty(rows)
     else:
         accepted, tokens = _new(stream, first, (sequences,), torch.int32), _new(stream, first, (rows,), torch.int32)
@@ -671,9 +696,8 @@ def verify(target, proposal, drafted, uniforms, finals, first, stream=None):
         a = _VERIFY_ARGS.pack(
             _DTYPES[dtype], sequences, rows, drafts, vocabulary, 0, target.data_ptr(), 0 if proposal is None else proposal.data_ptr(),
             drafted.data_ptr(), uniforms.data_ptr(), finals.data_ptr(), first.data_ptr(), accepted.data_ptr(), tokens.data_ptr(),
-            target.stride(0), 0 if proposal is None else proposal.stride(0))
+            target_stride[0], proposal_stride[0])
     except (struct.error, OverflowError) as e:
         raise _unfit(e) from None
-    at = target.get_device()
-    _call("emmy_verify", at, _current_stream(at) if stream is None else stream, a)
+    _call("emmy_verify", at, stream, a)
     return accepted, tokens

@@ -318,7 +318,7 @@ EMMY_API int emmy_quantised_plan_data(emmy_quantised_plan_t plan, const int32_t 
 EMMY_API void emmy_quantised_plan_free(emmy_quantised_plan_t plan);
 
 typedef struct {
-  emmy_paged_attention_args a; /* dtype: of q and out; page_size: a multiple of 8    */
+  emmy_paged_attention_args a; /* dtype: of q and out                                */
   uint64_t exponents;          /* int32 [2][kv_heads]: of keys, of values; 0: all 0  */
 } emmy_quantised_attention_args;
 EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, const emmy_quantised_attention_args *a,

@@ -269,7 +269,7 @@ def check(q_lens, kv_lens, heads, kv_heads, dim, page, dtype=BF16, layout="token
 
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("layout,page", [("token", 16), ("head", 64), ("token", 8), ("head", 128), ("token", 384), ("head", 8), ("token", 24)])
+@pytest.mark.parametrize("layout,page", [("token", 16), ("head", 64), ("token", 8), ("head", 128), ("token", 384), ("head", 8), ("token", 32)])
 def test_decode_types_pages_layouts(dim, dtype, layout, page):
     check([1] * 10, [1, 15, 16, 17, 31, 32, 33, 257, 640, 1000], 16, 4, dim, page, dtype, layout)
 
@@ -280,10 +280,10 @@ def test_head_groups(heads, kv_heads, dim):
     check([1, 3, 40, 129], [300, 3, 170, 513], heads, kv_heads, dim, 32)
 
 
-@pytest.mark.parametrize("tokens", [1, 2, 3, 7, 8, 9, 16, 17, 24, 31, 32, 33, 64, 65])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129, 255, 256, 257])
 @pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
 def test_rows_around_the_tiles(tokens, dim, dtype):
-    """Query rows about 8, 32 and 128, which the ways of computing begin at."""
+    """Query rows about 8, 16, 32, 128, 256 and 512, which the ways of computing begin at."""
     check([tokens, 1], [tokens + 100, 70], 4, 2, dim, 16, dtype)
 
 
@@ -291,7 +291,7 @@ def test_rows_around_the_tiles(tokens, dim, dtype):
     ([128], [128]), ([129], [129]), ([257], [300]), ([1, 200, 1, 31, 64], [900, 200, 1, 600, 65]), ([500, 1, 333], [500, 2000, 777]),
 ])
 @pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
-@pytest.mark.parametrize("page", [16, 48])
+@pytest.mark.parametrize("page", [8, 16, 64, 256])
 def test_chunks(q_lens, kv_lens, dim, dtype, page):
     check(q_lens, kv_lens, 8, 4, dim, page, dtype)
 
@@ -524,6 +524,7 @@ def test_attention_refuses():
     refused(ValueError, "different shapes", q, k, v[:, :8], e, table)
     refused(native.EmmyError, "does not hold", q, k, v, e, table[:, :3])
     refused(native.EmmyError, "scale", q, k, v, e, table, scale=0.0)
+    refused(native.EmmyError, "page_size", q, k[:, :12], v[:, :12], e, table)
     odd = torch.zeros(2, 4, 68, dtype=q.dtype, device="cuda")[..., :64]
     refused(native.EmmyError, "stride", odd, k, v, e, table)
     refused(ValueError, "lse", q, k, v, e, table, lse=torch.empty(4, 2, device="cuda").t())

@@ -12,7 +12,7 @@ from emmy_b200 import native, paged
 pytestmark = pytest.mark.usefixtures("native_lib")
 
 FIELDS = ("seq", "kvh", "tok0", "row0", "rows", "pos0", "lo", "hi", "kv_len", "slice0", "nslices", "split", "nsplit", "part_row")
-FEW = 128
+FEW, MIDDLE = 16, 128                 # rows of 64 components
 
 
 def parts_of(plan):
@@ -55,9 +55,8 @@ def test_pieces_cover_the_work_once(q_lens, kv_lens, hq, hkv, causal, window, ct
     pieces, first, warps = parts_of(plan)
     group = hq // hkv
     few = [q * group <= FEW for q in q_lens]
-    most = max([8] + [q * group for q, f in zip(q_lens, few) if f])
-    at_once = 8 if most <= 8 else 16 if most <= 16 else 32
-    assert warps == {8: 8, 16: 6, 32: 4}[at_once] and len(first) - 1 <= 2 * ctas * (warps + 1)
+    at_once = {8: 8, 6: 16}[warps]
+    assert len(first) - 1 <= 2 * ctas * (warps + 1)
     items = {}
     for u in pieces:
         assert few[u["seq"]] and 0 < u["rows"] <= at_once and 0 <= u["kvh"] < hkv
@@ -89,11 +88,11 @@ def test_pieces_cover_the_work_once(q_lens, kv_lens, hq, hkv, causal, window, ct
             scratch |= mine
     assert len(covered) == sum(q * hq for q, f in zip(q_lens, few) if f)
     assert scratch == set(range(len(scratch))) and joined == set(rows_to_join(plan, pieces, group))
-    # the others' keys: 4 bytes a component of whole pages of 128 tokens that some row sees, and parts
+    # keys that are read back: 4 bytes a component of whole pages of 128 tokens that some row sees; and parts
     blocks = 0
     for q, kv, f in zip(q_lens, kv_lens, few):
         hi, lo = kv, max(0, kv - q - window + 1) if window else 0
-        blocks += 0 if f or hi <= 0 else -(-hi // 128) - lo // 128
+        blocks += -(-hi // 128) - lo // 128 if q * group > MIDDLE and hi > 0 else 0
     assert plan.scratch.numel() >= len(scratch) * 68 * 4 + blocks * 128 * hkv * 64 * 4
     if all(few):
         assert plan.scratch.numel() == -(-len(scratch) * 68 * 4 // 128) * 128
@@ -102,7 +101,7 @@ def test_pieces_cover_the_work_once(q_lens, kv_lens, hq, hkv, causal, window, ct
 @pytest.mark.parametrize("q_lens,kv_lens,most", [
     ([1] * 64, [random.Random(s).randint(517, 8191) for s in range(64)], 1.03),
     ([1], [131071], 1.03),
-    ([5] * 24, [random.Random(s).randint(65, 4095) for s in range(24)], 1.1),
+    ([4] * 24, [random.Random(s).randint(65, 4095) for s in range(24)], 1.2),
 ])
 def test_work_is_even(q_lens, kv_lens, most):
     plan = paged.QuantisedPlan(q_lens, kv_lens, 32, 8, 128, device="cpu", ctas=148)
@@ -189,10 +188,10 @@ def test_c_norm_rotate_append_refuses(native_lib, change, words):
     assert words in said and b"norm_rotate_append" in said, said
 
 
-@pytest.mark.parametrize("q_lens", [[2], [300]])
+@pytest.mark.parametrize("q_lens", [[2], [100], [300]])
 @pytest.mark.parametrize("change,words", [
     (dict(dtype=7), b"dtype"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=3.4e38), b"scale"),
-    (dict(page_size=0), b"page_size"), (dict(page_size=12), b"page_size"), (dict(pages=0), b"pages"), (dict(table_width=1), b"does not hold"), (dict(q=0), b"null"),
+    (dict(page_size=0), b"page_size"), (dict(page_size=24), b"page_size"), (dict(page_size=192), b"page_size"), (dict(pages=0), b"pages"), (dict(table_width=1), b"does not hold"), (dict(q=0), b"null"),
     (dict(scratch=0), b"null"), (dict(q=4104), b"16 bytes"), (dict(scratch=4112), b"16 bytes"), (dict(table=4098), b"16 bytes"),
     (dict(exponents=4098), b"16 bytes"), (dict(k_cache=4104), b"16 bytes"), (dict(q_token=100), b"stride"), (dict(k_page=-2048), b"stride"),
     (dict(v_token=136), b"stride"), (dict(v_token=0), b"stride"),
