@@ -35,18 +35,18 @@ int emmy_internal_fail(int code, const char *msg);   // emmy_runtime.cpp
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kMostCtas = 8;
-constexpr int kBatch = 8;            // elements of a thread that are loaded together
+static_assert(kMostCtas * kWarps <= 64, "two segments a lane");
+constexpr int kEach = 8;             // elements of a thread where the token lies
+constexpr int kBatch = 16;           // elements of a thread that are loaded together, of both rows
 
 __device__ __forceinline__ double wide(float x) { return double(x); }
 __device__ __forceinline__ double wide(__half x) { return double(__half2float(x)); }
 __device__ __forceinline__ double wide(__nv_bfloat16 x) { return double(__bfloat162float(x)); }
 
-struct Chosen { int token, found; };
-
 // blockIdx.x: sequence x CTAs of its cluster + CTA.
 template <typename T> __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const __grid_constant__ emmy_verify_args a) {
-  __shared__ double sums[kWarps], all[kMostCtas * kWarps], warp_sums[kWarps];
-  __shared__ int kept_shared, segment_shared, positive_shared[kWarps];
+  __shared__ double sums[kWarps], warp_sums[kWarps];
+  __shared__ int kept_shared, segment_shared, positive_shared[kWarps], token_shared[kWarps];
   __shared__ double target_shared, before_shared;
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank(), seq = blockIdx.x / ctas;
@@ -101,19 +101,29 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) verify_kern
       const int s = rank * kWarps + warp, to = segment_begin(s + 1);
       double sum = 0.0;
       int j = segment_begin(s) + lane;
-      for (; j + 32 * (kBatch - 1) < to; j += 32 * kBatch) {
-        T x[kBatch], y[kBatch];
+      if (q_row) {
+        for (; j + 32 * (kBatch / 2 - 1) < to; j += 32 * (kBatch / 2)) {
+          T x[kBatch / 2], y[kBatch / 2];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) x[k] = p_row[j + 32 * k];
-        if (q_row) {
+          for (int k = 0; k < kBatch / 2; ++k) x[k] = p_row[j + 32 * k];
 #pragma unroll
-          for (int k = 0; k < kBatch; ++k) y[k] = q_row[j + 32 * k];
+          for (int k = 0; k < kBatch / 2; ++k) y[k] = q_row[j + 32 * k];
+#pragma unroll
+          for (int k = 0; k < kBatch / 2; ++k) {
+            const double d = wide(x[k]) - wide(y[k]);
+            sum += d > 0.0 ? d : 0.0;
+          }
         }
+      } else {
+        for (; j + 32 * (kBatch - 1) < to; j += 32 * kBatch) {
+          T x[kBatch];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          double d = wide(x[k]);
-          if (q_row) d -= wide(y[k]);
-          sum += d > 0.0 && j + 32 * k != without ? d : 0.0;
+          for (int k = 0; k < kBatch; ++k) x[k] = p_row[j + 32 * k];
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            const double d = wide(x[k]);
+            sum += d > 0.0 && j + 32 * k != without ? d : 0.0;
+          }
         }
       }
       for (; j < to; j += 32) sum += mass(j);
@@ -121,80 +131,100 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 4) verify_kern
       if (lane == 0) sums[warp] = sum;
     }
     cluster.sync();
-    if (tid < segments) all[tid] = cluster.map_shared_rank(sums, tid / kWarps)[tid % kWarps];
-    __syncthreads();
-    if (tid == 0) {
-      double total = 0.0;
-      for (int s = 0; s < segments; ++s) total += all[s];
-      const double goal = double(reinterpret_cast<const float *>(a.finals)[seq]) * total;
-      // the first segment whose end is past the goal; else the last that has anything
-      double sum = 0.0, before = 0.0;
-      int at = -1;
-      for (int s = 0; s < segments; ++s) {
-        if (all[s] > 0.0) at = s, before = sum;
-        sum += all[s];
-        if (sum > goal) break;
+    if (warp == 0) {
+      // a lane has two segments next to one another
+      double mine[2], upto;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int s = 2 * lane + k;
+        mine[k] = s < segments ? cluster.map_shared_rank(sums, s / kWarps)[s % kWarps] : 0.0;
       }
-      segment_shared = total > 0.0 ? at : -1;
-      target_shared = goal;
-      before_shared = before;
+      upto = mine[0] + mine[1];
+      for (int k = 1; k < 32; k *= 2) {
+        const double x = __shfl_up_sync(~0u, upto, k);
+        if (lane >= k) upto += x;
+      }
+      const double total = __shfl_sync(~0u, upto, 31), goal = double(reinterpret_cast<const float *>(a.finals)[seq]) * total;
+      double before = __shfl_up_sync(~0u, upto, 1);
+      if (lane == 0) before = 0.0;
+      // the first segment whose end is past the goal; else the last that has anything
+      const bool first_past = mine[0] > 0.0 && before + mine[0] > goal, past = first_past || (mine[1] > 0.0 && upto > goal);
+      const unsigned all_past = __ballot_sync(~0u, past), any = __ballot_sync(~0u, mine[0] > 0.0 || mine[1] > 0.0);
+      const int owner = all_past ? __ffs(all_past) - 1 : 31 - __clz(any);      // (-1: none)
+      if (lane == max(owner, 0)) {
+        const bool second = all_past ? !first_past : mine[1] > 0.0;
+        segment_shared = total > 0.0 && owner >= 0 ? 2 * lane + second : -1;
+        target_shared = goal;
+        before_shared = second ? before + mine[0] : before;
+      }
     }
     __syncthreads();
+    cluster.barrier_arrive();          // the sums have been read
     const int at = segment_shared;
     if (at < 0 && pass == 0 && (q_row || without >= 0)) {      // nothing is left of p: p itself
       q_row = nullptr;
       without = -1;
-      cluster.sync();                  // the sums have been read
+      cluster.barrier_wait();
       continue;
     }
     if (at < 0) {
       if (rank == 0 && tid == 0) tokens[kept] = -1;
     } else if (at / kWarps == rank) {
-      // a thread's elements of the segment, then the threads' sums in their order
-      const int from = segment_begin(at), to = segment_begin(at + 1), each = (to - from + kThreads - 1) / kThreads;
-      const int mine = min(to, from + tid * each), stop = min(to, mine + each);
-      double sum = 0.0;
-      int positive = -1;
-      for (int j = mine; j < stop; ++j) {
-        const double d = mass(j);
-        sum += d;
-        if (d > 0.0) positive = j;
-      }
-      double upto = sum;
-      for (int k = 1; k < 32; k *= 2) {
-        const double x = __shfl_up_sync(~0u, upto, k);
-        if (lane >= k) upto += x;
-      }
-      if (lane == 31) warp_sums[warp] = upto;
-      const int last = __reduce_max_sync(~0u, positive);
-      if (lane == 0) positive_shared[warp] = last;
-      if (tid == 0) kept_shared = INT_MAX;
-      __syncthreads();
-      double before = before_shared;
-      for (int w = 0; w < warp; ++w) before += warp_sums[w];
-      before += upto - sum;
+      // the segment once more, some elements next to one another a thread at a time, and
+      // the threads' sums in their order
+      const int to = segment_begin(at + 1);
       const double goal = target_shared;
-      // the first element past the goal, of the first thread that has one
-      for (int j = mine; j < stop; ++j) {
-        before += mass(j);
-        if (before > goal && mass(j) > 0.0) {
-          atomicMin(&kept_shared, j);
+      double before = before_shared;
+      int last = -1;
+      for (int from = segment_begin(at);; from += kThreads * kEach) {
+        double d[kEach], sum = 0.0;
+        int positive = -1, token = INT_MAX;
+        const int mine = from + tid * kEach;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) d[k] = mine + k < to ? mass(mine + k) : 0.0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+          sum += d[k];
+          if (d[k] > 0.0) positive = mine + k;
+        }
+        double upto = sum;
+        for (int k = 1; k < 32; k *= 2) {
+          const double x = __shfl_up_sync(~0u, upto, k);
+          if (lane >= k) upto += x;
+        }
+        if (lane == 31) warp_sums[warp] = upto;
+        positive = __reduce_max_sync(~0u, positive);
+        if (lane == 0) positive_shared[warp] = positive;
+        __syncthreads();
+        double reached = before + (upto - sum);
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) reached += warp_sums[w];
+          before += warp_sums[w];
+          last = max(last, positive_shared[w]);
+        }
+        // the first element past the goal
+#pragma unroll
+        for (int k = kEach - 1; k >= 0; --k) {
+          double s = reached;
+#pragma unroll
+          for (int e = 0; e <= k; ++e) s += d[e];
+          if (d[k] > 0.0 && s > goal) token = mine + k;
+        }
+        token = __reduce_min_sync(~0u, token);
+        if (lane == 0) token_shared[warp] = token;
+        __syncthreads();
+        for (int w = 0; w < kWarps; ++w) token = min(token, token_shared[w]);
+        const bool end = from >= to - kThreads * kEach;
+        if (token != INT_MAX || end) {
+          // (none: the goal is the end, or within a rounding of it)
+          if (tid == 0) tokens[kept] = token != INT_MAX ? token : last;
           break;
         }
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int token = kept_shared;
-        if (token == INT_MAX) {        // (the goal is the end, or within a rounding of it)
-          token = -1;
-          for (int w = 0; w < kWarps; ++w) token = max(token, positive_shared[w]);
-        }
-        tokens[kept] = token;
       }
     }
     break;
   }
-  cluster.sync();                      // a CTA's shared memory lasts while others read it
+  cluster.barrier_wait();              // a CTA's shared memory lasts while others read it
 }
 
 int fail(const char *fmt, long a = 0, long b = 0) {
