@@ -27,16 +27,21 @@
 // is in 32 bits; the one rounding is to the cache's or q_out's type.
 //
 // With norms (queries and keys of each head times the reciprocal of their root mean
-// square and a weight) and a cache of 8-bit floats it is the same walk: the squares'
-// sums of a head's threads meet in shared memory at the barrier that the angles have
-// anyway, the weights of a thread's two vectors stay in registers, and keys and values
-// are multiplied by a power of two -- exactly -- and rounded once.
+// square and a weight) or a cache of 8-bit floats (times a power of two -- exactly -- and
+// rounded once), each element takes twice the instructions, and that walk waited at its
+// barrier of each token: 8,191 tokens of 32 + 8 heads of 128 in 57 us, whatever the
+// tokens ahead.  A head of 2, 4, .. 32 threads goes through append_kernel instead, a
+// warp a token: its angles and weights stay in registers for all heads, the squares'
+// sums meet by shuffles, arithmetic is on pairs of floats (fma.rn.f32x2), the norm's
+// factor and the cache's power of two are one at the end, and nothing waits for another
+// warp.  Other heads take the walk above, with the squares in shared memory.
 #include "../../include/emmy_b200.h"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
 #include <cstdio>
@@ -55,6 +60,8 @@ struct Params {
   int lanes;                       // threads of a row: a head's vectors by two
   uint64_t q_weight, k_weight, exponents;
   float eps;
+  uint32_t page_inverse;           // slot / page_size = slot * page_inverse >> page_shift
+  int page_shift;
 };
 
 struct E4M3 { uint8_t bits; };     // an 8-bit float: 4 exponent bits, largest 448
@@ -129,6 +136,49 @@ template <int N> __device__ __forceinline__ void round_to(const float *f, Vec<E4
     else
       *reinterpret_cast<uint32_t *>(&v) = words[0];
   }
+}
+
+// ---- pairs of floats
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+template <typename T, int N> __device__ __forceinline__ void widen2(const Vec<T, N> &v, uint64_t *f) {
+  float x[N];
+  widen(v, x);
+#pragma unroll
+  for (int e = 0; e < N; e += 2) f[e / 2] = pair_of(x[e], x[e + 1]);
+}
+template <typename T, int N> __device__ __forceinline__ void round2(const uint64_t *f, float by, Vec<T, N> &v) {
+  float x[N];
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    const float2 t = unpair(mul2(f[e / 2], pair_of(by, by)));
+    x[e] = t.x, x[e + 1] = t.y;
+  }
+  round_to(x, v);
+}
+
+// cosine and sine of position * frequency, the angle formed in 64 bits as half turns
+__device__ __forceinline__ void angle_of(int position, float frequency, float &c, float &s) {
+  const double turned = double(position) * double(frequency) * 0.31830988618379067154;
+  sincospif(float(turned - 2.0 * rint(0.5 * turned)), &s, &c);
 }
 
 template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const void *from) {
@@ -411,6 +461,165 @@ __global__ void __launch_bounds__(kThreads, NORM ? kNormBlocks : kBlocks) rotate
   }
 }
 
+constexpr int kWarps = 4, kGroups = 4;      // of a block of append_kernel; groups of heads on their way or being turned
+
+// A warp has a token (of 4 a block) and every gridDim.y-th group of heads, `lanes` threads
+// a head: a power of two up to 32.  Thread's vectors and pairs as above.
+// LANES: `lanes` where it is known, else 0.
+template <typename T, typename C, int N, bool WITHIN, bool NORM, int LANES>
+__global__ void __launch_bounds__(32 * kWarps, 5) append_kernel(const __grid_constant__ Params p) {
+  using V = Vec<T, N>;
+  constexpr bool SMALL = !std::is_same<T, C>::value;
+  extern __shared__ __align__(16) float angles[];           // vectors [kWarps][kGroups][2][32], angles [kWarps][2][half]
+  const emmy_rotate_append_args &a = p.a;
+  const int half = a.rotary_dim / 2, heads = a.q_heads + 2 * a.kv_heads, lanes = LANES ? LANES : p.lanes;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, token = blockIdx.x * kWarps + warp;
+  if (token >= a.tokens) return;
+  const int at_once = 32 / lanes, mine = lane & (lanes - 1), step = at_once * gridDim.y;
+  int head = blockIdx.y * at_once + lane / lanes;
+  // its two vectors, `apart` elements from one another, and their first pairs
+  bool turn_one, turn_two;
+  int one, apart, first_pair, second_pair;
+  if (WITHIN) {
+    one = mine * N;
+    apart = lanes * N;
+    turn_one = one < a.rotary_dim;
+    turn_two = one + apart < a.rotary_dim;
+    first_pair = one / 2, second_pair = (one + apart) / 2;
+  } else {
+    turn_one = turn_two = mine * N < half;
+    one = turn_one ? mine * N : half + mine * N;
+    apart = turn_one ? half : lanes * N - half;
+    first_pair = second_pair = mine * N;
+  }
+  // a head's vectors go to shared memory, each to its thread's own place, some groups ahead
+  V *const ring = reinterpret_cast<V *>(angles) + warp * kGroups * 2 * 32 + lane;
+  auto fetch = [&](int h, int stage) {
+    if (h < heads) {
+      const T *at;
+      if (h < a.q_heads)
+        at = reinterpret_cast<const T *>(a.q) + token * a.q_stride[0] + h * a.q_stride[1];
+      else if (h < a.q_heads + a.kv_heads)
+        at = reinterpret_cast<const T *>(a.k) + token * a.k_stride[0] + (h - a.q_heads) * a.k_stride[1];
+      else
+        at = reinterpret_cast<const T *>(a.v) + token * a.v_stride[0] + (h - a.q_heads - a.kv_heads) * a.v_stride[1];
+      copy_async<16>(ring + stage * 64, at + one);
+      copy_async<16>(ring + stage * 64 + 32, at + one + apart);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int k = 0; k + 1 < kGroups; ++k) fetch(head + k * step, k);
+  int stage = 0;
+  int64_t k_at = -1, v_at = -1;                 // where the token's keys and values go; -1: nowhere
+  if (a.kv_heads) {
+    const int slot = __ldg(reinterpret_cast<const int *>(a.slots) + token);
+    if (slot >= 0 && slot < int64_t(a.pages) * a.page_size) {
+      const int page = static_cast<int>(uint64_t(slot) * p.page_inverse >> p.page_shift), within = slot - page * a.page_size;
+      k_at = page * a.k_cache_stride[0] + within * a.k_cache_stride[1];
+      v_at = page * a.v_cache_stride[0] + within * a.v_cache_stride[1];
+    }
+  }
+  // this token's angles, and of them those of this thread's pairs: c[0..N) and s[0..N);
+  // WITHIN: the first half of the first vector, the others of the second
+  float *const angle = angles + kWarps * kGroups * 64 * (sizeof(V) / 4) + warp * 2 * half;
+  for (int i = lane; i < half; i += 32) {
+    const int axis = a.pair_axis ? min(max(__ldg(reinterpret_cast<const int *>(a.pair_axis) + i), 0), a.axes - 1) : 0;
+    angle_of(__ldg(reinterpret_cast<const int *>(a.positions) + axis * a.positions_stride + token),
+             __ldg(reinterpret_cast<const float *>(a.frequencies) + i), angle[i], angle[half + i]);
+  }
+  __syncwarp();
+  float c[N], s[N], minus[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const int i = !WITHIN ? first_pair + e : e < N / 2 ? first_pair + e : second_pair + e - N / 2;
+    const bool used = !WITHIN || e < N / 2 ? turn_one : turn_two;
+    c[e] = used ? angle[i] : 1.f;
+    s[e] = used ? angle[half + i] : 0.f;
+    minus[e] = -s[e];
+  }
+  uint64_t weight[NORM ? N : 1];                // of both vectors, of queries or keys
+  int weights_of = -1;
+  const float reciprocal = 1.f / float(a.head_dim);
+#pragma unroll 1
+  for (int n = 0; blockIdx.y * at_once + n * step < heads; ++n, head += step) {
+    const bool query = head < a.q_heads, turns = head < a.q_heads + a.kv_heads;
+    uint64_t f[N / 2], g[N / 2];
+    fetch(head + (kGroups - 1) * step, (stage + kGroups - 1) % kGroups);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kGroups - 1) : "memory");
+    const V left = ring[stage * 64], right = ring[stage * 64 + 32];
+    stage = (stage + 1) % kGroups;
+    widen2(left, f);
+    widen2(right, g);
+    float by = 1.f;
+    if constexpr (NORM) {
+      uint64_t x = mul2(f[0], f[0]), y = mul2(g[0], g[0]);
+#pragma unroll
+      for (int e = 1; e < N / 2; ++e) x = fma2(f[e], f[e], x), y = fma2(g[e], g[e], y);
+      const float2 sx = unpair(x), sy = unpair(y);
+      float sum = (sx.x + sx.y) + (sy.x + sy.y);
+#pragma unroll
+      for (int k = 1; k < (LANES ? LANES : 32); k *= 2)
+        if (LANES || k < lanes) sum += __shfl_xor_sync(~0u, sum, k);
+      const int kind = turns ? !query : weights_of;
+      if (kind != weights_of) {
+        const T *w = reinterpret_cast<const T *>(kind ? p.k_weight : p.q_weight) + one;
+        widen2(*reinterpret_cast<const V *>(w), weight);
+        widen2(*reinterpret_cast<const V *>(w + apart), weight + N / 2);
+        weights_of = kind;
+      }
+      if (turns) {
+        by = rsqrtf(fmaf(sum, reciprocal, p.eps));
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) f[e] = mul2(f[e], weight[e]), g[e] = mul2(g[e], weight[N / 2 + e]);
+      }
+    }
+    if (turns && turn_one) {
+      if (WITHIN) {
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) {
+          const float2 x = unpair(f[e]), y = unpair(g[e]);
+          f[e] = fma2(f[e], pair_of(c[e], c[e]), mul2(pair_of(x.y, x.x), pair_of(minus[e], s[e])));
+          g[e] = fma2(g[e], pair_of(c[N / 2 + e], c[N / 2 + e]), mul2(pair_of(y.y, y.x), pair_of(minus[N / 2 + e], s[N / 2 + e])));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+          const uint64_t cosine = pair_of(c[e], c[e + 1]), x = f[e / 2], y = g[e / 2];
+          f[e / 2] = fma2(x, cosine, mul2(y, pair_of(minus[e], minus[e + 1])));
+          g[e / 2] = fma2(y, cosine, mul2(x, pair_of(s[e], s[e + 1])));
+        }
+      }
+    }
+    if (head >= heads) continue;
+    if (query) {
+      T *to = reinterpret_cast<T *>(a.q_out) + token * a.q_out_stride[0] + head * a.q_out_stride[1] + one;
+      V r;
+      round2(f, by, r);
+      *reinterpret_cast<V *>(to) = r;
+      round2(g, by, r);
+      *reinterpret_cast<V *>(to + apart) = r;
+    } else if (k_at >= 0) {
+      const int kv_head = head - a.q_heads - (turns ? 0 : a.kv_heads);
+      C *to = (turns ? reinterpret_cast<C *>(a.k_cache) + k_at + kv_head * a.k_cache_stride[2] : reinterpret_cast<C *>(a.v_cache) + v_at + kv_head * a.v_cache_stride[2]) + one;
+      Vec<C, N> r, t;
+      if constexpr (SMALL) {
+        const int e = p.exponents ? __ldg(reinterpret_cast<const int *>(p.exponents) + kv_head + (turns ? 0 : a.kv_heads)) : 0;
+        const float scale = by * __uint_as_float(uint32_t(127 - min(max(e, EMMY_MIN_EXPONENT), EMMY_MAX_EXPONENT)) << 23);
+        round2(f, scale, r);
+        round2(g, scale, t);
+      } else if (turns) {
+        round2(f, by, r);
+        round2(g, by, t);
+      } else {
+        r = left, t = right;
+      }
+      *reinterpret_cast<Vec<C, N> *>(to) = r;
+      *reinterpret_cast<Vec<C, N> *>(to + apart) = t;
+    }
+  }
+}
+
 int fail(const char *fmt, long a = 0, long b = 0) {
   char buf[256];
   snprintf(buf, sizeof buf, fmt, a, b);
@@ -426,6 +635,26 @@ int failed(cudaError_t e) {
 template <typename T, typename C, int N, bool WITHIN, bool NORM> int launch(Params &p, cudaStream_t s) {
   const emmy_rotate_append_args &a = p.a;
   p.lanes = (a.head_dim / N + 1) / 2;
+  if constexpr (N > 1 && (NORM || !std::is_same<T, C>::value)) {
+    if (p.lanes <= 32 && (p.lanes & (p.lanes - 1)) == 0) {
+      // a token's heads go to more warps where tokens are few: 16 warps an SM at least
+      const int groups = (a.q_heads + 2 * a.kv_heads + 32 / p.lanes - 1) / (32 / p.lanes);
+      const int64_t wanted = 148 * 32;
+      const int shares = static_cast<int>(std::min<int64_t>(groups, std::max<int64_t>(1, (wanted + a.tokens - 1) / a.tokens)));
+      const dim3 grid((a.tokens + kWarps - 1) / kWarps, shares);
+      const size_t smem = size_t(kWarps) * (kGroups * 64 * 16 + a.rotary_dim * sizeof(float));
+      if (p.lanes == 4)
+        append_kernel<T, C, N, WITHIN, NORM, 4><<<grid, 32 * kWarps, smem, s>>>(p);
+      else if (p.lanes == 8)
+        append_kernel<T, C, N, WITHIN, NORM, 8><<<grid, 32 * kWarps, smem, s>>>(p);
+      else if (p.lanes == 16)
+        append_kernel<T, C, N, WITHIN, NORM, 16><<<grid, 32 * kWarps, smem, s>>>(p);
+      else
+        append_kernel<T, C, N, WITHIN, NORM, 0><<<grid, 32 * kWarps, smem, s>>>(p);
+      const cudaError_t e = cudaGetLastError();
+      return e == cudaSuccess ? 0 : failed(e);
+    }
+  }
   // heads in shares of equal size, and a few tokens a block where one is small
   const int heads = a.q_heads + 2 * a.kv_heads, most = p.lanes < kThreads ? kThreads / p.lanes : 1;
   const int shares = (heads + most - 1) / most, rows = (heads + shares - 1) / shares;
@@ -498,6 +727,12 @@ template <typename T> int dispatch(Params &p, bool small, bool norm, cudaStream_
 // `name`: the entry's, for messages
 int run(const char *name, Params &p, bool small, bool norm, void *stream) {
   const emmy_rotate_append_args *const a = &p.a;
+  // 2^shift / page_size rounded up is too large by less than 1, which a slot times that,
+  // below 2^shift, forgives
+  int log = 0;
+  while ((int64_t(1) << log) < a->page_size) ++log;
+  p.page_shift = 31 + log;
+  p.page_inverse = a->page_size > 0 ? static_cast<uint32_t>(((uint64_t(1) << p.page_shift) + a->page_size - 1) / a->page_size) : 0;
   auto bad = [&](const char *fmt, long x = 0, long y = 0) {
     char with[256];
     snprintf(with, sizeof with, "%s: %s", name, fmt);
