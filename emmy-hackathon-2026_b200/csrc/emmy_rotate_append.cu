@@ -30,11 +30,11 @@
 // square and a weight) or a cache of 8-bit floats (times a power of two -- exactly -- and
 // rounded once), each element takes twice the instructions, and that walk waited at its
 // barrier of each token: 8,191 tokens of 32 + 8 heads of 128 in 57 us, whatever the
-// tokens ahead.  A head of 2, 4, .. 32 threads goes through append_kernel instead, a
-// warp a token: its angles and weights stay in registers for all heads, the squares'
-// sums meet by shuffles, arithmetic is on pairs of floats (fma.rn.f32x2), the norm's
-// factor and the cache's power of two are one at the end, and nothing waits for another
-// warp.  Other heads take the walk above, with the squares in shared memory.
+// tokens ahead.  Heads of vectors go through append_kernel instead, a warp a token: its
+// angles and weights stay in registers for all heads, the squares' sums meet by shuffles,
+// arithmetic is on pairs of floats (fma.rn.f32x2), the norm's factor and the cache's power
+// of two are one at the end, and nothing waits for another warp: 34.5 us, 5,400 GB/s.
+// Heads that are no vectors take the walk above, with the squares in shared memory.
 #include "../../include/emmy_b200.h"
 
 #include <cuda_bf16.h>
@@ -464,8 +464,8 @@ __global__ void __launch_bounds__(kThreads, NORM ? kNormBlocks : kBlocks) rotate
 constexpr int kWarps = 4, kGroups = 4;      // of a block of append_kernel; groups of heads on their way or being turned
 
 // A warp has a token (of 4 a block) and every gridDim.y-th group of heads, `lanes` threads
-// a head: a power of two up to 32.  Thread's vectors and pairs as above.
-// LANES: `lanes` where it is known, else 0.
+// a head, 32 at most (256 components of 4 bytes).  A thread's vectors and pairs as above.
+// LANES: `lanes` where it is one of the common ones, else 0.
 template <typename T, typename C, int N, bool WITHIN, bool NORM, int LANES>
 __global__ void __launch_bounds__(32 * kWarps, 5) append_kernel(const __grid_constant__ Params p) {
   using V = Vec<T, N>;
@@ -475,8 +475,9 @@ __global__ void __launch_bounds__(32 * kWarps, 5) append_kernel(const __grid_con
   const int half = a.rotary_dim / 2, heads = a.q_heads + 2 * a.kv_heads, lanes = LANES ? LANES : p.lanes;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, token = blockIdx.x * kWarps + warp;
   if (token >= a.tokens) return;
-  const int at_once = 32 / lanes, mine = lane & (lanes - 1), step = at_once * gridDim.y;
-  int head = blockIdx.y * at_once + lane / lanes;
+  const int at_once = 32 / lanes, mine = lane % lanes, step = at_once * gridDim.y;
+  // (of 32 lanes, those that are too few for another head have none)
+  int head = lane / lanes < at_once ? blockIdx.y * at_once + lane / lanes : heads;
   // its two vectors, `apart` elements from one another, and their first pairs
   bool turn_one, turn_two;
   int one, apart, first_pair, second_pair;
@@ -558,9 +559,14 @@ __global__ void __launch_bounds__(32 * kWarps, 5) append_kernel(const __grid_con
       for (int e = 1; e < N / 2; ++e) x = fma2(f[e], f[e], x), y = fma2(g[e], g[e], y);
       const float2 sx = unpair(x), sy = unpair(y);
       float sum = (sx.x + sx.y) + (sy.x + sy.y);
+      if constexpr (LANES != 0) {
 #pragma unroll
-      for (int k = 1; k < (LANES ? LANES : 32); k *= 2)
-        if (LANES || k < lanes) sum += __shfl_xor_sync(~0u, sum, k);
+        for (int k = 1; k < LANES; k *= 2) sum += __shfl_xor_sync(~0u, sum, k);
+      } else {
+        float all = 0.f;
+        for (int k = 0; k < lanes; ++k) all += __shfl_sync(~0u, sum, lane - mine + k);
+        sum = all;
+      }
       const int kind = turns ? !query : weights_of;
       if (kind != weights_of) {
         const T *w = reinterpret_cast<const T *>(kind ? p.k_weight : p.q_weight) + one;
@@ -636,63 +642,52 @@ template <typename T, typename C, int N, bool WITHIN, bool NORM> int launch(Para
   const emmy_rotate_append_args &a = p.a;
   p.lanes = (a.head_dim / N + 1) / 2;
   if constexpr (N > 1 && (NORM || !std::is_same<T, C>::value)) {
-    if (p.lanes <= 32 && (p.lanes & (p.lanes - 1)) == 0) {
-      // a token's heads go to more warps where tokens are few: 16 warps an SM at least
-      const int groups = (a.q_heads + 2 * a.kv_heads + 32 / p.lanes - 1) / (32 / p.lanes);
-      const int64_t wanted = 148 * 32;
-      const int shares = static_cast<int>(std::min<int64_t>(groups, std::max<int64_t>(1, (wanted + a.tokens - 1) / a.tokens)));
-      const dim3 grid((a.tokens + kWarps - 1) / kWarps, shares);
-      const size_t smem = size_t(kWarps) * (kGroups * 64 * 16 + a.rotary_dim * sizeof(float));
-      if (p.lanes == 4)
-        append_kernel<T, C, N, WITHIN, NORM, 4><<<grid, 32 * kWarps, smem, s>>>(p);
-      else if (p.lanes == 8)
-        append_kernel<T, C, N, WITHIN, NORM, 8><<<grid, 32 * kWarps, smem, s>>>(p);
-      else if (p.lanes == 16)
-        append_kernel<T, C, N, WITHIN, NORM, 16><<<grid, 32 * kWarps, smem, s>>>(p);
-      else
-        append_kernel<T, C, N, WITHIN, NORM, 0><<<grid, 32 * kWarps, smem, s>>>(p);
-      const cudaError_t e = cudaGetLastError();
-      return e == cudaSuccess ? 0 : failed(e);
-    }
-  }
-  // heads in shares of equal size, and a few tokens a block where one is small
-  const int heads = a.q_heads + 2 * a.kv_heads, most = p.lanes < kThreads ? kThreads / p.lanes : 1;
-  const int shares = (heads + most - 1) / most, rows = (heads + shares - 1) / shares;
-  int tokens = kThreads / 2 / (p.lanes * rows);
-  tokens = tokens < 1 ? 1 : tokens > 64 ? 64 : tokens;
-  if (tokens > a.tokens) tokens = a.tokens;
-  static std::atomic<int> known[64];         // SMs of each device
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return failed(e);
-  int sms = dev < 64 ? known[dev].load() : 0;
-  if (!sms) {
-    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    // a token's heads go to more warps where tokens are few: 16 warps an SM at least
+    const int groups = (a.q_heads + 2 * a.kv_heads + 32 / p.lanes - 1) / (32 / p.lanes);
+    const int64_t wanted = 148 * 32;
+    const int shares = static_cast<int>(std::min<int64_t>(groups, std::max<int64_t>(1, (wanted + a.tokens - 1) / a.tokens)));
+    const dim3 grid((a.tokens + kWarps - 1) / kWarps, shares);
+    const size_t smem = size_t(kWarps) * (kGroups * 64 * 16 + a.rotary_dim * sizeof(float));
+    if (p.lanes == 4)
+      append_kernel<T, C, N, WITHIN, NORM, 4><<<grid, 32 * kWarps, smem, s>>>(p);
+    else if (p.lanes == 8)
+      append_kernel<T, C, N, WITHIN, NORM, 8><<<grid, 32 * kWarps, smem, s>>>(p);
+    else if (p.lanes == 16)
+      append_kernel<T, C, N, WITHIN, NORM, 16><<<grid, 32 * kWarps, smem, s>>>(p);
+    else
+      append_kernel<T, C, N, WITHIN, NORM, 0><<<grid, 32 * kWarps, smem, s>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : failed(e);
+  } else {
+    // heads in shares of equal size, and a few tokens a block where one is small
+    const int heads = a.q_heads + 2 * a.kv_heads, most = p.lanes < kThreads ? kThreads / p.lanes : 1;
+    const int shares = (heads + most - 1) / most, rows = (heads + shares - 1) / shares;
+    int tokens = kThreads / 2 / (p.lanes * rows);
+    tokens = tokens < 1 ? 1 : tokens > 64 ? 64 : tokens;
+    if (tokens > a.tokens) tokens = a.tokens;
+    static std::atomic<int> known[64];         // SMs of each device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return failed(e);
-    if (dev < 64) known[dev].store(sms);
-  }
-  const int want = (a.tokens + tokens - 1) / tokens;
-  int resident = sms * ((NORM ? kNormBlocks : kBlocks) * kThreads / (p.lanes * rows * tokens)) / shares;
-  if (resident < 1) resident = 1;
-  const dim3 grid(want < resident ? want : resident, shares), block(p.lanes, rows, tokens);
-  // angles of two turns; vectors, slots and positions on their way (N > 1): with
-  // 256 components and 384 threads 47 KiB, under the 48 that need no asking
-  const size_t smem = size_t(tokens) * 2 * a.rotary_dim * sizeof(float) +
-                      (N > 1 ? size_t(kAhead) * 2 * p.lanes * rows * tokens * (16 + 4) : 0) +
-                      (NORM ? size_t(2) * p.lanes * rows * tokens * sizeof(float) : 0);
-  if constexpr (NORM) {
-    // up to 51 KiB with the squares
-    static std::atomic<uint64_t> ready{0};   // a bit for each device
-    const uint64_t bit = uint64_t(1) << (dev & 63);
-    if (smem > 48 * 1024 && (dev > 63 || !(ready.load() & bit))) {
-      e = cudaFuncSetAttribute(rotate_append_kernel<T, C, N, WITHIN, NORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
+    int sms = dev < 64 ? known[dev].load() : 0;
+    if (!sms) {
+      e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
       if (e != cudaSuccess) return failed(e);
-      if (dev <= 63) ready.fetch_or(bit);
+      if (dev < 64) known[dev].store(sms);
     }
+    const int want = (a.tokens + tokens - 1) / tokens;
+    int resident = sms * ((NORM ? kNormBlocks : kBlocks) * kThreads / (p.lanes * rows * tokens)) / shares;
+    if (resident < 1) resident = 1;
+    const dim3 grid(want < resident ? want : resident, shares), block(p.lanes, rows, tokens);
+    // angles of two turns; vectors, slots and positions on their way (N > 1): with
+    // 256 components and 384 threads 47 KiB, under the 48 that need no asking
+    const size_t smem = size_t(tokens) * 2 * a.rotary_dim * sizeof(float) +
+                        (N > 1 ? size_t(kAhead) * 2 * p.lanes * rows * tokens * (16 + 4) : 0) +
+                        (NORM ? size_t(2) * p.lanes * rows * tokens * sizeof(float) : 0);
+    rotate_append_kernel<T, C, N, WITHIN, NORM><<<grid, block, smem, s>>>(p);
+    e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : failed(e);
   }
-  rotate_append_kernel<T, C, N, WITHIN, NORM><<<grid, block, smem, s>>>(p);
-  e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : failed(e);
 }
 
 // 16-byte accesses need every address and stride to be a multiple of 16 bytes
