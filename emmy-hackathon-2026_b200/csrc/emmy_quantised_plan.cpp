@@ -28,6 +28,10 @@ namespace {
 // shared in 37 parts, 69 in 296; 8 sequences of 8,191: 36 us shared, 33 in 48 parts).
 constexpr int kSharedCost = 5, kOwnCost = 2, kMinShared = 16, kMinOwn = 4, kMostParts = 64;
 constexpr int kCtasAnSm = 2;
+// 8-bit keys and values of sequences that are read back with others, though a kernel
+// would take them as they are: 15 tokens (120 rows) over 4,110 keys of 4 heads of 64 took
+// 46 us on 64 SMs before 138 us for seven sequences with more.
+constexpr int64_t kSmallBytes = 32 << 20;
 
 int fail(const char *fmt, long a = 0, long b = 0) {
   char buf[256];
@@ -61,9 +65,22 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
   for (int s = 0; s < a.sequences; ++s) {
     const int64_t rows = int64_t(a.q_lens[s]) * group;
     kind[s] = rows <= kFewRows ? kFew : rows <= middle_rows(a.head_dim) ? kMiddle : kMany;
-    any[kind[s]] = true;
     plan.max_kv = std::max(plan.max_kv, a.kv_lens[s]);
   }
+  // Launches that would not fill the GPU one after the other are one: where some
+  // sequences are read back, others of few bytes are too.
+  int64_t bytes[3] = {}, small = 0;
+  for (int s = 0; s < a.sequences; ++s) {
+    const int64_t seen = a.window ? std::min<int64_t>(a.kv_lens[s], int64_t(a.window) + a.q_lens[s]) : a.kv_lens[s];
+    if (a.q_lens[s]) bytes[kind[s]] += seen * a.kv_heads * a.head_dim * 2;
+  }
+  for (const int k : {kMiddle, kFew})
+    if (bytes[kMany] && bytes[k] && small + bytes[k] <= kSmallBytes) {
+      small += bytes[k];
+      for (int s = 0; s < a.sequences; ++s)
+        if (kind[s] == k && a.q_lens[s]) kind[s] = kMany;
+    }
+  for (int s = 0; s < a.sequences; ++s) any[kind[s]] = true;
   plan.tiles = few_tiles(a, kind);
   const int keys = slice_keys(a.head_dim);
   const int at_once = 8 * plan.tiles;
@@ -218,6 +235,8 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
   };
   plan.middle = plan_of(kMiddle);
   plan.many = plan_of(kMany);
+  // (its kernel without the few rows' code, which costs the chunks 7 %: 174 us against 162)
+  if (plan.many && plan.many->spread) plan.many->spread = false, plan.many->tiled = true;
   if (plan.many) {
     plan.table_width = static_cast<int32_t>(div_up(plan.many->max_kv, kBlock));
     table.assign(int64_t(a.sequences) * plan.table_width, 0);
