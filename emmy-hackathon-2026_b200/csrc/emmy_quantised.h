@@ -16,11 +16,11 @@ constexpr int kFewRows = 16;
 constexpr int middle_rows(int head_dim) { return head_dim == 128 ? 256 : 128; }
 constexpr int kBlock = 128;         // tokens of a page of the workspace, which keys are read back to
 
-// Warps of a CTA whose pieces have up to `tiles` tiles of 8 query rows: as many as the
-// registers of their sums allow twice an SM (128, 168 or 255 a thread).
-constexpr int warps_of(int tiles) { return tiles == 1 ? 8 : tiles == 2 ? 6 : 4; }
+// Warps of a CTA whose pieces have one or two tiles of 8 query rows: as many as the
+// registers of their sums allow twice an SM (128 or 168 a thread).
+constexpr int warps_of(int tiles) { return tiles == 1 ? 8 : 6; }
 
-// A piece of work: up to 8, 16 or 32 query rows of one sequence and key head (row r is
+// A piece of work: up to 8 or 16 query rows of one sequence and key head (row r is
 // new token (row0 + r) / G of the sequence, query head (row0 + r) % G of the group)
 // against some of the key slices that they see between them.  The warps of a CTA share
 // its `shared` pieces, slice by slice in turn, and have others of their own after
@@ -66,7 +66,7 @@ struct emmy_quantised_plan_s {
   emmy_paged_plan_s *middle = nullptr, *many = nullptr;       // of the sequences with more rows; null: none
   int64_t tokens = 0, part_rows = 0, workspace_pages = 0;
   int32_t sequences = 0, q_heads = 0, kv_heads = 0, head_dim = 0, causal = 0, window = 0, max_kv = 0;
-  int32_t tiles = 1;                         // tiles of 8 rows that a piece may have: 1, 2 or 4
+  int32_t tiles = 1;                         // tiles of 8 rows that a piece may have: 1 or 2
   int32_t table_width = 0, n_jobs = 0, n_joined = 0;
   bool reads = false;                        // some row sees a key
   ~emmy_quantised_plan_s() {

@@ -26,9 +26,17 @@
 // f16; they start at 2^6 and grow to 2^14 before the base moves, so that small ones
 // keep their bits.
 //
-// Many rows: bound by the tensor cores.  The keys are read back to 16 bits once, into
-// pages of 128 tokens (unscaled values, exact in either type; read_back_kernel), and go
-// through the 16-bit cache's tcgen05 attention.
+// What bounds it: the memory, where sequences are long: 64 of 517 to 8,191 keys, 32 + 8
+// heads of 128, 95 us (1.09 of reading them once), a key's 256 bytes taking each SM 11
+// cycles where the work on it takes 8.  A warp on its own needs no barrier and joins
+// nothing in shared memory; pieces that eight warps shared, with a thread fence, a counter
+// and the joining of parts at their ends, took 120 us, since each such step takes 3 us
+// while the memory is busy.  Short calls are bound by their latencies: about 4 us from
+// the launch to the first keys (lists, piece, page, keys, each behind the one before).
+//
+// More rows go through the 16-bit cache's tcgen05 attention, which widens 8-bit tiles
+// itself, or, with many, over keys and values that read_back_kernel reads back to 16 bits
+// once, in pages of 128 tokens (times their power of two: exact in either type).
 #include "emmy_quantised.h"
 
 #include <cuda.h>
@@ -81,7 +89,7 @@ template <int D, int NT> struct Shape {
   static constexpr int kSteps = D / 16;                                    // products of 16 components
   static constexpr int kRounds = D / 32;                                   // of 4 of a thread's components, at a unit's end
   static constexpr bool kQueryRegs = NT * D <= 128;                        // queries in registers
-  static constexpr int kStages = NT == 4 && D == 128 ? 4 : NT == 4 ? 5 : 3;        // slices of a warp in flight or in use
+  static constexpr int kStages = 3;                                        // slices of a warp in flight or in use
   static constexpr int kRing = kStages * kStage, kQueryBytes = kQueryRegs ? 0 : NT * kSteps * 256;
   static constexpr int kQuery = kWarps * kRing;
   static constexpr int kScales = kQuery + kWarps * kQueryBytes;

@@ -116,12 +116,14 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
           plan.reads = true;
         }
         blocks.push_back({s, r, p.nslices, items.size(), false});
+        if (items.size() + a.kv_heads > (size_t(1) << 26)) throw 1;
         for (p.kvh = 0; p.kvh < a.kv_heads; ++p.kvh) items.push_back(p);
       }
     } else if (highest(n) > lowest(0)) {
       plan.reads = true;
       for (int b = lowest(0) / kBlock; kind[s] == kMany && b * kBlock < highest(n); ++b) {
         // (a token that no row sees is not used, but lies in a page that is)
+        if (plan.workspace_pages >= (int64_t(1) << 26)) throw 1;
         jobs.push_back({s, b * kBlock, std::min(kBlock, len - b * kBlock), static_cast<int32_t>(plan.workspace_pages++)});
       }
     }

@@ -512,11 +512,13 @@ __global__ void __launch_bounds__(32 * kWarps, 5) append_kernel(const __grid_con
 #pragma unroll
   for (int k = 0; k + 1 < kGroups; ++k) fetch(head + k * step, k);
   int stage = 0;
-  int64_t k_at = -1, v_at = -1;                 // where the token's keys and values go; -1: nowhere
+  int64_t k_at = 0, v_at = 0;                   // where the token's keys and values go
+  bool stored = false;
   if (a.kv_heads) {
     const int slot = __ldg(reinterpret_cast<const int *>(a.slots) + token);
     if (slot >= 0 && slot < int64_t(a.pages) * a.page_size) {
       const int page = static_cast<int>(uint64_t(slot) * p.page_inverse >> p.page_shift), within = slot - page * a.page_size;
+      stored = true;
       k_at = page * a.k_cache_stride[0] + within * a.k_cache_stride[1];
       v_at = page * a.v_cache_stride[0] + within * a.v_cache_stride[1];
     }
@@ -605,7 +607,7 @@ __global__ void __launch_bounds__(32 * kWarps, 5) append_kernel(const __grid_con
       *reinterpret_cast<V *>(to) = r;
       round2(g, by, r);
       *reinterpret_cast<V *>(to + apart) = r;
-    } else if (k_at >= 0) {
+    } else if (stored) {
       const int kv_head = head - a.q_heads - (turns ? 0 : a.kv_heads);
       C *to = (turns ? reinterpret_cast<C *>(a.k_cache) + k_at + kv_head * a.k_cache_stride[2] : reinterpret_cast<C *>(a.v_cache) + v_at + kv_head * a.v_cache_stride[2]) + one;
       Vec<C, N> r, t;

@@ -7,6 +7,7 @@ length.  Attention: as for a 16-bit cache -- a weight rounded to 16 bits moves a
 at most u sum(p|v|)/l, the last rounding by u|o|, 32-bit scores, exponentials and sums by
 less than 1e-4 of sum(p|v|)/l and, in the logarithm, 1e-4 -- as reading the cache is exact."""
 import math
+import random
 
 import pytest
 import torch
@@ -300,6 +301,17 @@ def test_chunks(q_lens, kv_lens, dim, dtype, page):
 @pytest.mark.parametrize("dim", [64, 128])
 def test_window(window, dim):
     check([1, 300, 5, 129, 20], [1500, 1000, 5, 640, 700], 8, 2, dim, 16, window=window)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_batches(seed):
+    """Decoding, drafts and chunks together: every kernel's sequences in one call."""
+    r = random.Random(seed)
+    n, kv_heads, group = r.randint(1, 12), r.choice((1, 2, 3, 4, 8)), r.choice((1, 2, 3, 4, 8, 16))
+    q_lens = [r.choice((0, 1, 1, 1, r.randint(2, 9), r.randint(10, 40), r.choice((3, 100, 300)))) for _ in range(n)]
+    kv_lens = [max(q, r.choice((0, r.randint(1, 200), r.randint(1, 3000)))) if r.random() < 0.9 else q // 2 for q in q_lens]
+    check(q_lens, kv_lens, group * kv_heads, kv_heads, r.choice((64, 128)), r.choice((8, 16, 32, 64, 128, 256)), r.choice((BF16, F16)),
+          r.choice(("token", "head")), window=r.choice((None, None, r.randint(1, 700))), ctas=r.choice((None, None, 2, 11)), seed=seed)
 
 
 @pytest.mark.parametrize("dim", [64, 128])
