@@ -175,10 +175,18 @@ template <typename T, int N> __device__ __forceinline__ void round2(const uint64
   round_to(x, v);
 }
 
-// cosine and sine of position * frequency, the angle formed in 64 bits as half turns
+// Cosine and sine of position * frequency.  The angle is formed in 64 bits as half turns
+// and goes on as 32 bits and the rest, a first-order step: left out, that is up to 2^-25
+// half turns, 9e-8 radians, as much as the other roundings of a key together (of 8 million
+// 8-bit keys 17 to 27 went to the other neighbour, 6 to 13 with it; the time is the same).
 __device__ __forceinline__ void angle_of(int position, float frequency, float &c, float &s) {
-  const double turned = double(position) * double(frequency) * 0.31830988618379067154;
-  sincospif(float(turned - 2.0 * rint(0.5 * turned)), &s, &c);
+  double turned = double(position) * double(frequency) * 0.31830988618379067154;
+  turned -= 2.0 * rint(0.5 * turned);
+  const float near = float(turned), rest = float(turned - double(near)) * 3.14159265f;
+  float c0, s0;
+  sincospif(near, &s0, &c0);
+  c = fmaf(-s0, rest, c0);
+  s = fmaf(c0, rest, s0);
 }
 
 template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const void *from) {
