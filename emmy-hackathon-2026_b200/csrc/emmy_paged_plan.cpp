@@ -40,7 +40,7 @@ int fail(const char *fmt, long a = 0, long b = 0) {
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-void make(const emmy_paged_plan_args &a, const uint8_t *left_out, emmy_paged_plan_s &plan) {
+void make(const emmy_paged_plan_args &a, const uint8_t *left_out, int least_part, emmy_paged_plan_s &plan) {
   const int group = a.q_heads / a.kv_heads, per_tile = kTile / group, per_unit = plan.narrow ? per_tile : 2 * per_tile;
   const Cost cost = a.head_dim == 64 ? kCost64 : kCost128;
   std::vector<Unit> wide, narrow;     // one unit an item, to be cut below
@@ -162,8 +162,9 @@ void make(const emmy_paged_plan_args &a, const uint8_t *left_out, emmy_paged_pla
     int64_t filled = load[0];
     for (size_t i = 0; i < narrow.size(); ++i) {
       int b = 0;
+      const int least = narrow[i].ntok * group > 32 ? least_part : kMinNarrow;
       do {
-        const int rest = narrow[i].ntiles - b, least_take = std::min(kMinNarrow, std::max(1, rest));
+        const int rest = narrow[i].ntiles - b, least_take = std::min(least, std::max(1, rest));
         int64_t room = (level - filled - cost.narrow_unit) / cost.narrow_tile;
         while (room < least_take) {
           if (++c == a.ctas) return false;
@@ -171,7 +172,7 @@ void make(const emmy_paged_plan_args &a, const uint8_t *left_out, emmy_paged_pla
           room = (level - filled - cost.narrow_unit) / cost.narrow_tile;
         }
         // a rest too small to be a piece of its own goes along
-        const int take = rest - room >= kMinNarrow ? static_cast<int>(room) : rest;
+        const int take = rest - room >= least ? static_cast<int>(room) : rest;
         pieces.push_back({static_cast<int>(i), c, b, b + take});
         filled += cost.narrow_unit + cost.narrow_tile * take;
         b += take;
@@ -235,7 +236,7 @@ void make(const emmy_paged_plan_args &a, const uint8_t *left_out, emmy_paged_pla
 
 }  // namespace
 
-int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_out, bool narrow, emmy_paged_plan_t *out) {
+int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_out, bool narrow, int least_part, emmy_paged_plan_t *out) {
   if (!a || !out || a->sequences < 0 || (a->sequences && (!a->q_lens || !a->kv_lens)))
     return fail("emmy_paged_plan_make: bad argument");
   *out = nullptr;
@@ -268,7 +269,7 @@ int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_
     plan->window = args.window;
     plan->narrow = narrow;
     try {
-      make(args, left_out, *plan);
+      make(args, left_out, std::max(least_part, kMinNarrow), *plan);
     } catch (...) {
       delete plan;
       throw;
@@ -287,7 +288,7 @@ int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_
 }
 
 extern "C" EMMY_API int emmy_paged_plan_make(const emmy_paged_plan_args *a, emmy_paged_plan_t *out) {
-  return emmy_internal_paged_plan(a, nullptr, false, out);
+  return emmy_internal_paged_plan(a, nullptr, false, 0, out);
 }
 
 extern "C" EMMY_API int emmy_paged_plan_data(emmy_paged_plan_t plan, const int32_t **words, size_t *n_words,

@@ -10,10 +10,12 @@ namespace emmy_quantised {
 constexpr int slice_keys(int head_dim) { return 2048 / head_dim; }      // that a warp takes at once: 2 KiB of 8-bit keys
 // Query rows of a sequence and key head up to which they are few, and up to which the
 // tensor-core kernel widens its keys itself (128 rows at a time) instead of reading them
-// back.  32 sequences of up to 8,191 keys, 8 heads of 128: 256 rows 284 us against 332;
-// 24 of up to 4,095, 32 heads of 64: 128 rows 199 us against 268, 160 rows 334 against 268.
-constexpr int kFewRows = 16;
-constexpr int middle_rows(int head_dim) { return head_dim == 128 ? 256 : 128; }
+// back.  32 sequences of up to 8,191 keys, 8 heads of 128: 17 rows 128 us widened, 136 as
+// few; 384 rows 431 widened, 504 read back; 512 rows 565 and 503.  24 of up to 4,095, 32
+// heads of 64: 24 rows 130 us as few, 140 widened; 32 rows 138 and 135; 128 rows 200
+// widened, 278 read back; 160 rows 374 and 328.
+constexpr int few_rows(int head_dim) { return head_dim == 128 ? 16 : 24; }
+constexpr int middle_rows(int head_dim) { return head_dim == 128 ? 384 : 128; }
 constexpr int kBlock = 128;         // tokens of a page of the workspace, which keys are read back to
 
 // Warps of a CTA whose pieces have one or two tiles of 8 query rows: as many as the
@@ -94,7 +96,8 @@ inline Scratch scratch_of(const emmy_quantised_plan_s &plan) {
 }  // namespace emmy_quantised
 
 // emmy_paged_plan.cpp: a plan without the sequences that left_out marks, whose rows it
-// leaves alone; `narrow`: without wide units
-int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_out, bool narrow, emmy_paged_plan_t *out);
+// leaves alone; `narrow`: without wide units; least_part: key tiles of a part of a narrow unit
+// of more than 32 rows
+int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_out, bool narrow, int least_part, emmy_paged_plan_t *out);
 // emmy_paged_attention.cu: over a cache of 8-bit floats
 int emmy_internal_paged_attention8(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, uint64_t exponents, void *stream);

@@ -1,6 +1,6 @@
 // emmy_quantised_plan.cpp -- cuts the attention over an 8-bit cache into work.
 //
-// A sequence whose query rows of a key head are few (kFewRows) is bound by reading
+// A sequence whose query rows of a key head are few (few_rows) is bound by reading
 // its keys, which a kernel of its own takes as they lie: its slices of keys are
 // poured over the CTAs up to a common level, an item being cut where a CTA is full.
 // The pieces go to the CTA's warps together or to each on its own (below).
@@ -32,6 +32,10 @@ constexpr int kCtasAnSm = 2;
 // would take them as they are: 15 tokens (120 rows) over 4,110 keys of 4 heads of 64 took
 // 46 us on 64 SMs before 138 us for seven sequences with more.
 constexpr int64_t kSmallBytes = 32 << 20;
+// Key tiles of a part where more than 32 rows share a tile: each part leaves 128 rows for
+// the last to join.  1 sequence of 8,192 keys, 8 heads of 128: 256 rows 38 us, 44 with parts
+// of 2, 41 of 16; 600 rows 81, 100 and 76; 16 of up to 8,192, 68 to 128 rows 88, 95, 87.
+constexpr int kLeastPart = 8;
 
 int fail(const char *fmt, long a = 0, long b = 0) {
   char buf[256];
@@ -64,7 +68,7 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
   bool any[3] = {};
   for (int s = 0; s < a.sequences; ++s) {
     const int64_t rows = int64_t(a.q_lens[s]) * group;
-    kind[s] = rows <= kFewRows ? kFew : rows <= middle_rows(a.head_dim) ? kMiddle : kMany;
+    kind[s] = rows <= few_rows(a.head_dim) ? kFew : rows <= middle_rows(a.head_dim) ? kMiddle : kMany;
     plan.max_kv = std::max(plan.max_kv, a.kv_lens[s]);
   }
   // Launches that would not fill the GPU one after the other are one: where some
@@ -232,7 +236,7 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
     std::vector<uint8_t> left_out(a.sequences);
     for (int s = 0; s < a.sequences; ++s) left_out[s] = kind[s] != which;
     emmy_paged_plan_t made = nullptr;
-    if (any[which] && emmy_internal_paged_plan(&a, left_out.data(), which == kMiddle, &made)) throw 2;
+    if (any[which] && emmy_internal_paged_plan(&a, left_out.data(), which == kMiddle, kLeastPart, &made)) throw 2;
     return made;
   };
   plan.middle = plan_of(kMiddle);

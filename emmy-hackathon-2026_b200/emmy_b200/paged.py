@@ -553,10 +553,11 @@ def norm_rotate_append(rotation, norm, q, k, v, positions, slots, k_cache, v_cac
 class QuantisedPlan(AttentionPlan):
     """An :class:`AttentionPlan` for :func:`quantised_attention`.
 
-    Sequences with many new tokens, of over 256 query rows a key head (tokens
-    times ``q_heads / kv_heads``; 128 with a head_dim of 64), have their keys and values read back to 16
-    bits once a call, into ``scratch``: 4 bytes x kv_heads x head_dim for each of
-    the cached tokens that they see.  The others read the 8-bit cache as it lies."""
+    Sequences with many new tokens, of over 384 query rows a key head (tokens times
+    ``q_heads / kv_heads``; 128 with a head_dim of 64), have their keys and values
+    read back to 16 bits once a call, into ``scratch``: 4 bytes x kv_heads x head_dim
+    for each of the cached tokens that they see, and those of others with them where
+    that is 32 MiB of the cache at most.  The others read the 8-bit cache as it lies."""
 
     _kind = "quantised"
 

@@ -281,10 +281,10 @@ def test_head_groups(heads, kv_heads, dim):
     check([1, 3, 40, 129], [300, 3, 170, 513], heads, kv_heads, dim, 32)
 
 
-@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129, 255, 256, 257])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 7, 8, 9, 12, 13, 16, 17, 32, 33, 64, 65, 128, 129, 192, 193, 255, 256, 257])
 @pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
 def test_rows_around_the_tiles(tokens, dim, dtype):
-    """Query rows about 8, 16, 32, 128, 256 and 512, which the ways of computing begin at."""
+    """Query rows about 8, 16, 24, 32, 128, 256, 384 and 512, which the ways of computing begin at."""
     check([tokens, 1], [tokens + 100, 70], 4, 2, dim, 16, dtype)
 
 

@@ -12,7 +12,7 @@ from test_gpu_quantised import BF16, E4M3, F16, make, wanted
 pytestmark = pytest.mark.gpu
 
 # few query rows of a key head (of 2 each), those that are widened, and those read back
-FEW, MIDDLE, MANY = [5], [30], [140]
+FEW, MIDDLE, MANY = [5], [30], [200]
 
 
 def plan_and_inputs(q_lens, kv_lens, dim=128, heads=8, kv_heads=2, page=16, dtype=BF16, seed=0, **how):

@@ -12,7 +12,7 @@ from emmy_b200 import native, paged
 pytestmark = pytest.mark.usefixtures("native_lib")
 
 FIELDS = ("seq", "kvh", "tok0", "row0", "rows", "pos0", "lo", "hi", "kv_len", "slice0", "nslices", "split", "nsplit", "part_row")
-FEW, MIDDLE = 16, 128                 # rows of 64 components
+FEW, MIDDLE = 24, 128                 # rows of 64 components
 
 
 def parts_of(plan):
