@@ -6,7 +6,7 @@
 // The pieces go to the CTA's warps together or to each on its own (below).
 // With more rows, which the tensor-core kernel takes, the keys are widened within it
 // (middle), or read back to 16 bits once, in pages of 128 tokens, where many tiles of
-// rows use them (many).
+// rows use them (many).  Little work goes to the first kernel whatever its rows.
 #include "emmy_quantised.h"
 
 #include <algorithm>
@@ -32,6 +32,13 @@ constexpr int kCtasAnSm = 2;
 // would take them as they are: 15 tokens (120 rows) over 4,110 keys of 4 heads of 64 took
 // 46 us on 64 SMs before 138 us for seven sequences with more.
 constexpr int64_t kSmallBytes = 32 << 20;
+// Units x keys x blocks x head_dim^2 up to which more rows go to the kernel for few:
+// heads of 128, one sequence of 8,192 keys and 8 heads: 32 rows 18 us against 23, 64 rows
+// 26 and 30; of 32,768 keys: 32 rows (2^36) 35 and 41, 64 rows 60 and 54; 400 rows over 1,000 keys 21
+// and 30; 8 sequences of 2,000 keys (2^38): 32 rows 25 and 23.  32 heads of 64, 2,000 keys:
+// 64 rows 19 and 22.
+constexpr int kFewBlock = 16;
+constexpr double kIdle = 68719476736.0;      // 2^36
 // Key tiles of a part where more than 32 rows share a tile: each part leaves 128 rows for
 // the last to join.  1 sequence of 8,192 keys, 8 heads of 128: 256 rows 38 us, 44 with parts
 // of 2, 41 of 16; 600 rows 81, 100 and 76; 16 of up to 8,192, 68 to 128 rows 88, 95, 87.
@@ -71,13 +78,31 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
     kind[s] = rows <= few_rows(a.head_dim) ? kFew : rows <= middle_rows(a.head_dim) ? kMiddle : kMany;
     plan.max_kv = std::max(plan.max_kv, a.kv_lens[s]);
   }
+  // Work that would leave most of the GPU idle goes to the kernel for few rows, which cuts
+  // it finest, in blocks of kFewBlock rows.  Its time grows with the keys times the blocks
+  // that read them; the others' shrinks with the units that they have.
+  auto keys_of = [&](int s) {
+    return a.window ? std::min<int64_t>(a.kv_lens[s], int64_t(a.window) + a.q_lens[s]) : int64_t(a.kv_lens[s]);
+  };
+  for (const int least : {kMiddle, kMany}) {       // with the fewer rows alone only where there are no others
+    int64_t units = 0, pieces = 0, read = 0, others = 0;
+    for (int s = 0; s < a.sequences; ++s) {
+      if (!a.q_lens[s] || kind[s] == kFew) continue;
+      if (kind[s] > least) ++others;
+      const int64_t blocks = div_up(int64_t(a.q_lens[s]) * group, kFewBlock);
+      units += a.kv_heads;
+      pieces += blocks * a.kv_heads;
+      read += keys_of(s) * blocks * a.kv_heads;
+    }
+    if (others || pieces > int64_t(kCtasAnSm) * a.ctas) continue;
+    if (double(units) * double(read) * (a.head_dim * a.head_dim) <= kIdle)
+      for (int s = 0; s < a.sequences; ++s) kind[s] = kFew;
+  }
   // Launches that would not fill the GPU one after the other are one: where some
   // sequences are read back, others of few bytes are too.
   int64_t bytes[3] = {}, small = 0;
-  for (int s = 0; s < a.sequences; ++s) {
-    const int64_t seen = a.window ? std::min<int64_t>(a.kv_lens[s], int64_t(a.window) + a.q_lens[s]) : a.kv_lens[s];
-    if (a.q_lens[s]) bytes[kind[s]] += seen * a.kv_heads * a.head_dim * 2;
-  }
+  for (int s = 0; s < a.sequences; ++s)
+    if (a.q_lens[s]) bytes[kind[s]] += keys_of(s) * a.kv_heads * a.head_dim * 2;
   for (const int k : {kMiddle, kFew})
     if (bytes[kMany] && bytes[k] && small + bytes[k] <= kSmallBytes) {
       small += bytes[k];

@@ -557,7 +557,8 @@ class QuantisedPlan(AttentionPlan):
     ``q_heads / kv_heads``; 128 with a head_dim of 64), have their keys and values
     read back to 16 bits once a call, into ``scratch``: 4 bytes x kv_heads x head_dim
     for each of the cached tokens that they see, and those of others with them where
-    that is 32 MiB of the cache at most.  The others read the 8-bit cache as it lies."""
+    that is 32 MiB of the cache at most.  The others, and a little work of any kind,
+    read the 8-bit cache as it lies."""
 
     _kind = "quantised"
 

@@ -223,6 +223,13 @@ def test_append_writes_are_known_to_autograd():
 
 
 # ------------------------------------------------------------------ quantised_attention
+@pytest.fixture(params=[None, 3])
+def ways(request, monkeypatch):
+    """Plans for as many CTAs as there are, which little work goes to as few rows, and for a few, which it does not."""
+    made = paged.QuantisedPlan.__init__
+    monkeypatch.setattr(paged.QuantisedPlan, "__init__", lambda self, *args, **how: made(self, *args, **{"ctas": request.param, **how}))
+
+
 def make(q_lens, kv_lens, heads, kv_heads, dim, page, dtype=BF16, layout="token", seed=0, size=16.0):
     """Inputs whose cache holds NaN wherever no sequence has a token, and whose table has
     page numbers from nowhere after each sequence's last; and the cache's values."""
@@ -260,11 +267,14 @@ def wanted(made, q_lens, kv_lens, scale, causal=True, window=None):
 
 
 def check(q_lens, kv_lens, heads, kv_heads, dim, page, dtype=BF16, layout="token", causal=True, window=None, scale=None, ctas=None, seed=0):
+    """With as many CTAs as there are, which little work goes to as few rows, and with a few, which it does not."""
     made = make(q_lens, kv_lens, heads, kv_heads, dim, page, dtype, layout, seed)
-    plan = paged.QuantisedPlan(q_lens, kv_lens, heads, kv_heads, dim, causal, window, ctas=ctas)
-    out, lse = paged.quantised_attention(plan, *made, scale=scale)
-    plan.check()
-    close(out, lse, wanted(made, q_lens, kv_lens, scale or dim ** -0.5, causal, window), UNIT[dtype])
+    want = wanted(made, q_lens, kv_lens, scale or dim ** -0.5, causal, window)
+    for n in (3, ctas):
+        plan = paged.QuantisedPlan(q_lens, kv_lens, heads, kv_heads, dim, causal, window, ctas=n)
+        out, lse = paged.quantised_attention(plan, *made, scale=scale)
+        plan.check()
+        close(out, lse, want, UNIT[dtype])
     return plan, made, out, lse
 
 
@@ -366,6 +376,7 @@ def test_few_ctas(ctas):
     check([1] * 40, [17 * s % 333 for s in range(40)], 8, 2, 128, 16, ctas=ctas)
 
 
+@pytest.mark.usefixtures("ways")
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_scores_that_grow(dim, dtype):
@@ -390,6 +401,7 @@ def test_scores_that_grow(dim, dtype):
         assert float((lse.double() - ls).abs().max()) < 8e-3
 
 
+@pytest.mark.usefixtures("ways")
 @pytest.mark.parametrize("dtype,size", [(BF16, 2.0 ** 100), (BF16, 2.0 ** -100), (BF16, 2.0 ** -130), (F16, 60000.0), (F16, 2.0 ** -20)])
 def test_queries_of_any_size(dtype, size):
     """The power of two that makes a row of queries f16 comes out of the scores again."""
@@ -404,6 +416,7 @@ def test_queries_of_any_size(dtype, size):
     close(out, lse, wanted((q, k, v, e, table), q_lens, kv_lens, float(torch.tensor(scale, dtype=F32))), UNIT[dtype])
 
 
+@pytest.mark.usefixtures("ways")
 def test_queries_of_many_sizes_in_a_row():
     """Components 2^-24 of the largest count for as much as their keys make of them."""
     q_lens, kv_lens = [1, 7], [100, 90]
@@ -418,6 +431,7 @@ def test_queries_of_many_sizes_in_a_row():
     close(out, lse, wanted((q, k, v, e, table), q_lens, kv_lens, 4.0), UNIT[BF16])
 
 
+@pytest.mark.usefixtures("ways")
 def test_keys_that_are_not_numbers_concern_the_tokens_that_see_them():
     q_lens, kv_lens = [3, 140], [40, 150]
     q, k, v, e, table = make(q_lens, kv_lens, 4, 2, 64, 16)
@@ -431,6 +445,7 @@ def test_keys_that_are_not_numbers_concern_the_tokens_that_see_them():
     assert torch.equal(lse.isnan(), nan) and torch.equal(out.isnan().all(-1), nan) and torch.equal(out.isnan().any(-1), nan)
 
 
+@pytest.mark.usefixtures("ways")
 def test_strided_views_and_given_outputs():
     q_lens, kv_lens = [3, 130, 5], [200, 300, 90]
     q, k, v, e, table = make(q_lens, kv_lens, 8, 2, 64, 16)
@@ -462,6 +477,7 @@ def test_no_exponents_are_zeros():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.usefixtures("ways")
 @pytest.mark.parametrize("exponent", [-15, 7])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_exponents_at_the_ends(exponent, dtype):
@@ -482,6 +498,7 @@ def test_exponents_at_the_ends(exponent, dtype):
     assert torch.equal(got[0].float(), values(v, e[1])[table[0, 0].long(), 0].repeat_interleave(2, 0))
 
 
+@pytest.mark.usefixtures("ways")
 def test_pages_outside_the_cache_read_as_zeros():
     for n in (1, 64):
         q, k, v, e, table = make([n], [64], 4, 2, 64, 16)
@@ -496,6 +513,7 @@ def test_pages_outside_the_cache_read_as_zeros():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.usefixtures("ways")
 @pytest.mark.parametrize("n", [4, 150])
 def test_cache_beyond_32_bit_offsets(n):
     page, kv_heads, dim = 64, 8, 128
@@ -553,6 +571,7 @@ def test_no_tokens():
     plan.check()
 
 
+@pytest.mark.usefixtures("ways")
 def test_streams_and_graphs():
     q_lens, kv_lens = [1, 1, 140, 5], [5000, 77, 640, 300]
     made = make(q_lens, kv_lens, 8, 2, 128, 16)
@@ -768,6 +787,7 @@ def test_verify_no_sequences():
 
 
 # ------------------------------------------------------------------ together
+@pytest.mark.usefixtures("ways")
 @pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64)])
 def test_a_serving_step_with_drafts(dtype, dim):
     """Prompts into the 8-bit cache, attention of a step with drafts over it, and their

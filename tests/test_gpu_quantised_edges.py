@@ -7,7 +7,7 @@ import torch
 from emmy_b200 import native, paged
 from test_gpu_paged import UNIT, close
 from test_gpu_paged_streams import PENDING, states
-from test_gpu_quantised import BF16, E4M3, F16, make, wanted
+from test_gpu_quantised import BF16, E4M3, F16, make, wanted, ways  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -46,7 +46,7 @@ def test_every_kernel_in_one_call(dim, kv_heads, dtype, window):
 def test_a_plan_that_gave_up_stays_so(q_lens, dim):
     """Once a wait ran out (here: the word that says so is set), later calls with the plan write nothing."""
     group = 2
-    plan, made = plan_and_inputs(q_lens, [2000], dim, 2 * group, 2)
+    plan, made = plan_and_inputs(q_lens, [2000], dim, 2 * group, 2, ctas=3)      # (too few for all to be few)
     status = 3 if q_lens is FEW else 16       # its own, or the first word of the other kernel's plan behind it
     plan.words[status] = 2
     out, lse = torch.full_like(made[0], 7.0), torch.full(made[0].shape[:2], 7.0, device="cuda")
@@ -60,6 +60,7 @@ def test_a_plan_that_gave_up_stays_so(q_lens, dim):
     close(out, lse, wanted(made, q_lens, [2000], dim ** -0.5), UNIT[BF16])
 
 
+@pytest.mark.usefixtures("ways")
 @pytest.mark.parametrize("q_lens", [[1] * 3, [30, 25, 20], [300, 200, 1]])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_sequences_that_share_pages(q_lens, dim):
@@ -71,6 +72,7 @@ def test_sequences_that_share_pages(q_lens, dim):
     close(*paged.quantised_attention(plan, *made), wanted(made, q_lens, kv_lens, dim ** -0.5), UNIT[BF16])
 
 
+@pytest.mark.usefixtures("ways")
 @pytest.mark.parametrize("tokens", [1, 20, 200])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("page", [8, 64])
@@ -88,6 +90,7 @@ def test_pages_before_the_window_may_be_anything(tokens, dim, page):
     close(*paged.quantised_attention(plan, q, k, v, e, table), want, UNIT[BF16])
 
 
+@pytest.mark.usefixtures("ways")
 def test_two_plans_on_two_streams():
     """Graphs of two plans replayed at once, and exponents that change between replays."""
     shapes = [([1, 9, 70], [9000, 3000, 400]), ([200, 1], [1200, 7000])]
@@ -114,6 +117,7 @@ def test_two_plans_on_two_streams():
             plan.check()
 
 
+@pytest.mark.usefixtures("ways")
 def test_results_are_the_same_every_time():
     for q_lens in ([1] * 20, [9] * 20, [40] * 20, [200] * 4):
         kv_lens = [2000 + 300 * i for i in range(len(q_lens))]

@@ -54,8 +54,12 @@ def test_pieces_cover_the_work_once(q_lens, kv_lens, hq, hkv, causal, window, ct
     plan = paged.QuantisedPlan(q_lens, kv_lens, hq, hkv, 64, causal, window or None, device="cpu", ctas=ctas)
     pieces, first, warps = parts_of(plan)
     group = hq // hkv
-    # (few and middle ones of little go with those that are read back)
     kinds = [0 if q * group <= FEW else 1 if q * group <= MIDDLE else 2 for q in q_lens]
+    # (all are few where that is not much, or the middle ones where there are no others)
+    more = [(kv if not window else min(kv, window + q), -(-q * group // 16)) for q, kv, k in zip(q_lens, kv_lens, kinds) if k and q]
+    if sum(b for _, b in more) * hkv <= 2 * ctas and len(more) * hkv * sum(n * b for n, b in more) * hkv * 64 ** 2 <= 2 ** 36:
+        kinds = [0] * len(kinds)
+    # (few and middle ones of little go with those that are read back)
     seen = [min(kv, window + q if window else kv) * hkv * 64 * 2 if q else 0 for q, kv in zip(q_lens, kv_lens)]
     small = 0
     for k in (1, 0):
