@@ -16,6 +16,10 @@ constexpr int slice_keys(int head_dim) { return 2048 / head_dim; }      // that 
 // widened, 278 read back; 160 rows 374 and 328.
 constexpr int few_rows(int head_dim) { return head_dim == 128 ? 16 : 24; }
 constexpr int middle_rows(int head_dim) { return head_dim == 128 ? 384 : 128; }
+// The kernel for few rows divides a sequence's row r by G as r * ceil(2^16 / G) >> 16, which
+// is too large by less than r G / 2^16 of 1 / G: right for r G under 2^16, and in 32 bits
+// for r / G under 2^15.
+constexpr int64_t kMostRowsGroup = 1 << 15;
 constexpr int kBlock = 128;         // tokens of a page of the workspace, which keys are read back to
 
 // Warps of a CTA whose pieces have one or two tiles of 8 query rows: as many as the

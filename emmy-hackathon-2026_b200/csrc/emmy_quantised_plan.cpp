@@ -88,8 +88,8 @@ void make(const emmy_paged_plan_args &a, emmy_quantised_plan_s &plan) {
     int64_t units = 0, pieces = 0, read = 0, others = 0;
     for (int s = 0; s < a.sequences; ++s) {
       if (!a.q_lens[s] || kind[s] == kFew) continue;
-      if (kind[s] > least) ++others;
-      const int64_t blocks = div_up(int64_t(a.q_lens[s]) * group, kFewBlock);
+      const int64_t rows = int64_t(a.q_lens[s]) * group, blocks = div_up(rows, kFewBlock);
+      if (kind[s] > least || rows * group >= kMostRowsGroup) ++others;
       units += a.kv_heads;
       pieces += blocks * a.kv_heads;
       read += keys_of(s) * blocks * a.kv_heads;

@@ -60,6 +60,15 @@ def test_a_plan_that_gave_up_stays_so(q_lens, dim):
     close(out, lse, wanted(made, q_lens, [2000], dim ** -0.5), UNIT[BF16])
 
 
+@pytest.mark.parametrize("heads,kv_heads,tokens", [(127, 1, 4), (127, 1, 5), (127, 1, 30), (96, 1, 7), (100, 2, 6), (100, 2, 9), (39, 3, 40), (3, 1, 900)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_rows_of_little_work(heads, kv_heads, tokens, dim):
+    """Groups that are no powers of two, whose rows are many."""
+    for n in (tokens, tokens + 200):
+        plan, made = plan_and_inputs([tokens], [n], dim, heads, kv_heads)
+        close(*paged.quantised_attention(plan, *made), wanted(made, [tokens], [n], dim ** -0.5), UNIT[BF16])
+
+
 @pytest.mark.usefixtures("ways")
 @pytest.mark.parametrize("q_lens", [[1] * 3, [30, 25, 20], [300, 200, 1]])
 @pytest.mark.parametrize("dim", [64, 128])

@@ -44,6 +44,9 @@ CASES = [
     ([7, 25], [65536, 5000], 5, 1, True, 333),
     ([500, 1, 300], [700, 9000, 200], 8, 2, True, 0),
     ([0, 0], [10, 0], 4, 4, True, 0),
+    ([4], [100], 127, 1, True, 0),
+    ([5], [100], 127, 1, True, 0),
+    ([9, 1], [100, 90], 100, 1, True, 0),
     ([], [], 4, 4, True, 0),
 ]
 
@@ -57,7 +60,7 @@ def test_pieces_cover_the_work_once(q_lens, kv_lens, hq, hkv, causal, window, ct
     kinds = [0 if q * group <= FEW else 1 if q * group <= MIDDLE else 2 for q in q_lens]
     # (all are few where that is not much, or the middle ones where there are no others)
     more = [(kv if not window else min(kv, window + q), -(-q * group // 16)) for q, kv, k in zip(q_lens, kv_lens, kinds) if k and q]
-    if sum(b for _, b in more) * hkv <= 2 * ctas and len(more) * hkv * sum(n * b for n, b in more) * hkv * 64 ** 2 <= 2 ** 36:
+    if all(q * group * group < 2 ** 15 for q, k in zip(q_lens, kinds) if k) and sum(b for _, b in more) * hkv <= 2 * ctas and len(more) * hkv * sum(n * b for n, b in more) * hkv * 64 ** 2 <= 2 ** 36:
         kinds = [0] * len(kinds)
     # (few and middle ones of little go with those that are read back)
     seen = [min(kv, window + q if window else kv) * hkv * 64 * 2 if q else 0 for q, kv in zip(q_lens, kv_lens)]
@@ -125,6 +128,14 @@ def test_work_is_even(q_lens, kv_lens, most):
         load.append(-(-shared // warps) + max(own))
     even = sum(u["nslices"] for u in pieces) / 296 / warps
     assert max(load) <= most * even + 4, (max(load), even)
+
+
+def test_rows_of_a_piece_can_be_divided():
+    """The kernel for few rows takes row * ceil(2^16 / G) >> 16 for row / G: right for every row that it is given."""
+    for group in range(1, 129):
+        most = max(24, (2 ** 15 - 1) // group)
+        inverse = -(-2 ** 16 // group)
+        assert most * inverse < 2 ** 31 and all(r * inverse >> 16 == r // group for r in range(most + 1)), group
 
 
 @pytest.mark.parametrize("seed", range(30))
