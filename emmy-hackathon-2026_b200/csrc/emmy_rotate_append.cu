@@ -596,7 +596,8 @@ __global__ void __launch_bounds__(32 * kWarps, 5) append_kernel(const __grid_con
         for (int e = 0; e < N / 2; ++e) {
           const float2 x = unpair(f[e]), y = unpair(g[e]);
           f[e] = fma2(f[e], pair_of(c[e], c[e]), mul2(pair_of(x.y, x.x), pair_of(minus[e], s[e])));
-          g[e] = fma2(g[e], pair_of(c[N / 2 + e], c[N / 2 + e]), mul2(pair_of(y.y, y.x), pair_of(minus[N / 2 + e], s[N / 2 + e])));
+          // (by an angle of 0 an infinity that does not turn would make its neighbour NaN)
+          if (turn_two) g[e] = fma2(g[e], pair_of(c[N / 2 + e], c[N / 2 + e]), mul2(pair_of(y.y, y.x), pair_of(minus[N / 2 + e], s[N / 2 + e])));
         }
       } else {
 #pragma unroll
