@@ -179,6 +179,7 @@ template <typename T, int N> __device__ __forceinline__ void round2(const uint64
 // and goes on as 32 bits and the rest, a first-order step: left out, that is up to 2^-25
 // half turns, 9e-8 radians, as much as the other roundings of a key together (of 8 million
 // 8-bit keys 17 to 27 went to the other neighbour, 6 to 13 with it; the time is the same).
+// Without norms and 8 bits the walk ends at 32 bits, and rotate_append's results stay as they are.
 __device__ __forceinline__ void angle_of(int position, float frequency, float &c, float &s) {
   double turned = double(position) * double(frequency) * 0.31830988618379067154;
   turned -= 2.0 * rint(0.5 * turned);
@@ -284,11 +285,15 @@ __global__ void __launch_bounds__(kThreads, NORM ? kNormBlocks : kBlocks) rotate
   const int *const slots = reinterpret_cast<const int *>(a.slots);
   const int64_t n_slots = int64_t(a.pages) * a.page_size;
   auto turn = [&](float *to, int i, int position, float f) {
-    const double turned = double(position) * double(f) * 0.31830988618379067154;     // half turns
-    float s, c;
-    sincospif(float(turned - 2.0 * rint(0.5 * turned)), &s, &c);
-    to[i] = c;
-    to[half + i] = s;
+    if constexpr (NORM || SMALL) {
+      angle_of(position, f, to[i], to[half + i]);
+    } else {
+      const double turned = double(position) * double(f) * 0.31830988618379067154;     // half turns
+      float s, c;
+      sincospif(float(turned - 2.0 * rint(0.5 * turned)), &s, &c);
+      to[i] = c;
+      to[half + i] = s;
+    }
   };
 
   // single elements (N = 1) are read where they are used: too small to copy

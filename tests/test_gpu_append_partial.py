@@ -1,12 +1,12 @@
 """norm_rotate_append where only a part of a head turns: what is not a number stays where
-the definition has it."""
+the definition has it, angles of large positions, and parts that are no whole vectors."""
 import math
 
 import pytest
 import torch
 
 from emmy_b200 import paged
-from test_gpu_quantised import BF16, E4M3, F32
+from test_gpu_quantised import BF16, E4M3, F16, F32, appended
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +70,35 @@ def test_components_that_are_not_finite(dim, rotary, interleaved, dtype, bits8, 
     there = want[2].clone()
     there[each, :, each] = stored
     assert same(got[2], there)
+
+
+@pytest.mark.parametrize("dim,rotary", [(64, 64), (128, 128), (96, 20), (80, 20), (96, 36), (7, 6), (33, 2)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_angles_of_large_positions(dim, rotary, interleaved):
+    """Pairs (1, 0) come out as cosine and sine, whichever kernel takes the head.  A cosine in 32 bits is
+    off by 2 units in its last place at most and the step to the angle's rest by half a unit: 2.5 x 2^-23 of
+    the value.  The angle in 64 bits: two roundings of up to 2^18.4 half turns, 2^-33.6 of one, 2^-31.9
+    radians.  (An angle that ends at 32 bits is off by 2^-25 half turns, 9e-8 radians.)"""
+    tokens, half = 4096, rotary // 2
+    g = torch.Generator(device="cuda").manual_seed(rotary)
+    x = torch.zeros(tokens, 3, dim, device="cuda")
+    left = torch.arange(half, device="cuda") * (2 if interleaved else 1)
+    right = left + (1 if interleaved else half)
+    x[..., left] = 1.0
+    frequencies = torch.rand(half, generator=g, device="cuda")
+    positions = torch.randint(-(1 << 20), 1 << 20, (tokens,), generator=g, device="cuda", dtype=torch.int32)
+    out, _, _ = append(paged.Rotation(frequencies, interleaved=interleaved), None, x, 1, 1, positions, E4M3)
+    angle = positions.double()[:, None] * frequencies.double()           # (exact: 20 and 24 bits)
+    for at, want in ((left, angle.cos()), (right, angle.sin())):
+        off = (out[:, 0, at].double() - want).abs()
+        assert bool((off <= 2.0 ** -21 * want.abs() + 2.0 ** -31).all()), float((off - 2.0 ** -21 * want.abs()).max())
+
+
+@pytest.mark.parametrize("dim,rotary", [(96, 24), (96, 48), (80, 40), (80, 20), (192, 72), (128, 8)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("bits8,norm", [(True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_halves_that_are_no_vectors(dim, rotary, interleaved, bits8, norm, dtype):
+    """Heads of whole vectors, of which a part turns whose halves are none."""
+    appended(37, 6, 2, dim, rotary, 16, dtype, bits8, norm, interleaved=interleaved)
+    appended(600, 12, 4, dim, rotary, 16, dtype, bits8, norm, interleaved=interleaved)
