@@ -84,6 +84,7 @@ struct alignas(64) Params {
   const int *cta_first;
   const int *table;
   unsigned *counters, *status;
+  unsigned *batch_status;              // of the plan that this one is a part of; its own where it is none
   float *part_o;
   float2 *part_ml;
   void *out;
@@ -154,7 +155,7 @@ __device__ __forceinline__ uint64_t now_ns() {
 }
 
 // What a role needs to give up: the CTA's flag (any role may set it) and the
-// plan's status word.
+// plan's status word, with that of the plan which it is a part of.
 struct Guard {
   uint32_t dead;          // shared-memory address
   const Params &p;
@@ -169,6 +170,7 @@ struct Guard {
       if (now_ns() - t0 > 2000000000ull) {
         asm volatile("st.volatile.shared.b32 [%0], 1;" ::"r"(dead) : "memory");
         atomicExch(p.status, code);
+        atomicExch(p.batch_status, code);
         return false;
       }
     }
@@ -1266,7 +1268,7 @@ __global__ void __launch_bounds__(Warps<BITS8>::kThreads, 1) paged_attention_ker
   sm.base = (smem_addr(raw) + 1023) & ~1023u;
   const int warp = threadIdx.x / 32;
   // the first unit is on its way while the CTA sets itself up
-  const unsigned status = threadIdx.x == 0 ? __ldcg(p.status) : 0;
+  const unsigned status = threadIdx.x == 0 ? __ldcg(p.status) | __ldcg(p.batch_status) : 0;
   const int first = __ldg(p.cta_first + blockIdx.x), last = __ldg(p.cta_first + blockIdx.x + 1);
   asm volatile("prefetch.global.L1 [%0];" ::"l"(p.units + first));
   if (threadIdx.x == 0) {
@@ -1374,8 +1376,9 @@ template <int D, bool BF16, bool SPREAD, bool BITS8> int launch(const Params &p,
   return e == cudaSuccess ? 0 : cuda_fail("emmy_paged_attention: launch", e);
 }
 
-// bits8: the caches hold 8-bit floats, with `exponents`
-int run(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, bool bits8, uint64_t exponents, void *stream) {
+// bits8: the caches hold 8-bit floats, with `exponents`; batch_status: of the plan that
+// this one is a part of, or 0
+int run(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, bool bits8, uint64_t exponents, uint64_t batch_status, void *stream) {
   if (!plan || !a) return fail("emmy_paged_attention: bad argument");
   if (bits8 && !plan->narrow) return fail("emmy_paged_attention: a plan with wide units");
   if (a->dtype != 6 && a->dtype != 9) return fail("emmy_paged_attention: dtype %ld (f16 or bf16)", a->dtype);
@@ -1425,6 +1428,7 @@ int run(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, bool bits8, 
   }
   int *words = reinterpret_cast<int *>(a->plan_words);
   p.status = reinterpret_cast<unsigned *>(words);
+  p.batch_status = batch_status ? reinterpret_cast<unsigned *>(batch_status) : p.status;
   p.cta_first = words + 4;
   p.counters = reinterpret_cast<unsigned *>(words + plan->at.counters);
   p.units = reinterpret_cast<const Unit *>(words + plan->at.units);
@@ -1468,11 +1472,12 @@ int run(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, bool bits8, 
 }  // namespace
 
 extern "C" EMMY_API int emmy_paged_attention(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, void *stream) {
-  return run(plan, a, false, 0, stream);
+  return run(plan, a, false, 0, 0, stream);
 }
 
-int emmy_internal_paged_attention8(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, uint64_t exponents, void *stream) {
-  return run(plan, a, true, exponents, stream);
+int emmy_internal_paged_attention(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, bool bits8, uint64_t exponents, uint64_t batch_status,
+                                  void *stream) {
+  return run(plan, a, bits8, exponents, batch_status, stream);
 }
 
 extern "C" EMMY_API int emmy_paged_plan_status(emmy_paged_plan_t plan, uint64_t plan_words, void *stream) {

@@ -58,7 +58,8 @@ static_assert(sizeof(Job) == 16, "jobs are read as 16-byte records");
 // pieces, the status; from 4 on where the pieces of each CTA begin that its warps share
 // and then those of each warp (ctas x (warps + 1) + 1); pieces, rows to join, the words
 // of the plans of the sequences with more rows, middle and many (emmy_paged.h), the page
-// table [sequences][width] of the latter in the workspace, and the jobs that fill it.  The kernel writes the status only.
+// table [sequences][width] of the latter in the workspace, and the jobs that fill it.  The kernels write the
+// status (that of every kernel of a call: where one gave up none does any more) and what the other plans have of their own.
 struct Layout {
   static constexpr int status = 3;
   int ctas = 0, pieces = 0, joined = 0, middle = 0, many = 0, table = 0, jobs = 0;
@@ -103,5 +104,6 @@ inline Scratch scratch_of(const emmy_quantised_plan_s &plan) {
 // leaves alone; `narrow`: without wide units; least_part: key tiles of a part of a narrow unit
 // of more than 32 rows
 int emmy_internal_paged_plan(const emmy_paged_plan_args *a, const uint8_t *left_out, bool narrow, int least_part, emmy_paged_plan_t *out);
-// emmy_paged_attention.cu: over a cache of 8-bit floats
-int emmy_internal_paged_attention8(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, uint64_t exponents, void *stream);
+// emmy_paged_attention.cu: as a part of a plan whose status is at batch_status; bits8: over a cache of 8-bit floats
+int emmy_internal_paged_attention(emmy_paged_plan_t plan, const emmy_paged_attention_args *a, bool bits8, uint64_t exponents, uint64_t batch_status,
+                                  void *stream);

@@ -757,6 +757,7 @@ template <int D> __global__ void __launch_bounds__(128) join_kernel(const __grid
 
 struct ReadParams {
   const Job *jobs;
+  const unsigned *status;
   const int *table, *exponents;
   const uint8_t *k, *v;
   uint16_t *k_out, *v_out;              // [page][head][kBlock][D]
@@ -769,6 +770,7 @@ struct ReadParams {
 // One job's keys or values of a head, blockIdx = (job, head, keys or values); 16 bytes
 // a thread at once.
 template <int D> __global__ void __launch_bounds__(256) read_back_kernel(const __grid_constant__ ReadParams p) {
+  if (__ldcg(p.status)) return;
   const int4 words = __ldg(reinterpret_cast<const int4 *>(p.jobs) + blockIdx.x);
   const Job job{words.x, words.y, words.z, words.w};
   const int head = blockIdx.y;
@@ -864,6 +866,8 @@ extern "C" EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, con
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int d = plan->head_dim;
   int *words = reinterpret_cast<int *>(a->plan_words);
+  unsigned *const status = reinterpret_cast<unsigned *>(words + plan->at.status);
+  const uint64_t status_at = reinterpret_cast<uint64_t>(status);
   char *scratch_at = reinterpret_cast<char *>(a->scratch);
   // key * inverse >> shift is key / page_size for keys up to 2^30: 2^shift / page_size
   // rounded up is too large by less than 1, which key times that, under 2^shift, forgives
@@ -887,7 +891,7 @@ extern "C" EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, con
         if (int e = emmy_tensormap_encode(i ? &p.v : &p.k, 0, 4, i ? a->v_cache : a->k_cache, dims, steps, box, d == 128 ? 3 : 2)) return e;
       }
     }
-    p.status = reinterpret_cast<unsigned *>(words + plan->at.status);
+    p.status = status;
     p.first = words + 4;
     p.pieces = reinterpret_cast<const Piece *>(words + plan->at.pieces);
     p.table = reinterpret_cast<const int *>(a->table);
@@ -945,7 +949,7 @@ extern "C" EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, con
   if (plan->middle) {
     b.plan_words = reinterpret_cast<uint64_t>(words + plan->at.middle);
     b.scratch = a->scratch + scratch.middle;
-    if (int e = emmy_internal_paged_attention8(plan->middle, &b, args->exponents, stream)) return e;
+    if (int e = emmy_internal_paged_attention(plan->middle, &b, true, args->exponents, status_at, stream)) return e;
   }
   if (!plan->many) return 0;
   const int64_t page = int64_t(kBlock) * plan->kv_heads * d;
@@ -963,6 +967,7 @@ extern "C" EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, con
   if (plan->n_jobs) {
     ReadParams p{};
     p.jobs = reinterpret_cast<const Job *>(words + plan->at.jobs);
+    p.status = status;
     p.table = reinterpret_cast<const int *>(a->table);
     p.exponents = reinterpret_cast<const int *>(args->exponents);
     p.k = reinterpret_cast<const uint8_t *>(a->k_cache);
@@ -984,7 +989,7 @@ extern "C" EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, con
       read_back_kernel<64><<<grid, 256, 0, s>>>(p);
     if (const cudaError_t e = cudaGetLastError()) return cuda_fail("emmy_quantised_attention: launch", e);
   }
-  return emmy_paged_attention(plan->many, &b, stream);
+  return emmy_internal_paged_attention(plan->many, &b, false, 0, status_at, stream);
 }
 
 extern "C" EMMY_API int emmy_quantised_plan_status(emmy_quantised_plan_t plan, uint64_t plan_words, void *stream) {

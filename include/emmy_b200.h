@@ -323,7 +323,8 @@ typedef struct {
 } emmy_quantised_attention_args;
 EMMY_API int emmy_quantised_attention(emmy_quantised_plan_t plan, const emmy_quantised_attention_args *a,
                                       void *stream);
-/* As emmy_paged_plan_status. */
+/* As emmy_paged_plan_status: where a kernel of a call gave up, none of them does     */
+/* anything in later calls.                                                          */
 EMMY_API int emmy_quantised_plan_status(emmy_quantised_plan_t plan, uint64_t plan_words, void *stream);
 
 /* Drafted tokens against the target's probabilities.  Sequence s has rows          */
