@@ -34,7 +34,9 @@
 // angles and weights stay in registers for all heads, the squares' sums meet by shuffles,
 // arithmetic is on pairs of floats (fma.rn.f32x2), the norm's factor and the cache's power
 // of two are one at the end, and nothing waits for another warp: 34.5 us, 5,400 GB/s.
-// Heads that are no vectors take the walk above, with the squares in shared memory.
+// Heads that are no whole vectors, or of which a part turns that is none (halves of 12 of 96
+// components, say), take the walk above an element at a time, with the squares in shared
+// memory.
 #include "../../include/emmy_b200.h"
 
 #include <cuda_bf16.h>
@@ -201,11 +203,13 @@ template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const 
 // blockDim = (lanes, heads, tokens); blockIdx.y: the block's share of the heads
 // of queries, keys and values.  WITHIN: the pairs lie inside a vector
 // (interleaved, N > 1); otherwise a pair is one element of each of the thread's
-// two vectors.  C: the cache's elements, T or 8-bit floats.
+// two vectors.  C: the cache's elements, T or 8-bit floats.  With norms or an 8-bit
+// cache: single elements only (append_kernel has the vectors).
 template <typename T, typename C, int N, bool WITHIN, bool NORM>
 __global__ void __launch_bounds__(kThreads, NORM ? kNormBlocks : kBlocks) rotate_append_kernel(const __grid_constant__ Params p) {
   using V = Vec<T, N>;
   constexpr bool SMALL = !std::is_same<T, C>::value;
+  static_assert(N == 1 || !(NORM || SMALL), "vectors with norms or 8 bits are append_kernel's");
   extern __shared__ __align__(16) float angles[];
   const emmy_rotate_append_args &a = p.a;
   const int half = a.rotary_dim / 2, heads = a.q_heads + 2 * a.kv_heads;
@@ -301,8 +305,8 @@ __global__ void __launch_bounds__(kThreads, NORM ? kNormBlocks : kBlocks) rotate
   const int threads = blockDim.x * blockDim.y * blockDim.z, me = (threadIdx.z * blockDim.y + threadIdx.y) * blockDim.x + lane;
   V *const vectors = reinterpret_cast<V *>(angles + blockDim.z * 2 * a.rotary_dim) + me;       // [kAhead][2][threads]
   int *const numbers = reinterpret_cast<int *>(vectors - me + (COPIED ? kAhead * 2 * threads : 0)) + me;   // [kAhead][2][threads]
-  // sums of squares of this token and the next in turn, [2][threads]
-  [[maybe_unused]] float *const squares = reinterpret_cast<float *>(numbers - me + (COPIED ? kAhead * 2 * threads : 0)) + me;
+  // (NORM, where nothing is copied) sums of squares of this token and the next in turn, [2][threads]
+  [[maybe_unused]] float *const squares = reinterpret_cast<float *>(vectors - me) + me;
   [[maybe_unused]] int odd = 0;
   auto fetch = [&](int token, int stage) {
     if (COPIED && token < a.tokens) {
@@ -330,8 +334,8 @@ __global__ void __launch_bounds__(kThreads, NORM ? kNormBlocks : kBlocks) rotate
       float sum = 0.f;
       if (token < a.tokens && moves) {
         const T *at = src + token * src_token;
-        read_one = COPIED ? vectors[stage * 2 * threads] : *reinterpret_cast<const V *>(at);
-        read_two = COPIED ? vectors[(stage * 2 + 1) * threads] : *reinterpret_cast<const V *>(at + apart);
+        read_one = *reinterpret_cast<const V *>(at);
+        read_two = *reinterpret_cast<const V *>(at + apart);
         float f[N], g[N];
         widen(read_one, f);
         widen(read_two, g);
@@ -416,10 +420,8 @@ __global__ void __launch_bounds__(kThreads, NORM ? kNormBlocks : kBlocks) rotate
                         cg = c[N / 2 + e / 2], sg = s[N / 2 + e / 2];
             f[e] = f0 * ce - f1 * se;
             f[e + 1] = f1 * ce + f0 * se;
-            if (!(NORM || SMALL) || turn_two) {      // (otherwise left out below)
-              g[e] = g0 * cg - g1 * sg;
-              g[e + 1] = g1 * cg + g0 * sg;
-            }
+            g[e] = g0 * cg - g1 * sg;      // (left out below where it does not turn)
+            g[e + 1] = g1 * cg + g0 * sg;
           }
         } else {
 #pragma unroll
