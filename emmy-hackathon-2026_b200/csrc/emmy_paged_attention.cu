@@ -109,6 +109,11 @@ template <int D, bool BITS8> struct Shape {
   static constexpr int kEnd = kPowers + (BITS8 ? 2 * kTile : 0);
   // tiles that are copied ahead, and bytes of an element there
   static constexpr int kCopied = BITS8 ? kRawStages : kStages, kElement = BITS8 ? 1 : 2;
+  // A loader waits for a stage by one bit of its phase, which two fills earlier has as well.
+  // It comes to a place of the ring at most 3 after its last (load_role), for which it saw
+  // the fill `kCopied` before that released, and stages are released in the ring's order: from
+  // 3 stages on that covers the fill 2 kCopied before the place.
+  static_assert(kCopied >= 3, "a stage's phase would be ambiguous");
   static_assert(kEnd + 1024 <= kSmem, "shared memory");
 };
 
@@ -432,7 +437,9 @@ __device__ __forceinline__ void load_queries(const Params &p, const Smem<D, SPRE
 // sees are left out; what the stage then holds in their place is masked (keys)
 // or cleared (values).  The order of the tiles in the ring is that of their use:
 // the first keys (one tile, or one for each stream), then values of tile n and
-// keys of tile n + ahead.  One warp for both took 2,400 cycles a tile pair, more
+// keys of tile n + ahead; a loader's next place is at most 3 on, in a unit (2) and from
+// one to the next alike: the last keys lie 3 before a unit's end, the first values 2
+// after its start.  One warp for both took 2,400 cycles a tile pair, more
 // than a pair of 64-component heads takes to arrive.
 template <bool VALUES, int D, bool SPREAD, bool BITS8>
 __device__ void load_role(const Params &p, const Smem<D, SPREAD, BITS8> &sm, const Guard &g, int first, int last) {
