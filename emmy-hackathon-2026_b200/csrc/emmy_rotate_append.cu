@@ -51,6 +51,18 @@
 
 int emmy_internal_fail(int code, const char *msg);   // emmy_runtime.cpp
 
+// SMs of the current device, which is asked once; a cudaError_t
+int emmy_internal_sms(int *sms) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev)) return e;
+  *sms = dev < 64 ? known[dev].load() : 0;
+  if (*sms) return cudaSuccess;
+  if (const cudaError_t e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev)) return e;
+  if (dev < 64) known[dev].store(*sms);
+  return cudaSuccess;
+}
+
 namespace {
 
 constexpr int kThreads = 384, kBlocks = 3;      // at most a block; at least an SM
@@ -659,10 +671,12 @@ int failed(cudaError_t e) {
 template <typename T, typename C, int N, bool WITHIN, bool NORM> int launch(Params &p, cudaStream_t s) {
   const emmy_rotate_append_args &a = p.a;
   p.lanes = (a.head_dim / N + 1) / 2;
+  int sms = 0;
+  if (const int e = emmy_internal_sms(&sms)) return failed(static_cast<cudaError_t>(e));
   if constexpr (N > 1 && (NORM || !std::is_same<T, C>::value)) {
     // a token's heads go to more warps where tokens are few: 16 warps an SM at least
     const int groups = (a.q_heads + 2 * a.kv_heads + 32 / p.lanes - 1) / (32 / p.lanes);
-    const int64_t wanted = 148 * 32;
+    const int64_t wanted = sms * 32;
     const int shares = static_cast<int>(std::min<int64_t>(groups, std::max<int64_t>(1, (wanted + a.tokens - 1) / a.tokens)));
     const dim3 grid((a.tokens + kWarps - 1) / kWarps, shares);
     const size_t smem = size_t(kWarps) * (kGroups * 64 * 16 + a.rotary_dim * sizeof(float));
@@ -683,16 +697,6 @@ template <typename T, typename C, int N, bool WITHIN, bool NORM> int launch(Para
     int tokens = kThreads / 2 / (p.lanes * rows);
     tokens = tokens < 1 ? 1 : tokens > 64 ? 64 : tokens;
     if (tokens > a.tokens) tokens = a.tokens;
-    static std::atomic<int> known[64];         // SMs of each device
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return failed(e);
-    int sms = dev < 64 ? known[dev].load() : 0;
-    if (!sms) {
-      e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-      if (e != cudaSuccess) return failed(e);
-      if (dev < 64) known[dev].store(sms);
-    }
     const int want = (a.tokens + tokens - 1) / tokens;
     int resident = sms * ((NORM ? kNormBlocks : kBlocks) * kThreads / (p.lanes * rows * tokens)) / shares;
     if (resident < 1) resident = 1;
@@ -703,7 +707,7 @@ template <typename T, typename C, int N, bool WITHIN, bool NORM> int launch(Para
                         (N > 1 ? size_t(kAhead) * 2 * p.lanes * rows * tokens * (16 + 4) : 0) +
                         (NORM ? size_t(2) * p.lanes * rows * tokens * sizeof(float) : 0);
     rotate_append_kernel<T, C, N, WITHIN, NORM><<<grid, block, smem, s>>>(p);
-    e = cudaGetLastError();
+    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : failed(e);
   }
 }

@@ -31,6 +31,7 @@
 namespace cg = cooperative_groups;
 
 int emmy_internal_fail(int code, const char *msg);   // emmy_runtime.cpp
+int emmy_internal_sms(int *sms);                     // emmy_rotate_append.cu
 
 namespace {
 
@@ -241,8 +242,9 @@ int cuda_fail(const char *what, cudaError_t e) {
 template <typename T> int launch(const emmy_verify_args &a, cudaStream_t s) {
   // CTAs of a cluster: as many as have 4,096 elements each, fewer where the sequences
   // fill the GPU's 4 CTAs an SM without
-  int ctas = 1;
-  while (ctas < kMostCtas && a.vocabulary > 4096 * ctas && int64_t(a.sequences) * 2 * ctas <= 4 * 148) ctas *= 2;
+  int ctas = 1, sms = 0;
+  if (const int e = emmy_internal_sms(&sms)) return cuda_fail("emmy_verify: device", static_cast<cudaError_t>(e));
+  while (ctas < kMostCtas && a.vocabulary > 4096 * ctas && int64_t(a.sequences) * 2 * ctas <= 4 * sms) ctas *= 2;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(a.sequences) * ctas);
   config.blockDim = dim3(kThreads);
