@@ -11,11 +11,16 @@
 // order (distributed shared memory), and the CTA with the segment in which v falls goes
 // through that segment again, a thread a few elements.  Nothing is kept between calls.
 //
-// Products, differences and sums are in 64 bits, where products and differences of
-// 32-bit numbers are exact or off by 2^-53: a token is another one than the definition's
-// only if v comes within 2^-50 or so of a border.  Sums in 32 bits of 131,071 elements
-// would move borders by 1e-6 and one token in a hundred.  At the rate of the memory an
-// SM has 3 elements a cycle, for which the conversions and additions in 64 bits suffice.
+// Products, differences and sums are in 64 bits.  Products and differences of 32-bit
+// numbers are exact or off by 2^-53.  A sum of numbers that are not negative is off by
+// 2^-53 of it for each addition on an element's way: those of its lane one after the
+// other (64 of 131,071 elements over 8 CTAs, 512 over one) and 30 or so of lanes, segments
+// and threads.  So a token is another one than with exact sums only if v comes within twice
+// that of a border: 2^-45 there, 2^-42 over one CTA, more as the vocabulary grows.  (Sums
+// one after the other in 64 bits are off by up to 2^-36 of as many.)  Sums in 32 bits of
+// 131,071 elements would move borders by 1e-6 and one token in a hundred.  At the rate of
+// the memory an SM has 3 elements a cycle, for which the conversions and additions in 64
+// bits suffice.
 #include "../../include/emmy_b200.h"
 
 #include <cooperative_groups.h>
