@@ -36,7 +36,8 @@
 // of two are one at the end, and nothing waits for another warp: 34.5 us, 5,400 GB/s.
 // Heads that are no whole vectors, or of which a part turns that is none (halves of 12 of 96
 // components, say), take the walk above an element at a time, with the squares in shared
-// memory.
+// memory: right, and slow, as each element is a load and a store of its own (8,191 tokens of
+// 32 + 8 heads of 96, bfloat16: 276 us, 39 where all of a head turns).
 #include "../../include/emmy_b200.h"
 
 #include <cuda_bf16.h>
@@ -192,7 +193,7 @@ template <typename T, int N> __device__ __forceinline__ void round2(const uint64
 // Cosine and sine of position * frequency.  The angle is formed in 64 bits as half turns
 // and goes on as 32 bits and the rest, a first-order step: left out, that is up to 2^-25
 // half turns, 9e-8 radians, as much as the other roundings of a key together (of 8 million
-// 8-bit keys 17 to 27 went to the other neighbour, 6 to 13 with it; the time is the same).
+// 8-bit keys 17 to 27 went to the other neighbour, 6 to 15 with it; the time is the same).
 // Without norms and 8 bits the walk ends at 32 bits, and rotate_append's results stay as they are.
 __device__ __forceinline__ void angle_of(int position, float frequency, float &c, float &s) {
   double turned = double(position) * double(frequency) * 0.31830988618379067154;

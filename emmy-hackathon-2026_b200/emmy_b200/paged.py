@@ -279,8 +279,8 @@ class AttentionPlan(_Kept):
     ``q_heads`` is ``kv_heads`` times at most 128; ``head_dim`` is 64 or 128.
     ``ctas``: over how many CTAs the work is spread, one for each SM by default.
     Made by the host, in 30 us for one sequence, 140 to 300 for 64 to 256 that
-    decode and 0.5 to 1.2 ms where chunks of hundreds of tokens are among them,
-    and copied from pageable memory: the host waits for the current stream.
+    decode and 0.5 to 1.2 ms where chunks of hundreds of tokens are among them
+    (:class:`QuantisedPlan`: see there), and copied from pageable memory: the host waits for the current stream.
 
     A plan holds device memory (``words``, ``scratch``) that its calls write:
     they must not overlap on the GPU, so calls on several streams need a plan
@@ -558,7 +558,16 @@ class QuantisedPlan(AttentionPlan):
     read back to 16 bits once a call, into ``scratch``: 4 bytes x kv_heads x head_dim
     for each of the cached tokens that they see, and those of others with them where
     that is 32 MiB of the cache at most.  The others, and a little work of any kind,
-    read the 8-bit cache as it lies."""
+    read the 8-bit cache as it lies.
+
+    Weights are rounded to float16 where the cache is read as it lies, to q's type where
+    it is read back, and sums are cut where the batch's work is.  So a sequence's result
+    may move within those roundings with the others of its batch; the same plan gives
+    the same bits.
+
+    Made by the host and copied, as an :class:`AttentionPlan`, in 45 to 95 us for one
+    sequence, 280, 400 and 800 for 8, 64 and 256 that decode and 0.5 to 1 ms with
+    chunks of hundreds of tokens."""
 
     _kind = "quantised"
 
