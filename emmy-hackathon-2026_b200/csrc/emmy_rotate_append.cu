@@ -193,7 +193,7 @@ template <typename T, int N> __device__ __forceinline__ void round2(const uint64
 // Cosine and sine of position * frequency.  The angle is formed in 64 bits as half turns
 // and goes on as 32 bits and the rest, a first-order step: left out, that is up to 2^-25
 // half turns, 9e-8 radians, as much as the other roundings of a key together (of 8 million
-// 8-bit keys 17 to 27 went to the other neighbour, 6 to 15 with it; the time is the same).
+// 8-bit keys 17 to 27 went to the other neighbour, 4 to 16 with it; the time is the same).
 // Without norms and 8 bits the walk ends at 32 bits, and rotate_append's results stay as they are.
 __device__ __forceinline__ void angle_of(int position, float frequency, float &c, float &s) {
   double turned = double(position) * double(frequency) * 0.31830988618379067154;
